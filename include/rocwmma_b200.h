@@ -353,6 +353,97 @@ int b200wmma_gemv_f64(uint32_t m, uint32_t n, const double* a, uint32_t lda, int
                       const double* x, double* y, double alpha, double beta, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Matrix-vector products with 4-bit weights and group scales (no counterpart in the reference):
+ *   y[r][i] = alpha * sum_k x[r][k] * s[i][k / group] * (q[i][k] - z[i][k / group]) + beta * y[r][i]
+ * for `rows` vectors x (one for a single token, a few for several sequences or drafted tokens; any number is right, the
+ * kernel is made for up to 64).
+ * A is m x n, row major, two 4-bit values per byte along n with the even column in the low nibble (the packing of
+ * b200wmma_gemm_i4), lda_bytes bytes per row.  zeros == NULL: q is signed, [-8, 7], and z = 0.  zeros != NULL: q is
+ * unsigned, [0, 15], and z = the low four bits of zeros[i * ld_zeros + k / group].
+ * scales[i * ld_scales + k / group], x and y hold data_type (B200WMMA_OUT_F16 or B200WMMA_OUT_BF16); y may hold fp32
+ * instead (out_type).  Products are exact, sums are fp32, y is rounded once.  beta == 0: y is not read.
+ * n and group are multiples of 32; the last group of a row may be short, group >= n is one scale per row.
+ * a, lda_bytes, x and ldx (in bytes) are multiples of 16.  y must not overlap the inputs.  No workspace.
+ * ------------------------------------------------------------------------------------------ */
+int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows,
+                     const uint8_t* a_packed, uint32_t lda_bytes,
+                     const void* scales, uint32_t ld_scales, const uint8_t* zeros, uint32_t ld_zeros, uint32_t group,
+                     const void* x, uint32_t ldx, void* y, uint32_t ldy, float alpha, float beta,
+                     int data_type, int out_type, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention: chained products with a softmax between them, forward and backward (no counterpart in the reference).
+ * For query i, key j of one batch entry and query head h (key head h / (heads_q / heads_kv)), off = len_kv - len_q:
+ *   t = scale * q_i . k_j;   c = cap > 0 ? cap * tanh(t / cap) : t;   s = c - slopes[h] * |i + off - j|
+ *   j is visible to i if (!causal or j <= i + off or j < prefix[batch]) and (no documents or doc_q[i] == doc_kv[j] >= 0)
+ *   p = exp(s - lse), lse = log(sum over visible j of exp(s));   o_i = sum over visible j of p * v_j
+ * A query that sees no key gets o = 0 and lse = -infinity, and no gradient flows through it.
+ * data_type is B200WMMA_OUT_F16 or B200WMMA_OUT_BF16 and holds for every matrix; p and the backward pass's ds are rounded
+ * to it between the two products, everything else (scores, sums, statistics, accumulators) is fp32.
+ * head_dim is a multiple of 8, at most 128.  Rows (one token of one head) are contiguous; the strides of batch entries,
+ * tokens and heads are free multiples of 8 elements (any value for an extent of 1), bases 16-byte aligned.
+ * slopes [heads_q] fp32, prefix [batch], doc_q [batch][len_q], doc_kv [batch][len_kv] int32 and may be NULL (doc_q and
+ * doc_kv only together).  A negative document marks padding: whatever the rows of padding hold, NaN included, has no
+ * influence; their outputs and gradients are zero.  All other elements of q, k, v and dout must be finite, visible or not.
+ * slopes are constants: there is no gradient for them.
+ * lse: [batch][heads_q][len_q] fp32; attn_fwd accepts NULL.  attn_bwd takes o and lse as attn_fwd wrote them and writes
+ * dq, dk and dv (sums over the query heads of a key head); results do not depend on the order of execution.
+ * Outputs must not overlap inputs.  workspace: device scratch of b200wmma_attn_workspace_bytes() bytes, 16-byte aligned;
+ * calls that may overlap on the GPU must not share one.  attn_fwd without documents needs none (NULL / 0).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct b200wmma_attn_strides
+{
+    int64_t batch, token, head; /* in elements */
+} b200wmma_attn_strides;
+
+typedef struct b200wmma_attn_args
+{
+    uint32_t batch, heads_q, heads_kv, len_q, len_kv, head_dim;
+    int32_t  data_type;
+    int32_t  causal;
+    float    scale;
+    float    cap; /* 0 = none */
+    const float*   slopes;
+    const int32_t* prefix;
+    const int32_t* doc_q;
+    const int32_t* doc_kv;
+    b200wmma_attn_strides q, k, v, o;
+    b200wmma_attn_strides dout, dq, dk, dv; /* attn_bwd only */
+} b200wmma_attn_args;
+
+size_t b200wmma_attn_workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv, int backward);
+int b200wmma_attn_fwd(const b200wmma_attn_args* args, const void* q, const void* k, const void* v, void* o, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, const void* k, const void* v, const void* o,
+                      const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention of drafted tokens over a paged cache (the serving form of the operator above; one token per sequence is
+ * drafts == 1).  Scores, cap and slopes are those of b200wmma_attn_fwd.
+ * Sequence b holds lens[b] tokens, its drafted tokens follow them: token p (drafted token t is p = lens[b] + t) has its
+ * key and value in row p % page_size of page block_table[b * ld_table + p / page_size] of k_cache / v_cache.
+ * Every drafted token sees the lens[b] tokens; drafted token i sees drafted token j if bit j of tree[b * drafts + i] is
+ * set (tree == NULL: j <= i).  Distances for slopes: token p < lens[b] stands at p, drafted token t at
+ * lens[b] + depths[b * drafts + t] (depths == NULL: t).
+ * drafts is 1 to 64.  n_drafts [batch] int32 or NULL: only the first n_drafts[b] drafted tokens exist; later rows of o
+ * are left as they were.  A drafted token that sees nothing gets o = 0.
+ * Strides of q and o: batch, token and head as above; of the caches: pages (args->k.batch), rows in a page (.token) and
+ * key heads (.head).  From args are used: batch, heads_q, heads_kv, head_dim (multiple of 8, at most 128), data_type,
+ * scale, cap, slopes and the strides q, k, v, o; every other field must be zero.
+ * Lengths and pages live on the device and are not checked on the host: a negative length counts as 0, tokens beyond
+ * ld_table * page_size and tokens in pages outside [0, num_pages) are not read and not visible.  Rows of the cache that
+ * no token of the batch occupies may hold anything, NaN included.
+ * workspace: b200wmma_attn_tree_workspace_bytes() bytes, max_tokens = ld_table * page_size; same rules as above.
+ * ------------------------------------------------------------------------------------------ */
+size_t b200wmma_attn_tree_workspace_bytes(uint32_t batch, uint32_t drafts, uint32_t heads_q, uint32_t heads_kv,
+                                          uint32_t head_dim, uint32_t max_tokens);
+int b200wmma_attn_tree(const b200wmma_attn_args* args, uint32_t drafts, const void* q, const void* k_cache,
+                       const void* v_cache, uint32_t num_pages, uint32_t page_size, const int32_t* block_table,
+                       uint32_t ld_table, const int32_t* lens, const int32_t* n_drafts, const uint64_t* tree,
+                       const int32_t* depths, void* o, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Host-buffer drivers.  These stand in for the reference samples' host functions
  * gemm_test (samples/perf_hgemm.cpp:713-941), dlrm_test (samples/simple_dlrm.cpp:443-710)
  * and sgemv_test (samples/simple_sgemv.cpp:157-273): allocate-or-reuse device buffers,

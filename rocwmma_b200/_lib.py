@@ -12,6 +12,20 @@ LIB_PATH = os.path.join(_PKG, "librocwmma_b200.so")
 
 u32, i32, f32, f64, vp, sz = C.c_uint32, C.c_int32, C.c_float, C.c_double, C.c_void_p, C.c_size_t
 
+
+class AttnStrides(C.Structure):
+    """b200wmma_attn_strides"""
+    _fields_ = [("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class AttnArgs(C.Structure):
+    """b200wmma_attn_args"""
+    _fields_ = ([(n, u32) for n in ("batch", "heads_q", "heads_kv", "len_q", "len_kv", "head_dim")]
+                + [("data_type", i32), ("causal", i32), ("scale", f32), ("cap", f32)]
+                + [(n, vp) for n in ("slopes", "prefix", "doc_q", "doc_kv")]
+                + [(n, AttnStrides) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")])
+
+
 # name -> (restype, argtypes); mirrors include/rocwmma_b200.h one to one
 SIGNATURES = {
     "b200wmma_last_error_string": (C.c_char_p, []),
@@ -64,6 +78,13 @@ SIGNATURES = {
     "b200wmma_dlrm_bwd_f32": (C.c_int, [vp, vp, vp, vp, u32, u32, u32, u32, u32, C.c_int, vp]),
     "b200wmma_gemv_f32": (C.c_int, [u32, u32, vp, u32, C.c_int, vp, vp, f32, f32, vp]),
     "b200wmma_gemv_f64": (C.c_int, [u32, u32, vp, u32, C.c_int, vp, vp, f64, f64, vp]),
+    "b200wmma_gemv_w4": (C.c_int, [u32, u32, u32, vp, u32, vp, u32, vp, u32, u32, vp, u32, vp, u32, f32, f32,
+                                   C.c_int, C.c_int, vp]),
+    "b200wmma_attn_workspace_bytes": (sz, [u32, u32, u32, u32, C.c_int]),
+    "b200wmma_attn_fwd": (C.c_int, [C.POINTER(AttnArgs), vp, vp, vp, vp, vp, vp, sz, vp]),
+    "b200wmma_attn_bwd": (C.c_int, [C.POINTER(AttnArgs), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "b200wmma_attn_tree_workspace_bytes": (sz, [u32, u32, u32, u32, u32, u32]),
+    "b200wmma_attn_tree": (C.c_int, [C.POINTER(AttnArgs), u32, vp, vp, vp, u32, u32, vp, u32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "b200wmma_mg_unique_id": (C.c_int, [vp]),
     "b200wmma_mg_create": (C.c_int, [C.POINTER(vp), vp, C.c_int, C.c_int]),
     "b200wmma_mg_broadcast": (C.c_int, [vp, vp, C.c_size_t, C.c_int, vp]),

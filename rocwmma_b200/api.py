@@ -12,7 +12,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import B200WmmaError, check, lib
+from ._lib import AttnArgs, B200WmmaError, check, lib
 
 ROW_MAJOR, COL_MAJOR = 0, 1
 OUT_F16, OUT_F32 = 0, 1
@@ -269,6 +269,150 @@ def gemv(m, n, a, lda, x, y, alpha, beta, layout_a=ROW_MAJOR):
         raise TypeError("gemv: a must be float32 or float64")
     _need(a, a.dtype, "a"); _need(x, a.dtype, "x"); _need(y, a.dtype, "y")
     check(fn(m, n, _ptr(a), lda, layout_a, _ptr(x), _ptr(y), alpha, beta, _stream()))
+
+
+_DATA_TYPES = {torch.float16: OUT_F16, torch.bfloat16: OUT_BF16}
+
+
+def _need_here(t, dtype, name):
+    """A CUDA tensor of this type on the current device (the library launches there)."""
+    _need(t, dtype, name)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def gemv_w4(m, n, rows, a_packed, lda_bytes, scales, ld_scales, group, x, ldx, y, ldy, alpha, beta, zeros=None, ld_zeros=0):
+    """y = alpha * W x + beta * y for `rows` vectors x, W = scale * (q - zero) from packed 4-bit values with one scale (and
+    zero point) to `group` columns of a row.  x and scales fp16 or bf16, y of that type or fp32.  zeros (uint8) makes the
+    values unsigned; without it they are signed."""
+    dt = x.dtype if isinstance(x, torch.Tensor) else None
+    if dt not in _DATA_TYPES:
+        raise TypeError("x must be a float16 or bfloat16 tensor")
+    _need_here(a_packed, torch.uint8, "a_packed"); _need_here(scales, dt, "scales"); _need_here(x, dt, "x")
+    out = y.dtype if isinstance(y, torch.Tensor) else None
+    if out not in (dt, torch.float32):
+        raise TypeError("y must have the type of x, or float32")
+    _need_here(y, out, "y")
+    if zeros is not None:
+        _need_here(zeros, torch.uint8, "zeros")
+    check(lib().b200wmma_gemv_w4(m, n, rows, _ptr(a_packed), lda_bytes, _ptr(scales), ld_scales, _ptr(zeros), ld_zeros, group,
+                                 _ptr(x), ldx, _ptr(y), ldy, alpha, beta, _DATA_TYPES[dt],
+                                 OUT_F32 if out == torch.float32 else _DATA_TYPES[dt], _stream()))
+
+
+def _attn_args(q, k, v, o, scale, cap, slopes):
+    """AttnArgs of q, o [batch, tokens, heads_q, dim] and k, v [batch or pages, tokens, heads_kv, dim]."""
+    dt = q.dtype if isinstance(q, torch.Tensor) else None
+    if dt not in _DATA_TYPES:
+        raise TypeError("q must be a float16 or bfloat16 tensor")
+    a = AttnArgs()
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o)):
+        _attn_tensor(a, name, t, dt)
+    if k.shape != v.shape or o.shape != q.shape or q.shape[3] != k.shape[3]:
+        raise ValueError("o must have the shape of q, v the shape of k, and both the same head size")
+    a.batch, _, a.heads_q, a.head_dim = q.shape
+    a.heads_kv = k.shape[2]
+    a.data_type, a.scale, a.cap = _DATA_TYPES[dt], scale, cap
+    if slopes is not None:
+        _attn_vector(slopes, torch.float32, (a.heads_q,), "slopes")
+        a.slopes = slopes.data_ptr()
+    return a
+
+
+def _attn_tensor(a, name, t, dt):
+    _need_here(t, dt, name)
+    if t.dim() != 4 or t.stride(3) != 1:
+        raise ValueError(f"{name} must have four dimensions, the last one contiguous")
+    s = getattr(a, name)
+    s.batch, s.token, s.head = t.stride()[:3]
+
+
+def _attn_vector(t, dtype, shape, name):
+    _need_here(t, dtype, name)
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, of shape {tuple(shape)}")
+
+
+def _attn_workspace(workspace):
+    if workspace is None:
+        return None, 0
+    _need_here(workspace, torch.uint8, "workspace")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return _ptr(workspace), workspace.numel()
+
+
+def _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv):
+    if k.shape[0] != q.shape[0]:
+        raise ValueError("q and k must have the same batch")
+    a.len_q, a.len_kv, a.causal = q.shape[1], k.shape[1], int(causal)
+    if prefix is not None:
+        _attn_vector(prefix, torch.int32, (a.batch,), "prefix")
+        a.prefix = prefix.data_ptr()
+    if doc_q is not None:
+        _attn_vector(doc_q, torch.int32, (a.batch, a.len_q), "doc_q")
+        a.doc_q = doc_q.data_ptr()
+    if doc_kv is not None:
+        _attn_vector(doc_kv, torch.int32, (a.batch, a.len_kv), "doc_kv")
+        a.doc_kv = doc_kv.data_ptr()
+    if lse is not None:
+        _attn_vector(lse, torch.float32, (a.batch, a.heads_q, a.len_q), "lse")
+
+
+def attn_workspace_bytes(batch, heads_q, len_q, len_kv, backward):
+    return lib().b200wmma_attn_workspace_bytes(batch, heads_q, len_q, len_kv, int(backward))
+
+
+def attn_fwd(q, k, v, o, lse, scale, causal=False, cap=0.0, slopes=None, prefix=None, doc_q=None, doc_kv=None, workspace=None):
+    """o = softmax(scores) v with scores = cap * tanh(scale * q k^T / cap) - slope * distance under causal, prefix and
+    document masks (b200wmma_attn_fwd has the definition).  q, o: [batch, len_q, heads_q, dim], k, v: [batch, len_kv,
+    heads_kv, dim], any strides of whole rows; lse: [batch, heads_q, len_q] fp32 or None."""
+    a = _attn_args(q, k, v, o, scale, cap, slopes)
+    _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv)
+    ws, size = _attn_workspace(workspace)
+    check(lib().b200wmma_attn_fwd(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), ws, size, _stream()))
+
+
+def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, scale, causal=False, cap=0.0, slopes=None, prefix=None, doc_q=None, doc_kv=None,
+             workspace=None):
+    """Gradients dq, dk, dv of attn_fwd for the gradient dout of its o; o and lse are what attn_fwd wrote."""
+    a = _attn_args(q, k, v, o, scale, cap, slopes)
+    for name, t, like in (("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        _attn_tensor(a, name, t, q.dtype)
+        if t.shape != like.shape:
+            raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
+    if lse is None:
+        raise TypeError("attn_bwd needs the lse of attn_fwd")
+    _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv)
+    ws, size = _attn_workspace(workspace)
+    check(lib().b200wmma_attn_bwd(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk),
+                                  _ptr(dv), ws, size, _stream()))
+
+
+def attn_tree_workspace_bytes(batch, drafts, heads_q, heads_kv, head_dim, max_tokens):
+    return lib().b200wmma_attn_tree_workspace_bytes(batch, drafts, heads_q, heads_kv, head_dim, max_tokens)
+
+
+def attn_tree(q, k_cache, v_cache, block_table, lens, o, scale, tree=None, depths=None, n_drafts=None, cap=0.0, slopes=None,
+              workspace=None):
+    """Attention of drafted tokens over a paged cache (b200wmma_attn_tree).  q, o: [batch, drafts, heads_q, dim]; caches:
+    [pages, page_size, heads_kv, dim]; block_table: [batch, pages of a sequence] int32; lens, n_drafts: [batch] int32;
+    tree: [batch, drafts] int64, bit j of word i set where drafted token i sees drafted token j (None: j <= i); depths:
+    [batch, drafts] int32, for the distances (None: 0, 1, 2, ...)."""
+    a = _attn_args(q, k_cache, v_cache, o, scale, cap, slopes)
+    drafts = q.shape[1]
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("block_table must have two dimensions")
+    _attn_vector(block_table, torch.int32, (a.batch, block_table.shape[1]), "block_table")
+    _attn_vector(lens, torch.int32, (a.batch,), "lens")
+    for t, dtype, shape, name in ((n_drafts, torch.int32, (a.batch,), "n_drafts"), (tree, torch.int64, (a.batch, drafts), "tree"),
+                                  (depths, torch.int32, (a.batch, drafts), "depths")):
+        if t is not None:
+            _attn_vector(t, dtype, shape, name)
+    ws, size = _attn_workspace(workspace)
+    check(lib().b200wmma_attn_tree(C.byref(a), drafts, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], k_cache.shape[1],
+                                   _ptr(block_table), block_table.shape[1], _ptr(lens), _ptr(n_drafts), _ptr(tree), _ptr(depths),
+                                   _ptr(o), ws, size, _stream()))
 
 
 class HostContext:

@@ -1,0 +1,124 @@
+// What the attention kernels share: the checked and flattened arguments, and the arithmetic of one score
+//   s = cap * tanh(scale * q.k / cap) - slope * |distance|,  masked by causality, prefix and documents.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <type_traits>
+
+namespace b200wmma
+{
+    namespace attn
+    {
+        constexpr uint32_t MAX_DIM = 128;
+        constexpr float    LOG2E   = 1.4426950408889634f;
+        constexpr float    LN2     = 0.6931471805599453f;
+
+        struct Strides
+        {
+            int64_t batch, token, head;
+        };
+
+        // Kernel parameters of the forward and backward pass.
+        struct Params
+        {
+            uint32_t batch, heads_q, heads_kv, len_q, len_kv, dim;
+            int32_t  off; // len_kv - len_q: query i stands at key position i + off
+            int32_t  causal;
+            float    scale, cap;
+            const float*   slopes;
+            const int32_t *prefix, *doc_q, *doc_kv;
+            Strides        q, k, v, o, dout, dq, dk, dv;
+        };
+
+        // tanh from one exponential: 1 - 2 / (1 + e^2x) is off by a few ulp of 1, absolutely, which is what a score needs
+        // (the hardware's tanh approximation is off by 2^-11 of its value: a capped score of 20 would move by 0.01).
+        // e^2x = infinity and 0 give 1 and -1, NaN stays NaN.
+        __device__ __forceinline__ float tanh_of(float x)
+        {
+            return 1.0f - __fdividef(2.0f, 1.0f + exp2f(x * (2.0f * LOG2E)));
+        }
+
+        template <typename T>
+        __device__ __forceinline__ float to_f32(T x)
+        {
+            if constexpr(std::is_same<T, __half>::value)
+                return __half2float(x);
+            else
+                return __bfloat162float(x);
+        }
+        template <typename T>
+        __device__ __forceinline__ T from_f32(float x)
+        {
+            if constexpr(std::is_same<T, __half>::value)
+                return __float2half_rn(x);
+            else
+                return __float2bfloat16_rn(x);
+        }
+
+        // ---- host side: argument checks -------------------------------------------------------
+        static int check_strides(const char* who, const char* name, const void* base, const b200wmma_attn_strides& s,
+                                 uint32_t batch, uint32_t tokens, uint32_t heads, Strides* out)
+        {
+            B200_REQUIRE(base, B200WMMA_ERR_INVALID_ARG, "%s: %s must be non-null", who, name);
+            B200_REQUIRE(aligned16(base), B200WMMA_ERR_ALIGNMENT, "%s: %s must be 16-byte aligned", who, name);
+            const int64_t  st[3]  = {s.batch, s.token, s.head};
+            const uint32_t ext[3] = {batch, tokens, heads};
+            static const char* const which[3] = {"batch", "token", "head"};
+            int64_t                  v[3];
+            for(int i = 0; i < 3; ++i)
+            {
+                v[i] = ext[i] > 1 ? st[i] : 8;
+                B200_REQUIRE(v[i] > 0, B200WMMA_ERR_INVALID_ARG, "%s: the %s stride of %s must be positive", who, which[i], name);
+                B200_REQUIRE(v[i] % 8 == 0, B200WMMA_ERR_ALIGNMENT, "%s: the %s stride of %s must be a multiple of 8 elements", who,
+                             which[i], name);
+                B200_REQUIRE(v[i] < (int64_t(1) << 38), B200WMMA_ERR_UNSUPPORTED, "%s: the %s stride of %s is too large", who,
+                             which[i], name);
+            }
+            *out = {v[0], v[1], v[2]};
+            return B200WMMA_OK;
+        }
+        // The elements that a call writes must not share memory among themselves.  Of three extents, sorted by stride, each
+        // stride has to clear what the smaller ones span; rows are `dim` elements.
+        static bool disjoint(const Strides& s, uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t dim)
+        {
+            int64_t  st[3] = {s.batch, s.token, s.head};
+            uint32_t n[3]  = {batch, tokens, heads};
+            for(int i = 0; i < 3; ++i)
+                for(int j = i + 1; j < 3; ++j)
+                    if(st[j] < st[i])
+                    {
+                        const int64_t t = st[i];
+                        st[i] = st[j], st[j] = t;
+                        const uint32_t u = n[i];
+                        n[i] = n[j], n[j] = u;
+                    }
+            int64_t span = dim;
+            for(int i = 0; i < 3; ++i)
+            {
+                if(n[i] <= 1)
+                    continue;
+                if(st[i] < span)
+                    return false;
+                span += st[i] * (int64_t(n[i]) - 1);
+            }
+            return true;
+        }
+
+        static int check_common(const char* who, const b200wmma_attn_args* a)
+        {
+            B200_REQUIRE(a, B200WMMA_ERR_INVALID_ARG, "%s: args must be non-null", who);
+            B200_REQUIRE(a->batch && a->heads_q && a->heads_kv && a->head_dim, B200WMMA_ERR_INVALID_ARG,
+                         "%s: batch, heads_q, heads_kv and head_dim must be non-zero", who);
+            B200_REQUIRE(a->heads_q % a->heads_kv == 0, B200WMMA_ERR_INVALID_ARG, "%s: heads_q must be a multiple of heads_kv", who);
+            B200_REQUIRE(a->head_dim % 8 == 0 && a->head_dim <= MAX_DIM, B200WMMA_ERR_UNSUPPORTED,
+                         "%s: head_dim must be a multiple of 8, at most %u", who, MAX_DIM);
+            B200_REQUIRE(a->data_type == B200WMMA_OUT_F16 || a->data_type == B200WMMA_OUT_BF16, B200WMMA_ERR_INVALID_ARG,
+                         "%s: data_type must be B200WMMA_OUT_F16 or B200WMMA_OUT_BF16", who);
+            B200_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, B200WMMA_ERR_INVALID_ARG, "%s: scale must be finite", who);
+            B200_REQUIRE(a->cap >= 0.0f && a->cap - a->cap == 0.0f, B200WMMA_ERR_INVALID_ARG,
+                         "%s: cap must be finite and not negative (0 = none)", who);
+            return B200WMMA_OK;
+        }
+    } // namespace attn
+} // namespace b200wmma
