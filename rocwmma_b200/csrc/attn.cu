@@ -1,5 +1,5 @@
 // Attention, forward and backward: the entry points b200wmma_attn_fwd / _bwd.
-#include "attn_common.cuh"
+#include "attn_fwd.cuh"
 
 namespace b200wmma
 {
@@ -20,7 +20,7 @@ namespace b200wmma
             return true;
         }
         // score of a dot product, and the derivative of the cap at it
-        __device__ __forceinline__ float score(const Params& p, float dot, uint32_t i, uint32_t j, float slope, float& slip)
+        __device__ __forceinline__ float score_of(const Params& p, float dot, uint32_t i, uint32_t j, float slope, float& slip)
         {
             float s = dot * p.scale;
             slip    = 1.0f;
@@ -61,41 +61,6 @@ namespace b200wmma
             return (buf[0] + buf[1]) + (buf[2] + buf[3]);
         }
 
-        // One block to a query: 128 scores at a time, then each thread adds up one column of o.
-        template <typename T>
-        __global__ void __launch_bounds__(CHUNK) fwd_kernel(const Params p, const T* q, const T* k, const T* v, T* o, float* lse)
-        {
-            __shared__ float w[CHUNK], buf[4];
-            const uint32_t   i = blockIdx.x % p.len_q, h = blockIdx.x / p.len_q % p.heads_q, b = blockIdx.x / p.len_q / p.heads_q;
-            const uint32_t   g = h / (p.heads_q / p.heads_kv), t = threadIdx.x;
-            const T*         qr     = q + b * p.q.batch + i * p.q.token + h * p.q.head;
-            const float      slope  = p.slopes ? p.slopes[h] : 0.0f;
-            const int32_t    prefix = p.prefix ? p.prefix[b] : 0;
-            float            top = -INFINITY, sum = 0.0f, acc = 0.0f;
-            for(uint32_t j0 = 0; j0 < p.len_kv; j0 += CHUNK)
-            {
-                const uint32_t j = j0 + t;
-                float          s = -INFINITY, slip;
-                if(j < p.len_kv && visible(p, b, i, j, prefix))
-                    s = score(p, dot_row(qr, k + b * p.k.batch + j * p.k.token + g * p.k.head, p.dim), i, j, slope, slip);
-                const float m2 = fmaxf(top, block_max(s, buf));
-                if(m2 == -INFINITY)
-                    continue;
-                const float f = exp2f((top - m2) * LOG2E), e = exp2f((s - m2) * LOG2E);
-                w[t]          = e;
-                sum           = sum * f + block_sum(e, buf);
-                acc *= f;
-                for(uint32_t c = 0; c < min(CHUNK, p.len_kv - j0); ++c)
-                    if(t < p.dim && w[c] != 0.0f)
-                        acc += w[c] * to_f32(v[b * p.v.batch + (j0 + c) * p.v.token + g * p.v.head + t]);
-                top = m2;
-            }
-            if(t < p.dim)
-                o[b * p.o.batch + i * p.o.token + h * p.o.head + t] = from_f32<T>(sum > 0.0f ? acc / sum : 0.0f);
-            if(t == 0 && lse)
-                lse[(size_t(b) * p.heads_q + h) * p.len_q + i] = sum > 0.0f ? top + logf(sum) : -INFINITY;
-        }
-
         // delta = rowsum(dout * o), one block to a query
         template <typename T>
         __global__ void __launch_bounds__(CHUNK) delta_kernel(const Params p, const T* o, const T* dout, const float* lse, float* delta)
@@ -132,7 +97,7 @@ namespace b200wmma
                 float          ds = 0.0f, slip;
                 if(j < p.len_kv && visible(p, b, i, j, prefix))
                 {
-                    const float s = score(p, dot_row(qr, k + b * p.k.batch + j * p.k.token + g * p.k.head, p.dim), i, j, slope, slip);
+                    const float s = score_of(p, dot_row(qr, k + b * p.k.batch + j * p.k.token + g * p.k.head, p.dim), i, j, slope, slip);
                     const float e = exp2f((s - lse[row]) * LOG2E);
                     ds = e * (dot_row(dr, v + b * p.v.batch + j * p.v.token + g * p.v.head, p.dim) - delta[row]) * slip;
                 }
@@ -169,7 +134,7 @@ namespace b200wmma
                     if(i < p.len_q && visible(p, b, i, j, prefix))
                     {
                         const size_t row = (size_t(b) * p.heads_q + h) * p.len_q + i;
-                        const float s = score(p, dot_row(q + b * p.q.batch + i * p.q.token + h * p.q.head, kr, p.dim), i, j, slope, slip);
+                        const float s = score_of(p, dot_row(q + b * p.q.batch + i * p.q.token + h * p.q.head, kr, p.dim), i, j, slope, slip);
                         pr = exp2f((s - lse[row]) * LOG2E);
                         ds = pr * (dot_row(dout + b * p.dout.batch + i * p.dout.token + h * p.dout.head, vr, p.dim) - delta[row]) * slip;
                     }
@@ -191,9 +156,29 @@ namespace b200wmma
             }
         }
 
-        static size_t workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t, int backward)
+        // Workspace: documents of the query and key tiles, then (backward) delta.
+        static size_t tiles_of(uint32_t len)
         {
-            return backward ? size_t(batch) * heads_q * len_q * sizeof(float) : 0;
+            return (len + TILE - 1) / TILE;
+        }
+        static size_t workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv, int backward)
+        {
+            const size_t docs = batch * (tiles_of(len_q) + tiles_of(len_kv)) * sizeof(DocTile);
+            return docs + (backward ? size_t(batch) * heads_q * len_q * sizeof(float) : 0);
+        }
+        static int list_documents(const Params& p, void* workspace, const DocTile** q, const DocTile** kv, cudaStream_t stream)
+        {
+            *q = *kv = nullptr;
+            if(!p.doc_q)
+                return B200WMMA_OK;
+            DocTile*       dq = static_cast<DocTile*>(workspace);
+            const uint32_t nq = uint32_t(tiles_of(p.len_q)), nk = uint32_t(tiles_of(p.len_kv));
+            DocTile*       dk = dq + size_t(p.batch) * nq;
+            doc_tiles_kernel<<<ceil_div(p.batch * nq, 4), 128, 0, stream>>>(p.doc_q, p.len_q, nq, p.batch * nq, dq);
+            doc_tiles_kernel<<<ceil_div(p.batch * nk, 4), 128, 0, stream>>>(p.doc_kv, p.len_kv, nk, p.batch * nk, dk);
+            B200_CHECK_CUDA(cudaGetLastError());
+            *q = dq, *kv = dk;
+            return B200WMMA_OK;
         }
 
         // Fills Params from checked arguments.
@@ -235,13 +220,31 @@ namespace b200wmma
             return B200WMMA_OK;
         }
 
-        template <typename T>
-        static int run_fwd(const Params& p, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t stream)
+        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
+        static int launch_fwd(const Params& p, const CUtensorMap (&maps)[3], void* o, float* lse, const DocTile* dq, const DocTile* dk,
+                              unsigned* status, cudaStream_t stream)
         {
-            fwd_kernel<T><<<p.batch * p.heads_q * p.len_q, CHUNK, 0, stream>>>(
-                p, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(o), lse);
+            auto kern = fwd_tc05_kernel<T, HD, CAP, BIAS, PLAIN>;
+            B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<HD>::BYTES));
+            const uint32_t q_blocks = ceil_div(p.len_q, 2 * TILE);
+            kern<<<q_blocks * p.batch * p.heads_q, FWD_THREADS, FwdSmem<HD>::BYTES, stream>>>(maps[0], maps[1], maps[2], p, static_cast<T*>(o), lse,
+                                                                                              dq, dk, q_blocks, status);
             B200_CHECK_CUDA(cudaGetLastError());
             return B200WMMA_OK;
+        }
+        template <typename T, uint32_t HD>
+        static int run_fwd(const Params& p, const CUtensorMap (&maps)[3], void* o, float* lse, const DocTile* dq, const DocTile* dk,
+                           unsigned* status, cudaStream_t stream)
+        {
+            const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
+            if(cap)
+                return bias ? launch_fwd<T, HD, true, true, false>(p, maps, o, lse, dq, dk, status, stream)
+                            : launch_fwd<T, HD, true, false, false>(p, maps, o, lse, dq, dk, status, stream);
+            if(bias)
+                return launch_fwd<T, HD, false, true, false>(p, maps, o, lse, dq, dk, status, stream);
+            // the softmax scales plain scores in the exponential's argument, which takes a positive scale
+            return p.scale > 0.0f ? launch_fwd<T, HD, false, false, true>(p, maps, o, lse, dq, dk, status, stream)
+                                  : launch_fwd<T, HD, false, false, false>(p, maps, o, lse, dq, dk, status, stream);
         }
         template <typename T>
         static int run_bwd(const Params& p, const void* q_, const void* k_, const void* v_, const void* o_, const void* dout_, const float* lse,
@@ -281,8 +284,24 @@ extern "C" int b200wmma_attn_fwd(const b200wmma_attn_args* args, const void* q, 
         return e;
     if(int e = require_sm100())
         return e;
-    return args->data_type == B200WMMA_OUT_F16 ? attn::run_fwd<__half>(p, q, k, v, o, lse, as_stream(stream))
-                                               : attn::run_fwd<__nv_bfloat16>(p, q, k, v, o, lse, as_stream(stream));
+    unsigned* status = nullptr;
+    if(int e = status_word_ptr(&status))
+        return e;
+    CUtensorMap maps[3];
+    if(int e = attn::make_map(&maps[0], args->data_type, q, p.dim, p.len_q, p.heads_q, p.batch, p.q))
+        return e;
+    if(int e = attn::make_map(&maps[1], args->data_type, k, p.dim, p.len_kv, p.heads_kv, p.batch, p.k))
+        return e;
+    if(int e = attn::make_map(&maps[2], args->data_type, v, p.dim, p.len_kv, p.heads_kv, p.batch, p.v))
+        return e;
+    const attn::DocTile *dq = nullptr, *dk = nullptr;
+    if(int e = attn::list_documents(p, workspace, &dq, &dk, as_stream(stream)))
+        return e;
+    if(args->data_type == B200WMMA_OUT_F16)
+        return p.dim <= 64 ? attn::run_fwd<__half, 64>(p, maps, o, lse, dq, dk, status, as_stream(stream))
+                           : attn::run_fwd<__half, 128>(p, maps, o, lse, dq, dk, status, as_stream(stream));
+    return p.dim <= 64 ? attn::run_fwd<__nv_bfloat16, 64>(p, maps, o, lse, dq, dk, status, as_stream(stream))
+                       : attn::run_fwd<__nv_bfloat16, 128>(p, maps, o, lse, dq, dk, status, as_stream(stream));
 }
 
 extern "C" int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, const void* k, const void* v, const void* o,
@@ -314,7 +333,8 @@ extern "C" int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, 
         return e;
     if(int e = require_sm100())
         return e;
-    float* delta = static_cast<float*>(workspace);
+    float* delta = reinterpret_cast<float*>(static_cast<attn::DocTile*>(workspace)
+                                            + p.batch * (attn::tiles_of(p.len_q) + attn::tiles_of(p.len_kv)));
     return args->data_type == B200WMMA_OUT_F16
                ? attn::run_bwd<__half>(p, q, k, v, o, dout, lse, dq, dk, dv, delta, as_stream(stream))
                : attn::run_bwd<__nv_bfloat16>(p, q, k, v, o, dout, lse, dq, dk, dv, delta, as_stream(stream));

@@ -1,0 +1,430 @@
+// Forward attention on tcgen05.
+//
+// A CTA owns 256 queries of one head as two tiles of 128 and walks the key tiles that either of them sees.  Per tile
+//   S = Q K^T (tensor cores, fp32 in tensor memory) -> softmax warps: running maximum and sum, P = 2^(x - m) in 16 bits over S
+//   -> O += P V (tensor cores, P from tensor memory).
+// The two tiles take turns: while the tensor cores work on one, 128 threads (one to a query) do the softmax of the other.
+// The running maximum of a row is only moved when a score passes it by more than 2^8 (RESCALE_STEP): until then P grows up to
+// 256, which both 16-bit types hold, and sums stay fp32, so O is rescaled in a few steps instead of at every one.
+#pragma once
+#include "attn_tc05.cuh"
+
+namespace b200wmma
+{
+    namespace attn
+    {
+        constexpr uint32_t FWD_THREADS  = 320; // warps 0-3: softmax of tile 0, 4-7: of tile 1, 8: TMA, 9: MMA
+        constexpr float    RESCALE_STEP = 8.0f;
+
+        template <uint32_t HD>
+        struct FwdSmem
+        {
+            static constexpr uint32_t TILE_BYTES = HD / 64 * BOX_BYTES;
+            static constexpr uint32_t STAGES     = HD == 128 ? 4 : 8; // key and value tiles in turn
+            static constexpr uint32_t Q          = 0;
+            static constexpr uint32_t KV         = Q + 2 * TILE_BYTES;
+            static constexpr uint32_t LIST       = KV + STAGES * TILE_BYTES; // SEG words
+            static constexpr uint32_t RAW        = LIST + SEG * 4; // SEG bytes of flags before they are listed
+            static constexpr uint32_t DOCS       = RAW + SEG; // 2 x 128 documents of the keys
+            static constexpr uint32_t BARS       = DOCS + 2 * TILE * 4;
+            static constexpr uint32_t Q_FULL = BARS, KV_FULL = Q_FULL + 8, KV_EMPTY = KV_FULL + 8 * STAGES, S_FULL = KV_EMPTY + 8 * STAGES,
+                                      P_FULL = S_FULL + 16, O_DONE = P_FULL + 16;
+            static constexpr uint32_t MISC  = O_DONE + 16; // tensor memory address, abort flag, list length
+            static constexpr uint32_t TOTAL = MISC + 16;
+            static constexpr uint32_t BYTES = TOTAL + 1024;
+        };
+
+        enum FwdRole : uint32_t
+        {
+            FWD_PRODUCER = 0x31,
+            FWD_MMA      = 0x32,
+            FWD_SOFTMAX  = 0x33
+        };
+
+        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
+        __global__ void __launch_bounds__(FWD_THREADS, 1)
+            fwd_tc05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p, T* __restrict__ o,
+                            float* __restrict__ lse, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv,
+                            uint32_t q_blocks, unsigned* status)
+        {
+            using L = FwdSmem<HD>;
+            extern __shared__ uint8_t smem_raw[];
+            const uint32_t            base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+            uint8_t*                  smem = smem_raw + (base - ptx::smem_u32(smem_raw));
+            uint32_t*                 list = reinterpret_cast<uint32_t*>(smem + L::LIST);
+            uint8_t*                  raw  = smem + L::RAW;
+            uint32_t*                 misc = reinterpret_cast<uint32_t*>(smem + L::MISC);
+            volatile uint32_t*        cta_abort = misc + 1;
+
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+            // the last queries first: under a causal mask they take longest
+            const uint32_t bh = blockIdx.x % (p.batch * p.heads_q), q_block = q_blocks - 1 - blockIdx.x / (p.batch * p.heads_q);
+            const uint32_t h = bh % p.heads_q, b = bh / p.heads_q, g = h / (p.heads_q / p.heads_kv);
+            const uint32_t row0 = q_block * 2 * TILE, q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
+            const int32_t  prefix = p.prefix ? p.prefix[b] : 0;
+            const bool     docs   = p.doc_q != nullptr;
+
+            if(threadIdx.x == 0)
+            {
+                ptx::prefetch_tensormap(&map_q);
+                ptx::prefetch_tensormap(&map_k);
+                ptx::prefetch_tensormap(&map_v);
+                ptx::mbar_init(base + L::Q_FULL, 1);
+                for(uint32_t s = 0; s < L::STAGES; ++s)
+                {
+                    ptx::mbar_init(base + L::KV_FULL + 8 * s, 1);
+                    ptx::mbar_init(base + L::KV_EMPTY + 8 * s, 1);
+                }
+                for(uint32_t t = 0; t < 2; ++t)
+                {
+                    ptx::mbar_init(base + L::S_FULL + 8 * t, 1);
+                    ptx::mbar_init(base + L::P_FULL + 8 * t, TILE);
+                    ptx::mbar_init(base + L::O_DONE + 8 * t, 1);
+                }
+                *cta_abort = 0u;
+                ptx::fence_barrier_init();
+                ptx::fence_proxy_async_smem();
+            }
+            if(warp == 9)
+            {
+                ptx::tmem_alloc(base + L::MISC, 512);
+                ptx::tmem_relinquish();
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            ptx::tc_fence_after_sync();
+            const uint32_t tmem = misc[0];
+            const uint32_t s_tmem[2] = {tmem, tmem + TILE}, o_tmem[2] = {tmem + 2 * TILE, tmem + 2 * TILE + HD};
+
+            // roles keep their place in the rings from one segment of the key tiles to the next
+            uint32_t   it = 0; // producer, MMA: key tiles so far (a key and a value stage each)
+            uint32_t   done[2] = {0, 0}; // MMA: S tiles so far of each query tile
+            const uint32_t t   = warp >> 2; // softmax: this thread's query tile
+            const uint32_t row = row0 + t * TILE + (threadIdx.x & 127u), quad = warp & 3u;
+            const int32_t  at  = int32_t(row) + p.off;
+            uint32_t       n_s = 0; // softmax: S tiles so far
+            float          m = -INFINITY, l = 0.0f;
+            bool           ok = true, q_here = false;
+            const ScoreConst sc = score_const(p, h);
+            const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
+            // keys [0, lim) of this row are visible as far as causality and lengths go
+            const int32_t lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
+
+            for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
+            {
+                // ---- list the key tiles of this segment that a query of the CTA sees ----
+                const uint32_t count = min(SEG, kv_tiles - seg);
+                for(uint32_t i = threadIdx.x; i < count; i += FWD_THREADS)
+                {
+                    uint32_t f = 0;
+                    const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + seg + i : nullptr;
+                    for(uint32_t u = 0; u < 2; ++u)
+                    {
+                        const uint32_t r0 = row0 + u * TILE;
+                        if(r0 < p.len_q)
+                            f |= tile_flags(p, r0, (seg + i) * TILE, prefix, docs ? doc_tiles_q + size_t(b) * q_tiles + r0 / TILE : nullptr, dk)
+                                 << (2 * u);
+                    }
+                    if(f && docs && dk->neg)
+                        f |= 16u;
+                    raw[i] = static_cast<uint8_t>(f);
+                }
+                __syncthreads();
+                if(warp == 0)
+                {
+                    uint32_t n = 0;
+                    for(uint32_t i0 = 0; i0 < count; i0 += 32)
+                    {
+                        const uint32_t f    = i0 + lane < count ? raw[i0 + lane] : 0u;
+                        const uint32_t vote = __ballot_sync(0xFFFFFFFFu, f != 0);
+                        if(f)
+                            list[n + __popc(vote & ((1u << lane) - 1u))] = (seg + i0 + lane) | f << 24;
+                        n += __popc(vote);
+                    }
+                    if(lane == 0)
+                        misc[2] = n;
+                }
+                __syncthreads();
+                const uint32_t entries = misc[2];
+
+                if(warp == 8)
+                {
+                    // ------------------------------ TMA producer ------------------------------
+                    if(lane == 0 && ok && entries)
+                    {
+                        if(!q_here)
+                        {
+                            const uint32_t n = row0 + TILE < p.len_q ? 2u : 1u;
+                            ptx::mbar_arrive_expect_tx(base + L::Q_FULL, n * L::TILE_BYTES);
+                            for(uint32_t u = 0; u < n; ++u)
+                                load_tile<HD>(base + L::Q + u * L::TILE_BYTES, &map_q, row0 + u * TILE, h, b, base + L::Q_FULL);
+                            q_here = true;
+                        }
+                        for(uint32_t e = 0; ok && e < entries; ++e, ++it)
+                            for(uint32_t half = 0; ok && half < 2; ++half)
+                            {
+                                const uint32_t n = 2 * it + half, st = n % L::STAGES, ph = (n / L::STAGES) & 1u;
+                                ok = ptx::mbar_wait_bounded(base + L::KV_EMPTY + 8 * st, ph ^ 1u, cta_abort, status,
+                                                            FWD_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS);
+                                if(!ok)
+                                    break;
+                                ptx::mbar_arrive_expect_tx(base + L::KV_FULL + 8 * st, L::TILE_BYTES);
+                                load_tile<HD>(base + L::KV + st * L::TILE_BYTES, half ? &map_v : &map_k, (list[e] & 0xFFFFFFu) * TILE, g, b,
+                                              base + L::KV_FULL + 8 * st);
+                            }
+                    }
+                    __syncwarp();
+                }
+                else if(warp == 9)
+                {
+                    // ------------------------------- MMA issuer -------------------------------
+                    // The whole warp waits (rows of padding are cleared by all lanes); lane 0 issues.
+                    const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
+                        ok = ok
+                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status,
+                                                            FWD_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        ptx::tc_fence_after_sync();
+                        return ok;
+                    };
+                    const auto arrive_kv = [&](uint32_t n, uint32_t e) { // waits for stage n, makes it fit for a product
+                        const uint32_t st = n % L::STAGES;
+                        if(!wait(base + L::KV_FULL + 8 * st, (n / L::STAGES) & 1u, 1))
+                            return false;
+                        if(list[e] >> 28 & 1u)
+                        {
+                            const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
+                            clear_padding<HD>(smem + L::KV + st * L::TILE_BYTES, p.doc_kv + size_t(b) * p.len_kv + c0, min(TILE, p.len_kv - c0),
+                                              lane);
+                        }
+                        return true;
+                    };
+                    const auto scores = [&](uint32_t u, uint32_t e, uint32_t n) { // S of query tile u
+                        if(lane == 0 && (list[e] >> (24 + 2 * u) & TILE_NEED))
+                        {
+                            mma_over_head<T, HD>(s_tmem[u], base + L::Q + u * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::S_FULL + 8 * u);
+                        }
+                    };
+                    const auto free_stage = [&](uint32_t n) {
+                        if(lane == 0)
+                            ptx::tc_commit(base + L::KV_EMPTY + 8 * (n % L::STAGES));
+                    };
+                    if(entries && ok)
+                    {
+                        if(!q_here)
+                            wait(base + L::Q_FULL, 0, 0);
+                        q_here = true;
+                        if(ok && arrive_kv(2 * it, 0))
+                        {
+                            scores(0, 0, 2 * it);
+                            scores(1, 0, 2 * it);
+                            free_stage(2 * it);
+                        }
+                        for(uint32_t e = 0; ok && e < entries; ++e, ++it)
+                        {
+                            if(!arrive_kv(2 * it + 1, e))
+                                break;
+                            const bool more = e + 1 < entries;
+                            if(more && !arrive_kv(2 * it + 2, e + 1))
+                                break;
+                            for(uint32_t u = 0; ok && u < 2; ++u)
+                            {
+                                if(list[e] >> (24 + 2 * u) & TILE_NEED)
+                                {
+                                    if(!wait(base + L::P_FULL + 8 * u, done[u] & 1u, 2 + u))
+                                        break;
+                                    if(lane == 0)
+                                    {
+                                        mma_over_tokens<T, HD>(o_tmem[u], s_tmem[u], base + L::KV + ((2 * it + 1) % L::STAGES) * L::TILE_BYTES,
+                                                               done[u] != 0);
+                                        ptx::tc_commit(base + L::O_DONE + 8 * u);
+                                    }
+                                    ++done[u];
+                                }
+                                if(more)
+                                    scores(u, e + 1, 2 * it + 2);
+                            }
+                            if(!ok)
+                                break;
+                            free_stage(2 * it + 1);
+                            if(more)
+                                free_stage(2 * it + 2);
+                        }
+                    }
+                    __syncwarp();
+                }
+                else
+                {
+                    // --------------------------------- softmax --------------------------------
+                    const uint32_t lane_tmem = (quad * 32u) << 16;
+                    for(uint32_t e = 0; ok && e < entries; ++e)
+                    {
+                        const uint32_t f = list[e] >> (24 + 2 * t);
+                        if(!(f & TILE_NEED))
+                            continue;
+                        const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
+                        ok = ptx::mbar_wait_bounded_warp(base + L::S_FULL + 8 * t, n_s & 1u, cta_abort, status,
+                                                         FWD_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        if(!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        uint32_t v[4][32];
+#pragma unroll
+                        for(int i = 0; i < 4; ++i)
+                            ptx::tmem_ld_32x32b_x32(s_tmem[t] + lane_tmem + 32 * i, v[i]);
+                        ptx::tmem_ld_wait();
+                        if constexpr(!PLAIN)
+                        {
+                            const float from = static_cast<float>(at - int32_t(c0));
+#pragma unroll
+                            for(int i = 0; i < 128; ++i)
+                            {
+                                float unused;
+                                v[i >> 5][i & 31] = __float_as_uint(
+                                    score<CAP, BIAS>(sc, __uint_as_float(v[i >> 5][i & 31]), from - static_cast<float>(i), unused));
+                            }
+                        }
+                        if(f & TILE_MASK)
+                        {
+                            const int32_t rel = lim - int32_t(c0);
+                            if(docs)
+                            {
+                                int32_t* dk = reinterpret_cast<int32_t*>(smem + L::DOCS) + t * TILE;
+                                const uint32_t c = c0 + (threadIdx.x & 127u);
+                                ptx::named_bar_sync(1 + t, TILE); // everyone is done with the last tile's documents
+                                dk[threadIdx.x & 127u] = c < p.len_kv ? p.doc_kv[size_t(b) * p.len_kv + c] : -1;
+                                ptx::named_bar_sync(1 + t, TILE);
+#pragma unroll
+                                for(int i = 0; i < 128; ++i)
+                                    if(i >= rel || dk[i] != doc)
+                                        v[i >> 5][i & 31] = 0xFF800000u; // -infinity
+                            }
+                            else
+#pragma unroll
+                                for(int i = 0; i < 128; ++i)
+                                    if(i >= rel)
+                                        v[i >> 5][i & 31] = 0xFF800000u;
+                        }
+                        float top = __uint_as_float(v[0][0]);
+#pragma unroll
+                        for(int i = 1; i < 128; ++i)
+                            top = fmaxf(top, __uint_as_float(v[i >> 5][i & 31]));
+                        if constexpr(PLAIN)
+                            top *= sc.c; // scale > 0
+                        // move the maximum where some row of this warp has outgrown it
+                        if(__any_sync(0xFFFFFFFFu, top > m + RESCALE_STEP))
+                        {
+                            const float m2 = fmaxf(m, top);
+                            const float by = m2 == -INFINITY ? 1.0f : ex2(m - m2);
+                            l *= by;
+                            m = m2;
+                            if(n_s != 0)
+                            {
+                                ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
+                                                                 FWD_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu),
+                                                                 tc05::WAIT_TIMEOUT_NS, lane);
+                                if(!ok)
+                                    break;
+                                ptx::tc_fence_after_sync();
+#pragma unroll 1
+                                for(uint32_t c = 0; c < HD; c += 32)
+                                {
+                                    uint32_t w[32];
+                                    ptx::tmem_ld_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
+                                    ptx::tmem_ld_wait();
+#pragma unroll
+                                    for(int i = 0; i < 32; ++i)
+                                        w[i] = __float_as_uint(__uint_as_float(w[i]) * by);
+                                    tmem_st_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
+                                }
+                            }
+                        }
+                        const float sub = m == -INFINITY ? 0.0f : -m;
+                        float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for(int i = 0; i < 4; ++i)
+                        {
+                            uint32_t w[16];
+#pragma unroll
+                            for(int j = 0; j < 16; ++j)
+                            {
+                                float x = __uint_as_float(v[i][2 * j]), y = __uint_as_float(v[i][2 * j + 1]);
+                                x = ex2(PLAIN ? fmaf(x, sc.c, sub) : x + sub);
+                                y = ex2(PLAIN ? fmaf(y, sc.c, sub) : y + sub);
+                                sum[j & 3] += x + y;
+                                w[j] = pack2<T>(x, y);
+                            }
+                            tmem_st_32x32b_x16(s_tmem[t] + lane_tmem + 16 * i, w);
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        ptx::mbar_arrive(base + L::P_FULL + 8 * t);
+                        ++n_s;
+                    }
+                }
+                if(seg + SEG < kv_tiles)
+                    __syncthreads(); // the list is written anew
+            }
+
+            // ---- results ----
+            if(warp < 8)
+            {
+                bool have = n_s != 0;
+                if(have && ok)
+                {
+                    ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
+                                                     FWD_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    ptx::tc_fence_after_sync();
+                }
+                if(ok)
+                {
+                    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); // NaN stays NaN
+                    T*          out = o + int64_t(b) * p.o.batch + int64_t(row) * p.o.token + int64_t(h) * p.o.head;
+#pragma unroll 1
+                    for(uint32_t c = 0; c < HD; c += 32)
+                    {
+                        uint32_t w[32];
+                        if(have)
+                        {
+                            ptx::tmem_ld_32x32b_x32(o_tmem[t] + ((quad * 32u) << 16) + c, w);
+                            ptx::tmem_ld_wait();
+                        }
+                        if(row < p.len_q)
+#pragma unroll
+                            for(int i = 0; i < 4; ++i)
+                                if(c + 8 * i < p.dim)
+                                {
+                                    uint32_t u[4];
+#pragma unroll
+                                    for(int j = 0; j < 4; ++j)
+                                        u[j] = (have && l != 0.0f) ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * inv,
+                                                                              __uint_as_float(w[8 * i + 2 * j + 1]) * inv)
+                                                                   : 0u;
+                                    *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(u[0], u[1], u[2], u[3]);
+                                }
+                    }
+                    if(lse && row < p.len_q)
+                        lse[(size_t(b) * p.heads_q + h) * p.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                }
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            if(*cta_abort)
+            {
+                // A wait was abandoned: copies or products of this CTA may still be in flight.  Give them a bounded grace
+                // period before shared and tensor memory are released.
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while(ptx::globaltimer_ns() - t0 < 2000000ull)
+                    __nanosleep(1000);
+                __syncthreads();
+            }
+            if(warp == 9)
+            {
+                ptx::tc_fence_after_sync();
+                ptx::tmem_dealloc(tmem, 512);
+            }
+        }
+    } // namespace attn
+} // namespace b200wmma

@@ -1,0 +1,242 @@
+// Pieces of the tcgen05 attention kernels: the instruction forms the GEMM does not use, masks by tile, the arithmetic of a
+// score in registers, operand tiles and tensor maps.
+//
+// Tiles are 128 queries x 128 keys.  An operand tile is 128 rows of HD = 64 or 128 elements (a smaller head is padded with
+// zeros by TMA), stored as HD / 64 boxes of 128 rows x 128 bytes with the 128-byte swizzle.  The same bytes serve as a
+// K-major operand (the head is the contraction) and as an MN-major one (the tokens are the contraction).
+// A product whose left operand comes out of a softmax takes it from tensor memory: its 16-bit values overwrite the fp32
+// scores that they were computed from, two to a 32-bit column.
+#pragma once
+#include "attn_common.cuh"
+#include "gemm_tc05_common.cuh"
+
+namespace b200wmma
+{
+    namespace attn
+    {
+        constexpr uint32_t TILE      = 128;
+        constexpr uint32_t BOX_BYTES = TILE * 128; // 128 rows x 64 elements of 16 bits
+        constexpr uint32_t SEG       = 512; // key (or query) tiles that are listed at a time
+
+        template <typename T>
+        constexpr int kind_of = std::is_same<T, __half>::value ? tc05::KIND_F16 : tc05::KIND_BF16;
+
+        // ---- instructions ---------------------------------------------------------------------
+        // D[tmem] (+)= A[tmem] * B[smem]
+        __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+        {
+            asm volatile("{\n"
+                         ".reg .pred p;\n"
+                         "setp.ne.b32 p, %4, 0;\n"
+                         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+                         "}" ::"r"(d_tmem),
+                         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                         : "memory");
+        }
+        __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32])
+        {
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+                         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                         "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+                         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+                         "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+                         "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+                         : "memory");
+        }
+        __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16])
+        {
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+                         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+                         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                         : "memory");
+        }
+        __device__ __forceinline__ void tmem_st_wait()
+        {
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        __device__ __forceinline__ void tma_load_4d(uint32_t dst_smem, const void* tmap, int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                                    uint32_t bar)
+        {
+            asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                         " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst_smem),
+                         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                         : "memory");
+        }
+        __device__ __forceinline__ float ex2(float x)
+        {
+            float y;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+            return y;
+        }
+        __device__ __forceinline__ float rcp(float x)
+        {
+            float y;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+            return y;
+        }
+        template <typename T>
+        __device__ __forceinline__ uint32_t pack2(float lo, float hi)
+        {
+            return tc05::Pack16<T>::narrow(lo, hi);
+        }
+
+        // ---- operand tiles --------------------------------------------------------------------
+        template <uint32_t HD>
+        __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t token, uint32_t head, uint32_t batch,
+                                                  uint32_t bar)
+        {
+#pragma unroll
+            for(uint32_t s = 0; s < HD / 64; ++s)
+                tma_load_4d(dst + s * BOX_BYTES, map, s * 64, token, head, batch, bar);
+        }
+        // D (+)= A B^T over the head: both operands K-major tiles
+        template <typename T, uint32_t HD>
+        __device__ __forceinline__ void mma_over_head(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem)
+        {
+            constexpr uint32_t idesc = tc05::make_idesc<kind_of<T>, TILE, TILE>();
+            const uint64_t     a = ptx::make_kmajor_sw128_desc(a_smem), b = ptx::make_kmajor_sw128_desc(b_smem);
+#pragma unroll
+            for(uint32_t k = 0; k < HD / 16; ++k)
+            {
+                const uint32_t at = (k / 4) * (BOX_BYTES >> 4) + (k % 4) * 2;
+                ptx::mma_f16_ss(d_tmem, a + at, b + at, idesc, k != 0);
+            }
+        }
+        // D (+)= A B over 128 tokens: A 16-bit values in tensor memory, B an MN-major tile
+        template <typename T, uint32_t HD>
+        __device__ __forceinline__ void mma_over_tokens(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem, bool accumulate)
+        {
+            constexpr uint32_t idesc = tc05::make_idesc<kind_of<T>, TILE, HD, false, true>();
+            const uint64_t     b     = ptx::make_mnmajor_sw128_desc(b_smem, BOX_BYTES);
+#pragma unroll
+            for(uint32_t k = 0; k < TILE / 16; ++k)
+                mma_f16_ts(d_tmem, a_tmem + 8 * k, b + k * (2048u >> 4), idesc, (accumulate || k != 0) ? 1u : 0u);
+        }
+        // Rows of padding may hold anything: zeroed before a product contracts over them.  One warp; `docs` are the tile's.
+        template <uint32_t HD>
+        __device__ __forceinline__ void clear_padding(uint8_t* tile, const int32_t* docs, uint32_t rows, uint32_t lane)
+        {
+            for(uint32_t r = lane; r < rows; r += 32)
+                if(docs[r] < 0)
+                    for(uint32_t s = 0; s < HD / 64; ++s)
+                        for(uint32_t c = 0; c < 8; ++c)
+                            *reinterpret_cast<uint4*>(tile + s * BOX_BYTES + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+        }
+
+        // ---- masks by tile --------------------------------------------------------------------
+        // Documents of a tile: {smallest, largest, any padding}; smallest > largest where there is nothing but padding.
+        struct DocTile
+        {
+            int32_t lo, hi, neg, unused;
+        };
+        enum : uint32_t
+        {
+            TILE_NEED = 1, // some pair of the tile is visible
+            TILE_MASK = 2, // some pair is not: each one is looked at
+        };
+        // Tile of queries [r0, r0 + 128) x keys [c0, c0 + 128).
+        __device__ __forceinline__ uint32_t tile_flags(const Params& p, uint32_t r0, uint32_t c0, int32_t prefix, const DocTile* dq,
+                                                       const DocTile* dk)
+        {
+            if(r0 >= p.len_q || c0 >= p.len_kv)
+                return 0;
+            const int32_t r1 = min(r0 + TILE, p.len_q) - 1, c1 = min(c0 + TILE, p.len_kv) - 1;
+            bool          mask = c0 + TILE > p.len_kv;
+            if(p.causal)
+            {
+                if(int32_t(c0) > r1 + p.off && int32_t(c0) >= prefix)
+                    return 0;
+                mask |= c1 > int32_t(r0) + p.off && c1 >= prefix;
+            }
+            if(dq)
+            {
+                const DocTile q = *dq, k = *dk;
+                if(q.lo > q.hi || k.lo > k.hi || q.hi < k.lo || k.hi < q.lo)
+                    return 0;
+                mask |= q.neg || k.neg || q.lo != q.hi || k.lo != k.hi || q.lo != k.lo;
+            }
+            return TILE_NEED | (mask ? TILE_MASK : 0u);
+        }
+
+        // One warp to a tile of a batch entry.
+        __global__ void __launch_bounds__(128) doc_tiles_kernel(const int32_t* docs, uint32_t len, uint32_t tiles, uint32_t total, DocTile* out)
+        {
+            const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+            if(at >= total)
+                return;
+            const int32_t* d = docs + size_t(at / tiles) * len;
+            const uint32_t i0 = at % tiles * TILE;
+            int32_t        lo = INT32_MAX, hi = -1, neg = 0;
+            for(uint32_t i = i0 + lane; i < min(i0 + TILE, len); i += 32)
+                if(d[i] < 0)
+                    neg = 1;
+                else
+                    lo = min(lo, d[i]), hi = max(hi, d[i]);
+            lo  = __reduce_min_sync(0xFFFFFFFFu, lo);
+            hi  = __reduce_max_sync(0xFFFFFFFFu, hi);
+            neg = __any_sync(0xFFFFFFFFu, neg);
+            if(lane == 0)
+                out[at] = {lo, hi, neg, 0};
+        }
+
+        // ---- scores ---------------------------------------------------------------------------
+        // Constants of a score in units of log 2: x = log2(e) * (cap * tanh(scale * dot / cap) - slope * distance).
+        struct ScoreConst
+        {
+            float c;     // log2(e) * scale (no cap)
+            float k1;    // 2 log2(e) scale / cap: e^(2 scale dot / cap) = 2^(k1 dot)
+            float cap2;  // log2(e) * cap
+            float slope; // log2(e) * slope of this head
+        };
+        __device__ __forceinline__ ScoreConst score_const(const Params& p, uint32_t head)
+        {
+            ScoreConst s;
+            s.c     = p.scale * LOG2E;
+            s.k1    = p.cap > 0.0f ? 2.0f * LOG2E * (p.scale / p.cap) : 0.0f;
+            s.cap2  = p.cap * LOG2E;
+            s.slope = p.slopes ? p.slopes[head] * LOG2E : 0.0f;
+            return s;
+        }
+        // tanh from one exponential: 1 - 2 / (1 + 2^(k1 dot)) is off by a few ulp of 1, absolutely, which is what a score
+        // needs (the hardware's tanh approximation is off by 2^-11 of its value: a capped score of 20 would move by 0.01).
+        // An infinite or zero power gives 1 and -1, NaN stays NaN.
+        template <bool CAP, bool BIAS>
+        __device__ __forceinline__ float score(const ScoreConst& s, float dot, float dist, float& tanh)
+        {
+            float x;
+            if constexpr(CAP)
+            {
+                tanh = fmaf(-2.0f, rcp(1.0f + ex2(dot * s.k1)), 1.0f);
+                x    = s.cap2 * tanh;
+            }
+            else
+                x = dot * s.c;
+            if constexpr(BIAS)
+                x = fmaf(-s.slope, fabsf(dist), x);
+            return x;
+        }
+
+        // ---- host side ------------------------------------------------------------------------
+        // [batch][tokens][heads][dim] with free strides, in boxes of 64 elements x 128 tokens; zero fill out of bounds.
+        static int make_map(CUtensorMap* out, int data_type, const void* ptr, uint32_t dim, uint32_t tokens, uint32_t heads, uint32_t batch,
+                            const Strides& s)
+        {
+            tc05::EncodeTiledFn fn = tc05::get_encode_fn();
+            B200_REQUIRE(fn != nullptr, B200WMMA_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+            cuuint64_t gdim[4]    = {dim, tokens, heads, batch};
+            cuuint64_t gstride[3] = {cuuint64_t(s.token) * 2, cuuint64_t(s.head) * 2, cuuint64_t(s.batch) * 2};
+            cuuint32_t box[4]     = {64, TILE, 1, 1};
+            cuuint32_t estr[4]    = {1, 1, 1, 1};
+            CUresult   r          = fn(out, data_type == B200WMMA_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                            const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            B200_REQUIRE(r == CUDA_SUCCESS, B200WMMA_ERR_CUDA, "cuTensorMapEncodeTiled (attention operand) failed with CUresult %d",
+                         static_cast<int>(r));
+            return B200WMMA_OK;
+        }
+    } // namespace attn
+} // namespace b200wmma

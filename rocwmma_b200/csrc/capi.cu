@@ -80,9 +80,14 @@ namespace b200wmma
         std::lock_guard<std::mutex> lock(mu);
         if(!cache[dev])
         {
-            void* p = nullptr;
-            B200_CHECK_CUDA(cudaGetSymbolAddress(&p, g_status_word));
-            B200_CHECK_CUDA(cudaMemset(p, 0, sizeof(unsigned) * 4));
+            // The word is zero when its module is loaded.  The first call may come while some stream of this thread is
+            // captured into a graph: looking up an address enqueues nothing, so it is allowed in the relaxed mode.
+            void*                   p    = nullptr;
+            cudaStreamCaptureMode   mode = cudaStreamCaptureModeRelaxed;
+            B200_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            const cudaError_t found = cudaGetSymbolAddress(&p, g_status_word);
+            B200_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            B200_CHECK_CUDA(found);
             cache[dev] = static_cast<unsigned*>(p);
         }
         *out = cache[dev];
