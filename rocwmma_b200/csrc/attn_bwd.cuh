@@ -1,0 +1,751 @@
+// Backward attention on tcgen05: delta = rowsum(dout * o) in one pass over the rows, then two kernels that both recompute
+// P = 2^(x - lse), so that no sum is shared between blocks and no atomics are needed (seven products where one kernel
+// with shared sums would do five).
+//   dkv: a block owns 128 keys of one key head and walks the queries of all its heads, with keys as tensor memory lanes:
+//        S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   dq:  a block owns 128 queries and walks the keys:  S = Q K^T, dP = dO V^T, dQ += dS K
+// with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
+// 256 threads compute, two to a lane (64 columns each); one warp issues the products, one the copies.
+#pragma once
+#include "attn_tc05.cuh"
+
+namespace b200wmma
+{
+    namespace attn
+    {
+        constexpr uint32_t BWD_THREADS = 320; // warps 0-7: columns 0-63 (0-3) and 64-127 (4-7); 8: TMA, 9: MMA
+
+        template <uint32_t HD>
+        struct BwdSmem
+        {
+            static constexpr uint32_t TILE_BYTES = HD / 64 * BOX_BYTES;
+            static constexpr uint32_t OWN  = 0; // the two tiles of the block itself
+            static constexpr uint32_t RING = 2 * TILE_BYTES; // two stages of each of the two tiles that are walked
+            static constexpr uint32_t LIST = RING + 4 * TILE_BYTES;
+            static constexpr uint32_t RAW  = LIST + SEG * 4;
+            static constexpr uint32_t DOCS = RAW + SEG; // 128 documents
+            static constexpr uint32_t STAT = DOCS + TILE * 4; // dkv: two stages of 128 lse and 128 delta
+            static constexpr uint32_t BARS = STAT + 4 * TILE * 4;
+            static constexpr uint32_t OWN_FULL = BARS, FULL = OWN_FULL + 8, EMPTY = FULL + 32, // [2 tiles][2 stages]
+                                      S_FULL = EMPTY + 32, DP_FULL = S_FULL + 8, P_FULL = DP_FULL + 16, DS_FULL = P_FULL + 8,
+                                      DONE = DS_FULL + 16;
+            static constexpr uint32_t MISC  = DONE + 8;
+            static constexpr uint32_t BYTES = MISC + 16 + 1024;
+        };
+        enum BwdRole : uint32_t
+        {
+            DKV_PRODUCER = 0x41,
+            DKV_MMA      = 0x42,
+            DKV_COMPUTE  = 0x43,
+            DQ_PRODUCER  = 0x51,
+            DQ_MMA       = 0x52,
+            DQ_COMPUTE   = 0x53
+        };
+
+        // delta = rowsum(dout * o) and the row statistics in units of log 2, rows padded to whole tiles.  Rows that see nothing
+        // and rows behind the last one get lse = +infinity, so that every P of theirs is 0.  16 lanes to a row.
+        template <typename T>
+        __global__ void __launch_bounds__(256)
+            bwd_rows_kernel(const __grid_constant__ Params p, const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse,
+                            float* __restrict__ lse2, float* __restrict__ delta, uint32_t padded, uint32_t total)
+        {
+            const uint32_t at = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15u;
+            const uint32_t i = at % padded, bh = at / padded, h = bh % p.heads_q, b = bh / p.heads_q;
+            float          sum = 0.0f, s = -INFINITY;
+            if(at < total && i < p.len_q)
+            {
+                s = lse[size_t(bh) * p.len_q + i];
+                if(s != -INFINITY && lane * 8 < p.dim)
+                {
+                    const uint4 x = *reinterpret_cast<const uint4*>(o + int64_t(b) * p.o.batch + int64_t(i) * p.o.token + int64_t(h) * p.o.head + lane * 8);
+                    const uint4 y = *reinterpret_cast<const uint4*>(dout + int64_t(b) * p.dout.batch + int64_t(i) * p.dout.token
+                                                                    + int64_t(h) * p.dout.head + lane * 8);
+                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for(int j = 0; j < 4; ++j)
+                    {
+                        const float2 u = tc05::Pack16<T>::widen(xs[j]), v = tc05::Pack16<T>::widen(ys[j]);
+                        sum = fmaf(u.x, v.x, sum);
+                        sum = fmaf(u.y, v.y, sum);
+                    }
+                }
+            }
+#pragma unroll
+            for(int d = 8; d > 0; d >>= 1)
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            if(at < total && lane == 0)
+            {
+                lse2[at]  = s == -INFINITY ? INFINITY : s * LOG2E;
+                delta[at] = sum;
+            }
+        }
+
+        // Bit j: document j of 64 is `doc`.
+        __device__ __forceinline__ uint64_t same_docs(const int32_t* docs, int32_t doc)
+        {
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for(int j = 0; j < 32; ++j)
+            {
+                lo |= uint32_t(docs[j] == doc) << j;
+                hi |= uint32_t(docs[32 + j] == doc) << j;
+            }
+            return uint64_t(hi) << 32 | lo;
+        }
+        // A row of HD fp32 columns in tensor memory, times `by`, to 16-bit memory.  `live`: the accumulator was written.
+        template <typename T, uint32_t HD>
+        __device__ __forceinline__ void store_row(T* out, uint32_t taddr, float by, bool live, bool mine, uint32_t dim)
+        {
+#pragma unroll 1
+            for(uint32_t c = 0; c < HD; c += 32)
+            {
+                uint32_t w[32];
+                ptx::tmem_ld_32x32b_x32(taddr + c, w);
+                ptx::tmem_ld_wait();
+                if(mine)
+#pragma unroll
+                    for(int i = 0; i < 4; ++i)
+                        if(c + 8 * i < dim)
+                        {
+                            uint32_t u[4];
+#pragma unroll
+                            for(int j = 0; j < 4; ++j)
+                                u[j] = live ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * by, __uint_as_float(w[8 * i + 2 * j + 1]) * by) : 0u;
+                            *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
+            }
+        }
+        // D (+)= A B over 128 tokens; the left operand's halves of 64 tokens start 64 columns apart
+        template <typename T, uint32_t HD>
+        __device__ __forceinline__ void mma_over_tokens_halves(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem, bool accumulate)
+        {
+            constexpr uint32_t idesc = tc05::make_idesc<kind_of<T>, TILE, HD, false, true>();
+            const uint64_t     b     = ptx::make_mnmajor_sw128_desc(b_smem, BOX_BYTES);
+#pragma unroll
+            for(uint32_t k = 0; k < TILE / 16; ++k)
+                mma_f16_ts(d_tmem, a_tmem + (k / 4) * 64 + (k % 4) * 8, b + k * (2048u >> 4), idesc, (accumulate || k != 0) ? 1u : 0u);
+        }
+
+        // ---------------------------------------------------------------------------------------------------------------
+        template <typename T, uint32_t HD, bool CAP, bool BIAS>
+        __global__ void __launch_bounds__(BWD_THREADS, 1)
+            bwd_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                           const __grid_constant__ Params p, const float* __restrict__ lse2, const float* __restrict__ delta, T* __restrict__ dk,
+                           T* __restrict__ dv, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+        {
+            using L = BwdSmem<HD>;
+            extern __shared__ uint8_t smem_raw[];
+            const uint32_t            base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+            uint8_t*                  smem = smem_raw + (base - ptx::smem_u32(smem_raw));
+            uint32_t*                 list = reinterpret_cast<uint32_t*>(smem + L::LIST);
+            uint32_t*                 misc = reinterpret_cast<uint32_t*>(smem + L::MISC);
+            volatile uint32_t*        cta_abort = misc + 1;
+
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+            const uint32_t bg = blockIdx.x % (p.batch * p.heads_kv), kv_tile = blockIdx.x / (p.batch * p.heads_kv);
+            const uint32_t g = bg % p.heads_kv, b = bg / p.heads_kv, share = p.heads_q / p.heads_kv;
+            const uint32_t c0 = kv_tile * TILE, q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
+            const int32_t  prefix = p.prefix ? p.prefix[b] : 0;
+            const bool     docs   = p.doc_q != nullptr;
+
+            if(threadIdx.x == 0)
+            {
+                ptx::prefetch_tensormap(&map_q);
+                ptx::prefetch_tensormap(&map_k);
+                ptx::prefetch_tensormap(&map_v);
+                ptx::prefetch_tensormap(&map_do);
+                ptx::mbar_init(base + L::OWN_FULL, 1);
+                for(uint32_t s = 0; s < 4; ++s)
+                {
+                    ptx::mbar_init(base + L::FULL + 8 * s, 1);
+                    ptx::mbar_init(base + L::EMPTY + 8 * s, 1);
+                }
+                ptx::mbar_init(base + L::S_FULL, 1);
+                ptx::mbar_init(base + L::DP_FULL, 1);
+                ptx::mbar_init(base + L::P_FULL, 256);
+                ptx::mbar_init(base + L::DS_FULL, 256);
+                ptx::mbar_init(base + L::DONE, 1);
+                *cta_abort = 0u;
+                ptx::fence_barrier_init();
+                ptx::fence_proxy_async_smem();
+            }
+            if(warp == 9)
+            {
+                ptx::tmem_alloc(base + L::MISC, 512);
+                ptx::tmem_relinquish();
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            ptx::tc_fence_after_sync();
+            const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dv_tmem = tmem + 2 * TILE, dk_tmem = dv_tmem + HD;
+
+            const uint32_t   n_stat = q_tiles * TILE; // padded rows of a head
+            uint32_t         it = 0; // pairs (head, query tile) so far, in every role
+            bool             ok = true;
+            const uint32_t   half = warp >> 2, quad = warp & 3u; // compute: columns [64 half, 64 half + 64) of lane 32 quad + lane
+            const uint32_t   col = c0 + quad * 32u + lane; // its key
+            const uint32_t   lane_tmem = ((quad * 32u) << 16) + half * 64u;
+            const int32_t    doc = (docs && col < p.len_kv) ? p.doc_kv[size_t(b) * p.len_kv + col] : 0;
+
+            for(uint32_t seg = 0; seg < q_tiles; seg += SEG)
+            {
+                const uint32_t entries
+                    = list_tiles<BWD_THREADS>(seg, min(SEG, q_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
+                          const DocTile* dq = docs ? doc_tiles_q + size_t(b) * q_tiles + tile : nullptr;
+                          const uint32_t f  = tile_flags(p, tile * TILE, c0, prefix, dq, docs ? doc_tiles_kv + size_t(b) * kv_tiles + kv_tile : nullptr);
+                          return f && docs && dq->neg ? f | TILE_DIRTY : f;
+                      });
+                const uint32_t steps = entries * share; // all tiles of one head, then those of the next
+                if(warp == 8)
+                {
+                    // ------------------------------ TMA producer ------------------------------
+                    if(lane == 0 && ok && steps)
+                    {
+                        if(it == 0)
+                        {
+                            ptx::mbar_arrive_expect_tx(base + L::OWN_FULL, 2 * L::TILE_BYTES);
+                            load_tile<HD>(base + L::OWN, &map_k, c0, g, b, base + L::OWN_FULL);
+                            load_tile<HD>(base + L::OWN + L::TILE_BYTES, &map_v, c0, g, b, base + L::OWN_FULL);
+                        }
+                        for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                        {
+                            const uint32_t h = g * share + n / entries, r0 = (list[n % entries] & 0xFFFFFFu) * TILE;
+                            const uint32_t st = it & 1u, ph = (it >> 1) & 1u;
+                            const size_t   stat = (size_t(b) * p.heads_q + h) * n_stat + r0;
+                            for(uint32_t what = 0; ok && what < 2; ++what) // q with the row statistics (read until dS), dout
+                            {
+                                const uint32_t full = base + L::FULL + 16 * what + 8 * st;
+                                ok = ptx::mbar_wait_bounded(base + L::EMPTY + 16 * what + 8 * st, ph ^ 1u, cta_abort, status,
+                                                            DKV_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS);
+                                if(!ok)
+                                    break;
+                                ptx::mbar_arrive_expect_tx(full, L::TILE_BYTES + (what ? 0u : 2 * TILE * 4));
+                                load_tile<HD>(base + L::RING + (2 * what + st) * L::TILE_BYTES, what ? &map_do : &map_q, r0, h, b, full);
+                                if(what == 0)
+                                {
+                                    ptx::bulk_load_1d(base + L::STAT + st * TILE * 4, lse2 + stat, TILE * 4, full);
+                                    ptx::bulk_load_1d(base + L::STAT + (2 + st) * TILE * 4, delta + stat, TILE * 4, full);
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                else if(warp == 9)
+                {
+                    // ------------------------------- MMA issuer -------------------------------
+                    const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
+                        ok = ok
+                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status,
+                                                            DKV_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        ptx::tc_fence_after_sync();
+                        return ok;
+                    };
+                    // waits for tile `what` (0 q, 1 dout) of step n and clears its rows of padding
+                    const auto arrive = [&](uint32_t what, uint32_t at, uint32_t n) {
+                        if(!wait(base + L::FULL + 16 * what + 8 * (at & 1u), (at >> 1) & 1u, what))
+                            return false;
+                        const uint32_t e = list[n % entries];
+                        if(e >> 24 & TILE_DIRTY)
+                        {
+                            const uint32_t r0 = (e & 0xFFFFFFu) * TILE;
+                            clear_padding<HD>(smem + L::RING + (2 * what + (at & 1u)) * L::TILE_BYTES, p.doc_q + size_t(b) * p.len_q + r0,
+                                              min(TILE, p.len_q - r0), lane);
+                        }
+                        return true;
+                    };
+                    const auto scores = [&](uint32_t at) {
+                        if(lane == 0)
+                        {
+                            mma_over_head<T, HD>(s_tmem, base + L::OWN, base + L::RING + (at & 1u) * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::S_FULL);
+                        }
+                    };
+                    const auto grads = [&](uint32_t at) {
+                        if(lane == 0)
+                        {
+                            mma_over_head<T, HD>(dp_tmem, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + (at & 1u)) * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::DP_FULL);
+                        }
+                    };
+                    if(steps && ok)
+                    {
+                        if(it == 0)
+                            wait(base + L::OWN_FULL, 0, 2);
+                        if(ok && arrive(0, it, 0))
+                            scores(it);
+                        if(ok && arrive(1, it, 0))
+                            grads(it);
+                        for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                        {
+                            const bool more = n + 1 < steps;
+                            if(!wait(base + L::P_FULL, it & 1u, 3))
+                                break;
+                            if(lane == 0)
+                            {
+                                mma_over_tokens_halves<T, HD>(dv_tmem, s_tmem, base + L::RING + (2 + (it & 1u)) * L::TILE_BYTES, it != 0);
+                                ptx::tc_commit(base + L::EMPTY + 16 + 8 * (it & 1u));
+                            }
+                            if(more)
+                            {
+                                if(!arrive(0, it + 1, n + 1))
+                                    break;
+                                scores(it + 1);
+                            }
+                            if(!wait(base + L::DS_FULL, it & 1u, 4))
+                                break;
+                            if(lane == 0)
+                            {
+                                mma_over_tokens_halves<T, HD>(dk_tmem, dp_tmem, base + L::RING + (it & 1u) * L::TILE_BYTES, it != 0);
+                                ptx::tc_commit(base + L::EMPTY + 8 * (it & 1u));
+                            }
+                            if(more)
+                            {
+                                if(!arrive(1, it + 1, n + 1))
+                                    break;
+                                grads(it + 1);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                else
+                {
+                    // --------------------------------- compute --------------------------------
+                    for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                    {
+                        const uint32_t e = list[n % entries], r0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
+                        const auto     wait = [&](uint32_t bar, uint32_t what) {
+                            ok = ptx::mbar_wait_bounded_warp(bar, it & 1u, cta_abort, status,
+                                                                 DKV_COMPUTE << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                            ptx::tc_fence_after_sync();
+                            return ok;
+                        };
+                        const ScoreConst sc = score_const(p, g * share + n / entries);
+                        // the statistics came with the tiles: an acquire of the same barriers
+                        ok = ptx::mbar_wait_bounded_warp(base + L::FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
+                                                         DKV_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        if(!ok || !wait(base + L::S_FULL, 0))
+                            break;
+                        uint32_t v[2][32];
+                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem, v[0]);
+                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
+                        ptx::tmem_ld_wait();
+                        // v becomes P, and then P (1 - tanh^2)
+                        const float4* ls   = reinterpret_cast<const float4*>(smem + L::STAT + st * TILE * 4) + half * 16;
+                        const float   from = static_cast<float>(int32_t(r0 + half * 64) + p.off - int32_t(col));
+                        uint64_t seen = ~uint64_t(0); // bit j: this key is visible to query j of the 64
+                        if(e >> 24 & TILE_MASK)
+                        {
+                            const int32_t first = col >= p.len_kv                           ? 64
+                                                  : (p.causal && int32_t(col) >= prefix) ? int32_t(col) - p.off - int32_t(r0 + half * 64)
+                                                                                         : 0;
+                            seen = first >= 64 ? 0 : first > 0 ? seen << first : seen;
+                            if(docs)
+                            {
+                                int32_t*       dq = reinterpret_cast<int32_t*>(smem + L::DOCS) + half * 64;
+                                const uint32_t i  = threadIdx.x & 127u, r = r0 + half * 64 + i;
+                                ptx::named_bar_sync(1 + half, TILE); // everyone is done with the last tile's documents
+                                if(i < 64)
+                                    dq[i] = r < p.len_q ? p.doc_q[size_t(b) * p.len_q + r] : -1;
+                                ptx::named_bar_sync(1 + half, TILE);
+                                seen = doc < 0 ? 0 : seen & same_docs(dq, doc);
+                            }
+                        }
+                        const auto weights = [&](auto masked) {
+#pragma unroll
+                            for(int i = 0; i < 2; ++i)
+                            {
+                                uint32_t w[16];
+#pragma unroll
+                                for(int j4 = 0; j4 < 8; ++j4)
+                                {
+                                    const float4 s4    = ls[i * 8 + j4];
+                                    const float  sv[4] = {s4.x, s4.y, s4.z, s4.w};
+                                    float        pr[4];
+#pragma unroll
+                                    for(int k = 0; k < 4; ++k)
+                                    {
+                                        const int j    = i * 32 + j4 * 4 + k;
+                                        float     slip = 1.0f, x;
+                                        if constexpr(CAP || BIAS)
+                                            x = score<CAP, BIAS>(sc, __uint_as_float(v[i][j4 * 4 + k]), from + static_cast<float>(j), slip) - sv[k];
+                                        else
+                                            x = fmaf(__uint_as_float(v[i][j4 * 4 + k]), sc.c, -sv[k]);
+                                        if constexpr(decltype(masked)::value)
+                                            if(!(seen >> j & 1u))
+                                                x = -INFINITY, slip = 0.0f; // the product may be NaN
+                                        pr[k]            = ex2(x);
+                                        v[i][j4 * 4 + k] = __float_as_uint(CAP ? pr[k] * slip : pr[k]);
+                                    }
+                                    w[2 * j4] = pack2<T>(pr[0], pr[1]), w[2 * j4 + 1] = pack2<T>(pr[2], pr[3]);
+                                }
+                                tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
+                            }
+                        };
+                        if(e >> 24 & TILE_MASK)
+                            weights(std::true_type{});
+                        else
+                            weights(std::false_type{});
+                        tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        ptx::mbar_arrive(base + L::P_FULL);
+
+                        if(!wait(base + L::DP_FULL, 1))
+                            break;
+                        const float4* de = reinterpret_cast<const float4*>(smem + L::STAT + (2 + st) * TILE * 4) + half * 16;
+                        uint32_t ds[32];
+#pragma unroll
+                        for(int i = 0; i < 2; ++i)
+                        {
+                            uint32_t u[32];
+                            ptx::tmem_ld_32x32b_x32(dp_tmem + lane_tmem + 32 * i, u);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for(int j4 = 0; j4 < 8; ++j4)
+                            {
+                                const float4 d4    = de[i * 8 + j4];
+                                const float  dl[4] = {d4.x, d4.y, d4.z, d4.w};
+                                float        x[4];
+#pragma unroll
+                                for(int k = 0; k < 4; ++k)
+                                {
+                                    const float pr = __uint_as_float(v[i][j4 * 4 + k]);
+                                    x[k]           = pr * (__uint_as_float(u[j4 * 4 + k]) - dl[k]);
+                                    if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
+                                        x[k] = pr == 0.0f ? 0.0f : x[k];
+                                }
+                                ds[i * 16 + 2 * j4] = pack2<T>(x[0], x[1]), ds[i * 16 + 2 * j4 + 1] = pack2<T>(x[2], x[3]);
+                            }
+                        }
+                        tmem_st_32x32b_x32(dp_tmem + lane_tmem, ds);
+                        tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        ptx::mbar_arrive(base + L::DS_FULL);
+                    }
+                }
+                if(seg + SEG < q_tiles)
+                    __syncthreads();
+            }
+
+            // ---- results: dv by the first four warps, dk by the next four ----
+            if(warp == 9 && lane == 0 && ok)
+                ptx::tc_commit(base + L::DONE);
+            if(warp < 8)
+            {
+                if(ok)
+                    ok = ptx::mbar_wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DKV_COMPUTE << 24 | 4u << 20 | (blockIdx.x & 0xFFFFFu),
+                                                     tc05::WAIT_TIMEOUT_NS, lane);
+                if(ok)
+                {
+                    ptx::tc_fence_after_sync();
+                    const Strides& s   = half ? p.dk : p.dv;
+                    T*             out = (half ? dk : dv) + int64_t(b) * s.batch + int64_t(col) * s.token + int64_t(g) * s.head;
+                    store_row<T, HD>(out, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), half ? p.scale : 1.0f, it != 0, col < p.len_kv, p.dim);
+                }
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            if(*cta_abort)
+            {
+                // A wait was abandoned: give copies and products in flight a bounded grace period before memory is released.
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while(ptx::globaltimer_ns() - t0 < 2000000ull)
+                    __nanosleep(1000);
+                __syncthreads();
+            }
+            if(warp == 9)
+            {
+                ptx::tc_fence_after_sync();
+                ptx::tmem_dealloc(tmem, 512);
+            }
+        }
+
+        // ---------------------------------------------------------------------------------------------------------------
+        // S has one place in tensor memory, dP (later dS) two, so that the products of the next step run under the arithmetic
+        // of this one.
+        template <typename T, uint32_t HD, bool CAP, bool BIAS>
+        __global__ void __launch_bounds__(BWD_THREADS, 1)
+            bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ Params p,
+                          const float* __restrict__ lse2, const float* __restrict__ delta, T* __restrict__ dq,
+                          const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+        {
+            using L = BwdSmem<HD>;
+            extern __shared__ uint8_t smem_raw[];
+            const uint32_t            base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+            uint8_t*                  smem = smem_raw + (base - ptx::smem_u32(smem_raw));
+            uint32_t*                 list = reinterpret_cast<uint32_t*>(smem + L::LIST);
+            uint32_t*                 misc = reinterpret_cast<uint32_t*>(smem + L::MISC);
+            volatile uint32_t*        cta_abort = misc + 1;
+
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+            const uint32_t q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
+            const uint32_t bh = blockIdx.x % (p.batch * p.heads_q), q_tile = q_tiles - 1 - blockIdx.x / (p.batch * p.heads_q);
+            const uint32_t h = bh % p.heads_q, b = bh / p.heads_q, g = h / (p.heads_q / p.heads_kv);
+            const uint32_t row0   = q_tile * TILE;
+            const int32_t  prefix = p.prefix ? p.prefix[b] : 0;
+            const bool     docs   = p.doc_q != nullptr;
+
+            if(threadIdx.x == 0)
+            {
+                ptx::prefetch_tensormap(&map_q);
+                ptx::prefetch_tensormap(&map_k);
+                ptx::prefetch_tensormap(&map_v);
+                ptx::prefetch_tensormap(&map_do);
+                ptx::mbar_init(base + L::OWN_FULL, 1);
+                for(uint32_t s = 0; s < 4; ++s)
+                {
+                    ptx::mbar_init(base + L::FULL + 8 * s, 1);
+                    ptx::mbar_init(base + L::EMPTY + 8 * s, 1);
+                }
+                ptx::mbar_init(base + L::S_FULL, 1);
+                ptx::mbar_init(base + L::P_FULL, 256); // S has been read
+                for(uint32_t s = 0; s < 2; ++s)
+                {
+                    ptx::mbar_init(base + L::DP_FULL + 8 * s, 1);
+                    ptx::mbar_init(base + L::DS_FULL + 8 * s, 256);
+                }
+                ptx::mbar_init(base + L::DONE, 1);
+                *cta_abort = 0u;
+                ptx::fence_barrier_init();
+                ptx::fence_proxy_async_smem();
+            }
+            if(warp == 9)
+            {
+                ptx::tmem_alloc(base + L::MISC, 512);
+                ptx::tmem_relinquish();
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            ptx::tc_fence_after_sync();
+            const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dq_tmem = tmem + 3 * TILE;
+
+            uint32_t         it = 0;
+            bool             ok = true;
+            const uint32_t   half = warp >> 2, quad = warp & 3u;
+            const uint32_t   row = row0 + quad * 32u + lane, lane_tmem = ((quad * 32u) << 16) + half * 64u;
+            const int32_t    at  = int32_t(row) + p.off;
+            const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
+            const int32_t    lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
+            const ScoreConst sc  = score_const(p, h);
+            float            ls = 0.0f, de = 0.0f;
+            if(warp < 8)
+            {
+                const size_t stat = (size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row;
+                ls = lse2[stat], de = delta[stat];
+            }
+
+            for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
+            {
+                const uint32_t entries
+                    = list_tiles<BWD_THREADS>(seg, min(SEG, kv_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
+                          const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + tile : nullptr;
+                          const uint32_t f  = tile_flags(p, row0, tile * TILE, prefix, docs ? doc_tiles_q + size_t(b) * q_tiles + q_tile : nullptr, dk);
+                          return f && docs && dk->neg ? f | TILE_DIRTY : f;
+                      });
+                if(warp == 8)
+                {
+                    if(lane == 0 && ok && entries)
+                    {
+                        if(it == 0)
+                        {
+                            ptx::mbar_arrive_expect_tx(base + L::OWN_FULL, 2 * L::TILE_BYTES);
+                            load_tile<HD>(base + L::OWN, &map_q, row0, h, b, base + L::OWN_FULL);
+                            load_tile<HD>(base + L::OWN + L::TILE_BYTES, &map_do, row0, h, b, base + L::OWN_FULL);
+                        }
+                        for(uint32_t n = 0; ok && n < entries; ++n, ++it)
+                            for(uint32_t what = 0; ok && what < 2; ++what) // k, v
+                            {
+                                const uint32_t st = it & 1u, full = base + L::FULL + 16 * what + 8 * st;
+                                ok = ptx::mbar_wait_bounded(base + L::EMPTY + 16 * what + 8 * st, ((it >> 1) & 1u) ^ 1u, cta_abort, status,
+                                                            DQ_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS);
+                                if(!ok)
+                                    break;
+                                ptx::mbar_arrive_expect_tx(full, L::TILE_BYTES);
+                                load_tile<HD>(base + L::RING + (2 * what + st) * L::TILE_BYTES, what ? &map_v : &map_k, (list[n] & 0xFFFFFFu) * TILE, g,
+                                              b, full);
+                            }
+                    }
+                    __syncwarp();
+                }
+                else if(warp == 9)
+                {
+                    const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
+                        ok = ok
+                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status, DQ_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu),
+                                                            tc05::WAIT_TIMEOUT_NS, lane);
+                        ptx::tc_fence_after_sync();
+                        return ok;
+                    };
+                    // S and dP of step n (number `a` over all segments)
+                    const auto products = [&](uint32_t a, uint32_t n) {
+                        const uint32_t st = a & 1u;
+                        if(!wait(base + L::FULL + 8 * st, (a >> 1) & 1u, 0))
+                            return;
+                        if(list[n] >> 24 & TILE_DIRTY) // the keys are contracted over; the values' rows only reach their own columns
+                        {
+                            const uint32_t c0 = (list[n] & 0xFFFFFFu) * TILE;
+                            clear_padding<HD>(smem + L::RING + st * L::TILE_BYTES, p.doc_kv + size_t(b) * p.len_kv + c0, min(TILE, p.len_kv - c0), lane);
+                        }
+                        if(a != 0 && !wait(base + L::P_FULL, (a - 1) & 1u, 1)) // the last S has been read
+                            return;
+                        if(lane == 0)
+                        {
+                            mma_over_head<T, HD>(s_tmem, base + L::OWN, base + L::RING + st * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::S_FULL);
+                        }
+                        if(!wait(base + L::FULL + 16 + 8 * st, (a >> 1) & 1u, 2))
+                            return;
+                        if(lane == 0)
+                        {
+                            mma_over_head<T, HD>(dp_tmem + st * TILE, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + st) * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::DP_FULL + 8 * st);
+                            ptx::tc_commit(base + L::EMPTY + 16 + 8 * st);
+                        }
+                    };
+                    if(entries && ok)
+                    {
+                        if(it == 0)
+                            wait(base + L::OWN_FULL, 0, 3);
+                        if(ok)
+                            products(it, 0);
+                        for(uint32_t n = 0; ok && n < entries; ++n, ++it)
+                        {
+                            if(n + 1 < entries)
+                                products(it + 1, n + 1);
+                            const uint32_t st = it & 1u;
+                            if(!ok || !wait(base + L::DS_FULL + 8 * st, (it >> 1) & 1u, 4))
+                                break;
+                            if(lane == 0)
+                            {
+                                mma_over_tokens_halves<T, HD>(dq_tmem, dp_tmem + st * TILE, base + L::RING + st * L::TILE_BYTES, it != 0);
+                                ptx::tc_commit(base + L::EMPTY + 8 * st);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                else
+                {
+                    for(uint32_t n = 0; ok && n < entries; ++n, ++it)
+                    {
+                        const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
+                        ok = ptx::mbar_wait_bounded_warp(base + L::S_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu),
+                                                         tc05::WAIT_TIMEOUT_NS, lane);
+                        if(!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        uint32_t v[2][32];
+                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem, v[0]);
+                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
+                        ptx::tmem_ld_wait();
+                        ptx::tc_fence_before_sync();
+                        ptx::mbar_arrive(base + L::P_FULL);
+                        uint64_t seen = ~uint64_t(0); // bit j: key j of the 64 is visible to this query
+                        if(e >> 24 & TILE_MASK)
+                        {
+                            const int32_t rel = lim - int32_t(c0 + half * 64);
+                            seen              = rel <= 0 ? 0 : rel < 64 ? seen >> (64 - rel) : seen;
+                            if(docs)
+                            {
+                                int32_t*       dk = reinterpret_cast<int32_t*>(smem + L::DOCS) + half * 64;
+                                const uint32_t i  = threadIdx.x & 127u, c = c0 + half * 64 + i;
+                                ptx::named_bar_sync(1 + half, TILE); // everyone is done with the last tile's documents
+                                if(i < 64)
+                                    dk[i] = c < p.len_kv ? p.doc_kv[size_t(b) * p.len_kv + c] : -1;
+                                ptx::named_bar_sync(1 + half, TILE);
+                                seen &= same_docs(dk, doc);
+                            }
+                        }
+                        const float from    = static_cast<float>(at - int32_t(c0 + half * 64));
+                        const auto  weights = [&](auto masked) {
+#pragma unroll
+                            for(int j = 0; j < 64; ++j)
+                            {
+                                float slip = 1.0f, x;
+                                if constexpr(CAP || BIAS)
+                                    x = score<CAP, BIAS>(sc, __uint_as_float(v[j >> 5][j & 31]), from - static_cast<float>(j), slip) - ls;
+                                else
+                                    x = fmaf(__uint_as_float(v[j >> 5][j & 31]), sc.c, -ls);
+                                if constexpr(decltype(masked)::value)
+                                    if(!(seen >> j & 1u))
+                                        x = -INFINITY, slip = 0.0f; // the product may be NaN
+                                x                 = ex2(x);
+                                v[j >> 5][j & 31] = __float_as_uint(CAP ? x * slip : x);
+                            }
+                        };
+                        if(e >> 24 & TILE_MASK)
+                            weights(std::true_type{});
+                        else
+                            weights(std::false_type{});
+                        ok = ptx::mbar_wait_bounded_warp(base + L::DP_FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
+                                                         DQ_COMPUTE << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        if(!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        uint32_t ds[32];
+#pragma unroll
+                        for(int i = 0; i < 2; ++i)
+                        {
+                            uint32_t u[32];
+                            ptx::tmem_ld_32x32b_x32(dp_tmem + st * TILE + lane_tmem + 32 * i, u);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for(int j = 0; j < 16; ++j)
+                            {
+                                float x[2];
+#pragma unroll
+                                for(int k = 0; k < 2; ++k)
+                                {
+                                    const float pr = __uint_as_float(v[i][2 * j + k]);
+                                    x[k]           = pr * (__uint_as_float(u[2 * j + k]) - de);
+                                    if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
+                                        x[k] = pr == 0.0f ? 0.0f : x[k];
+                                }
+                                ds[i * 16 + j] = pack2<T>(x[0], x[1]);
+                            }
+                        }
+                        tmem_st_32x32b_x32(dp_tmem + st * TILE + lane_tmem, ds);
+                        tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        ptx::mbar_arrive(base + L::DS_FULL + 8 * st);
+                    }
+                }
+                if(seg + SEG < kv_tiles)
+                    __syncthreads();
+            }
+
+            if(warp == 9 && lane == 0 && ok)
+                ptx::tc_commit(base + L::DONE);
+            if(warp < 4)
+            {
+                if(ok)
+                    ok = ptx::mbar_wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu),
+                                                     tc05::WAIT_TIMEOUT_NS, lane);
+                if(ok)
+                {
+                    ptx::tc_fence_after_sync();
+                    T* out = dq + int64_t(b) * p.dq.batch + int64_t(row) * p.dq.token + int64_t(h) * p.dq.head;
+                    store_row<T, HD>(out, dq_tmem + ((quad * 32u) << 16), p.scale, it != 0, row < p.len_q, p.dim);
+                }
+            }
+            ptx::tc_fence_before_sync();
+            __syncthreads();
+            if(*cta_abort)
+            {
+                // A wait was abandoned: give copies and products in flight a bounded grace period before memory is released.
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while(ptx::globaltimer_ns() - t0 < 2000000ull)
+                    __nanosleep(1000);
+                __syncthreads();
+            }
+            if(warp == 9)
+            {
+                ptx::tc_fence_after_sync();
+                ptx::tmem_dealloc(tmem, 512);
+            }
+        }
+    } // namespace attn
+} // namespace b200wmma

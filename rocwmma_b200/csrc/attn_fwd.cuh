@@ -113,40 +113,19 @@ namespace b200wmma
 
             for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
             {
-                // ---- list the key tiles of this segment that a query of the CTA sees ----
-                const uint32_t count = min(SEG, kv_tiles - seg);
-                for(uint32_t i = threadIdx.x; i < count; i += FWD_THREADS)
-                {
-                    uint32_t f = 0;
-                    const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + seg + i : nullptr;
+                // the key tiles of this segment that a query of the CTA sees, with the flags of both query tiles
+                const uint32_t entries = list_tiles<FWD_THREADS>(seg, min(SEG, kv_tiles - seg), list, raw, misc + 2, [&](uint32_t tile) {
+                    uint32_t       f  = 0;
+                    const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + tile : nullptr;
                     for(uint32_t u = 0; u < 2; ++u)
                     {
                         const uint32_t r0 = row0 + u * TILE;
                         if(r0 < p.len_q)
-                            f |= tile_flags(p, r0, (seg + i) * TILE, prefix, docs ? doc_tiles_q + size_t(b) * q_tiles + r0 / TILE : nullptr, dk)
+                            f |= tile_flags(p, r0, tile * TILE, prefix, docs ? doc_tiles_q + size_t(b) * q_tiles + r0 / TILE : nullptr, dk)
                                  << (2 * u);
                     }
-                    if(f && docs && dk->neg)
-                        f |= 16u;
-                    raw[i] = static_cast<uint8_t>(f);
-                }
-                __syncthreads();
-                if(warp == 0)
-                {
-                    uint32_t n = 0;
-                    for(uint32_t i0 = 0; i0 < count; i0 += 32)
-                    {
-                        const uint32_t f    = i0 + lane < count ? raw[i0 + lane] : 0u;
-                        const uint32_t vote = __ballot_sync(0xFFFFFFFFu, f != 0);
-                        if(f)
-                            list[n + __popc(vote & ((1u << lane) - 1u))] = (seg + i0 + lane) | f << 24;
-                        n += __popc(vote);
-                    }
-                    if(lane == 0)
-                        misc[2] = n;
-                }
-                __syncthreads();
-                const uint32_t entries = misc[2];
+                    return f && docs && dk->neg ? f | TILE_DIRTY : f;
+                });
 
                 if(warp == 8)
                 {
@@ -191,7 +170,7 @@ namespace b200wmma
                         const uint32_t st = n % L::STAGES;
                         if(!wait(base + L::KV_FULL + 8 * st, (n / L::STAGES) & 1u, 1))
                             return false;
-                        if(list[e] >> 28 & 1u)
+                        if(list[e] >> 24 & TILE_DIRTY)
                         {
                             const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
                             clear_padding<HD>(smem + L::KV + st * L::TILE_BYTES, p.doc_kv + size_t(b) * p.len_kv + c0, min(TILE, p.len_kv - c0),

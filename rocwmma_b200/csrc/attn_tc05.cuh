@@ -137,6 +137,7 @@ namespace b200wmma
         {
             TILE_NEED = 1, // some pair of the tile is visible
             TILE_MASK = 2, // some pair is not: each one is looked at
+            TILE_DIRTY = 16, // the tile that is listed holds rows of padding
         };
         // Tile of queries [r0, r0 + 128) x keys [c0, c0 + 128).
         __device__ __forceinline__ uint32_t tile_flags(const Params& p, uint32_t r0, uint32_t c0, int32_t prefix, const DocTile* dq,
@@ -162,6 +163,31 @@ namespace b200wmma
             return TILE_NEED | (mask ? TILE_MASK : 0u);
         }
 
+        // Lists tiles seg .. seg + count that flags_of(tile) says something about, as tile | flags << 24, in order.  Every
+        // thread of the block calls it; `raw` holds SEG bytes, `list` SEG words, `length` one.  Returns the list's length.
+        template <uint32_t THREADS, typename F>
+        __device__ __forceinline__ uint32_t list_tiles(uint32_t seg, uint32_t count, uint32_t* list, uint8_t* raw, uint32_t* length, F flags_of)
+        {
+            for(uint32_t i = threadIdx.x; i < count; i += THREADS)
+                raw[i] = static_cast<uint8_t>(flags_of(seg + i));
+            __syncthreads();
+            if(threadIdx.x < 32)
+            {
+                uint32_t n = 0;
+                for(uint32_t i0 = 0; i0 < count; i0 += 32)
+                {
+                    const uint32_t f    = i0 + threadIdx.x < count ? raw[i0 + threadIdx.x] : 0u;
+                    const uint32_t vote = __ballot_sync(0xFFFFFFFFu, f != 0);
+                    if(f)
+                        list[n + __popc(vote & ((1u << threadIdx.x) - 1u))] = (seg + i0 + threadIdx.x) | f << 24;
+                    n += __popc(vote);
+                }
+                if(threadIdx.x == 0)
+                    *length = n;
+            }
+            __syncthreads();
+            return *length;
+        }
         // One warp to a tile of a batch entry.
         __global__ void __launch_bounds__(128) doc_tiles_kernel(const int32_t* docs, uint32_t len, uint32_t tiles, uint32_t total, DocTile* out)
         {
@@ -205,13 +231,14 @@ namespace b200wmma
         // needs (the hardware's tanh approximation is off by 2^-11 of its value: a capped score of 20 would move by 0.01).
         // An infinite or zero power gives 1 and -1, NaN stays NaN.
         template <bool CAP, bool BIAS>
-        __device__ __forceinline__ float score(const ScoreConst& s, float dot, float dist, float& tanh)
+        __device__ __forceinline__ float score(const ScoreConst& s, float dot, float dist, float& slip)
         {
             float x;
             if constexpr(CAP)
             {
-                tanh = fmaf(-2.0f, rcp(1.0f + ex2(dot * s.k1)), 1.0f);
-                x    = s.cap2 * tanh;
+                const float tanh = fmaf(-2.0f, rcp(1.0f + ex2(dot * s.k1)), 1.0f);
+                slip             = fmaf(-tanh, tanh, 1.0f); // the cap's derivative
+                x                = s.cap2 * tanh;
             }
             else
                 x = dot * s.c;
