@@ -1,62 +1,500 @@
 // Matrix-vector products with 4-bit weights and group scales: the entry point b200wmma_gemv_w4.
 //   y[r][i] = alpha * sum_k x[r][k] * s[i][k / G] * (q[i][k] - z[i][k / G]) + beta * y[r][i]
+//
+// Bound: the packed weights, m * n / 2 bytes, are read once.  What competes is the arithmetic on each weight, so
+//  - values become 16-bit numbers two at a time, by putting the nibble into the mantissa of 1024 (fp16) or 128 (bf16) and
+//    subtracting that with the zero point: exact, since |q - z| <= 15;
+//  - the products are warp-level matrix instructions (16 outputs x 8 vectors x 16 columns, fp32 sums) even for one vector:
+//    a fused multiply-add per weight and vector would take the issue slots that the conversion needs.  tcgen05 would want
+//    tiles of 128 outputs in shared memory and has nothing to gain at 8 vectors;
+//  - sums of a group are scaled in fp32, so nothing is rounded before y.
+// The columns' order inside a group of 32 is free as long as weights and x agree: lane t of four takes word t of each 16-byte
+// piece (8 weights), whose nibbles i and i + 4 come out as one pair, and x is permuted to that by four byte selections.
 #include "attn_common.cuh"
+#include "gemm_tc05_common.cuh"
 
 namespace b200wmma
 {
     namespace gemv_w4
     {
-        using attn::from_f32;
-        using attn::to_f32;
+        constexpr uint32_t WARPS   = 8;
+        constexpr uint32_t THREADS = 32 * WARPS;
 
-        // One warp to an output of one vector, 8 weights (4 bytes) to a lane at a time.
-        template <typename T, typename OutT>
-        __global__ void __launch_bounds__(256)
-            gemv_w4_kernel(uint32_t m, uint32_t n, const uint8_t* a, uint32_t lda, const T* scales, uint32_t ld_scales, const uint8_t* zeros,
-                           uint32_t ld_zeros, uint32_t group, const T* x, uint32_t ldx, OutT* y, uint32_t ldy, float alpha, float beta)
+        struct Args
         {
-            const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-            if(row >= m)
-                return;
-            x += size_t(blockIdx.y) * ldx;
-            float acc = 0.0f;
-            for(uint32_t k = lane * 8; k < n; k += 256)
+            uint32_t       m, n, rows;
+            const uint8_t* a;
+            uint32_t       lda;
+            const void*    scales;
+            uint32_t       ld_scales;
+            const uint8_t* zeros;
+            uint32_t       ld_zeros, group, groups;
+            const void*    x;
+            uint32_t       ldx;
+            void*          y;
+            uint32_t       ldy;
+            float          alpha, beta;
+        };
+
+        __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
+        {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+        }
+        __device__ __forceinline__ void copy_commit()
+        {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        template <int N>
+        __device__ __forceinline__ void copy_wait()
+        {
+            asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+        }
+        __device__ __forceinline__ uint32_t lds32(uint32_t at)
+        {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+            return v;
+        }
+        __device__ __forceinline__ uint4 lds128(uint32_t at)
+        {
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+            return v;
+        }
+        template <typename T>
+        __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+        {
+            if constexpr(std::is_same<T, __half>::value)
+                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+            else
+                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        }
+
+        // What a group subtracts: 1024 + z and 64 + z as fp16 pairs, 128 + z as a bf16 pair (z = 8 for signed values).
+        template <typename T>
+        struct Offset
+        {
+            uint32_t low, high;
+            __device__ __forceinline__ void set(uint32_t z)
             {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(a + size_t(row) * lda + k / 2);
-                const uint32_t g = k / group;
-                const int      z = zeros ? (zeros[size_t(row) * ld_zeros + g] & 15) : 0;
-                float          s = 0.0f;
-                for(int i = 0; i < 8; ++i)
+                if constexpr(std::is_same<T, __half>::value)
                 {
-                    int q = (w >> (4 * i)) & 15;
-                    q     = zeros ? q - z : (q ^ 8) - 8;
-                    s     = fmaf(to_f32(x[k + i]), static_cast<float>(q), s);
+                    low  = (0x6400u + z) * 0x10001u; // 1024 + z
+                    high = (0x5400u + (z << 4)) * 0x10001u; // 64 + z: a step there is 1/16
                 }
-                acc = fmaf(s, to_f32(scales[size_t(row) * ld_scales + g]), acc);
-            }
-            for(int o = 16; o > 0; o >>= 1)
-                acc += __shfl_xor_sync(0xFFFFFFFFu, acc, o);
-            if(lane == 0)
-            {
-                OutT* out = y + size_t(blockIdx.y) * ldy + row;
-                acc *= alpha;
-                if constexpr(sizeof(OutT) == 4)
-                    *out = beta != 0.0f ? acc + beta * *out : acc;
                 else
-                    *out = from_f32<OutT>(beta != 0.0f ? acc + beta * to_f32(*out) : acc);
+                    low = (0x4300u + z) * 0x10001u; // 128 + z
+            }
+        };
+        // Eight weights of a word as pairs (0, 4), (1, 5), (2, 6), (3, 7).  flip = 8 turns signed nibbles into unsigned ones.
+        template <typename T, bool SIGNED>
+        __device__ __forceinline__ void unpack(uint32_t w, const Offset<T>& z, uint32_t (&p)[4])
+        {
+            if constexpr(std::is_same<T, __half>::value)
+            {
+                constexpr uint32_t LOW = SIGNED ? 0x64086408u : 0x64006400u, HIGH = SIGNED ? 0x64806480u : 0x64006400u;
+                const __half2      zl = *reinterpret_cast<const __half2*>(&z.low), zh = *reinterpret_cast<const __half2*>(&z.high);
+                const uint32_t     w8 = w >> 8;
+                uint32_t           u[4] = {(w & 0x000F000Fu) ^ LOW, (w & 0x00F000F0u) ^ HIGH, (w8 & 0x000F000Fu) ^ LOW, (w8 & 0x00F000F0u) ^ HIGH};
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                {
+                    const __half2 h = *reinterpret_cast<const __half2*>(&u[i]);
+                    // 1024 + 16 q comes down to 64 + q exactly
+                    const __half2 r = (i & 1) ? __hfma2(h, __float2half2_rn(0.0625f), __hneg2(zh)) : __hsub2(h, zl);
+                    p[i]            = *reinterpret_cast<const uint32_t*>(&r);
+                }
+            }
+            else
+            {
+                constexpr uint32_t   BASE = SIGNED ? 0x43084308u : 0x43004300u;
+                const __nv_bfloat162 zl   = *reinterpret_cast<const __nv_bfloat162*>(&z.low);
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                {
+                    const uint32_t       u = ((w >> (4 * i)) & 0x000F000Fu) ^ BASE;
+                    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), zl);
+                    p[i]                   = *reinterpret_cast<const uint32_t*>(&r);
+                }
+            }
+        }
+
+        // Scales (and zero points) of the groups that a stretch of columns touches, for the two rows of a lane: lane t of four
+        // holds groups t, t + 4, ...; the upper half belongs to the second row.
+        template <typename T, bool SIGNED, int N>
+        struct GroupInfo
+        {
+            uint32_t scale[N], zero[N];
+            __device__ __forceinline__ void load(const Args& p, uint32_t row0, uint32_t row1, uint32_t k, uint32_t k_end, uint32_t t)
+            {
+                const uint32_t first = k / p.group, last = min(p.groups - 1, (min(k_end, p.n) - 1) / p.group);
+#pragma unroll
+                for(int i = 0; i < N; ++i)
+                {
+                    const uint32_t g = first + t + 4 * i;
+                    scale[i] = zero[i] = 0;
+                    if(g <= last)
+                    {
+                        const uint16_t* s = static_cast<const uint16_t*>(p.scales);
+                        scale[i]          = __ldg(s + size_t(row0) * p.ld_scales + g) | uint32_t(__ldg(s + size_t(row1) * p.ld_scales + g)) << 16;
+                        if constexpr(!SIGNED)
+                            zero[i] = (__ldg(p.zeros + size_t(row0) * p.ld_zeros + g) & 15u)
+                                      | uint32_t(__ldg(p.zeros + size_t(row1) * p.ld_zeros + g) & 15u) << 16;
+                    }
+                }
+            }
+            __device__ __forceinline__ uint32_t pick(const uint32_t (&from)[N], uint32_t i, uint32_t lane) const
+            {
+                uint32_t v = from[0];
+                if constexpr(N == 2)
+                    v = i >= 4 ? from[1] : from[0];
+                return __shfl_sync(0xFFFFFFFFu, v, (lane & ~3u) | (i & 3u));
+            }
+            __device__ __forceinline__ void offsets(uint32_t i, uint32_t lane, Offset<T> (&z)[2]) const
+            {
+                if constexpr(SIGNED)
+                    z[0].set(8), z[1].set(8);
+                else
+                {
+                    const uint32_t v = pick(zero, i, lane);
+                    z[0].set(v & 0xFFFFu), z[1].set(v >> 16);
+                }
+            }
+            // sum += scale * part, part = 0
+            template <int NT>
+            __device__ __forceinline__ void flush(uint32_t i, uint32_t lane, float (&sum)[NT][4], float (&part)[NT][4]) const
+            {
+                const float2 s = tc05::Pack16<T>::widen(pick(scale, i, lane));
+#pragma unroll
+                for(int c = 0; c < NT; ++c)
+#pragma unroll
+                    for(int j = 0; j < 4; ++j)
+                    {
+                        sum[c][j]  = fmaf(j < 2 ? s.x : s.y, part[c][j], sum[c][j]);
+                        part[c][j] = 0.0f;
+                    }
+            }
+        };
+
+        // 32 columns: words of the two rows, 16 bytes of x for each block of 8 vectors
+        template <typename T, bool SIGNED, int NT>
+        __device__ __forceinline__ void step(uint32_t w0, uint32_t w1, const uint4 (&x)[NT], const Offset<T> (&z)[2], float (&part)[NT][4])
+        {
+            uint32_t p[4], q[4];
+            unpack<T, SIGNED>(w0, z[0], p);
+            unpack<T, SIGNED>(w1, z[1], q);
+#pragma unroll
+            for(int c = 0; c < NT; ++c)
+            {
+                mma<T>(part[c], p[0], q[0], p[1], q[1], __byte_perm(x[c].x, x[c].z, 0x5410), __byte_perm(x[c].x, x[c].z, 0x7632));
+                mma<T>(part[c], p[2], q[2], p[3], q[3], __byte_perm(x[c].y, x[c].w, 0x5410), __byte_perm(x[c].y, x[c].w, 0x7632));
             }
         }
 
         template <typename T, typename OutT>
-        static int launch(uint32_t m, uint32_t n, uint32_t rows, const uint8_t* a, uint32_t lda, const void* scales, uint32_t ld_scales,
-                          const uint8_t* zeros, uint32_t ld_zeros, uint32_t group, const void* x, uint32_t ldx, void* y, uint32_t ldy,
-                          float alpha, float beta, cudaStream_t stream)
+        __device__ __forceinline__ void put(const Args& p, uint32_t r, uint32_t i, float s)
         {
-            gemv_w4_kernel<T, OutT><<<dim3(ceil_div(m, 8u), rows), 256, 0, stream>>>(m, n, a, lda, static_cast<const T*>(scales), ld_scales,
-                                                                                    zeros, ld_zeros, group, static_cast<const T*>(x), ldx,
-                                                                                    static_cast<OutT*>(y), ldy, alpha, beta);
-            B200_CHECK_CUDA(cudaGetLastError());
+            OutT* out = static_cast<OutT*>(p.y) + size_t(r) * p.ldy + i;
+            s *= p.alpha;
+            if constexpr(sizeof(OutT) == 4)
+                *out = p.beta != 0.0f ? fmaf(p.beta, *out, s) : s;
+            else
+                *out = attn::from_f32<OutT>(p.beta != 0.0f ? fmaf(p.beta, attn::to_f32(*out), s) : s);
+        }
+
+        // Up to 8 vectors.  A block owns 16 outputs; its warps share the columns in stretches of 256, each through a ring of
+        // its own in shared memory (128 bytes of each row and the x that belongs to them), so warps never wait for one
+        // another before the sums meet.  Few outputs: a cluster of blocks shares the columns too and the sums meet in the
+        // first block's shared memory.
+        constexpr uint32_t FEW_K = 256, FEW_STAGES = 4;
+        static __host__ __device__ constexpr uint32_t few_stage_bytes(uint32_t rows)
+        {
+            return 16 * (FEW_K / 2) + rows * FEW_K * 2;
+        }
+        static constexpr uint32_t few_smem(uint32_t rows)
+        {
+            return WARPS * FEW_STAGES * few_stage_bytes(rows) + WARPS * 128 * 4;
+        }
+        template <typename T, typename OutT, bool SIGNED>
+        __global__ void __launch_bounds__(THREADS) few_kernel(const __grid_constant__ Args p, uint32_t parts)
+        {
+            extern __shared__ __align__(128) uint8_t smem[];
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+            const uint32_t part_id = blockIdx.x % parts, row0 = blockIdx.x / parts * 16;
+            const uint32_t stage_bytes = few_stage_bytes(p.rows), ring = ptx::smem_u32(smem) + warp * FEW_STAGES * stage_bytes;
+            const uint32_t stretches = (p.n + FEW_K - 1) / FEW_K, stride = WARPS * parts, first = part_id * WARPS + warp;
+            const uint32_t mine = first < stretches ? (stretches - first - 1) / stride + 1 : 0;
+            const uint32_t ra = min(row0 + g, p.m - 1), rb = min(row0 + g + 8, p.m - 1);
+
+            const auto fetch = [&](uint32_t i) {
+                const uint32_t k0 = (first + i * stride) * FEW_K, at = ring + (i % FEW_STAGES) * stage_bytes;
+#pragma unroll
+                for(uint32_t j = 0; j < 4; ++j) // 16 rows x 8 pieces
+                {
+                    const uint32_t r = j * 4 + (lane >> 3), c = lane & 7u, k = k0 + c * 32;
+                    const bool     there = k < p.n;
+                    copy16(at + r * 128 + ((c ^ (r & 7u)) << 4), p.a + size_t(min(row0 + r, p.m - 1)) * p.lda + (there ? k / 2 : 0), there);
+                }
+                const T* x = static_cast<const T*>(p.x);
+                for(uint32_t r = 0; r < p.rows; ++r) // 32 pieces of a vector
+                {
+                    const uint32_t k = k0 + lane * 8;
+                    const bool     there = k < p.n;
+                    copy16(at + 2048 + r * 512 + ((lane ^ ((r & 1u) << 2)) << 4), x + size_t(r) * p.ldx + (there ? k : 0), there);
+                }
+            };
+            float sum[1][4] = {}, part[1][4] = {};
+            GroupInfo<T, SIGNED, 2> info, next;
+            const auto groups_of = [&](uint32_t i, GroupInfo<T, SIGNED, 2>& to) {
+                const uint32_t k0 = (first + i * stride) * FEW_K;
+                to.load(p, ra, rb, k0, k0 + FEW_K, t);
+            };
+#pragma unroll
+            for(uint32_t i = 0; i < FEW_STAGES; ++i)
+            {
+                if(i < mine)
+                    fetch(i);
+                copy_commit();
+            }
+            if(mine)
+                groups_of(0, next);
+            for(uint32_t i = 0; i < mine; ++i)
+            {
+                info = next;
+                if(i + 1 < mine)
+                    groups_of(i + 1, next);
+                copy_wait<FEW_STAGES - 1>();
+                __syncwarp();
+                const uint32_t k0 = (first + i * stride) * FEW_K, at = ring + (i % FEW_STAGES) * stage_bytes;
+                const uint32_t xa = at + 2048 + g * 512;
+                uint32_t       grp = 0, left = p.group - k0 % p.group; // columns left of the current group
+                Offset<T>      z[2];
+                info.offsets(0, lane, z);
+#pragma unroll
+                for(uint32_t c = 0; c < 8; ++c)
+                {
+                    const uint32_t w0 = lds32(at + g * 128 + ((c ^ g) << 4) + t * 4), w1 = lds32(at + (g + 8) * 128 + ((c ^ g) << 4) + t * 4);
+                    uint4          x[1] = {make_uint4(0, 0, 0, 0)};
+                    if(g < p.rows)
+                        x[0] = lds128(xa + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4));
+                    step<T, SIGNED, 1>(w0, w1, x, z, part);
+                    left -= 32;
+                    if(left == 0 || c == 7)
+                    {
+                        info.template flush<1>(grp, lane, sum, part);
+                        if(left == 0)
+                        {
+                            left = p.group;
+                            ++grp;
+                            if(!SIGNED && c != 7)
+                                info.offsets(grp, lane, z);
+                        }
+                    }
+                }
+                __syncwarp(); // everyone has read the stage
+                if(i + FEW_STAGES < mine)
+                    fetch(i + FEW_STAGES);
+                copy_commit();
+            }
+            // sums of the warps, [warp][vector][output]
+            float* red = reinterpret_cast<float*>(smem + WARPS * FEW_STAGES * stage_bytes);
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+                red[warp * 128 + (t * 2 + (j & 1)) * 16 + g + 8 * (j >> 1)] = sum[0][j];
+            __syncthreads();
+            const uint32_t r = threadIdx.x >> 4, i = row0 + (threadIdx.x & 15u);
+            float          s = 0.0f;
+            if(threadIdx.x < 128)
+#pragma unroll
+                for(uint32_t w = 0; w < WARPS; ++w)
+                    s += red[w * 128 + threadIdx.x];
+            if(parts > 1)
+            {
+                if(threadIdx.x < 128)
+                    red[threadIdx.x] = s; // only this thread reads or writes the place
+                ptx::cluster_sync();
+                if(part_id == 0 && threadIdx.x < 128)
+                    for(uint32_t c = 1; c < parts; ++c)
+                        s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + threadIdx.x), c)));
+                ptx::cluster_sync();
+                if(part_id != 0)
+                    return;
+            }
+            if(threadIdx.x < 128 && r < p.rows && i < p.m)
+                put<T, OutT>(p, r, i, s);
+        }
+
+        // More vectors, 8 NT to a block: its warps own 16 outputs each and share x in shared memory.  A cluster of blocks
+        // shares the columns where there are few blocks.
+        constexpr uint32_t MANY_K = 128, MANY_ROWS = 16 * WARPS;
+        template <int NT>
+        struct Many
+        {
+            static constexpr uint32_t W_BYTES = MANY_ROWS * MANY_K / 2, X_BYTES = 8 * NT * MANY_K * 2, STAGE = W_BYTES + X_BYTES;
+            static constexpr uint32_t STAGES = NT == 8 ? 4 : 6;
+            static constexpr uint32_t BYTES  = STAGES * STAGE;
+            static_assert(BYTES >= MANY_ROWS * 8 * NT * 4, "the sums of a cluster reuse the ring");
+        };
+        template <typename T, typename OutT, bool SIGNED, int NT>
+        __global__ void __launch_bounds__(THREADS) many_kernel(const __grid_constant__ Args p, uint32_t parts)
+        {
+            using S = Many<NT>;
+            extern __shared__ __align__(128) uint8_t smem[];
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+            const uint32_t part_id = blockIdx.x % parts, row0 = blockIdx.x / parts * MANY_ROWS, vec0 = blockIdx.y * 8 * NT;
+            const uint32_t ring = ptx::smem_u32(smem), stretches = (p.n + MANY_K - 1) / MANY_K;
+            const uint32_t from = uint32_t(uint64_t(stretches) * part_id / parts), mine = uint32_t(uint64_t(stretches) * (part_id + 1) / parts) - from;
+            const uint32_t ra = min(row0 + warp * 16 + g, p.m - 1), rb = min(row0 + warp * 16 + g + 8, p.m - 1);
+
+            const auto fetch = [&](uint32_t i) {
+                const uint32_t k0 = (from + i) * MANY_K, at = ring + (i % S::STAGES) * S::STAGE;
+#pragma unroll
+                for(uint32_t j = threadIdx.x; j < MANY_ROWS * 4; j += THREADS)
+                {
+                    const uint32_t r = j >> 2, c = j & 3u, k = k0 + c * 32;
+                    const bool     there = k < p.n;
+                    copy16(at + r * 64 + ((c ^ ((r >> 1) & 3u)) << 4), p.a + size_t(min(row0 + r, p.m - 1)) * p.lda + (there ? k / 2 : 0), there);
+                }
+                const T* x = static_cast<const T*>(p.x);
+#pragma unroll
+                for(uint32_t j = threadIdx.x; j < 8 * NT * 16; j += THREADS)
+                {
+                    const uint32_t r = j >> 4, c = j & 15u, k = k0 + c * 8;
+                    const bool     there = k < p.n && vec0 + r < p.rows;
+                    copy16(at + S::W_BYTES + r * 256 + ((c ^ ((r & 1u) << 2)) << 4), x + (there ? size_t(vec0 + r) * p.ldx + k : 0), there);
+                }
+            };
+            float sum[NT][4] = {}, part[NT][4] = {};
+            GroupInfo<T, SIGNED, 1> info, next;
+            const auto groups_of = [&](uint32_t i, GroupInfo<T, SIGNED, 1>& to) {
+                const uint32_t k0 = (from + i) * MANY_K;
+                to.load(p, ra, rb, k0, k0 + MANY_K, t);
+            };
+#pragma unroll
+            for(uint32_t i = 0; i < S::STAGES - 1; ++i)
+            {
+                if(i < mine)
+                    fetch(i);
+                copy_commit();
+            }
+            if(mine)
+                groups_of(0, next);
+            for(uint32_t i = 0; i < mine; ++i)
+            {
+                info = next;
+                if(i + 1 < mine)
+                    groups_of(i + 1, next);
+                copy_wait<S::STAGES - 2>();
+                __syncthreads(); // the stage is there for everyone, and everyone has read the one that is fetched into next
+                if(i + S::STAGES - 1 < mine)
+                    fetch(i + S::STAGES - 1);
+                copy_commit();
+                const uint32_t k0 = (from + i) * MANY_K, at = ring + (i % S::STAGES) * S::STAGE;
+                const uint32_t wa = at + (warp * 16 + g) * 64, flip = (g >> 1) & 3u;
+                uint32_t       grp = 0, left = p.group - k0 % p.group;
+                Offset<T>      z[2];
+                info.offsets(0, lane, z);
+#pragma unroll
+                for(uint32_t c = 0; c < 4; ++c)
+                {
+                    const uint32_t w0 = lds32(wa + ((c ^ flip) << 4) + t * 4), w1 = lds32(wa + 512 + ((c ^ flip) << 4) + t * 4);
+                    uint4          x[NT];
+#pragma unroll
+                    for(int v = 0; v < NT; ++v)
+                        x[v] = lds128(at + S::W_BYTES + (v * 8 + g) * 256 + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4));
+                    step<T, SIGNED, NT>(w0, w1, x, z, part);
+                    left -= 32;
+                    if(left == 0 || c == 3)
+                    {
+                        info.template flush<NT>(grp, lane, sum, part);
+                        if(left == 0)
+                        {
+                            left = p.group;
+                            ++grp;
+                            if(!SIGNED && c != 3)
+                                info.offsets(grp, lane, z);
+                        }
+                    }
+                }
+            }
+            copy_wait<0>();
+            __syncthreads();
+            // [vector][output] in shared memory, so that outputs are written next to one another
+            float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for(int v = 0; v < NT; ++v)
+#pragma unroll
+                for(int j = 0; j < 4; ++j)
+                    red[(v * 8 + t * 2 + (j & 1)) * MANY_ROWS + warp * 16 + g + 8 * (j >> 1)] = sum[v][j];
+            if(parts > 1)
+                ptx::cluster_sync();
+            else
+                __syncthreads();
+            // the blocks of a cluster share the outputs among them
+            for(uint32_t e = part_id * THREADS + threadIdx.x; e < MANY_ROWS * 8 * NT; e += parts * THREADS)
+            {
+                const uint32_t r = vec0 + e / MANY_ROWS, i = row0 + e % MANY_ROWS;
+                if(r >= p.rows || i >= p.m)
+                    continue;
+                float s = 0.0f;
+                if(parts > 1)
+                    for(uint32_t c = 0; c < parts; ++c)
+                        s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + e), c)));
+                else
+                    s = red[e];
+                put<T, OutT>(p, r, i, s);
+            }
+            if(parts > 1)
+                ptx::cluster_sync(); // no block leaves while another reads its sums
+        }
+
+        template <typename K>
+        static int launch_clusters(K kern, const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem, cudaStream_t stream)
+        {
+            B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(blocks * parts, blocks_y), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+            cudaLaunchAttribute attr{};
+            attr.id               = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr, cfg.numAttrs = parts > 1 ? 1 : 0;
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p, parts));
             return B200WMMA_OK;
+        }
+        // Blocks of a cluster: as many as keep every part busy for a stretch, up to 8 and to two blocks per SM.
+        static uint32_t parts_of(uint64_t blocks, uint32_t most)
+        {
+            uint32_t parts = 1;
+            while(parts < 8 && 2 * parts <= most && blocks * parts * 2 <= 2 * 148)
+                parts *= 2;
+            return parts;
+        }
+        template <typename T, typename OutT, bool SIGNED, int NT>
+        static int launch_many(const Args& p, cudaStream_t stream)
+        {
+            const uint32_t blocks = ceil_div(p.m, MANY_ROWS), blocks_y = ceil_div(p.rows, 8 * NT);
+            return launch_clusters(many_kernel<T, OutT, SIGNED, NT>, p, blocks, blocks_y, parts_of(uint64_t(blocks) * blocks_y, ceil_div(p.n, 4 * MANY_K)),
+                                   Many<NT>::BYTES, stream);
+        }
+        template <typename T, typename OutT, bool SIGNED>
+        static int launch_signed(const Args& p, cudaStream_t stream)
+        {
+            if(p.rows <= 8)
+            {
+                const uint32_t blocks = ceil_div(p.m, 16);
+                return launch_clusters(few_kernel<T, OutT, SIGNED>, p, blocks, 1, parts_of(blocks, ceil_div(p.n, WARPS * FEW_K)), few_smem(p.rows), stream);
+            }
+            return p.rows <= 16 ? launch_many<T, OutT, SIGNED, 2>(p, stream)
+                   : p.rows <= 32 ? launch_many<T, OutT, SIGNED, 4>(p, stream) : launch_many<T, OutT, SIGNED, 8>(p, stream);
+        }
+        template <typename T, typename OutT>
+        static int launch(const Args& p, cudaStream_t stream)
+        {
+            return p.zeros ? launch_signed<T, OutT, false>(p, stream) : launch_signed<T, OutT, true>(p, stream);
         }
     } // namespace gemv_w4
 } // namespace b200wmma
@@ -74,7 +512,8 @@ extern "C" int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows, const uin
     B200_REQUIRE(out_type == data_type || out_type == B200WMMA_OUT_F32, B200WMMA_ERR_INVALID_ARG,
                  "gemv_w4: out_type must be data_type or B200WMMA_OUT_F32");
     B200_REQUIRE(n % 32 == 0 && group % 32 == 0, B200WMMA_ERR_UNSUPPORTED, "gemv_w4: n and group must be multiples of 32");
-    B200_REQUIRE(m < (1u << 31) && rows < 65536u, B200WMMA_ERR_UNSUPPORTED, "gemv_w4: m must be below 2^31 and rows below 65536");
+    B200_REQUIRE(m < (1u << 30) && n < (1u << 30) && rows < 65536u, B200WMMA_ERR_UNSUPPORTED,
+                 "gemv_w4: m and n must be below 2^30 and rows below 65536");
     const uint32_t groups = (n - 1) / group + 1;
     B200_REQUIRE(lda_bytes >= n / 2 && ldx >= n && ldy >= m && ld_scales >= groups && (!zeros || ld_zeros >= groups),
                  B200WMMA_ERR_INVALID_ARG, "gemv_w4: a leading dimension is smaller than its row");
@@ -82,10 +521,10 @@ extern "C" int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows, const uin
                  "gemv_w4: a, x and their leading dimensions must be multiples of 16 bytes");
     if(int e = require_sm100())
         return e;
-    const auto run = [&](auto fn) {
-        return fn(m, n, rows, a, lda_bytes, scales, ld_scales, zeros, ld_zeros, group, x, ldx, y, ldy, alpha, beta, as_stream(stream));
-    };
+    // a group that outlasts the row is the row: what is left of it never runs out
+    const gemv_w4::Args p{m, n, rows, a, lda_bytes, scales, ld_scales, zeros, ld_zeros, group, groups, x, ldx, y, ldy, alpha, beta};
+    const cudaStream_t  s = as_stream(stream);
     if(data_type == B200WMMA_OUT_F16)
-        return out_type == B200WMMA_OUT_F32 ? run(gemv_w4::launch<__half, float>) : run(gemv_w4::launch<__half, __half>);
-    return out_type == B200WMMA_OUT_F32 ? run(gemv_w4::launch<__nv_bfloat16, float>) : run(gemv_w4::launch<__nv_bfloat16, __nv_bfloat16>);
+        return out_type == B200WMMA_OUT_F32 ? gemv_w4::launch<__half, float>(p, s) : gemv_w4::launch<__half, __half>(p, s);
+    return out_type == B200WMMA_OUT_F32 ? gemv_w4::launch<__nv_bfloat16, float>(p, s) : gemv_w4::launch<__nv_bfloat16, __nv_bfloat16>(p, s);
 }
