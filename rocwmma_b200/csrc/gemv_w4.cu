@@ -34,6 +34,7 @@ namespace b200wmma
             void*          y;
             uint32_t       ldy;
             float          alpha, beta;
+            bool           y_f32;
         };
 
         __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
@@ -55,23 +56,29 @@ namespace b200wmma
             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
             return v;
         }
+        __device__ __forceinline__ void sts128(uint32_t at, const uint4& v)
+        {
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
         __device__ __forceinline__ uint4 lds128(uint32_t at)
         {
             uint4 v;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
             return v;
         }
+        // c = a b + d: `d` is c, or 0 for the first product of a sum
         template <typename T>
-        __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+        __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool fresh)
         {
+            const float d0 = fresh ? 0.0f : c[0], d1 = fresh ? 0.0f : c[1], d2 = fresh ? 0.0f : c[2], d3 = fresh ? 0.0f : c[3];
             if constexpr(std::is_same<T, __half>::value)
-                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                             : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
             else
-                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                             : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
         }
 
         // What a group subtracts: 1024 + z and 64 + z as fp16 pairs, 128 + z as a bf16 pair (z = 8 for signed values).
@@ -90,6 +97,13 @@ namespace b200wmma
                     low = (0x4300u + z) * 0x10001u; // 128 + z
             }
         };
+        // (w & mask) ^ flip in one instruction (written in C, with both constants known, it becomes two)
+        __device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t mask, uint32_t flip)
+        {
+            uint32_t r;
+            asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(mask), "r"(flip));
+            return r;
+        }
         // Eight weights of a word as pairs (0, 4), (1, 5), (2, 6), (3, 7).  flip = 8 turns signed nibbles into unsigned ones.
         template <typename T, bool SIGNED>
         __device__ __forceinline__ void unpack(uint32_t w, const Offset<T>& z, uint32_t (&p)[4])
@@ -99,7 +113,8 @@ namespace b200wmma
                 constexpr uint32_t LOW = SIGNED ? 0x64086408u : 0x64006400u, HIGH = SIGNED ? 0x64806480u : 0x64006400u;
                 const __half2      zl = *reinterpret_cast<const __half2*>(&z.low), zh = *reinterpret_cast<const __half2*>(&z.high);
                 const uint32_t     w8 = w >> 8;
-                uint32_t           u[4] = {(w & 0x000F000Fu) ^ LOW, (w & 0x00F000F0u) ^ HIGH, (w8 & 0x000F000Fu) ^ LOW, (w8 & 0x00F000F0u) ^ HIGH};
+                uint32_t           u[4] = {and_xor(w, 0x000F000Fu, LOW), and_xor(w, 0x00F000F0u, HIGH), and_xor(w8, 0x000F000Fu, LOW),
+                                               and_xor(w8, 0x00F000F0u, HIGH)};
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
                 {
@@ -116,7 +131,7 @@ namespace b200wmma
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
                 {
-                    const uint32_t       u = ((w >> (4 * i)) & 0x000F000Fu) ^ BASE;
+                    const uint32_t       u = and_xor(w >> (4 * i), 0x000F000Fu, BASE);
                     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), zl);
                     p[i]                   = *reinterpret_cast<const uint32_t*>(&r);
                 }
@@ -129,21 +144,22 @@ namespace b200wmma
         struct GroupInfo
         {
             uint32_t scale[N], zero[N];
-            __device__ __forceinline__ void load(const Args& p, uint32_t row0, uint32_t row1, uint32_t k, uint32_t k_end, uint32_t t)
+            __device__ __forceinline__ void load(const Args& p, uint32_t row0, uint32_t row1, uint32_t first, uint32_t last)
             {
-                const uint32_t first = k / p.group, last = min(p.groups - 1, (min(k_end, p.n) - 1) / p.group);
+                const uint16_t* s0 = static_cast<const uint16_t*>(p.scales) + size_t(row0) * p.ld_scales;
+                const uint16_t* s1 = static_cast<const uint16_t*>(p.scales) + size_t(row1) * p.ld_scales;
+                const uint8_t*  z0 = SIGNED ? nullptr : p.zeros + size_t(row0) * p.ld_zeros;
+                const uint8_t*  z1 = SIGNED ? nullptr : p.zeros + size_t(row1) * p.ld_zeros;
 #pragma unroll
                 for(int i = 0; i < N; ++i)
                 {
-                    const uint32_t g = first + t + 4 * i;
+                    const uint32_t g = first + 4 * i;
                     scale[i] = zero[i] = 0;
                     if(g <= last)
                     {
-                        const uint16_t* s = static_cast<const uint16_t*>(p.scales);
-                        scale[i]          = __ldg(s + size_t(row0) * p.ld_scales + g) | uint32_t(__ldg(s + size_t(row1) * p.ld_scales + g)) << 16;
+                        scale[i] = __ldg(s0 + g) | uint32_t(__ldg(s1 + g)) << 16;
                         if constexpr(!SIGNED)
-                            zero[i] = (__ldg(p.zeros + size_t(row0) * p.ld_zeros + g) & 15u)
-                                      | uint32_t(__ldg(p.zeros + size_t(row1) * p.ld_zeros + g) & 15u) << 16;
+                            zero[i] = (__ldg(z0 + g) | uint32_t(__ldg(z1 + g)) << 16) & 0xF000Fu;
                     }
                 }
             }
@@ -164,7 +180,7 @@ namespace b200wmma
                     z[0].set(v & 0xFFFFu), z[1].set(v >> 16);
                 }
             }
-            // sum += scale * part, part = 0
+            // sum += scale * part
             template <int NT>
             __device__ __forceinline__ void flush(uint32_t i, uint32_t lane, float (&sum)[NT][4], float (&part)[NT][4]) const
             {
@@ -174,15 +190,20 @@ namespace b200wmma
 #pragma unroll
                     for(int j = 0; j < 4; ++j)
                     {
-                        sum[c][j]  = fmaf(j < 2 ? s.x : s.y, part[c][j], sum[c][j]);
-                        part[c][j] = 0.0f;
+                        sum[c][j] = fmaf(j < 2 ? s.x : s.y, part[c][j], sum[c][j]);
                     }
             }
         };
 
-        // 32 columns: words of the two rows, 16 bytes of x for each block of 8 vectors
+        // The order that unpack gives its pairs in, for 8 elements of x.
+        __device__ __forceinline__ uint4 pair_up(const uint4& x)
+        {
+            return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
+                              __byte_perm(x.y, x.w, 0x7632));
+        }
+        // 32 columns: words of the two rows, 8 paired elements of x for each block of 8 vectors
         template <typename T, bool SIGNED, int NT>
-        __device__ __forceinline__ void step(uint32_t w0, uint32_t w1, const uint4 (&x)[NT], const Offset<T> (&z)[2], float (&part)[NT][4])
+        __device__ __forceinline__ void step(uint32_t w0, uint32_t w1, const uint4 (&x)[NT], const Offset<T> (&z)[2], float (&part)[NT][4], bool fresh)
         {
             uint32_t p[4], q[4];
             unpack<T, SIGNED>(w0, z[0], p);
@@ -190,68 +211,104 @@ namespace b200wmma
 #pragma unroll
             for(int c = 0; c < NT; ++c)
             {
-                mma<T>(part[c], p[0], q[0], p[1], q[1], __byte_perm(x[c].x, x[c].z, 0x5410), __byte_perm(x[c].x, x[c].z, 0x7632));
-                mma<T>(part[c], p[2], q[2], p[3], q[3], __byte_perm(x[c].y, x[c].w, 0x5410), __byte_perm(x[c].y, x[c].w, 0x7632));
+                mma<T>(part[c], p[0], q[0], p[1], q[1], x[c].x, x[c].y, fresh);
+                mma<T>(part[c], p[2], q[2], p[3], q[3], x[c].z, x[c].w, false);
             }
         }
 
-        template <typename T, typename OutT>
+        template <typename T>
         __device__ __forceinline__ void put(const Args& p, uint32_t r, uint32_t i, float s)
         {
-            OutT* out = static_cast<OutT*>(p.y) + size_t(r) * p.ldy + i;
+            const size_t at = size_t(r) * p.ldy + i;
             s *= p.alpha;
-            if constexpr(sizeof(OutT) == 4)
-                *out = p.beta != 0.0f ? fmaf(p.beta, *out, s) : s;
+            if(p.y_f32)
+            {
+                float* out = static_cast<float*>(p.y) + at;
+                *out       = p.beta != 0.0f ? fmaf(p.beta, *out, s) : s;
+            }
             else
-                *out = attn::from_f32<OutT>(p.beta != 0.0f ? fmaf(p.beta, attn::to_f32(*out), s) : s);
+            {
+                T* out = static_cast<T*>(p.y) + at;
+                *out   = attn::from_f32<T>(p.beta != 0.0f ? fmaf(p.beta, attn::to_f32(*out), s) : s);
+            }
         }
 
-        // Up to 8 vectors.  A block owns 16 outputs; its warps share the columns in stretches of 256, each through a ring of
-        // its own in shared memory (128 bytes of each row and the x that belongs to them), so warps never wait for one
-        // another before the sums meet.  Few outputs: a cluster of blocks shares the columns too and the sums meet in the
-        // first block's shared memory.
-        constexpr uint32_t FEW_K = 256, FEW_STAGES = 4;
-        static __host__ __device__ constexpr uint32_t few_stage_bytes(uint32_t rows)
+        // Up to 8 vectors.  A block owns 16 outputs; its W warps share the columns in stretches of 256, each through a ring of its
+        // own in shared memory (128 bytes of each row, and the x that belongs to them), so warps never wait for one another
+        // before the sums meet.  Few outputs: a cluster of blocks shares the columns too and the sums meet in the first
+        // block's shared memory.
+        // STEPS: pieces of 32 columns to a group inside a stretch, where groups and stretches are aligned (groups of 32, 64,
+        // 128 and multiples of 256); 0: counted at run time.
+        // ONE: a single vector.  Each warp pairs up its part of x once, before the weights are there.
+        constexpr uint32_t FEW_K = 256, FEW_STAGES = 2, FEW_ROWS = 16;
+        struct Few
         {
-            return 16 * (FEW_K / 2) + rows * FEW_K * 2;
-        }
-        static constexpr uint32_t few_smem(uint32_t rows)
+            static constexpr uint32_t W_STAGE = FEW_ROWS * FEW_K / 2, ZERO = 512; // zeros: the x of vectors that do not exist
+            uint32_t x_warp, bytes; // bytes of a warp's x
+            __host__ __device__ Few(uint32_t w, uint32_t rows, uint32_t n, uint32_t parts)
+            {
+                const uint32_t stretches = (n + FEW_K - 1) / FEW_K;
+                x_warp = rows == 1 ? (stretches + w * parts - 1) / (w * parts) * FEW_K * 2 : FEW_STAGES * rows * FEW_K * 2;
+                const uint32_t ring = w * (FEW_STAGES * W_STAGE + x_warp), red = w * 128 * 4; // the sums reuse the ring
+                bytes = ZERO + (ring > red ? ring : red);
+            }
+        };
+        template <typename T, bool SIGNED, int W, int STEPS, bool ONE>
+        __global__ void __launch_bounds__(32 * W) few_kernel(const __grid_constant__ Args p, uint32_t parts)
         {
-            return WARPS * FEW_STAGES * few_stage_bytes(rows) + WARPS * 128 * 4;
-        }
-        template <typename T, typename OutT, bool SIGNED>
-        __global__ void __launch_bounds__(THREADS) few_kernel(const __grid_constant__ Args p, uint32_t parts)
-        {
-            extern __shared__ __align__(128) uint8_t smem[];
+            constexpr int GROUPS = STEPS == 0 ? 8 : 8 / STEPS, INFO = GROUPS > 4 ? 2 : 1;
+            extern __shared__ __align__(1024) uint8_t smem[];
+            const Few      f(W, ONE ? 1 : p.rows, p.n, parts);
             const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-            const uint32_t part_id = blockIdx.x % parts, row0 = blockIdx.x / parts * 16;
-            const uint32_t stage_bytes = few_stage_bytes(p.rows), ring = ptx::smem_u32(smem) + warp * FEW_STAGES * stage_bytes;
-            const uint32_t stretches = (p.n + FEW_K - 1) / FEW_K, stride = WARPS * parts, first = part_id * WARPS + warp;
+            const uint32_t part_id = parts > 1 ? blockIdx.x % parts : 0, row0 = (parts > 1 ? blockIdx.x / parts : blockIdx.x) * FEW_ROWS;
+            const uint32_t zero = ptx::smem_u32(smem), ring = zero + Few::ZERO + warp * (FEW_STAGES * Few::W_STAGE + f.x_warp);
+            const uint32_t ring_x = ring + FEW_STAGES * Few::W_STAGE, x_stage = f.x_warp / FEW_STAGES;
+            const uint32_t stretches = (p.n + FEW_K - 1) / FEW_K, stride = W * parts, first = part_id * W + warp;
             const uint32_t mine = first < stretches ? (stretches - first - 1) / stride + 1 : 0;
-            const uint32_t ra = min(row0 + g, p.m - 1), rb = min(row0 + g + 8, p.m - 1);
+            const bool     rows_full = row0 + FEW_ROWS <= p.m;
 
-            const auto fetch = [&](uint32_t i) {
-                const uint32_t k0 = (first + i * stride) * FEW_K, at = ring + (i % FEW_STAGES) * stage_bytes;
+            // a lane copies piece lane % 8 of rows lane / 8, lane / 8 + 4, ... and piece `lane` of each vector
+            const uint8_t* src_a = p.a + size_t(row0 + (lane >> 3)) * p.lda + (lane & 7u) * 16 + size_t(first) * (FEW_K / 2);
+            const T*       src_x = static_cast<const T*>(p.x) + size_t(first) * FEW_K + lane * 8;
+            const uint32_t place[2] = {ring + (lane >> 3) * 128 + (((lane & 7u) ^ (lane >> 3)) << 4),
+                                       ring + (lane >> 3) * 128 + (((lane & 7u) ^ ((lane >> 3) + 4)) << 4)};
+            const size_t   rows4    = size_t(p.lda) * 4;
+            uint32_t       k_next   = first * FEW_K;
+            const auto     fetch    = [&](uint32_t slot) {
+                const uint8_t* from = src_a;
+                if(rows_full && k_next + FEW_K <= p.n)
+                {
 #pragma unroll
-                for(uint32_t j = 0; j < 4; ++j) // 16 rows x 8 pieces
-                {
-                    const uint32_t r = j * 4 + (lane >> 3), c = lane & 7u, k = k0 + c * 32;
-                    const bool     there = k < p.n;
-                    copy16(at + r * 128 + ((c ^ (r & 7u)) << 4), p.a + size_t(min(row0 + r, p.m - 1)) * p.lda + (there ? k / 2 : 0), there);
+                    for(uint32_t j = 0; j < 4; ++j, from += rows4)
+                        copy16(place[j & 1u] + slot * Few::W_STAGE + j * 512, from, true);
                 }
-                const T* x = static_cast<const T*>(p.x);
-                for(uint32_t r = 0; r < p.rows; ++r) // 32 pieces of a vector
+                else
+#pragma unroll
+                    for(uint32_t j = 0; j < 4; ++j, from += rows4)
+                    {
+                        const bool there = row0 + (lane >> 3) + j * 4 < p.m && k_next + (lane & 7u) * 32 < p.n;
+                        copy16(place[j & 1u] + slot * Few::W_STAGE + j * 512, there ? from : p.a, there);
+                    }
+                if constexpr(!ONE)
                 {
-                    const uint32_t k = k0 + lane * 8;
-                    const bool     there = k < p.n;
-                    copy16(at + 2048 + r * 512 + ((lane ^ ((r & 1u) << 2)) << 4), x + size_t(r) * p.ldx + (there ? k : 0), there);
+                    const bool there = k_next + lane * 8 < p.n;
+                    for(uint32_t r = 0; r < p.rows; ++r)
+                        copy16(ring_x + slot * x_stage + r * 512 + ((lane ^ ((r & 1u) << 2)) << 4),
+                               there ? src_x + size_t(r) * p.ldx : static_cast<const T*>(p.x), there);
+                    src_x += size_t(stride) * FEW_K;
                 }
+                src_a += size_t(stride) * (FEW_K / 2), k_next += stride * FEW_K;
             };
-            float sum[1][4] = {}, part[1][4] = {};
-            GroupInfo<T, SIGNED, 2> info, next;
-            const auto groups_of = [&](uint32_t i, GroupInfo<T, SIGNED, 2>& to) {
-                const uint32_t k0 = (first + i * stride) * FEW_K;
-                to.load(p, ra, rb, k0, k0 + FEW_K, t);
+            float                      sum[1][4] = {}, part[1][4] = {};
+            GroupInfo<T, SIGNED, INFO> info, next;
+            const uint32_t             ra = min(row0 + g, p.m - 1), rb = min(row0 + g + 8, p.m - 1);
+            uint32_t                   k_info = first * FEW_K, g_info = k_info / p.group; // first group of the stretch
+            const auto                 groups = [&]() {
+                if constexpr(STEPS == 0 || STEPS == 8)
+                    g_info = k_info / p.group;
+                const uint32_t last = STEPS == 8 ? g_info : STEPS == 0 ? min(p.groups - 1, (k_info + FEW_K - 1) / p.group) : p.groups - 1;
+                next.load(p, ra, rb, g_info + t, min(last, g_info + GROUPS - 1));
+                k_info += stride * FEW_K, g_info += stride * GROUPS;
             };
 #pragma unroll
             for(uint32_t i = 0; i < FEW_STAGES; ++i)
@@ -261,32 +318,62 @@ namespace b200wmma
                 copy_commit();
             }
             if(mine)
-                groups_of(0, next);
+                groups();
+            if constexpr(ONE)
+            {
+#pragma unroll 4
+                for(uint32_t i = 0; i < mine; ++i)
+                {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if((first + i * stride) * FEW_K + lane * 8 < p.n)
+                        x = __ldg(reinterpret_cast<const uint4*>(src_x + size_t(i) * stride * FEW_K));
+                    sts128(ring_x + i * 512 + lane * 16, pair_up(x));
+                }
+            }
+            if(threadIdx.x < Few::ZERO / 16)
+                sts128(zero + threadIdx.x * 16, make_uint4(0, 0, 0, 0));
+            __syncthreads();
+            uint32_t       slot = 0, k0 = first * FEW_K;
+            const uint32_t wa = ring + g * 128 + (g << 4) + t * 4; // pieces are 16 bytes apart and swizzled by their row
+            // lanes of vectors that do not exist read zeros
+            uint32_t xa = g >= p.rows ? zero + t * 16 : ring_x + t * 16 + (ONE ? 0u : g * 512 + ((g & 1u) << 6));
             for(uint32_t i = 0; i < mine; ++i)
             {
                 info = next;
                 if(i + 1 < mine)
-                    groups_of(i + 1, next);
+                    groups();
                 copy_wait<FEW_STAGES - 1>();
                 __syncwarp();
-                const uint32_t k0 = (first + i * stride) * FEW_K, at = ring + (i % FEW_STAGES) * stage_bytes;
-                const uint32_t xa = at + 2048 + g * 512;
-                uint32_t       grp = 0, left = p.group - k0 % p.group; // columns left of the current group
+                const uint32_t ws = wa + slot * Few::W_STAGE, xs = ONE || g >= p.rows ? xa : xa + slot * x_stage;
+                uint32_t       grp = 0, left = STEPS == 0 ? p.group - k0 % p.group : 0; // columns left of the current group
+                bool           fresh = true;
                 Offset<T>      z[2];
                 info.offsets(0, lane, z);
 #pragma unroll
                 for(uint32_t c = 0; c < 8; ++c)
                 {
-                    const uint32_t w0 = lds32(at + g * 128 + ((c ^ g) << 4) + t * 4), w1 = lds32(at + (g + 8) * 128 + ((c ^ g) << 4) + t * 4);
-                    uint4          x[1] = {make_uint4(0, 0, 0, 0)};
-                    if(g < p.rows)
-                        x[0] = lds128(xa + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4));
-                    step<T, SIGNED, 1>(w0, w1, x, z, part);
-                    left -= 32;
-                    if(left == 0 || c == 7)
+                    uint4 x[1];
+                    if constexpr(ONE)
+                        x[0] = lds128(xs + c * 64);
+                    else
+                        x[0] = pair_up(lds128(xs ^ (c << 6)));
+                    if constexpr(STEPS != 0)
+                        fresh = c % STEPS == 0;
+                    step<T, SIGNED, 1>(lds32(ws ^ (c << 4)), lds32((ws ^ (c << 4)) + 1024), x, z, part, fresh);
+                    fresh    = false;
+                    bool end = c == 7;
+                    if constexpr(STEPS == 0)
+                    {
+                        left -= 32;
+                        end |= left == 0;
+                    }
+                    else
+                        end |= (c + 1) % STEPS == 0;
+                    if(end)
                     {
                         info.template flush<1>(grp, lane, sum, part);
-                        if(left == 0)
+                        fresh = true;
+                        if(STEPS != 0 || left == 0)
                         {
                             left = p.group;
                             ++grp;
@@ -297,35 +384,48 @@ namespace b200wmma
                 }
                 __syncwarp(); // everyone has read the stage
                 if(i + FEW_STAGES < mine)
-                    fetch(i + FEW_STAGES);
+                    fetch(slot);
                 copy_commit();
+                slot ^= 1u;
+                k0 += stride * FEW_K;
+                if(ONE && g == 0)
+                    xa += 512;
             }
+            copy_wait<0>();
+            __syncthreads();
             // sums of the warps, [warp][vector][output]
-            float* red = reinterpret_cast<float*>(smem + WARPS * FEW_STAGES * stage_bytes);
+            float* red = reinterpret_cast<float*>(smem + Few::ZERO);
 #pragma unroll
             for(int j = 0; j < 4; ++j)
-                red[warp * 128 + (t * 2 + (j & 1)) * 16 + g + 8 * (j >> 1)] = sum[0][j];
+                if(!ONE || (t == 0 && (j & 1) == 0))
+                    red[warp * 128 + (t * 2 + (j & 1)) * FEW_ROWS + g + 8 * (j >> 1)] = sum[0][j];
             __syncthreads();
-            const uint32_t r = threadIdx.x >> 4, i = row0 + (threadIdx.x & 15u);
-            float          s = 0.0f;
-            if(threadIdx.x < 128)
+            const uint32_t outs = (ONE ? 1 : p.rows) * FEW_ROWS;
+            for(uint32_t e = threadIdx.x; e < outs; e += 32 * W)
+            {
+                float s = 0.0f;
 #pragma unroll
-                for(uint32_t w = 0; w < WARPS; ++w)
-                    s += red[w * 128 + threadIdx.x];
+                for(uint32_t w = 0; w < W; ++w)
+                    s += red[w * 128 + e];
+                if(parts > 1)
+                    red[e] = s; // no other thread reads or writes the place
+                else if(row0 + e % FEW_ROWS < p.m)
+                    put<T>(p, e / FEW_ROWS, row0 + e % FEW_ROWS, s);
+            }
             if(parts > 1)
             {
-                if(threadIdx.x < 128)
-                    red[threadIdx.x] = s; // only this thread reads or writes the place
                 ptx::cluster_sync();
-                if(part_id == 0 && threadIdx.x < 128)
-                    for(uint32_t c = 1; c < parts; ++c)
-                        s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + threadIdx.x), c)));
-                ptx::cluster_sync();
-                if(part_id != 0)
-                    return;
+                if(part_id == 0)
+                    for(uint32_t e = threadIdx.x; e < outs; e += 32 * W)
+                    {
+                        float s = red[e];
+                        for(uint32_t c = 1; c < parts; ++c)
+                            s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + e), c)));
+                        if(row0 + e % FEW_ROWS < p.m)
+                            put<T>(p, e / FEW_ROWS, row0 + e % FEW_ROWS, s);
+                    }
+                ptx::cluster_sync(); // no block leaves while another reads its sums
             }
-            if(threadIdx.x < 128 && r < p.rows && i < p.m)
-                put<T, OutT>(p, r, i, s);
         }
 
         // More vectors, 8 NT to a block: its warps own 16 outputs each and share x in shared memory.  A cluster of blocks
@@ -339,7 +439,7 @@ namespace b200wmma
             static constexpr uint32_t BYTES  = STAGES * STAGE;
             static_assert(BYTES >= MANY_ROWS * 8 * NT * 4, "the sums of a cluster reuse the ring");
         };
-        template <typename T, typename OutT, bool SIGNED, int NT>
+        template <typename T, bool SIGNED, int NT>
         __global__ void __launch_bounds__(THREADS) many_kernel(const __grid_constant__ Args p, uint32_t parts)
         {
             using S = Many<NT>;
@@ -372,7 +472,7 @@ namespace b200wmma
             GroupInfo<T, SIGNED, 1> info, next;
             const auto groups_of = [&](uint32_t i, GroupInfo<T, SIGNED, 1>& to) {
                 const uint32_t k0 = (from + i) * MANY_K;
-                to.load(p, ra, rb, k0, k0 + MANY_K, t);
+                to.load(p, ra, rb, k0 / p.group + t, min(p.groups - 1, (k0 + MANY_K - 1) / p.group));
             };
 #pragma unroll
             for(uint32_t i = 0; i < S::STAGES - 1; ++i)
@@ -405,12 +505,15 @@ namespace b200wmma
                     uint4          x[NT];
 #pragma unroll
                     for(int v = 0; v < NT; ++v)
-                        x[v] = lds128(at + S::W_BYTES + (v * 8 + g) * 256 + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4));
-                    step<T, SIGNED, NT>(w0, w1, x, z, part);
+                        x[v] = pair_up(lds128(at + S::W_BYTES + (v * 8 + g) * 256 + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4)));
+                    step<T, SIGNED, NT>(w0, w1, x, z, part, false);
                     left -= 32;
                     if(left == 0 || c == 3)
                     {
                         info.template flush<NT>(grp, lane, sum, part);
+#pragma unroll
+                        for(int v = 0; v < NT; ++v)
+                            part[v][0] = part[v][1] = part[v][2] = part[v][3] = 0.0f;
                         if(left == 0)
                         {
                             left = p.group;
@@ -446,18 +549,19 @@ namespace b200wmma
                         s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + e), c)));
                 else
                     s = red[e];
-                put<T, OutT>(p, r, i, s);
+                put<T>(p, r, i, s);
             }
             if(parts > 1)
                 ptx::cluster_sync(); // no block leaves while another reads its sums
         }
 
         template <typename K>
-        static int launch_clusters(K kern, const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem, cudaStream_t stream)
+        static int launch_clusters(K kern, const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem,
+                                   uint32_t threads, cudaStream_t stream)
         {
             B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(blocks * parts, blocks_y), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+            cfg.gridDim = dim3(blocks * parts, blocks_y), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
             cudaLaunchAttribute attr{};
             attr.id               = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
@@ -473,28 +577,40 @@ namespace b200wmma
                 parts *= 2;
             return parts;
         }
-        template <typename T, typename OutT, bool SIGNED, int NT>
+        template <typename T, bool SIGNED, int NT>
         static int launch_many(const Args& p, cudaStream_t stream)
         {
             const uint32_t blocks = ceil_div(p.m, MANY_ROWS), blocks_y = ceil_div(p.rows, 8 * NT);
-            return launch_clusters(many_kernel<T, OutT, SIGNED, NT>, p, blocks, blocks_y, parts_of(uint64_t(blocks) * blocks_y, ceil_div(p.n, 4 * MANY_K)),
-                                   Many<NT>::BYTES, stream);
+            return launch_clusters(many_kernel<T, SIGNED, NT>, p, blocks, blocks_y, parts_of(uint64_t(blocks) * blocks_y, ceil_div(p.n, 4 * MANY_K)),
+                                   Many<NT>::BYTES, THREADS, stream);
         }
-        template <typename T, typename OutT, bool SIGNED>
-        static int launch_signed(const Args& p, cudaStream_t stream)
+#ifndef W4_W
+#define W4_W 8
+#endif
+        template <typename T, bool SIGNED, int W, int STEPS>
+        static int launch_warps(const Args& p, uint32_t blocks, cudaStream_t stream)
         {
-            if(p.rows <= 8)
-            {
-                const uint32_t blocks = ceil_div(p.m, 16);
-                return launch_clusters(few_kernel<T, OutT, SIGNED>, p, blocks, 1, parts_of(blocks, ceil_div(p.n, WARPS * FEW_K)), few_smem(p.rows), stream);
-            }
-            return p.rows <= 16 ? launch_many<T, OutT, SIGNED, 2>(p, stream)
-                   : p.rows <= 32 ? launch_many<T, OutT, SIGNED, 4>(p, stream) : launch_many<T, OutT, SIGNED, 8>(p, stream);
+            const uint32_t parts = parts_of(blocks, ceil_div(p.n, W * FEW_K));
+            const Few      f(W, p.rows, p.n, parts);
+            return p.rows == 1 ? launch_clusters(few_kernel<T, SIGNED, W, STEPS, true>, p, blocks, 1, parts, f.bytes, 32 * W, stream)
+                               : launch_clusters(few_kernel<T, SIGNED, W, STEPS, false>, p, blocks, 1, parts, f.bytes, 32 * W, stream);
         }
-        template <typename T, typename OutT>
+        template <typename T, bool SIGNED, int STEPS>
+        static int launch_few(const Args& p, cudaStream_t stream)
+        {
+            return launch_warps<T, SIGNED, W4_W, STEPS>(p, ceil_div(p.m, FEW_ROWS), stream);
+        }
+        template <typename T, bool SIGNED>
         static int launch(const Args& p, cudaStream_t stream)
         {
-            return p.zeros ? launch_signed<T, OutT, false>(p, stream) : launch_signed<T, OutT, true>(p, stream);
+            if(p.rows > 8)
+                return p.rows <= 16 ? launch_many<T, SIGNED, 2>(p, stream)
+                       : p.rows <= 32 ? launch_many<T, SIGNED, 4>(p, stream) : launch_many<T, SIGNED, 8>(p, stream);
+            if(p.group % FEW_K == 0)
+                return launch_few<T, SIGNED, 8>(p, stream);
+            return p.group == 128 ? launch_few<T, SIGNED, 4>(p, stream)
+                   : p.group == 64 ? launch_few<T, SIGNED, 2>(p, stream)
+                   : p.group == 32 ? launch_few<T, SIGNED, 1>(p, stream) : launch_few<T, SIGNED, 0>(p, stream);
         }
     } // namespace gemv_w4
 } // namespace b200wmma
@@ -522,9 +638,10 @@ extern "C" int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows, const uin
     if(int e = require_sm100())
         return e;
     // a group that outlasts the row is the row: what is left of it never runs out
-    const gemv_w4::Args p{m, n, rows, a, lda_bytes, scales, ld_scales, zeros, ld_zeros, group, groups, x, ldx, y, ldy, alpha, beta};
+    const gemv_w4::Args p{m, n, rows, a, lda_bytes, scales, ld_scales, zeros, ld_zeros, group, groups, x, ldx, y, ldy, alpha, beta,
+                          out_type == B200WMMA_OUT_F32};
     const cudaStream_t  s = as_stream(stream);
     if(data_type == B200WMMA_OUT_F16)
-        return out_type == B200WMMA_OUT_F32 ? gemv_w4::launch<__half, float>(p, s) : gemv_w4::launch<__half, __half>(p, s);
-    return out_type == B200WMMA_OUT_F32 ? gemv_w4::launch<__nv_bfloat16, float>(p, s) : gemv_w4::launch<__nv_bfloat16, __nv_bfloat16>(p, s);
+        return zeros ? gemv_w4::launch<__half, false>(p, s) : gemv_w4::launch<__half, true>(p, s);
+    return zeros ? gemv_w4::launch<__nv_bfloat16, false>(p, s) : gemv_w4::launch<__nv_bfloat16, true>(p, s);
 }
