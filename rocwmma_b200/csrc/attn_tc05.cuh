@@ -189,7 +189,7 @@ namespace b200wmma
             return *length;
         }
         // One warp to a tile of a batch entry.
-        __global__ void __launch_bounds__(128) doc_tiles_kernel(const int32_t* docs, uint32_t len, uint32_t tiles, uint32_t total, DocTile* out)
+        static __global__ void __launch_bounds__(128) doc_tiles_kernel(const int32_t* docs, uint32_t len, uint32_t tiles, uint32_t total, DocTile* out)
         {
             const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
             if(at >= total)
