@@ -248,15 +248,15 @@ namespace b200wmma
         }
 
         // ---- host side ------------------------------------------------------------------------
-        // [batch][tokens][heads][dim] with free strides, in boxes of 64 elements x 128 tokens; zero fill out of bounds.
+        // [batch][tokens][heads][dim] with free strides, in boxes of 64 elements x box_tokens tokens; zero fill out of bounds.
         static int make_map(CUtensorMap* out, int data_type, const void* ptr, uint32_t dim, uint32_t tokens, uint32_t heads, uint32_t batch,
-                            const Strides& s)
+                            const Strides& s, uint32_t box_tokens = TILE)
         {
             tc05::EncodeTiledFn fn = tc05::get_encode_fn();
             B200_REQUIRE(fn != nullptr, B200WMMA_ERR_CUDA, "cuTensorMapEncodeTiled not available");
             cuuint64_t gdim[4]    = {dim, tokens, heads, batch};
             cuuint64_t gstride[3] = {cuuint64_t(s.token) * 2, cuuint64_t(s.head) * 2, cuuint64_t(s.batch) * 2};
-            cuuint32_t box[4]     = {64, TILE, 1, 1};
+            cuuint32_t box[4]     = {64, box_tokens, 1, 1};
             cuuint32_t estr[4]    = {1, 1, 1, 1};
             CUresult   r          = fn(out, data_type == B200WMMA_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                             const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

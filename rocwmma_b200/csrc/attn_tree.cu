@@ -1,8 +1,9 @@
 // Attention of drafted tokens over a paged cache: the entry point b200wmma_attn_tree.
 //
 // Bound: keys and values are read once.  Rows that share a key head (its query heads times the drafted tokens) are the rows of
-// one product, so a block reads 64 tokens of the cache at a time into shared memory (a ring of asynchronous copies, 16 bytes
-// each, rows found through the page table) and every row uses them.  With up to 64 rows a token's 2 x head_dim values meet
+// one product, so a block reads 64 tokens of the cache at a time into shared memory and every row uses them.  One warp walks the
+// page table and issues the copies (TMA boxes of as many tokens as surely lie in one page; a page number outside the cache
+// reads as zeros), the others wait for a stage and never for one another.  With up to 64 rows a token's 2 x head_dim values meet
 // 4 x 64 x head_dim flops, which warp-level matrix instructions keep up with; tcgen05 tiles would be 128 rows high and mostly
 // empty.  One pass: running maximum and sum per row, the weights go from accumulators to operands in registers.
 // The tokens are split over blocks where rows, heads and sequences alone do not fill the machine; a second kernel joins the
@@ -17,13 +18,15 @@ namespace b200wmma
         using attn::LOG2E;
         constexpr uint32_t MAX_DRAFTS = 64;
         constexpr uint32_t KEYS       = 64; // tokens of a stage
-        constexpr uint32_t STAGES     = 3;
-        constexpr uint32_t THREADS    = 128;
+        constexpr uint32_t THREADS    = 160; // warps 0-3 compute, warp 4 copies
         constexpr uint32_t MAX_SPLITS = 256;
 
         struct Params
         {
             uint32_t batch, heads_q, heads_kv, share, dim, drafts, num_pages, page_size, ld_table, splits, tiles;
+            uint32_t page_shift; // log2 of page_size, 32 where it is no power of two
+            uint32_t box; // tokens of a copy: a power of two that divides page_size, at most 64
+            unsigned* status;
             float    scale, cap;
             const float*    slopes;
             const int32_t * block_table, *lens, *n_drafts, *depths;
@@ -32,10 +35,6 @@ namespace b200wmma
             float *         part_o, *part_ml; // [split][row][HD], [split][row][2]; rows: batch x heads_kv x share x drafts
         };
 
-        __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
-        {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-        }
         __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at)
         {
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -71,29 +70,54 @@ namespace b200wmma
             return int64_t(b) * s.batch + int64_t(t) * s.token + int64_t(h) * s.head;
         }
 
+        enum Role : uint32_t
+        {
+            TREE_PRODUCER = 0x61,
+            TREE_COMPUTE  = 0x62
+        };
         template <uint32_t HD>
         struct Smem
         {
-            static constexpr uint32_t ROW = HD * 2, TILE = KEYS * ROW; // a stage is a tile of keys and one of values
-            static constexpr uint32_t TABLE = STAGES * 2 * TILE; // 2 x 64 {page, row in it}; page -1: not there
-            static constexpr uint32_t VALID = TABLE + 2 * KEYS * 8; // STAGES words of 64 bits
-            static constexpr uint32_t BYTES = VALID + 8 * (STAGES + 1);
-            static_assert(STAGES * 2 * TILE >= 4 * 16 * (HD + 2) * 4, "sums of the warps reuse the ring");
+            static constexpr uint32_t HALF   = KEYS * 128; // 64 tokens x 64 elements, rows of 128 bytes with the 128-byte swizzle
+            static constexpr uint32_t TILE   = HD / 64 * HALF; // a stage is a tile of keys and one of values
+            static constexpr uint32_t STAGES = HD == 128 ? 3 : 4;
+            static constexpr uint32_t SUMS = 4 * 16 * (HD + 2) * 4, RING = STAGES * 2 * TILE; // sums of the warps reuse the ring
+            static constexpr uint32_t BARS  = RING;
+            static constexpr uint32_t VALID = BARS + 16 * STAGES; // STAGES words of 64 bits: tokens that are there
+            static constexpr uint32_t ABORT = VALID + 8 * STAGES;
+            static constexpr uint32_t BYTES = ABORT + 16 + 1024;
+            static_assert(RING >= SUMS, "");
         };
 
         // A block: 16 WM rows of one key head and the tokens of one split.  4 warps: WM along the rows, 4 / WM along the 64
         // tokens of a stage, each with its own running maximum.
         template <typename T, uint32_t HD, uint32_t WM, bool CAP, bool BIAS>
-        __global__ void __launch_bounds__(THREADS) tree_kernel(const __grid_constant__ Params p, const T* __restrict__ q, const T* __restrict__ k,
-                                                               const T* __restrict__ v, T* __restrict__ o)
+        __global__ void __launch_bounds__(THREADS, 2)
+            tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p,
+                        const T* __restrict__ q, T* __restrict__ o)
         {
-            using L                   = Smem<HD>;
-            constexpr uint32_t WN     = 4 / WM, MINE = KEYS / WN, CHUNKS = HD / 8; // tokens of a warp, 16-byte pieces of a row
-            extern __shared__ __align__(1024) uint8_t smem[];
-            const uint32_t base = ptx::smem_u32(smem), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
-            const uint32_t wm = warp % WM, wn = warp / WM;
-            int2*          table = reinterpret_cast<int2*>(smem + L::TABLE);
-            uint32_t*      valid = reinterpret_cast<uint32_t*>(smem + L::VALID);
+            using L               = Smem<HD>;
+            constexpr uint32_t WN = 4 / WM, MINE = KEYS / WN, STAGES = L::STAGES; // tokens of a warp
+            extern __shared__ uint8_t smem_raw[];
+            const uint32_t     base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+            uint8_t*           smem = smem_raw + (base - ptx::smem_u32(smem_raw));
+            const uint32_t     tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+            const uint32_t     wm = warp % WM, wn = (warp & 3u) / WM;
+            uint32_t*          valid     = reinterpret_cast<uint32_t*>(smem + L::VALID);
+            volatile uint32_t* cta_abort = reinterpret_cast<uint32_t*>(smem + L::ABORT);
+            if(tid == 0)
+            {
+                ptx::prefetch_tensormap(&map_k);
+                ptx::prefetch_tensormap(&map_v);
+                for(uint32_t s = 0; s < STAGES; ++s)
+                {
+                    ptx::mbar_init(base + L::BARS + 16 * s, 1); // full
+                    ptx::mbar_init(base + L::BARS + 16 * s + 8, 4); // empty
+                }
+                *cta_abort = 0u;
+                ptx::fence_barrier_init();
+                ptx::fence_proxy_async_smem();
+            }
 
             uint32_t       x     = blockIdx.x;
             const uint32_t split = x % p.splits;
@@ -140,62 +164,88 @@ namespace b200wmma
                                            : 0u;
                 }
 
-            // where the tokens of step i are, for the copies of the step after the next barrier
-            const auto look_up = [&](uint32_t i) {
-                if(tid < KEYS)
-                {
-                    const uint32_t j = (from + i) * KEYS + tid;
-                    int2           e = make_int2(-1, 0);
-                    if(i < steps && j < end)
+            __syncthreads();
+            bool ok = true;
+            if(warp == 4)
+            {
+                const uint32_t boxes = KEYS / p.box; // a lane takes boxes lane, lane + 32
+                int32_t        page[2], slot[2];
+                const auto     ask = [&](uint32_t i) { // starts the loads of the pages of step i
+#pragma unroll
+                    for(int u = 0; u < 2; ++u)
                     {
-                        const uint32_t n = j / p.page_size;
-                        e                = make_int2(__ldg(p.block_table + size_t(b) * p.ld_table + n), int32_t(j - n * p.page_size));
-                        if(uint32_t(e.x) >= p.num_pages)
-                            e.x = -1;
+                        const uint32_t at_box = lane + 32 * u, j = (from + i) * KEYS + at_box * p.box;
+                        page[u] = -1, slot[u] = 0;
+                        if(at_box < boxes && i < steps && j < end)
+                        {
+                            const uint32_t n = p.page_shift < 32 ? j >> p.page_shift : j / p.page_size;
+                            slot[u]          = int32_t(j - n * p.page_size);
+                            page[u]          = __ldg(p.block_table + size_t(b) * p.ld_table + n);
+                        }
                     }
-                    table[(i & 1u) * KEYS + tid] = e;
-                    const uint32_t there = __ballot_sync(0xFFFFFFFFu, e.x >= 0);
-                    if(lane == 0)
-                        valid[2 * (i % (STAGES + 1)) + warp] = there;
-                }
-            };
-            const auto fetch = [&](uint32_t i) {
-                const uint32_t stage = base + (i % STAGES) * 2 * L::TILE, c = tid % CHUNKS;
-                const T *      kh = k + int64_t(head) * p.k.head, *vh = v + int64_t(head) * p.v.head;
-#pragma unroll 4
-                for(uint32_t key = tid / CHUNKS; key < KEYS; key += THREADS / CHUNKS)
+                };
+                ask(0);
+                for(uint32_t i = 0; i < steps; ++i)
                 {
-                    const int2     e     = table[(i & 1u) * KEYS + key];
-                    const bool     there = e.x >= 0 && c * 8 < p.dim;
-                    const uint32_t to    = stage + key * L::ROW + ((c ^ (key & 7u)) << 4);
-                    copy16(to, there ? kh + int64_t(e.x) * p.k.batch + int64_t(e.y) * p.k.token + c * 8 : k, there);
-                    copy16(to + L::TILE, there ? vh + int64_t(e.x) * p.v.batch + int64_t(e.y) * p.v.token + c * 8 : v, there);
+                    const uint32_t st = i % STAGES, full = base + L::BARS + 16 * st, stage = base + st * 2 * L::TILE;
+                    const int32_t  pg[2] = {page[0], page[1]}, sl[2] = {slot[0], slot[1]};
+                    ask(i + 1);
+                    ok = ptx::mbar_wait_bounded_warp(full + 8, (i / STAGES & 1u) ^ 1u, cta_abort, p.status,
+                                                     TREE_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    if(!ok)
+                        break;
+                    // which of the 64 tokens are there: their box's page is, and they lie before the end
+                    const uint64_t box_bits = p.box < 64 ? (uint64_t(1) << p.box) - 1 : ~uint64_t(0);
+                    uint64_t       there    = 0;
+#pragma unroll
+                    for(int u = 0; u < 2; ++u)
+                        if(uint32_t(pg[u]) < p.num_pages && lane + 32 * u < boxes)
+                            there |= box_bits << ((lane + 32 * u) * p.box);
+                    const uint32_t left = end - (from + i) * KEYS;
+                    uint32_t       lo = __reduce_or_sync(0xFFFFFFFFu, uint32_t(there)), hi = __reduce_or_sync(0xFFFFFFFFu, uint32_t(there >> 32));
+                    if(left < 64)
+                    {
+                        lo &= left < 32 ? (1u << left) - 1u : 0xFFFFFFFFu;
+                        hi &= left <= 32 ? 0u : (1u << (left - 32)) - 1u;
+                    }
+                    if(lane == 0)
+                    {
+                        valid[2 * st] = lo, valid[2 * st + 1] = hi;
+                        ptx::mbar_arrive_expect_tx(full, 2 * L::TILE);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for(int u = 0; u < 2; ++u)
+                    {
+                        const uint32_t at_box = lane + 32 * u;
+                        if(at_box < boxes)
+                        {
+                            // a page that is not there: one behind the last, which reads as zeros
+                            const int32_t c3 = uint32_t(pg[u]) < p.num_pages ? pg[u] : int32_t(p.num_pages);
+#pragma unroll
+                            for(uint32_t h = 0; h < HD / 64; ++h)
+                            {
+                                const uint32_t to = stage + h * L::HALF + at_box * p.box * 128;
+                                attn::tma_load_4d(to, &map_k, h * 64, sl[u], head, c3, full);
+                                attn::tma_load_4d(to + L::TILE, &map_v, h * 64, sl[u], head, c3, full);
+                            }
+                        }
+                    }
                 }
-            };
+            }
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, acc[HD / 8][4];
 #pragma unroll
             for(uint32_t i = 0; i < HD / 8; ++i)
                 acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
 
-#pragma unroll
-            for(uint32_t i = 0; i < STAGES - 1; ++i)
+            for(uint32_t i = 0; warp < 4 && i < steps; ++i)
             {
-                look_up(i);
-                __syncthreads();
-                if(i < steps)
-                    fetch(i);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-            look_up(STAGES - 1);
-            for(uint32_t i = 0; i < steps; ++i)
-            {
-                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-                __syncthreads(); // the stage is there for everyone, as is the table; the stage that is fetched into has been read
-                if(i + STAGES - 1 < steps)
-                    fetch(i + STAGES - 1);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-
-                const uint32_t keys_at = base + (i % STAGES) * 2 * L::TILE + wn * MINE * L::ROW, values_at = keys_at + L::TILE;
+                const uint32_t st = i % STAGES;
+                ok = ptx::mbar_wait_bounded_warp(base + L::BARS + 16 * st, i / STAGES & 1u, cta_abort, p.status,
+                                                 TREE_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                if(!ok)
+                    break;
+                const uint32_t keys_at = base + st * 2 * L::TILE + wn * MINE * 128, values_at = keys_at + L::TILE;
                 float          s[MINE / 8][4];
 #pragma unroll
                 for(uint32_t n = 0; n < MINE / 8; ++n)
@@ -207,14 +257,14 @@ namespace b200wmma
                     for(uint32_t c = 0; c < HD / 32; ++c)
                     {
                         uint32_t f[4];
-                        ldmatrix4(f, keys_at + key * L::ROW + (((c * 4 + piece) ^ (key & 7u)) << 4));
+                        ldmatrix4(f, keys_at + (c / 2) * L::HALF + key * 128 + ((((c % 2) * 4 + piece) ^ (key & 7u)) << 4));
                         mma<T>(s[n], qf[2 * c], f[0], f[1]);
                         mma<T>(s[n], qf[2 * c + 1], f[2], f[3]);
                     }
                 }
                 // scores in units of log 2, masked
                 const uint32_t j0 = (from + i) * KEYS + wn * MINE;
-                const uint32_t v0 = valid[2 * (i % (STAGES + 1))], v1 = valid[2 * (i % (STAGES + 1)) + 1];
+                const uint32_t v0 = valid[2 * st], v1 = valid[2 * st + 1];
                 const bool     masked = (v0 & v1) != 0xFFFFFFFFu || (from + i + 1) * KEYS > len;
                 const uint64_t there  = (uint64_t(v1) << 32 | v0) >> (wn * MINE);
                 float          top[2] = {-INFINITY, -INFINITY};
@@ -275,6 +325,17 @@ namespace b200wmma
                     l[0] += w[0] + w[1], l[1] += w[2] + w[3];
                     pf[n / 2][2 * (n & 1)] = attn::pack2<T>(w[0], w[1]), pf[n / 2][2 * (n & 1) + 1] = attn::pack2<T>(w[2], w[3]);
                 }
+                // rows behind the last token hold anything; only the last step has them, whose stage is not filled again
+                if((from + i + 1) * KEYS > end)
+                {
+                    for(uint32_t e = lane; e < MINE * (HD / 8); e += 32)
+                    {
+                        const uint32_t key = e / (HD / 8), c = e % (HD / 8);
+                        if(j0 + key >= end)
+                            *reinterpret_cast<uint4*>(smem + (values_at - base) + (c / 8) * L::HALF + key * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
 #pragma unroll
                 for(uint32_t n = 0; n < MINE / 16; ++n)
                 {
@@ -284,14 +345,15 @@ namespace b200wmma
                     for(uint32_t c = 0; c < HD / 16; ++c)
                     {
                         uint32_t f[4];
-                        ldmatrix4_trans(f, values_at + key * L::ROW + (((c * 2 + (lane >> 4)) ^ (key & 7u)) << 4));
+                        ldmatrix4_trans(f, values_at + (c / 4) * L::HALF + key * 128 + ((((c % 4) * 2 + (lane >> 4)) ^ (key & 7u)) << 4));
                         mma<T>(acc[2 * c], pf[n], f[0], f[1]);
                         mma<T>(acc[2 * c + 1], pf[n], f[2], f[3]);
                     }
                 }
-                look_up(i + STAGES); // into the half of the table that the copies above have left
+                __syncwarp();
+                if(lane == 0)
+                    ptx::mbar_arrive(base + L::BARS + 16 * st + 8);
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
             for(int h = 0; h < 2; ++h)
             {
@@ -300,16 +362,27 @@ namespace b200wmma
             }
             // join the warps that share the rows: [warp][16 rows][HD] sums, [warp][16 rows] maximum and sum of weights
             __syncthreads();
+            if(*cta_abort)
+            {
+                // A wait was abandoned: copies may still be in flight.  Give them a bounded grace period, then leave.
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while(ptx::globaltimer_ns() - t0 < 2000000ull)
+                    __nanosleep(1000);
+                return;
+            }
             float *sums = reinterpret_cast<float*>(smem), *stats = sums + 4 * 16 * HD;
+            if(warp < 4)
+            {
 #pragma unroll
-            for(uint32_t c = 0; c < HD / 8; ++c)
+                for(uint32_t c = 0; c < HD / 8; ++c)
 #pragma unroll
-                for(int h = 0; h < 2; ++h)
-                    *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8 * h) * HD + c * 8 + t * 2) = make_float2(acc[c][2 * h], acc[c][2 * h + 1]);
-            if(t == 0)
+                    for(int h = 0; h < 2; ++h)
+                        *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8 * h) * HD + c * 8 + t * 2) = make_float2(acc[c][2 * h], acc[c][2 * h + 1]);
+                if(t == 0)
 #pragma unroll
-                for(int h = 0; h < 2; ++h)
-                    stats[(warp * 16 + g + 8 * h) * 2] = m[h], stats[(warp * 16 + g + 8 * h) * 2 + 1] = l[h];
+                    for(int h = 0; h < 2; ++h)
+                        stats[(warp * 16 + g + 8 * h) * 2] = m[h], stats[(warp * 16 + g + 8 * h) * 2 + 1] = l[h];
+            }
             __syncthreads();
             // four elements of a row to a thread
             for(uint32_t e = tid; e < 16 * WM * (HD / 4); e += THREADS)
@@ -351,46 +424,71 @@ namespace b200wmma
             ptx::grid_dep_launch_dependents();
         }
 
-        // Joins the splits: one warp to a row, four (HD = 128) or two elements to a lane, splits in order.
+        // Joins the splits: a block to a row.  The splits' maxima and sums become weights in shared memory, then four warps add
+        // up a quarter of the splits each, four (HD = 128) or two elements to a lane; all in a fixed order.
         template <typename T, uint32_t HD>
         __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, T* __restrict__ o)
         {
             constexpr uint32_t E = HD / 32;
+            __shared__ float   by[MAX_SPLITS], red[4][HD], top[4], total[4];
             ptx::grid_dep_wait();
-            const uint32_t rows = p.share * p.drafts, row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+            const uint32_t rows = p.share * p.drafts, row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
             const uint32_t all_rows = p.batch * p.heads_kv * rows;
-            if(row >= all_rows)
-                return;
             const uint32_t r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
             if(draft >= drafts_of(p, b))
                 return;
-            float mx = -INFINITY;
-            for(uint32_t s = lane; s < p.splits; s += 32)
-                mx = fmaxf(mx, p.part_ml[(size_t(s) * all_rows + row) * 2]);
+            static_assert(MAX_SPLITS == 256, "two splits to a thread");
+            float2 ml[2];
+            float  mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for(int i = 0; i < 2; ++i)
+            {
+                const uint32_t s = threadIdx.x + 128 * i;
+                ml[i] = s < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (size_t(s) * all_rows + row) * 2) : make_float2(-INFINITY, 0.0f);
+                mx    = fmaxf(mx, ml[i].x);
+            }
 #pragma unroll
             for(int d = 16; d > 0; d >>= 1)
                 mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-            float sum = 0.0f, y[E] = {};
-            if(mx != -INFINITY)
-                for(uint32_t s = 0; s < p.splits; ++s)
+            if(lane == 0)
+                top[warp] = mx;
+            __syncthreads();
+            mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+#pragma unroll
+            for(int i = 0; i < 2; ++i)
+            {
+                const float w = ml[i].x == -INFINITY ? 0.0f : ex2(ml[i].x - mx);
+                by[threadIdx.x + 128 * i] = w;
+                sum = ml[i].x == -INFINITY ? sum : fmaf(w, ml[i].y, sum);
+            }
+#pragma unroll
+            for(int d = 16; d > 0; d >>= 1)
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            if(lane == 0)
+                total[warp] = sum;
+            __syncthreads();
+            float y[E] = {};
+#pragma unroll 8
+            for(uint32_t s = warp; s < p.splits; s += 4)
+                if(by[s] != 0.0f) // NaN counts; splits without a visible token have written no sums
                 {
-                    const size_t part = size_t(s) * all_rows + row;
-                    const float2 ml   = *reinterpret_cast<const float2*>(p.part_ml + part * 2);
-                    if(ml.x == -INFINITY)
-                        continue;
-                    const float by = ex2(ml.x - mx);
-                    sum += by * ml.y;
+                    const float* from = p.part_o + (size_t(s) * all_rows + row) * HD + lane * E;
 #pragma unroll
                     for(uint32_t e = 0; e < E; ++e)
-                        y[e] = fmaf(by, p.part_o[part * HD + lane * E + e], y[e]);
+                        y[e] = fmaf(by[s], from[e], y[e]);
                 }
-            const float inv = sum > 0.0f ? 1.0f / sum : sum;
-            if(lane * E < p.dim)
-            {
-                uint32_t* out = reinterpret_cast<uint32_t*>(o + row_of(p.o, b, draft, head * p.share + r % p.share) + lane * E);
 #pragma unroll
-                for(uint32_t e = 0; e < E; e += 2)
-                    out[e / 2] = attn::pack2<T>(y[e] * inv, y[e + 1] * inv);
+            for(uint32_t e = 0; e < E; ++e)
+                red[warp][lane * E + e] = y[e];
+            __syncthreads();
+            sum             = (total[0] + total[1]) + (total[2] + total[3]);
+            const float inv = sum > 0.0f ? 1.0f / sum : sum;
+            const uint32_t d = threadIdx.x * 2;
+            if(d < p.dim)
+            {
+                const float u = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+                const float v = (red[0][d + 1] + red[1][d + 1]) + (red[2][d + 1] + red[3][d + 1]);
+                *reinterpret_cast<uint32_t*>(o + row_of(p.o, b, draft, head * p.share + r % p.share) + d) = attn::pack2<T>(u * inv, v * inv);
             }
         }
 
@@ -399,12 +497,16 @@ namespace b200wmma
         {
             return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
         }
+#ifndef SPLIT_STAGES
+#define SPLIT_STAGES 4
+#define SPLIT_BLOCKS (2 * 148)
+#endif
         // Splits of the tokens: enough blocks for two to four rounds of two per SM, but at least 8 stages (512 tokens) to a
         // block if a sequence is as long as its table allows.
         static uint32_t splits_of(uint32_t batch, uint32_t heads_kv, uint32_t rows, uint32_t max_tokens)
         {
             const uint64_t blocks = uint64_t(batch) * heads_kv * ceil_div(rows, 16 * rows_of_block(rows));
-            const uint64_t want = (4 * 148 + blocks - 1) / blocks, most = (uint64_t(max_tokens) + 8 * KEYS - 1) / (8 * KEYS);
+            const uint64_t want = (SPLIT_BLOCKS + blocks - 1) / blocks, most = (uint64_t(max_tokens) + SPLIT_STAGES * KEYS - 1) / (SPLIT_STAGES * KEYS);
             const uint64_t n = want < most ? want : most;
             return n < 1 ? 1u : n > MAX_SPLITS ? MAX_SPLITS : uint32_t(n);
         }
@@ -414,17 +516,17 @@ namespace b200wmma
         }
 
         template <typename T, uint32_t HD, uint32_t WM, bool CAP, bool BIAS>
-        static int launch(const Params& p, const void* q, const void* k, const void* v, void* o, cudaStream_t stream)
+        static int launch(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
             auto kern = tree_kernel<T, HD, WM, CAP, BIAS>;
             B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::BYTES));
-            kern<<<p.batch * p.heads_kv * p.tiles * p.splits, THREADS, Smem<HD>::BYTES, stream>>>(p, static_cast<const T*>(q), static_cast<const T*>(k),
-                                                                                             static_cast<const T*>(v), static_cast<T*>(o));
+            kern<<<p.batch * p.heads_kv * p.tiles * p.splits, THREADS, Smem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q),
+                                                                                             static_cast<T*>(o));
             B200_CHECK_CUDA(cudaGetLastError());
             if(p.splits > 1)
             {
                 cudaLaunchConfig_t cfg{};
-                cfg.gridDim = dim3(ceil_div(p.batch * p.heads_kv * p.share * p.drafts, 4)), cfg.blockDim = dim3(128), cfg.stream = stream;
+                cfg.gridDim = dim3(p.batch * p.heads_kv * p.share * p.drafts), cfg.blockDim = dim3(128), cfg.stream = stream;
                 cudaLaunchAttribute attr{};
                 attr.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
                 attr.val.programmaticStreamSerializationAllowed = 1;
@@ -434,23 +536,23 @@ namespace b200wmma
             return B200WMMA_OK;
         }
         template <typename T, uint32_t HD, uint32_t WM>
-        static int launch_scores(const Params& p, const void* q, const void* k, const void* v, void* o, cudaStream_t stream)
+        static int launch_scores(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
             if(p.cap > 0.0f)
-                return p.slopes ? launch<T, HD, WM, true, true>(p, q, k, v, o, stream) : launch<T, HD, WM, true, false>(p, q, k, v, o, stream);
-            return p.slopes ? launch<T, HD, WM, false, true>(p, q, k, v, o, stream) : launch<T, HD, WM, false, false>(p, q, k, v, o, stream);
+                return p.slopes ? launch<T, HD, WM, true, true>(p, maps, q, o, stream) : launch<T, HD, WM, true, false>(p, maps, q, o, stream);
+            return p.slopes ? launch<T, HD, WM, false, true>(p, maps, q, o, stream) : launch<T, HD, WM, false, false>(p, maps, q, o, stream);
         }
         template <typename T, uint32_t HD>
-        static int launch_rows(const Params& p, const void* q, const void* k, const void* v, void* o, cudaStream_t stream)
+        static int launch_rows(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
             const uint32_t wm = rows_of_block(p.share * p.drafts);
-            return wm == 1   ? launch_scores<T, HD, 1>(p, q, k, v, o, stream)
-                   : wm == 2 ? launch_scores<T, HD, 2>(p, q, k, v, o, stream) : launch_scores<T, HD, 4>(p, q, k, v, o, stream);
+            return wm == 1   ? launch_scores<T, HD, 1>(p, maps, q, o, stream)
+                   : wm == 2 ? launch_scores<T, HD, 2>(p, maps, q, o, stream) : launch_scores<T, HD, 4>(p, maps, q, o, stream);
         }
         template <typename T>
-        static int launch_dim(const Params& p, const void* q, const void* k, const void* v, void* o, cudaStream_t stream)
+        static int launch_dim(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
-            return p.dim <= 64 ? launch_rows<T, 64>(p, q, k, v, o, stream) : launch_rows<T, 128>(p, q, k, v, o, stream);
+            return p.dim <= 64 ? launch_rows<T, 64>(p, maps, q, o, stream) : launch_rows<T, 128>(p, maps, q, o, stream);
         }
     } // namespace attn_tree
 } // namespace b200wmma
@@ -503,6 +605,10 @@ extern "C" int b200wmma_attn_tree(const b200wmma_attn_args* a, uint32_t drafts, 
     if(int e = require_sm100())
         return e;
     p.batch = a->batch, p.heads_q = a->heads_q, p.heads_kv = a->heads_kv, p.share = a->heads_q / a->heads_kv, p.dim = a->head_dim;
+    p.page_shift = 32;
+    for(uint32_t i = 0; i < 32; ++i)
+        if(page_size == 1u << i)
+            p.page_shift = i;
     p.drafts = drafts, p.num_pages = num_pages, p.page_size = page_size, p.ld_table = ld_table, p.scale = a->scale, p.cap = a->cap;
     p.slopes = a->slopes, p.block_table = block_table, p.lens = lens, p.n_drafts = n_drafts, p.depths = depths, p.tree = tree;
     const uint32_t rows = p.share * drafts;
@@ -510,6 +616,16 @@ extern "C" int b200wmma_attn_tree(const b200wmma_attn_args* a, uint32_t drafts, 
     p.tiles   = ceil_div(rows, 16 * attn_tree::rows_of_block(rows));
     p.part_o  = static_cast<float*>(workspace);
     p.part_ml = p.part_o + size_t(p.splits) * p.batch * p.heads_kv * rows * attn_tree::padded_dim(p.dim);
-    return a->data_type == B200WMMA_OUT_F16 ? attn_tree::launch_dim<__half>(p, q, k_cache, v_cache, o, as_stream(stream))
-                                            : attn_tree::launch_dim<__nv_bfloat16>(p, q, k_cache, v_cache, o, as_stream(stream));
+    p.box = 64;
+    while(page_size % p.box != 0)
+        p.box /= 2;
+    if(int e = status_word_ptr(&p.status))
+        return e;
+    CUtensorMap maps[2];
+    if(int e = attn::make_map(&maps[0], a->data_type, k_cache, p.dim, page_size, p.heads_kv, num_pages, p.k, p.box))
+        return e;
+    if(int e = attn::make_map(&maps[1], a->data_type, v_cache, p.dim, page_size, p.heads_kv, num_pages, p.v, p.box))
+        return e;
+    return a->data_type == B200WMMA_OUT_F16 ? attn_tree::launch_dim<__half>(p, maps, q, o, as_stream(stream))
+                                            : attn_tree::launch_dim<__nv_bfloat16>(p, maps, q, o, as_stream(stream));
 }
