@@ -100,6 +100,7 @@ namespace b200wmma
             for(uint32_t c = 0; c < HD; c += 32)
             {
                 uint32_t w[32];
+                __syncwarp();
                 ptx::tmem_ld_32x32b_x32(taddr + c, w);
                 ptx::tmem_ld_wait();
                 if(mine)

@@ -365,6 +365,7 @@ namespace b200wmma
                     for(uint32_t c = 0; c < HD; c += 32)
                     {
                         uint32_t w[32];
+                        __syncwarp();
                         if(have)
                         {
                             ptx::tmem_ld_32x32b_x32(o_tmem[t] + ((quad * 32u) << 16) + c, w);

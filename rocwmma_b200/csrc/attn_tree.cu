@@ -65,11 +65,29 @@ namespace b200wmma
         {
             return p.n_drafts ? min(uint32_t(max(__ldg(p.n_drafts + b), 0)), p.drafts) : p.drafts;
         }
+        // Bit i: a row whose tree word is `bits` sees the token that stands `rel` + i behind the cached ones (before them: rel < 0).
+        __device__ __forceinline__ uint32_t seen_of(uint64_t bits, int32_t rel)
+        {
+            if(rel >= 64)
+                return 0;
+            if(rel >= 0)
+                return uint32_t(bits >> rel);
+            return rel <= -32 ? 0xFFFFFFFFu : uint32_t(bits << -rel) | ((1u << -rel) - 1u);
+        }
         __device__ __forceinline__ int64_t row_of(const attn::Strides& s, uint32_t b, uint32_t t, uint32_t h)
         {
             return int64_t(b) * s.batch + int64_t(t) * s.token + int64_t(h) * s.head;
         }
 
+    } // namespace attn_tree
+} // namespace b200wmma
+
+#include "attn_tree_tc05.cuh"
+
+namespace b200wmma
+{
+    namespace attn_tree
+    {
         enum Role : uint32_t
         {
             TREE_PRODUCER = 0x61,
@@ -266,31 +284,52 @@ namespace b200wmma
                 const uint32_t j0 = (from + i) * KEYS + wn * MINE;
                 const uint32_t v0 = valid[2 * st], v1 = valid[2 * st + 1];
                 const bool     masked = (v0 & v1) != 0xFFFFFFFFu || (from + i + 1) * KEYS > len;
-                const uint64_t there  = (uint64_t(v1) << 32 | v0) >> (wn * MINE);
+                const int32_t  rel0   = int32_t(int64_t(j0) - len); // place of the warp's first token behind the cached ones
                 float          top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for(uint32_t n = 0; n < MINE / 8; ++n)
-#pragma unroll
-                    for(int e = 0; e < 4; ++e)
+                const auto     scores = [&](auto mask) {
+                    constexpr bool MASK = decltype(mask)::value;
+                    uint32_t       see[2][(MINE + 31) / 32]; // of this lane's first token on
+                    if constexpr(MASK)
                     {
-                        const uint32_t off = n * 8 + t * 2 + (e & 1), j = j0 + off;
-                        const int32_t  rel = int32_t(int64_t(j) - len); // place behind the cached tokens
-                        float          dist = 0.0f, unused;
-                        if constexpr(BIAS)
+#pragma unroll
+                        for(uint32_t w = 0; w < (MINE + 31) / 32; ++w)
                         {
-                            int32_t where = rel;
-                            if(rel >= 0 && p.depths && j < end)
-                                where = __ldg(p.depths + size_t(b) * p.drafts + rel);
-                            dist = static_cast<float>(at[e >> 1] - where);
+                            const uint32_t bit = wn * MINE + 32 * w, there = (bit < 32 ? v0 : v1) >> (bit & 31u);
+                            see[0][w] = (there & seen_of(bits[0], rel0 + int32_t(32 * w))) >> (t * 2);
+                            see[1][w] = (there & seen_of(bits[1], rel0 + int32_t(32 * w))) >> (t * 2);
                         }
-                        sc.slope = slope[e >> 1];
-                        float y  = attn::score<CAP, BIAS>(sc, s[n][e], dist, unused);
-                        if(masked)
-                            if(!(there >> off & 1u) || (rel >= 0 && !(bits[e >> 1] >> (rel & 63) & 1u)))
-                                y = -INFINITY;
-                        s[n][e]     = y;
-                        top[e >> 1] = fmaxf(top[e >> 1], y);
                     }
+#pragma unroll
+                    for(uint32_t n = 0; n < MINE / 8; ++n)
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            const uint32_t off = n * 8 + (e & 1); // and t * 2
+                            const int      h   = e >> 1;
+                            float          dist = 0.0f, unused;
+                            if constexpr(BIAS)
+                            {
+                                dist = static_cast<float>(at[h] - rel0 - int32_t(t * 2)) - static_cast<float>(off);
+                                if constexpr(MASK)
+                                {
+                                    const int32_t rel = rel0 + int32_t(off + t * 2);
+                                    if(rel >= 0 && p.depths && j0 + off + t * 2 < end)
+                                        dist = static_cast<float>(at[h] - __ldg(p.depths + size_t(b) * p.drafts + rel));
+                                }
+                            }
+                            sc.slope = slope[h];
+                            float y  = attn::score<CAP, BIAS>(sc, s[n][e], dist, unused);
+                            if constexpr(MASK)
+                                if(!(see[h][off / 32] >> (off & 31u) & 1u))
+                                    y = -INFINITY;
+                            s[n][e] = y;
+                            top[h]  = fmaxf(top[h], y);
+                        }
+                };
+                if(masked)
+                    scores(std::true_type{});
+                else
+                    scores(std::false_type{});
 #pragma unroll
                 for(int h = 0; h < 2; ++h)
                 {
@@ -492,21 +531,29 @@ namespace b200wmma
             }
         }
 
-        // Rows of a block in units of 16: 1, 2 or 4.
-        static uint32_t rows_of_block(uint32_t rows)
-        {
-            return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-        }
-#ifndef SPLIT_STAGES
+#ifndef TC_ROWS
+#define TC_ROWS 16
 #define SPLIT_STAGES 4
 #define SPLIT_BLOCKS (2 * 148)
+#define TC_STAGES 2
+#define TC_BLOCKS 148
 #endif
-        // Splits of the tokens: enough blocks for two to four rounds of two per SM, but at least 8 stages (512 tokens) to a
-        // block if a sequence is as long as its table allows.
+        // More rows than this take the tcgen05 form.
+        static bool many_rows(uint32_t rows)
+        {
+            return rows > TC_ROWS;
+        }
+        static uint32_t rows_of_block(uint32_t rows)
+        {
+            return many_rows(rows) ? TILE : rows <= 16 ? 16 : 32;
+        }
+        // Splits of the tokens: a round of blocks over the machine, but at least 256 tokens to a block if a sequence is as long
+        // as its table allows.
         static uint32_t splits_of(uint32_t batch, uint32_t heads_kv, uint32_t rows, uint32_t max_tokens)
         {
-            const uint64_t blocks = uint64_t(batch) * heads_kv * ceil_div(rows, 16 * rows_of_block(rows));
-            const uint64_t want = (SPLIT_BLOCKS + blocks - 1) / blocks, most = (uint64_t(max_tokens) + SPLIT_STAGES * KEYS - 1) / (SPLIT_STAGES * KEYS);
+            const uint64_t blocks = uint64_t(batch) * heads_kv * ceil_div(rows, rows_of_block(rows));
+            const uint64_t slots = many_rows(rows) ? TC_BLOCKS : SPLIT_BLOCKS, least = many_rows(rows) ? TC_STAGES * TILE : SPLIT_STAGES * KEYS;
+            const uint64_t want = slots / blocks, most = (uint64_t(max_tokens) + least - 1) / least;
             const uint64_t n = want < most ? want : most;
             return n < 1 ? 1u : n > MAX_SPLITS ? MAX_SPLITS : uint32_t(n);
         }
@@ -515,13 +562,23 @@ namespace b200wmma
             return dim <= 64 ? 64 : 128;
         }
 
+        // WM: rows of a block of the warp-level kernel in units of 16; 0: the tcgen05 kernel
         template <typename T, uint32_t HD, uint32_t WM, bool CAP, bool BIAS>
         static int launch(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
-            auto kern = tree_kernel<T, HD, WM, CAP, BIAS>;
-            B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::BYTES));
-            kern<<<p.batch * p.heads_kv * p.tiles * p.splits, THREADS, Smem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q),
-                                                                                             static_cast<T*>(o));
+            const uint32_t grid = p.batch * p.heads_kv * p.tiles * p.splits;
+            if constexpr(WM == 0)
+            {
+                auto kern = tree_tc05_kernel<T, HD, CAP, BIAS>;
+                B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<HD>::BYTES));
+                kern<<<grid, TC_THREADS, TcSmem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q), static_cast<T*>(o));
+            }
+            else
+            {
+                auto kern = tree_kernel<T, HD, WM, CAP, BIAS>;
+                B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::BYTES));
+                kern<<<grid, THREADS, Smem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q), static_cast<T*>(o));
+            }
             B200_CHECK_CUDA(cudaGetLastError());
             if(p.splits > 1)
             {
@@ -545,9 +602,9 @@ namespace b200wmma
         template <typename T, uint32_t HD>
         static int launch_rows(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
-            const uint32_t wm = rows_of_block(p.share * p.drafts);
-            return wm == 1   ? launch_scores<T, HD, 1>(p, maps, q, o, stream)
-                   : wm == 2 ? launch_scores<T, HD, 2>(p, maps, q, o, stream) : launch_scores<T, HD, 4>(p, maps, q, o, stream);
+            const uint32_t rows = p.share * p.drafts;
+            return many_rows(rows) ? launch_scores<T, HD, 0>(p, maps, q, o, stream)
+                   : rows <= 16    ? launch_scores<T, HD, 1>(p, maps, q, o, stream) : launch_scores<T, HD, 2>(p, maps, q, o, stream);
         }
         template <typename T>
         static int launch_dim(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
@@ -613,7 +670,7 @@ extern "C" int b200wmma_attn_tree(const b200wmma_attn_args* a, uint32_t drafts, 
     p.slopes = a->slopes, p.block_table = block_table, p.lens = lens, p.n_drafts = n_drafts, p.depths = depths, p.tree = tree;
     const uint32_t rows = p.share * drafts;
     p.splits  = attn_tree::splits_of(p.batch, p.heads_kv, rows, max_tokens);
-    p.tiles   = ceil_div(rows, 16 * attn_tree::rows_of_block(rows));
+    p.tiles   = ceil_div(rows, attn_tree::rows_of_block(rows));
     p.part_o  = static_cast<float*>(workspace);
     p.part_ml = p.part_o + size_t(p.splits) * p.batch * p.heads_kv * rows * attn_tree::padded_dim(p.dim);
     p.box = 64;
