@@ -238,8 +238,8 @@ namespace b200wmma
                     // ------------------------------- MMA issuer -------------------------------
                     const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
                         ok = ok
-                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status,
-                                                            DKV_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                             && wait_bounded_warp(bar, parity, cta_abort, status,
+                                                            DKV_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu));
                         ptx::tc_fence_after_sync();
                         return ok;
                     };
@@ -318,15 +318,15 @@ namespace b200wmma
                     {
                         const uint32_t e = list[n % entries], r0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
                         const auto     wait = [&](uint32_t bar, uint32_t what) {
-                            ok = ptx::mbar_wait_bounded_warp(bar, it & 1u, cta_abort, status,
-                                                                 DKV_COMPUTE << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                            ok = wait_bounded_warp(bar, it & 1u, cta_abort, status,
+                                                                 DKV_COMPUTE << 24 | what << 20 | (blockIdx.x & 0xFFFFFu));
                             ptx::tc_fence_after_sync();
                             return ok;
                         };
                         const ScoreConst sc = score_const(p, g * share + n / entries);
                         // the statistics came with the tiles: an acquire of the same barriers
-                        ok = ptx::mbar_wait_bounded_warp(base + L::FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
-                                                         DKV_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        ok = wait_bounded_warp(base + L::FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
+                                                         DKV_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                         if(!ok || !wait(base + L::S_FULL, 0))
                             break;
                         uint32_t v[2][32];
@@ -436,8 +436,7 @@ namespace b200wmma
             if(warp < 8)
             {
                 if(ok)
-                    ok = ptx::mbar_wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DKV_COMPUTE << 24 | 4u << 20 | (blockIdx.x & 0xFFFFFu),
-                                                     tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DKV_COMPUTE << 24 | 4u << 20 | (blockIdx.x & 0xFFFFFu));
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
@@ -575,8 +574,7 @@ namespace b200wmma
                 {
                     const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
                         ok = ok
-                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status, DQ_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu),
-                                                            tc05::WAIT_TIMEOUT_NS, lane);
+                             && wait_bounded_warp(bar, parity, cta_abort, status, DQ_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu));
                         ptx::tc_fence_after_sync();
                         return ok;
                     };
@@ -633,8 +631,7 @@ namespace b200wmma
                     for(uint32_t n = 0; ok && n < entries; ++n, ++it)
                     {
                         const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
-                        ok = ptx::mbar_wait_bounded_warp(base + L::S_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu),
-                                                         tc05::WAIT_TIMEOUT_NS, lane);
+                        ok = wait_bounded_warp(base + L::S_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
@@ -681,8 +678,8 @@ namespace b200wmma
                             weights(std::true_type{});
                         else
                             weights(std::false_type{});
-                        ok = ptx::mbar_wait_bounded_warp(base + L::DP_FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
-                                                         DQ_COMPUTE << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        ok = wait_bounded_warp(base + L::DP_FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
+                                                         DQ_COMPUTE << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
@@ -723,8 +720,7 @@ namespace b200wmma
             if(warp < 4)
             {
                 if(ok)
-                    ok = ptx::mbar_wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu),
-                                                     tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();

@@ -161,8 +161,8 @@ namespace b200wmma
                     // The whole warp waits (rows of padding are cleared by all lanes); lane 0 issues.
                     const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
                         ok = ok
-                             && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, status,
-                                                            FWD_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                             && wait_bounded_warp(bar, parity, cta_abort, status,
+                                                            FWD_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu));
                         ptx::tc_fence_after_sync();
                         return ok;
                     };
@@ -243,8 +243,8 @@ namespace b200wmma
                         if(!(f & TILE_NEED))
                             continue;
                         const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
-                        ok = ptx::mbar_wait_bounded_warp(base + L::S_FULL + 8 * t, n_s & 1u, cta_abort, status,
-                                                         FWD_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                        ok = wait_bounded_warp(base + L::S_FULL + 8 * t, n_s & 1u, cta_abort, status,
+                                                         FWD_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
@@ -300,9 +300,8 @@ namespace b200wmma
                             m = m2;
                             if(n_s != 0)
                             {
-                                ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
-                                                                 FWD_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu),
-                                                                 tc05::WAIT_TIMEOUT_NS, lane);
+                                ok = wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
+                                                                 FWD_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
                                 if(!ok)
                                     break;
                                 ptx::tc_fence_after_sync();
@@ -353,8 +352,8 @@ namespace b200wmma
                 bool have = n_s != 0;
                 if(have && ok)
                 {
-                    ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
-                                                     FWD_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
+                                                     FWD_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                     ptx::tc_fence_after_sync();
                 }
                 if(ok)

@@ -82,6 +82,34 @@ namespace b200wmma
             return tc05::Pack16<T>::narrow(lo, hi);
         }
 
+        // Bounded wait of a whole warp on the critical path: every lane polls (one instruction for all of them) instead of being
+        // parked until the barrier's completion wakes it, which takes longer than these waits last.
+        __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile uint32_t* cta_abort, unsigned* status, uint32_t who)
+        {
+            if(ptx::mbar_try_wait(bar, parity))
+                return true;
+            const uint64_t t0    = ptx::globaltimer_ns();
+            uint32_t       spins = 0;
+            while(!ptx::mbar_try_wait(bar, parity))
+                if((++spins & 63u) == 0u)
+                {
+                    if(*cta_abort)
+                        return false;
+                    if(ptx::globaltimer_ns() - t0 > tc05::WAIT_TIMEOUT_NS)
+                    {
+                        *cta_abort = 1u;
+                        if(atomicCAS(status, 0u, ptx::STATUS_TIMEOUT_CODE) == 0u)
+                            status[1] = who;
+                        return false;
+                    }
+                }
+            return true;
+        }
+        __device__ __forceinline__ bool wait_bounded_warp(uint32_t bar, uint32_t parity, volatile uint32_t* cta_abort, unsigned* status, uint32_t who)
+        {
+            return __all_sync(0xFFFFFFFFu, wait_bounded(bar, parity, cta_abort, status, who));
+        }
+
         // ---- operand tiles --------------------------------------------------------------------
         template <uint32_t HD>
         __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t token, uint32_t head, uint32_t batch,

@@ -183,6 +183,7 @@ namespace b200wmma
                 }
 
             __syncthreads();
+            ptx::grid_dep_launch_dependents();
             bool ok = true;
             if(warp == 4)
             {
@@ -208,8 +209,8 @@ namespace b200wmma
                     const uint32_t st = i % STAGES, full = base + L::BARS + 16 * st, stage = base + st * 2 * L::TILE;
                     const int32_t  pg[2] = {page[0], page[1]}, sl[2] = {slot[0], slot[1]};
                     ask(i + 1);
-                    ok = ptx::mbar_wait_bounded_warp(full + 8, (i / STAGES & 1u) ^ 1u, cta_abort, p.status,
-                                                     TREE_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = attn::wait_bounded_warp(full + 8, (i / STAGES & 1u) ^ 1u, cta_abort, p.status,
+                                                     TREE_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu));
                     if(!ok)
                         break;
                     // which of the 64 tokens are there: their box's page is, and they lie before the end
@@ -259,8 +260,8 @@ namespace b200wmma
             for(uint32_t i = 0; warp < 4 && i < steps; ++i)
             {
                 const uint32_t st = i % STAGES;
-                ok = ptx::mbar_wait_bounded_warp(base + L::BARS + 16 * st, i / STAGES & 1u, cta_abort, p.status,
-                                                 TREE_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                ok = attn::wait_bounded_warp(base + L::BARS + 16 * st, i / STAGES & 1u, cta_abort, p.status,
+                                                 TREE_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu));
                 if(!ok)
                     break;
                 const uint32_t keys_at = base + st * 2 * L::TILE + wn * MINE * 128, values_at = keys_at + L::TILE;
@@ -460,10 +461,56 @@ namespace b200wmma
                         *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(mx, sum);
                 }
             }
-            ptx::grid_dep_launch_dependents();
         }
 
-        // Joins the splits: a block to a row.  The splits' maxima and sums become weights in shared memory, then four warps add
+        // Joins few splits: a warp to a row, a split's maximum and sum to a lane, four (HD = 128) or two elements to a lane; splits
+        // in order.
+        template <typename T, uint32_t HD>
+        __global__ void __launch_bounds__(256) join_few_kernel(const __grid_constant__ Params p, T* __restrict__ o)
+        {
+            constexpr uint32_t E = HD / 32;
+            const uint32_t     rows = p.share * p.drafts, row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+            const uint32_t     all_rows = p.batch * p.heads_kv * rows;
+            if(row >= all_rows)
+                return;
+            const uint32_t r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
+            if(draft >= drafts_of(p, b))
+                return;
+            ptx::grid_dep_wait();
+            const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (size_t(lane) * all_rows + row) * 2)
+                                              : make_float2(-INFINITY, 0.0f);
+            float        mx = ml.x;
+#pragma unroll
+            for(int d = 16; d > 0; d >>= 1)
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+            const float by  = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mx); // splits without a visible token have written no sums
+            float       sum = ml.x == -INFINITY ? 0.0f : by * ml.y, y[E] = {};
+#pragma unroll
+            for(int d = 16; d > 0; d >>= 1)
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+#pragma unroll 4
+            for(uint32_t s = 0; s < p.splits; ++s)
+            {
+                const float w = __shfl_sync(0xFFFFFFFFu, by, s);
+                if(w != 0.0f) // NaN counts
+                {
+                    const float* from = p.part_o + (size_t(s) * all_rows + row) * HD + lane * E;
+#pragma unroll
+                    for(uint32_t e = 0; e < E; ++e)
+                        y[e] = fmaf(w, from[e], y[e]);
+                }
+            }
+            const float inv = sum > 0.0f ? 1.0f / sum : sum;
+            if(lane * E < p.dim)
+            {
+                uint32_t* out = reinterpret_cast<uint32_t*>(o + row_of(p.o, b, draft, head * p.share + r % p.share) + lane * E);
+#pragma unroll
+                for(uint32_t e = 0; e < E; e += 2)
+                    out[e / 2] = attn::pack2<T>(y[e] * inv, y[e + 1] * inv);
+            }
+        }
+
+        // Joins many splits: a block to a row.  The splits' maxima and sums become weights in shared memory, then four warps add
         // up a quarter of the splits each, four (HD = 128) or two elements to a lane; all in a fixed order.
         template <typename T, uint32_t HD>
         __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, T* __restrict__ o)
@@ -532,10 +579,10 @@ namespace b200wmma
         }
 
 #ifndef TC_ROWS
-#define TC_ROWS 16
+#define TC_ROWS 32
 #define SPLIT_STAGES 4
 #define SPLIT_BLOCKS (2 * 148)
-#define TC_STAGES 2
+#define TC_STAGES 4
 #define TC_BLOCKS 148
 #endif
         // More rows than this take the tcgen05 form.
@@ -582,13 +629,16 @@ namespace b200wmma
             B200_CHECK_CUDA(cudaGetLastError());
             if(p.splits > 1)
             {
+                const uint32_t     rows = p.batch * p.heads_kv * p.share * p.drafts;
+                const bool         few  = p.splits <= 32;
                 cudaLaunchConfig_t cfg{};
-                cfg.gridDim = dim3(p.batch * p.heads_kv * p.share * p.drafts), cfg.blockDim = dim3(128), cfg.stream = stream;
+                cfg.gridDim = dim3(few ? ceil_div(rows, 8) : rows), cfg.blockDim = dim3(few ? 256 : 128), cfg.stream = stream;
+                // launched while the last blocks of the kernel above still run; it waits for them before it reads
                 cudaLaunchAttribute attr{};
                 attr.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
                 attr.val.programmaticStreamSerializationAllowed = 1;
                 cfg.attrs = &attr, cfg.numAttrs = 1;
-                B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, HD>, p, static_cast<T*>(o)));
+                B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, few ? join_few_kernel<T, HD> : join_kernel<T, HD>, p, static_cast<T*>(o)));
             }
             return B200WMMA_OK;
         }

@@ -113,6 +113,7 @@ namespace b200wmma
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(base + L::Q_FULL);
             }
+            ptx::grid_dep_launch_dependents();
             const uint32_t tmem = misc[0], s_tmem = tmem, o_tmem = tmem + 2 * TILE; // tile u: + u * TILE, + u * HD
             bool           ok = true;
             const uint32_t u = warp >> 2, quad = warp & 3u, lane_tmem = (quad * 32u) << 16, r = row_tile * TILE + (tid & 127u);
@@ -181,8 +182,8 @@ namespace b200wmma
                 const auto load = [&](uint32_t n, bool values) {
                     const uint32_t st = c % L::STAGES, full = base + L::FULL + 8 * st, stage = base + L::KV + st * L::TILE_BYTES;
                     ok = ok
-                         && ptx::mbar_wait_bounded_warp(base + L::EMPTY + 8 * st, (c / L::STAGES & 1u) ^ 1u, cta_abort, p.status,
-                                                        TREE_TC_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                         && attn::wait_bounded_warp(base + L::EMPTY + 8 * st, (c / L::STAGES & 1u) ^ 1u, cta_abort, p.status,
+                                                        TREE_TC_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu));
                     if(!ok)
                         return;
                     ++c;
@@ -218,8 +219,7 @@ namespace b200wmma
                 uint32_t   c = 0;
                 const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
                     ok = ok
-                         && ptx::mbar_wait_bounded_warp(bar, parity, cta_abort, p.status, TREE_TC_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu),
-                                                        tc05::WAIT_TIMEOUT_NS, lane);
+                         && attn::wait_bounded_warp(bar, parity, cta_abort, p.status, TREE_TC_MMA << 24 | what << 20 | (blockIdx.x & 0xFFFFFu));
                     ptx::tc_fence_after_sync();
                     return ok;
                 };
@@ -281,8 +281,8 @@ namespace b200wmma
                 const int32_t at = BIAS && live ? (p.depths ? __ldg(p.depths + size_t(b) * p.drafts + draft) : int32_t(draft)) : 0;
                 for(uint32_t n = u; ok && n < steps; n += 2, ++mine)
                 {
-                    ok = ptx::mbar_wait_bounded_warp(base + L::S_FULL + 8 * u, mine & 1u, cta_abort, p.status,
-                                                     TREE_TC_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = attn::wait_bounded_warp(base + L::S_FULL + 8 * u, mine & 1u, cta_abort, p.status,
+                                                     TREE_TC_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu));
                     if(!ok)
                         break;
                     ptx::tc_fence_after_sync();
@@ -337,8 +337,8 @@ namespace b200wmma
                         m = m2;
                         if(mine != 0)
                         {
-                            ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * u, (mine - 1) & 1u, cta_abort, p.status,
-                                                             TREE_TC_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                            ok = attn::wait_bounded_warp(base + L::O_DONE + 8 * u, (mine - 1) & 1u, cta_abort, p.status,
+                                                             TREE_TC_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
                             if(!ok)
                                 break;
                             ptx::tc_fence_after_sync();
@@ -377,8 +377,8 @@ namespace b200wmma
                 }
                 if(ok && mine != 0)
                 {
-                    ok = ptx::mbar_wait_bounded_warp(base + L::O_DONE + 8 * u, (mine - 1) & 1u, cta_abort, p.status,
-                                                     TREE_TC_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu), tc05::WAIT_TIMEOUT_NS, lane);
+                    ok = attn::wait_bounded_warp(base + L::O_DONE + 8 * u, (mine - 1) & 1u, cta_abort, p.status,
+                                                     TREE_TC_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                     ptx::tc_fence_after_sync();
                 }
             }
@@ -450,7 +450,6 @@ namespace b200wmma
                     }
                 }
             }
-            ptx::grid_dep_launch_dependents();
             ptx::tc_fence_before_sync();
             __syncthreads();
             if(*cta_abort)
