@@ -164,8 +164,8 @@ namespace b200wmma
                 }
                 ptx::mbar_init(base + L::S_FULL, 1);
                 ptx::mbar_init(base + L::DP_FULL, 1);
-                ptx::mbar_init(base + L::P_FULL, 256);
-                ptx::mbar_init(base + L::DS_FULL, 256);
+                ptx::mbar_init(base + L::P_FULL, 8); // warps
+                ptx::mbar_init(base + L::DS_FULL, 8);
                 ptx::mbar_init(base + L::DONE, 1);
                 *cta_abort = 0u;
                 ptx::fence_barrier_init();
@@ -391,7 +391,9 @@ namespace b200wmma
                             weights(std::false_type{});
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
-                        ptx::mbar_arrive(base + L::P_FULL);
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::P_FULL);
 
                         if(!wait(base + L::DP_FULL, 1))
                             break;
@@ -423,7 +425,9 @@ namespace b200wmma
                         tmem_st_32x32b_x32(dp_tmem + lane_tmem, ds);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
-                        ptx::mbar_arrive(base + L::DS_FULL);
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::DS_FULL);
                     }
                 }
                 if(seg + SEG < q_tiles)
@@ -501,11 +505,11 @@ namespace b200wmma
                     ptx::mbar_init(base + L::EMPTY + 8 * s, 1);
                 }
                 ptx::mbar_init(base + L::S_FULL, 1);
-                ptx::mbar_init(base + L::P_FULL, 256); // S has been read
+                ptx::mbar_init(base + L::P_FULL, 8); // S has been read by a warp
                 for(uint32_t s = 0; s < 2; ++s)
                 {
                     ptx::mbar_init(base + L::DP_FULL + 8 * s, 1);
-                    ptx::mbar_init(base + L::DS_FULL + 8 * s, 256);
+                    ptx::mbar_init(base + L::DS_FULL + 8 * s, 8);
                 }
                 ptx::mbar_init(base + L::DONE, 1);
                 *cta_abort = 0u;
@@ -640,7 +644,9 @@ namespace b200wmma
                         ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
                         ptx::tmem_ld_wait();
                         ptx::tc_fence_before_sync();
-                        ptx::mbar_arrive(base + L::P_FULL);
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::P_FULL);
                         uint64_t seen = ~uint64_t(0); // bit j: key j of the 64 is visible to this query
                         if(e >> 24 & TILE_MASK)
                         {
@@ -708,7 +714,9 @@ namespace b200wmma
                         tmem_st_32x32b_x32(dp_tmem + st * TILE + lane_tmem, ds);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
-                        ptx::mbar_arrive(base + L::DS_FULL + 8 * st);
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::DS_FULL + 8 * st);
                     }
                 }
                 if(seg + SEG < kv_tiles)

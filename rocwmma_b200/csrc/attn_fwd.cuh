@@ -79,7 +79,7 @@ namespace b200wmma
                 for(uint32_t t = 0; t < 2; ++t)
                 {
                     ptx::mbar_init(base + L::S_FULL + 8 * t, 1);
-                    ptx::mbar_init(base + L::P_FULL + 8 * t, TILE);
+                    ptx::mbar_init(base + L::P_FULL + 8 * t, 4); // warps
                     ptx::mbar_init(base + L::O_DONE + 8 * t, 1);
                 }
                 *cta_abort = 0u;
@@ -285,10 +285,7 @@ namespace b200wmma
                                     if(i >= rel)
                                         v[i >> 5][i & 31] = 0xFF800000u;
                         }
-                        float top = __uint_as_float(v[0][0]);
-#pragma unroll
-                        for(int i = 1; i < 128; ++i)
-                            top = fmaxf(top, __uint_as_float(v[i >> 5][i & 31]));
+                        float top = max_of(v);
                         if constexpr(PLAIN)
                             top *= sc.c; // scale > 0
                         // move the maximum where some row of this warp has outgrown it
@@ -319,26 +316,12 @@ namespace b200wmma
                             }
                         }
                         const float sub = m == -INFINITY ? 0.0f : -m;
-                        float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for(int i = 0; i < 4; ++i)
-                        {
-                            uint32_t w[16];
-#pragma unroll
-                            for(int j = 0; j < 16; ++j)
-                            {
-                                float x = __uint_as_float(v[i][2 * j]), y = __uint_as_float(v[i][2 * j + 1]);
-                                x = ex2(PLAIN ? fmaf(x, sc.c, sub) : x + sub);
-                                y = ex2(PLAIN ? fmaf(y, sc.c, sub) : y + sub);
-                                sum[j & 3] += x + y;
-                                w[j] = pack2<T>(x, y);
-                            }
-                            tmem_st_32x32b_x16(s_tmem[t] + lane_tmem + 16 * i, w);
-                        }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        l += weights<T>(v, s_tmem[t] + lane_tmem, PLAIN ? sc.c : 1.0f, sub);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
-                        ptx::mbar_arrive(base + L::P_FULL + 8 * t);
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::P_FULL + 8 * t);
                         ++n_s;
                     }
                 }

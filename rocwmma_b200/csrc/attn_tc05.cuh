@@ -76,6 +76,43 @@ namespace b200wmma
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
             return y;
         }
+        // Two fp32 numbers in a register pair: one instruction for both.
+        __device__ __forceinline__ uint64_t pair(float lo, float hi)
+        {
+            uint64_t r;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+            return r;
+        }
+        __device__ __forceinline__ void unpair(uint64_t x, float& lo, float& hi)
+        {
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+        }
+        __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+        {
+            uint64_t r;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+            return r;
+        }
+        __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+        {
+            uint64_t r;
+            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+            return r;
+        }
+        // Largest of 128 numbers in four independent chains of three-input steps.
+        __device__ __forceinline__ float max_of(const uint32_t (&v)[4][32])
+        {
+            float t[4];
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                t[i] = fmaxf(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]));
+#pragma unroll
+            for(int k = 2; k < 32; k += 2)
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                    t[i] = fmaxf(fmaxf(t[i], __uint_as_float(v[i][k])), __uint_as_float(v[i][k + 1]));
+            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        }
         template <typename T>
         __device__ __forceinline__ uint32_t pack2(float lo, float hi)
         {
@@ -153,6 +190,32 @@ namespace b200wmma
                             *reinterpret_cast<uint4*>(tile + s * BOX_BYTES + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
             ptx::fence_proxy_async_smem();
             __syncwarp();
+        }
+
+        // P of 128 scores: P = 2^(x c - m) in 16 bits over the scores' own columns; returns the sum of the unrounded P.
+        template <typename T>
+        __device__ __forceinline__ float weights(const uint32_t (&v)[4][32], uint32_t taddr, float c, float sub)
+        {
+            const uint64_t cc = pair(c, c), ss = pair(sub, sub);
+            uint64_t       sum[2] = {0, 0};
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                uint32_t w[16];
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                {
+                    float x, y;
+                    unpair(fma2(pair(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1])), cc, ss), x, y);
+                    x = ex2(x), y = ex2(y);
+                    sum[j & 1] = add2(sum[j & 1], pair(x, y));
+                    w[j]       = pack2<T>(x, y);
+                }
+                tmem_st_32x32b_x16(taddr + 16 * i, w);
+            }
+            float a, b;
+            unpair(add2(sum[0], sum[1]), a, b);
+            return a + b;
         }
 
         // ---- masks by tile --------------------------------------------------------------------

@@ -76,7 +76,7 @@ namespace b200wmma
                 for(uint32_t u = 0; u < 2; ++u)
                 {
                     ptx::mbar_init(base + L::S_FULL + 8 * u, 1);
-                    ptx::mbar_init(base + L::P_FULL + 8 * u, TILE);
+                    ptx::mbar_init(base + L::P_FULL + 8 * u, 4); // warps
                     ptx::mbar_init(base + L::O_DONE + 8 * u, 1);
                 }
                 ptx::mbar_init(base + L::Q_FULL, 256);
@@ -295,7 +295,6 @@ namespace b200wmma
                     for(int i = 0; i < 4; ++i)
                         ptx::tmem_ld_32x32b_x32(s_tmem + u * TILE + lane_tmem + 32 * i, v[i]);
                     ptx::tmem_ld_wait();
-                    float      top    = -INFINITY;
                     const auto scores = [&](auto mask) {
                         constexpr bool MASK = decltype(mask)::value;
 #pragma unroll
@@ -321,7 +320,6 @@ namespace b200wmma
                                     if(!(see >> k & 1u))
                                         y = -INFINITY;
                                 v[i][k] = __float_as_uint(y);
-                                top     = fmaxf(top, y);
                             }
                         }
                     };
@@ -329,6 +327,7 @@ namespace b200wmma
                         scores(std::true_type{});
                     else
                         scores(std::false_type{});
+                    const float top = attn::max_of(v);
                     // the maximum moves only where a score passes it by more than 2^8: until then weights grow up to 256
                     if(__any_sync(0xFFFFFFFFu, top > m + 8.0f))
                     {
@@ -356,24 +355,12 @@ namespace b200wmma
                         }
                     }
                     const float sub = m == -INFINITY ? 0.0f : m;
-                    float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for(int i = 0; i < 4; ++i)
-                    {
-                        uint32_t w[16];
-#pragma unroll
-                        for(int k = 0; k < 16; ++k)
-                        {
-                            const float y0 = ex2(__uint_as_float(v[i][2 * k]) - sub), y1 = ex2(__uint_as_float(v[i][2 * k + 1]) - sub);
-                            sum[k & 3] += y0 + y1;
-                            w[k] = attn::pack2<T>(y0, y1);
-                        }
-                        attn::tmem_st_32x32b_x16(s_tmem + u * TILE + lane_tmem + 16 * i, w);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    l += attn::weights<T>(v, s_tmem + u * TILE + lane_tmem, 1.0f, -sub);
                     attn::tmem_st_wait();
                     ptx::tc_fence_before_sync();
-                    ptx::mbar_arrive(base + L::P_FULL + 8 * u);
+                    __syncwarp();
+                    if(lane == 0)
+                        ptx::mbar_arrive(base + L::P_FULL + 8 * u);
                 }
                 if(ok && mine != 0)
                 {
