@@ -257,14 +257,14 @@ namespace b200wmma
                         return true;
                     };
                     const auto scores = [&](uint32_t at) {
-                        if(lane == 0)
+                        if(elect_one())
                         {
                             mma_over_head<T, HD>(s_tmem, base + L::OWN, base + L::RING + (at & 1u) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL);
                         }
                     };
                     const auto grads = [&](uint32_t at) {
-                        if(lane == 0)
+                        if(elect_one())
                         {
                             mma_over_head<T, HD>(dp_tmem, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + (at & 1u)) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::DP_FULL);
@@ -283,7 +283,7 @@ namespace b200wmma
                             const bool more = n + 1 < steps;
                             if(!wait(base + L::P_FULL, it & 1u, 3))
                                 break;
-                            if(lane == 0)
+                            if(elect_one())
                             {
                                 mma_over_tokens_halves<T, HD>(dv_tmem, s_tmem, base + L::RING + (2 + (it & 1u)) * L::TILE_BYTES, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 16 + 8 * (it & 1u));
@@ -296,7 +296,7 @@ namespace b200wmma
                             }
                             if(!wait(base + L::DS_FULL, it & 1u, 4))
                                 break;
-                            if(lane == 0)
+                            if(elect_one())
                             {
                                 mma_over_tokens_halves<T, HD>(dk_tmem, dp_tmem, base + L::RING + (it & 1u) * L::TILE_BYTES, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 8 * (it & 1u));
@@ -435,7 +435,7 @@ namespace b200wmma
             }
 
             // ---- results: dv by the first four warps, dk by the next four ----
-            if(warp == 9 && lane == 0 && ok)
+            if(warp == 9 && ok && elect_one())
                 ptx::tc_commit(base + L::DONE);
             if(warp < 8)
             {
@@ -594,14 +594,14 @@ namespace b200wmma
                         }
                         if(a != 0 && !wait(base + L::P_FULL, (a - 1) & 1u, 1)) // the last S has been read
                             return;
-                        if(lane == 0)
+                        if(elect_one())
                         {
                             mma_over_head<T, HD>(s_tmem, base + L::OWN, base + L::RING + st * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL);
                         }
                         if(!wait(base + L::FULL + 16 + 8 * st, (a >> 1) & 1u, 2))
                             return;
-                        if(lane == 0)
+                        if(elect_one())
                         {
                             mma_over_head<T, HD>(dp_tmem + st * TILE, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + st) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::DP_FULL + 8 * st);
@@ -621,7 +621,7 @@ namespace b200wmma
                             const uint32_t st = it & 1u;
                             if(!ok || !wait(base + L::DS_FULL + 8 * st, (it >> 1) & 1u, 4))
                                 break;
-                            if(lane == 0)
+                            if(elect_one())
                             {
                                 mma_over_tokens_halves<T, HD>(dq_tmem, dp_tmem + st * TILE, base + L::RING + st * L::TILE_BYTES, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 8 * st);
@@ -723,7 +723,7 @@ namespace b200wmma
                     __syncthreads();
             }
 
-            if(warp == 9 && lane == 0 && ok)
+            if(warp == 9 && ok && elect_one())
                 ptx::tc_commit(base + L::DONE);
             if(warp < 4)
             {

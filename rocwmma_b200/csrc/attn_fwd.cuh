@@ -179,14 +179,14 @@ namespace b200wmma
                         return true;
                     };
                     const auto scores = [&](uint32_t u, uint32_t e, uint32_t n) { // S of query tile u
-                        if(lane == 0 && (list[e] >> (24 + 2 * u) & TILE_NEED))
+                        if((list[e] >> (24 + 2 * u) & TILE_NEED) && elect_one())
                         {
                             mma_over_head<T, HD>(s_tmem[u], base + L::Q + u * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL + 8 * u);
                         }
                     };
                     const auto free_stage = [&](uint32_t n) {
-                        if(lane == 0)
+                        if(elect_one())
                             ptx::tc_commit(base + L::KV_EMPTY + 8 * (n % L::STAGES));
                     };
                     if(entries && ok)
@@ -213,7 +213,7 @@ namespace b200wmma
                                 {
                                     if(!wait(base + L::P_FULL + 8 * u, done[u] & 1u, 2 + u))
                                         break;
-                                    if(lane == 0)
+                                    if(elect_one())
                                     {
                                         mma_over_tokens<T, HD>(o_tmem[u], s_tmem[u], base + L::KV + ((2 * it + 1) % L::STAGES) * L::TILE_BYTES,
                                                                done[u] != 0);

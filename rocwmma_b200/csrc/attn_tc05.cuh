@@ -21,7 +21,21 @@ namespace b200wmma
         template <typename T>
         constexpr int kind_of = std::is_same<T, __half>::value ? tc05::KIND_F16 : tc05::KIND_BF16;
 
-        // ---- instructions ---------------------------------------------------------------------
+        // ---- instructions ----
+        // True in one lane of a converged warp, always the same one.  The compiler knows the branch on it to be taken by a single
+        // lane and keeps descriptors and addresses of tensor instructions in uniform registers; behind `lane == 0` it moved them
+        // there for every instruction, and issuing the 16 products of a tile took longer than the products.
+        __device__ __forceinline__ bool elect_one()
+        {
+            uint32_t yes;
+            asm volatile("{\n"
+                         ".reg .pred p;\n"
+                         "elect.sync _|p, 0xFFFFFFFF;\n"
+                         "selp.u32 %0, 1, 0, p;\n"
+                         "}"
+                         : "=r"(yes));
+            return yes != 0;
+        }
         // D[tmem] (+)= A[tmem] * B[smem]
         __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
         {

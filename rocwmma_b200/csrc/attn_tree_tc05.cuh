@@ -228,7 +228,7 @@ namespace b200wmma
                     if(!wait(base + L::FULL + 8 * st, c / L::STAGES & 1u, 0))
                         return;
                     ++c;
-                    if(lane == 0)
+                    if(attn::elect_one())
                     {
                         attn::mma_over_head<T, HD>(s_tmem + (n & 1u) * TILE, base + L::Q, base + L::KV + st * L::TILE_BYTES);
                         ptx::tc_commit(base + L::S_FULL + 8 * (n & 1u));
@@ -259,7 +259,7 @@ namespace b200wmma
                     }
                     if(!wait(base + L::P_FULL + 8 * (n & 1u), n >> 1 & 1u, 2))
                         break;
-                    if(lane == 0)
+                    if(attn::elect_one())
                     {
                         attn::mma_over_tokens<T, HD>(o_tmem + (n & 1u) * HD, s_tmem + (n & 1u) * TILE, base + L::KV + st * L::TILE_BYTES, n >= 2);
                         ptx::tc_commit(base + L::O_DONE + 8 * (n & 1u));
