@@ -23,8 +23,7 @@ namespace b200wmma
             static constexpr uint32_t RING = 2 * TILE_BYTES; // two stages of each of the two tiles that are walked
             static constexpr uint32_t LIST = RING + 4 * TILE_BYTES;
             static constexpr uint32_t RAW  = LIST + SEG * 4;
-            static constexpr uint32_t DOCS = RAW + SEG; // 128 documents
-            static constexpr uint32_t STAT = DOCS + TILE * 4; // dkv: two stages of 128 lse and 128 delta
+            static constexpr uint32_t STAT = RAW + SEG; // dkv: two stages of 128 lse and 128 delta
             static constexpr uint32_t BARS = STAT + 4 * TILE * 4;
             static constexpr uint32_t OWN_FULL = BARS, FULL = OWN_FULL + 8, EMPTY = FULL + 32, // [2 tiles][2 stages]
                                       S_FULL = EMPTY + 32, DP_FULL = S_FULL + 8, P_FULL = DP_FULL + 16, DS_FULL = P_FULL + 8,
@@ -80,18 +79,6 @@ namespace b200wmma
             }
         }
 
-        // Bit j: document j of 64 is `doc`.
-        __device__ __forceinline__ uint64_t same_docs(const int32_t* docs, int32_t doc)
-        {
-            uint32_t lo = 0, hi = 0;
-#pragma unroll
-            for(int j = 0; j < 32; ++j)
-            {
-                lo |= uint32_t(docs[j] == doc) << j;
-                hi |= uint32_t(docs[32 + j] == doc) << j;
-            }
-            return uint64_t(hi) << 32 | lo;
-        }
         // A row of HD fp32 columns in tensor memory, times `by`, to 16-bit memory.  `live`: the accumulator was written.
         template <typename T, uint32_t HD>
         __device__ __forceinline__ void store_row(T* out, uint32_t taddr, float by, bool live, bool mine, uint32_t dim)
@@ -324,6 +311,14 @@ namespace b200wmma
                             return ok;
                         };
                         const ScoreConst sc = score_const(p, g * share + n / entries);
+                        int32_t          query_docs[2]; // on their way while the product is
+                        if(docs && (e >> 24 & TILE_MASK))
+#pragma unroll
+                            for(uint32_t i = 0; i < 2; ++i)
+                            {
+                                const uint32_t r = r0 + half * 64 + 32 * i + lane;
+                                query_docs[i]    = r < p.len_q ? __ldg(p.doc_q + size_t(b) * p.len_q + r) : -1;
+                            }
                         // the statistics came with the tiles: an acquire of the same barriers
                         ok = wait_bounded_warp(base + L::FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
                                                          DKV_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
@@ -345,13 +340,9 @@ namespace b200wmma
                             seen = first >= 64 ? 0 : first > 0 ? seen << first : seen;
                             if(docs)
                             {
-                                int32_t*       dq = reinterpret_cast<int32_t*>(smem + L::DOCS) + half * 64;
-                                const uint32_t i  = threadIdx.x & 127u, r = r0 + half * 64 + i;
-                                ptx::named_bar_sync(1 + half, TILE); // everyone is done with the last tile's documents
-                                if(i < 64)
-                                    dq[i] = r < p.len_q ? p.doc_q[size_t(b) * p.len_q + r] : -1;
-                                ptx::named_bar_sync(1 + half, TILE);
-                                seen = doc < 0 ? 0 : seen & same_docs(dq, doc);
+                                uint32_t same[2] = {0, 0};
+                                same_docs(query_docs, doc, same);
+                                seen = doc < 0 ? 0 : seen & (uint64_t(same[1]) << 32 | same[0]);
                             }
                         }
                         const auto weights = [&](auto masked) {
@@ -635,6 +626,14 @@ namespace b200wmma
                     for(uint32_t n = 0; ok && n < entries; ++n, ++it)
                     {
                         const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
+                        int32_t        key_docs[2]; // on their way while the product is
+                        if(docs && (e >> 24 & TILE_MASK))
+#pragma unroll
+                            for(uint32_t i = 0; i < 2; ++i)
+                            {
+                                const uint32_t c = c0 + half * 64 + 32 * i + lane;
+                                key_docs[i]      = c < p.len_kv ? __ldg(p.doc_kv + size_t(b) * p.len_kv + c) : -1;
+                            }
                         ok = wait_bounded_warp(base + L::S_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu));
                         if(!ok)
                             break;
@@ -654,13 +653,9 @@ namespace b200wmma
                             seen              = rel <= 0 ? 0 : rel < 64 ? seen >> (64 - rel) : seen;
                             if(docs)
                             {
-                                int32_t*       dk = reinterpret_cast<int32_t*>(smem + L::DOCS) + half * 64;
-                                const uint32_t i  = threadIdx.x & 127u, c = c0 + half * 64 + i;
-                                ptx::named_bar_sync(1 + half, TILE); // everyone is done with the last tile's documents
-                                if(i < 64)
-                                    dk[i] = c < p.len_kv ? p.doc_kv[size_t(b) * p.len_kv + c] : -1;
-                                ptx::named_bar_sync(1 + half, TILE);
-                                seen &= same_docs(dk, doc);
+                                uint32_t same[2] = {0, 0};
+                                same_docs(key_docs, doc, same);
+                                seen &= uint64_t(same[1]) << 32 | same[0];
                             }
                         }
                         const float from    = static_cast<float>(at - int32_t(c0 + half * 64));

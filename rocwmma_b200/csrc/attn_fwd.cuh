@@ -25,8 +25,7 @@ namespace b200wmma
             static constexpr uint32_t KV         = Q + 2 * TILE_BYTES;
             static constexpr uint32_t LIST       = KV + STAGES * TILE_BYTES; // SEG words
             static constexpr uint32_t RAW        = LIST + SEG * 4; // SEG bytes of flags before they are listed
-            static constexpr uint32_t DOCS       = RAW + SEG; // 2 x 128 documents of the keys
-            static constexpr uint32_t BARS       = DOCS + 2 * TILE * 4;
+            static constexpr uint32_t BARS       = RAW + SEG;
             static constexpr uint32_t Q_FULL = BARS, KV_FULL = Q_FULL + 8, KV_EMPTY = KV_FULL + 8 * STAGES, S_FULL = KV_EMPTY + 8 * STAGES,
                                       P_FULL = S_FULL + 16, O_DONE = P_FULL + 16;
             static constexpr uint32_t MISC  = O_DONE + 16; // tensor memory address, abort flag, list length
@@ -243,8 +242,12 @@ namespace b200wmma
                         if(!(f & TILE_NEED))
                             continue;
                         const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
-                        ok = wait_bounded_warp(base + L::S_FULL + 8 * t, n_s & 1u, cta_abort, status,
-                                                         FWD_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu));
+                        int32_t        key_docs[4]; // on their way while the product is
+                        if(docs && (f & TILE_MASK))
+#pragma unroll
+                            for(uint32_t i = 0; i < 4; ++i)
+                                key_docs[i] = c0 + 32 * i + lane < p.len_kv ? __ldg(p.doc_kv + size_t(b) * p.len_kv + c0 + 32 * i + lane) : -1;
+                        ok = wait_bounded_warp(base + L::S_FULL + 8 * t, n_s & 1u, cta_abort, status, FWD_SOFTMAX << 24 | (blockIdx.x & 0xFFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
@@ -266,24 +269,22 @@ namespace b200wmma
                         }
                         if(f & TILE_MASK)
                         {
-                            const int32_t rel = lim - int32_t(c0);
+                            uint32_t see[4];
+#pragma unroll
+                            for(int i = 0; i < 4; ++i)
+                                see[i] = below(lim - int32_t(c0), i);
                             if(docs)
                             {
-                                int32_t* dk = reinterpret_cast<int32_t*>(smem + L::DOCS) + t * TILE;
-                                const uint32_t c = c0 + (threadIdx.x & 127u);
-                                ptx::named_bar_sync(1 + t, TILE); // everyone is done with the last tile's documents
-                                dk[threadIdx.x & 127u] = c < p.len_kv ? p.doc_kv[size_t(b) * p.len_kv + c] : -1;
-                                ptx::named_bar_sync(1 + t, TILE);
+                                uint32_t same[4] = {0, 0, 0, 0};
+                                same_docs(key_docs, doc, same);
 #pragma unroll
-                                for(int i = 0; i < 128; ++i)
-                                    if(i >= rel || dk[i] != doc)
-                                        v[i >> 5][i & 31] = 0xFF800000u; // -infinity
+                                for(int i = 0; i < 4; ++i)
+                                    see[i] &= same[i];
                             }
-                            else
 #pragma unroll
-                                for(int i = 0; i < 128; ++i)
-                                    if(i >= rel)
-                                        v[i >> 5][i & 31] = 0xFF800000u;
+                            for(int i = 0; i < 128; ++i)
+                                if(!(see[i >> 5] >> (i & 31) & 1u))
+                                    v[i >> 5][i & 31] = 0xFF800000u; // -infinity
                         }
                         float top = max_of(v);
                         if constexpr(PLAIN)

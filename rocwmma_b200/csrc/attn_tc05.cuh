@@ -268,6 +268,32 @@ namespace b200wmma
             return TILE_NEED | (mask ? TILE_MASK : 0u);
         }
 
+        // Bit i: document i of 32 N is `doc`, where lane l of the warp holds documents l, 32 + l, ... in `of`.  One round of votes
+        // for each document that rows of the warp belong to, mostly one or two.
+        template <int N>
+        __device__ __forceinline__ void same_docs(const int32_t (&of)[N], int32_t doc, uint32_t (&same)[N])
+        {
+            uint32_t todo = 0xFFFFFFFFu;
+            while(todo)
+            {
+                const int32_t d = __shfl_sync(0xFFFFFFFFu, doc, __ffs(todo) - 1);
+                todo &= ~__ballot_sync(0xFFFFFFFFu, doc == d);
+#pragma unroll
+                for(int i = 0; i < N; ++i)
+                {
+                    const uint32_t vote = __ballot_sync(0xFFFFFFFFu, of[i] == d);
+                    if(doc == d)
+                        same[i] = vote;
+                }
+            }
+        }
+        // Bit i of word w: 32 w + i < count.
+        __device__ __forceinline__ uint32_t below(int32_t count, int32_t w)
+        {
+            const int32_t n = count - 32 * w;
+            return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+        }
+
         // Lists tiles seg .. seg + count that flags_of(tile) says something about, as tile | flags << 24, in order.  Every
         // thread of the block calls it; `raw` holds SEG bytes, `list` SEG words, `length` one.  Returns the list's length.
         template <uint32_t THREADS, typename F>
