@@ -71,38 +71,37 @@ namespace b200wmma
         }
 
         template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
-        static int launch_fwd(const Params& p, const CUtensorMap (&maps)[3], void* o, float* lse, const DocTile* dq, const DocTile* dk,
+        static int launch_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
                               unsigned* status, cudaStream_t stream)
         {
             auto kern = fwd_tc05_kernel<T, HD, CAP, BIAS, PLAIN>;
             B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<HD>::BYTES));
             const uint32_t q_blocks = ceil_div(p.len_q, 2 * TILE);
-            kern<<<q_blocks * p.batch * p.heads_q, FWD_THREADS, FwdSmem<HD>::BYTES, stream>>>(maps[0], maps[1], maps[2], p, static_cast<T*>(o), lse,
+            kern<<<q_blocks * p.batch * p.heads_q, FWD_THREADS, FwdSmem<HD>::BYTES, stream>>>(maps[0], maps[1], maps[2], maps[3], p, lse,
                                                                                               dq, dk, q_blocks, status);
             B200_CHECK_CUDA(cudaGetLastError());
             return B200WMMA_OK;
         }
         template <typename T, uint32_t HD>
-        static int run_fwd(const Params& p, const CUtensorMap (&maps)[3], void* o, float* lse, const DocTile* dq, const DocTile* dk,
+        static int run_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
                            unsigned* status, cudaStream_t stream)
         {
             const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
             if(cap)
-                return bias ? launch_fwd<T, HD, true, true, false>(p, maps, o, lse, dq, dk, status, stream)
-                            : launch_fwd<T, HD, true, false, false>(p, maps, o, lse, dq, dk, status, stream);
+                return bias ? launch_fwd<T, HD, true, true, false>(p, maps, lse, dq, dk, status, stream)
+                            : launch_fwd<T, HD, true, false, false>(p, maps, lse, dq, dk, status, stream);
             if(bias)
-                return launch_fwd<T, HD, false, true, false>(p, maps, o, lse, dq, dk, status, stream);
+                return launch_fwd<T, HD, false, true, false>(p, maps, lse, dq, dk, status, stream);
             // the softmax scales plain scores in the exponential's argument, which takes a positive scale
-            return p.scale > 0.0f ? launch_fwd<T, HD, false, false, true>(p, maps, o, lse, dq, dk, status, stream)
-                                  : launch_fwd<T, HD, false, false, false>(p, maps, o, lse, dq, dk, status, stream);
+            return p.scale > 0.0f ? launch_fwd<T, HD, false, false, true>(p, maps, lse, dq, dk, status, stream)
+                                  : launch_fwd<T, HD, false, false, false>(p, maps, lse, dq, dk, status, stream);
         }
         struct BwdCall
         {
-            CUtensorMap    maps[4]; // q, k, v, dout
+            CUtensorMap    maps[7]; // q, k, v, dout, dq, dk, dv
             const void *   o, *dout;
             const float*   lse;
             float *        lse2, *delta;
-            void *         dq, *dk, *dv;
             const DocTile *docs_q, *docs_kv;
             unsigned*      status;
             cudaStream_t   stream;
@@ -118,10 +117,10 @@ namespace b200wmma
             bwd_rows_kernel<T><<<rows / 16, 256, 0, c.stream>>>(p, static_cast<const T*>(c.o), static_cast<const T*>(c.dout), c.lse, c.lse2, c.delta,
                                                                 padded, rows);
             dkv<<<uint32_t(tiles_of(p.len_kv)) * p.batch * p.heads_kv, BWD_THREADS, BwdSmem<HD>::BYTES, c.stream>>>(
-                c.maps[0], c.maps[1], c.maps[2], c.maps[3], p, c.lse2, c.delta, static_cast<T*>(c.dk), static_cast<T*>(c.dv), c.docs_q, c.docs_kv,
+                c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[5], c.maps[6], p, c.lse2, c.delta, c.docs_q, c.docs_kv,
                 c.status);
             dq<<<uint32_t(tiles_of(p.len_q)) * p.batch * p.heads_q, BWD_THREADS, BwdSmem<HD>::BYTES, c.stream>>>(
-                c.maps[0], c.maps[1], c.maps[2], c.maps[3], p, c.lse2, c.delta, static_cast<T*>(c.dq), c.docs_q, c.docs_kv, c.status);
+                c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[4], p, c.lse2, c.delta, c.docs_q, c.docs_kv, c.status);
             B200_CHECK_CUDA(cudaGetLastError());
             return B200WMMA_OK;
         }
@@ -161,21 +160,23 @@ extern "C" int b200wmma_attn_fwd(const b200wmma_attn_args* args, const void* q, 
     unsigned* status = nullptr;
     if(int e = status_word_ptr(&status))
         return e;
-    CUtensorMap maps[3];
+    CUtensorMap maps[4];
     if(int e = attn::make_map(&maps[0], args->data_type, q, p.dim, p.len_q, p.heads_q, p.batch, p.q))
         return e;
     if(int e = attn::make_map(&maps[1], args->data_type, k, p.dim, p.len_kv, p.heads_kv, p.batch, p.k))
         return e;
     if(int e = attn::make_map(&maps[2], args->data_type, v, p.dim, p.len_kv, p.heads_kv, p.batch, p.v))
         return e;
+    if(int e = attn::make_map(&maps[3], args->data_type, o, p.dim, p.len_q, p.heads_q, p.batch, p.o))
+        return e;
     const attn::DocTile *dq = nullptr, *dk = nullptr;
     if(int e = attn::list_documents(p, workspace, &dq, &dk, as_stream(stream)))
         return e;
     if(args->data_type == B200WMMA_OUT_F16)
-        return p.dim <= 64 ? attn::run_fwd<__half, 64>(p, maps, o, lse, dq, dk, status, as_stream(stream))
-                           : attn::run_fwd<__half, 128>(p, maps, o, lse, dq, dk, status, as_stream(stream));
-    return p.dim <= 64 ? attn::run_fwd<__nv_bfloat16, 64>(p, maps, o, lse, dq, dk, status, as_stream(stream))
-                       : attn::run_fwd<__nv_bfloat16, 128>(p, maps, o, lse, dq, dk, status, as_stream(stream));
+        return p.dim <= 64 ? attn::run_fwd<__half, 64>(p, maps, lse, dq, dk, status, as_stream(stream))
+                           : attn::run_fwd<__half, 128>(p, maps, lse, dq, dk, status, as_stream(stream));
+    return p.dim <= 64 ? attn::run_fwd<__nv_bfloat16, 64>(p, maps, lse, dq, dk, status, as_stream(stream))
+                       : attn::run_fwd<__nv_bfloat16, 128>(p, maps, lse, dq, dk, status, as_stream(stream));
 }
 
 extern "C" int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, const void* k, const void* v, const void* o,
@@ -218,10 +219,16 @@ extern "C" int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, 
         return e;
     if(int e = attn::make_map(&c.maps[3], args->data_type, dout, p.dim, p.len_q, p.heads_q, p.batch, p.dout))
         return e;
+    if(int e = attn::make_map(&c.maps[4], args->data_type, dq, p.dim, p.len_q, p.heads_q, p.batch, p.dq))
+        return e;
+    if(int e = attn::make_map(&c.maps[5], args->data_type, dk, p.dim, p.len_kv, p.heads_kv, p.batch, p.dk))
+        return e;
+    if(int e = attn::make_map(&c.maps[6], args->data_type, dv, p.dim, p.len_kv, p.heads_kv, p.batch, p.dv))
+        return e;
     const size_t doc_tiles = p.batch * (attn::tiles_of(p.len_q) + attn::tiles_of(p.len_kv));
     c.lse2  = reinterpret_cast<float*>(static_cast<attn::DocTile*>(workspace) + doc_tiles);
     c.delta = c.lse2 + size_t(p.batch) * p.heads_q * attn::tiles_of(p.len_q) * attn::TILE;
-    c.o = o, c.dout = dout, c.lse = lse, c.dq = dq, c.dk = dk, c.dv = dv, c.stream = as_stream(stream);
+    c.o = o, c.dout = dout, c.lse = lse, c.stream = as_stream(stream);
     if(int e = attn::list_documents(p, workspace, &c.docs_q, &c.docs_kv, c.stream))
         return e;
     if(args->data_type == B200WMMA_OUT_F16)

@@ -79,30 +79,6 @@ namespace b200wmma
             }
         }
 
-        // A row of HD fp32 columns in tensor memory, times `by`, to 16-bit memory.  `live`: the accumulator was written.
-        template <typename T, uint32_t HD>
-        __device__ __forceinline__ void store_row(T* out, uint32_t taddr, float by, bool live, bool mine, uint32_t dim)
-        {
-#pragma unroll 1
-            for(uint32_t c = 0; c < HD; c += 32)
-            {
-                uint32_t w[32];
-                __syncwarp();
-                ptx::tmem_ld_32x32b_x32(taddr + c, w);
-                ptx::tmem_ld_wait();
-                if(mine)
-#pragma unroll
-                    for(int i = 0; i < 4; ++i)
-                        if(c + 8 * i < dim)
-                        {
-                            uint32_t u[4];
-#pragma unroll
-                            for(int j = 0; j < 4; ++j)
-                                u[j] = live ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * by, __uint_as_float(w[8 * i + 2 * j + 1]) * by) : 0u;
-                            *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(u[0], u[1], u[2], u[3]);
-                        }
-            }
-        }
         // D (+)= A B over 128 tokens; the left operand's halves of 64 tokens start 64 columns apart
         template <typename T, uint32_t HD>
         __device__ __forceinline__ void mma_over_tokens_halves(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem, bool accumulate)
@@ -119,8 +95,8 @@ namespace b200wmma
         __global__ void __launch_bounds__(BWD_THREADS, 1)
             bwd_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                           const __grid_constant__ Params p, const float* __restrict__ lse2, const float* __restrict__ delta, T* __restrict__ dk,
-                           T* __restrict__ dv, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                           const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ Params p,
+                           const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
         {
             using L = BwdSmem<HD>;
             extern __shared__ uint8_t smem_raw[];
@@ -435,9 +411,13 @@ namespace b200wmma
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
-                    const Strides& s   = half ? p.dk : p.dv;
-                    T*             out = (half ? dk : dv) + int64_t(b) * s.batch + int64_t(col) * s.token + int64_t(g) * s.head;
-                    store_row<T, HD>(out, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), half ? p.scale : 1.0f, it != 0, col < p.len_kv, p.dim);
+                    // every product is done: the tiles of K and V make room
+                    stage_row<T>(smem + L::OWN + half * L::TILE_BYTES, threadIdx.x & 127u, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), 0, HD,
+                                 half ? p.scale : 1.0f, it != 0);
+                    ptx::fence_proxy_async_smem();
+                    ptx::named_bar_sync(1 + half, TILE);
+                    if((threadIdx.x & 127u) == 0)
+                        store_tile<HD>(half ? &map_dk : &map_dv, base + L::OWN + half * L::TILE_BYTES, c0, g, b);
                 }
             }
             ptx::tc_fence_before_sync();
@@ -463,9 +443,8 @@ namespace b200wmma
         template <typename T, uint32_t HD, bool CAP, bool BIAS>
         __global__ void __launch_bounds__(BWD_THREADS, 1)
             bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ Params p,
-                          const float* __restrict__ lse2, const float* __restrict__ delta, T* __restrict__ dq,
-                          const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dq,
+                          const __grid_constant__ Params p, const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
         {
             using L = BwdSmem<HD>;
             extern __shared__ uint8_t smem_raw[];
@@ -720,15 +699,19 @@ namespace b200wmma
 
             if(warp == 9 && ok && elect_one())
                 ptx::tc_commit(base + L::DONE);
-            if(warp < 4)
+            if(warp < 8)
             {
                 if(ok)
                     ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
-                    T* out = dq + int64_t(b) * p.dq.batch + int64_t(row) * p.dq.token + int64_t(h) * p.dq.head;
-                    store_row<T, HD>(out, dq_tmem + ((quad * 32u) << 16), p.scale, it != 0, row < p.len_q, p.dim);
+                    // every product is done: the tile of Q makes room; both halves of the threads take half of the columns
+                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2), p.scale, it != 0);
+                    ptx::fence_proxy_async_smem();
+                    ptx::named_bar_sync(1, 256);
+                    if(threadIdx.x == 0)
+                        store_tile<HD>(&map_dq, base + L::OWN, row0, h, b);
                 }
             }
             ptx::tc_fence_before_sync();

@@ -43,7 +43,8 @@ namespace b200wmma
         template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
         __global__ void __launch_bounds__(FWD_THREADS, 1)
             fwd_tc05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p, T* __restrict__ o,
+                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                            const __grid_constant__ Params p,
                             float* __restrict__ lse, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv,
                             uint32_t q_blocks, unsigned* status)
         {
@@ -126,6 +127,8 @@ namespace b200wmma
                     return f && docs && dk->neg ? f | TILE_DIRTY : f;
                 });
 
+                if(warp < 8)
+                    q_here |= entries != 0;
                 if(warp == 8)
                 {
                     // ------------------------------ TMA producer ------------------------------
@@ -333,7 +336,9 @@ namespace b200wmma
             // ---- results ----
             if(warp < 8)
             {
-                bool have = n_s != 0;
+                const bool have = n_s != 0;
+                if(q_here && ok) // the copies of Q, whose place is used below, are over also where this tile sees nothing
+                    ok = wait_bounded_warp(base + L::Q_FULL, 0, cta_abort, status, FWD_SOFTMAX << 24 | 3u << 20 | (blockIdx.x & 0xFFFFFu));
                 if(have && ok)
                 {
                     ok = wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
@@ -342,32 +347,13 @@ namespace b200wmma
                 }
                 if(ok)
                 {
-                    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); // NaN stays NaN
-                    T*          out = o + int64_t(b) * p.o.batch + int64_t(row) * p.o.token + int64_t(h) * p.o.head;
-#pragma unroll 1
-                    for(uint32_t c = 0; c < HD; c += 32)
-                    {
-                        uint32_t w[32];
-                        __syncwarp();
-                        if(have)
-                        {
-                            ptx::tmem_ld_32x32b_x32(o_tmem[t] + ((quad * 32u) << 16) + c, w);
-                            ptx::tmem_ld_wait();
-                        }
-                        if(row < p.len_q)
-#pragma unroll
-                            for(int i = 0; i < 4; ++i)
-                                if(c + 8 * i < p.dim)
-                                {
-                                    uint32_t u[4];
-#pragma unroll
-                                    for(int j = 0; j < 4; ++j)
-                                        u[j] = (have && l != 0.0f) ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * inv,
-                                                                              __uint_as_float(w[8 * i + 2 * j + 1]) * inv)
-                                                                   : 0u;
-                                    *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(u[0], u[1], u[2], u[3]);
-                                }
-                    }
+                    const float inv = l > 0.0f ? 1.0f / l : l; // NaN stays NaN
+                    // every product of this tile is done: its Q makes room
+                    stage_row<T>(smem + L::Q + t * L::TILE_BYTES, threadIdx.x & 127u, o_tmem[t] + ((quad * 32u) << 16), 0, HD, inv, have && l != 0.0f);
+                    ptx::fence_proxy_async_smem();
+                    ptx::named_bar_sync(1 + t, TILE);
+                    if((threadIdx.x & 127u) == 0 && row < p.len_q)
+                        store_tile<HD>(&map_o, base + L::Q + t * L::TILE_BYTES, row, h, b);
                     if(lse && row < p.len_q)
                         lse[(size_t(b) * p.heads_q + h) * p.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 }

@@ -232,6 +232,51 @@ namespace b200wmma
             return a + b;
         }
 
+        // ---- results ----
+        __device__ __forceinline__ void tma_store_4d(const void* tmap, int32_t c0, int32_t c1, int32_t c2, int32_t c3, uint32_t src_smem)
+        {
+            asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                             reinterpret_cast<uint64_t>(tmap)),
+                         "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src_smem)
+                         : "memory");
+        }
+        // Columns [from, to) of this thread's row of an fp32 accumulator, times `by`, as 16-bit values into row `row` of a tile in
+        // shared memory with the 128-byte swizzle, from where TMA writes whole rows (a thread's own 16-byte stores to its row
+        // would each touch a line of their own: 2.5 us for a tile).  `live`: the accumulator counts, otherwise zeros.
+        template <typename T>
+        __device__ __forceinline__ void stage_row(uint8_t* tile, uint32_t row, uint32_t taddr, uint32_t from, uint32_t to, float by, bool live)
+        {
+#pragma unroll 1
+            for(uint32_t c = from; c < to; c += 32)
+            {
+                uint32_t w[32];
+                __syncwarp();
+                ptx::tmem_ld_32x32b_x32(taddr + c, w);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                {
+                    uint32_t u[4];
+#pragma unroll
+                    for(int j = 0; j < 4; ++j)
+                        u[j] = live ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * by, __uint_as_float(w[8 * i + 2 * j + 1]) * by) : 0u;
+                    const uint32_t at = c / 8 + i; // 16-byte piece of the row
+                    *reinterpret_cast<uint4*>(tile + (at / 8) * BOX_BYTES + row * 128 + (((at % 8) ^ (row & 7u)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            }
+        }
+        // One thread, after a barrier over those that staged (each with a proxy fence): writes the tile and waits until it has
+        // been read.  Rows and columns out of bounds are left out.
+        template <uint32_t HD>
+        __device__ __forceinline__ void store_tile(const CUtensorMap* map, uint32_t tile_smem, uint32_t token, uint32_t head, uint32_t batch)
+        {
+#pragma unroll
+            for(uint32_t s = 0; s < HD / 64; ++s)
+                tma_store_4d(map, s * 64, token, head, batch, tile_smem + s * BOX_BYTES);
+            ptx::bulk_commit_group();
+            ptx::bulk_wait_group_read<0>();
+        }
+
         // ---- masks by tile --------------------------------------------------------------------
         // Documents of a tile: {smallest, largest, any padding}; smallest > largest where there is nothing but padding.
         struct DocTile
