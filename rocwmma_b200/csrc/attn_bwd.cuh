@@ -333,19 +333,27 @@ namespace b200wmma
                                     const float  sv[4] = {s4.x, s4.y, s4.z, s4.w};
                                     float        pr[4];
 #pragma unroll
-                                    for(int k = 0; k < 4; ++k)
+                                    for(int k = 0; k < 4; k += 2)
                                     {
-                                        const int j    = i * 32 + j4 * 4 + k;
-                                        float     slip = 1.0f, x;
+                                        const int      j   = i * 32 + j4 * 4 + k;
+                                        const uint64_t dot = pair(__uint_as_float(v[i][j4 * 4 + k]), __uint_as_float(v[i][j4 * 4 + k + 1]));
+                                        const uint64_t sub = pair(-sv[k], -sv[k + 1]);
+                                        uint64_t       slip2 = pair(1.0f, 1.0f);
+                                        float          x[2], slip[2];
                                         if constexpr(CAP || BIAS)
-                                            x = score<CAP, BIAS>(sc, __uint_as_float(v[i][j4 * 4 + k]), from + static_cast<float>(j), slip) - sv[k];
+                                            unpair(add2(score2<CAP, BIAS>(sc, dot, from + static_cast<float>(j), 1.0f, slip2), sub), x[0], x[1]);
                                         else
-                                            x = fmaf(__uint_as_float(v[i][j4 * 4 + k]), sc.c, -sv[k]);
-                                        if constexpr(decltype(masked)::value)
-                                            if(!(seen >> j & 1u))
-                                                x = -INFINITY, slip = 0.0f; // the product may be NaN
-                                        pr[k]            = ex2(x);
-                                        v[i][j4 * 4 + k] = __float_as_uint(CAP ? pr[k] * slip : pr[k]);
+                                            unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
+                                        unpair(slip2, slip[0], slip[1]);
+#pragma unroll
+                                        for(int u = 0; u < 2; ++u)
+                                        {
+                                            if constexpr(decltype(masked)::value)
+                                                if(!(seen >> (j + u) & 1u))
+                                                    x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
+                                            pr[k + u]            = ex2(x[u]);
+                                            v[i][j4 * 4 + k + u] = __float_as_uint(CAP ? pr[k + u] * slip[u] : pr[k + u]);
+                                        }
                                     }
                                     w[2 * j4] = pack2<T>(pr[0], pr[1]), w[2 * j4 + 1] = pack2<T>(pr[2], pr[3]);
                                 }
@@ -640,18 +648,26 @@ namespace b200wmma
                         const float from    = static_cast<float>(at - int32_t(c0 + half * 64));
                         const auto  weights = [&](auto masked) {
 #pragma unroll
-                            for(int j = 0; j < 64; ++j)
+                            for(int j = 0; j < 64; j += 2)
                             {
-                                float slip = 1.0f, x;
+                                const uint64_t dot = pair(__uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1]));
+                                const uint64_t sub = pair(-ls, -ls);
+                                uint64_t       slip2 = pair(1.0f, 1.0f);
+                                float          x[2], slip[2];
                                 if constexpr(CAP || BIAS)
-                                    x = score<CAP, BIAS>(sc, __uint_as_float(v[j >> 5][j & 31]), from - static_cast<float>(j), slip) - ls;
+                                    unpair(add2(score2<CAP, BIAS>(sc, dot, from - static_cast<float>(j), -1.0f, slip2), sub), x[0], x[1]);
                                 else
-                                    x = fmaf(__uint_as_float(v[j >> 5][j & 31]), sc.c, -ls);
-                                if constexpr(decltype(masked)::value)
-                                    if(!(seen >> j & 1u))
-                                        x = -INFINITY, slip = 0.0f; // the product may be NaN
-                                x                 = ex2(x);
-                                v[j >> 5][j & 31] = __float_as_uint(CAP ? x * slip : x);
+                                    unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
+                                unpair(slip2, slip[0], slip[1]);
+#pragma unroll
+                                for(int u = 0; u < 2; ++u)
+                                {
+                                    if constexpr(decltype(masked)::value)
+                                        if(!(seen >> (j + u) & 1u))
+                                            x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
+                                    x[u]                    = ex2(x[u]);
+                                    v[j >> 5][(j & 31) + u] = __float_as_uint(CAP ? x[u] * slip[u] : x[u]);
+                                }
                             }
                         };
                         if(e >> 24 & TILE_MASK)

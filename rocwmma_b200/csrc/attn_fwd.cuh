@@ -263,11 +263,14 @@ namespace b200wmma
                         {
                             const float from = static_cast<float>(at - int32_t(c0));
 #pragma unroll
-                            for(int i = 0; i < 128; ++i)
+                            for(int i = 0; i < 128; i += 2)
                             {
-                                float unused;
-                                v[i >> 5][i & 31] = __float_as_uint(
-                                    score<CAP, BIAS>(sc, __uint_as_float(v[i >> 5][i & 31]), from - static_cast<float>(i), unused));
+                                uint64_t  unused;
+                                uint32_t *x = &v[i >> 5][i & 31], *y = x + 1;
+                                float     lo, hi;
+                                unpair(score2<CAP, BIAS>(sc, pair(__uint_as_float(*x), __uint_as_float(*y)), from - static_cast<float>(i), -1.0f, unused),
+                                       lo, hi);
+                                *x = __float_as_uint(lo), *y = __float_as_uint(hi);
                             }
                         }
                         if(f & TILE_MASK)

@@ -113,6 +113,12 @@ namespace b200wmma
             asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
             return r;
         }
+        __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+        {
+            uint64_t r;
+            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+            return r;
+        }
         // Largest of 128 numbers in four independent chains of three-input steps.
         __device__ __forceinline__ float max_of(const uint32_t (&v)[4][32])
         {
@@ -420,6 +426,33 @@ namespace b200wmma
                 x = dot * s.c;
             if constexpr(BIAS)
                 x = fmaf(-s.slope, fabsf(dist), x);
+            return x;
+        }
+
+        // The same for two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.  (Powers by a
+        // polynomial on the fused multiply-add pipe and one reciprocal for both measured slower: 332 us against 307 for 2 x 16
+        // heads of 4096 x 128, causal.  Instructions count here, not the unit behind ex2 and rcp.)
+        template <bool CAP, bool BIAS>
+        __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
+        {
+            uint64_t x;
+            if constexpr(CAP)
+            {
+                float a, b;
+                unpair(mul2(dot, pair(s.k1, s.k1)), a, b);
+                unpair(add2(pair(ex2(a), ex2(b)), pair(1.0f, 1.0f)), a, b);
+                const uint64_t tanh = fma2(pair(rcp(a), rcp(b)), pair(-2.0f, -2.0f), pair(1.0f, 1.0f));
+                slip = fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
+                x    = mul2(tanh, pair(s.cap2, s.cap2));
+            }
+            else
+                x = mul2(dot, pair(s.c, s.c));
+            if constexpr(BIAS)
+            {
+                float a, b;
+                unpair(x, a, b);
+                x = pair(fmaf(-s.slope, fabsf(dist), a), fmaf(-s.slope, fabsf(dist + step), b));
+            }
             return x;
         }
 

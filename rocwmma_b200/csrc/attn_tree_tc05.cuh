@@ -302,24 +302,36 @@ namespace b200wmma
                         {
                             const uint32_t see = MASK ? valid[i] & seen_of(bits, rel0 + 32 * i) : 0u;
 #pragma unroll
-                            for(int k = 0; k < 32; ++k)
+                            for(int k = 0; k < 32; k += 2)
                             {
-                                float unused, dist = 0.0f;
+                                uint64_t unused;
+                                float    dist = 0.0f, step = -1.0f, y[2];
                                 if constexpr(BIAS)
                                 {
                                     dist = static_cast<float>(at - rel0) - static_cast<float>(i * 32 + k);
                                     if constexpr(MASK)
-                                    {
-                                        const int32_t rel = rel0 + i * 32 + k;
-                                        if(rel >= 0 && p.depths && j0 + i * 32 + k < end)
-                                            dist = static_cast<float>(at - __ldg(p.depths + size_t(b) * p.drafts + rel));
-                                    }
+                                        if(p.depths && rel0 + i * 32 + k + 1 >= 0) // drafted tokens stand at their depths
+                                        {
+                                            const int32_t rel = rel0 + i * 32 + k;
+                                            const auto    d   = [&](int32_t to) {
+                                                return static_cast<float>(
+                                                    at - (to >= 0 && to < int32_t(n_drafts) ? __ldg(p.depths + size_t(b) * p.drafts + to) : to));
+                                            };
+                                            dist = d(rel);
+                                            step = d(rel + 1) - dist;
+                                        }
                                 }
-                                float y = attn::score<CAP, BIAS>(sc, __uint_as_float(v[i][k]), dist, unused);
-                                if constexpr(MASK)
-                                    if(!(see >> k & 1u))
-                                        y = -INFINITY;
-                                v[i][k] = __float_as_uint(y);
+                                attn::unpair(attn::score2<CAP, BIAS>(sc, attn::pair(__uint_as_float(v[i][k]), __uint_as_float(v[i][k + 1])), dist, step,
+                                                                     unused),
+                                             y[0], y[1]);
+#pragma unroll
+                                for(int e = 0; e < 2; ++e)
+                                {
+                                    if constexpr(MASK)
+                                        if(!(see >> (k + e) & 1u))
+                                            y[e] = -INFINITY;
+                                    v[i][k + e] = __float_as_uint(y[e]);
+                                }
                             }
                         }
                     };
