@@ -254,25 +254,24 @@ namespace b200wmma
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
-                        uint32_t v[4][32];
-#pragma unroll
-                        for(int i = 0; i < 4; ++i)
-                            ptx::tmem_ld_32x32b_x32(s_tmem[t] + lane_tmem + 32 * i, v[i]);
-                        ptx::tmem_ld_wait();
-                        if constexpr(!PLAIN)
-                        {
-                            const float from = static_cast<float>(at - int32_t(c0));
-#pragma unroll
-                            for(int i = 0; i < 128; i += 2)
+                        const uint32_t s_row = s_tmem[t] + lane_tmem;
+                        const float    from  = static_cast<float>(at - int32_t(c0));
+                        const auto     transform = [&](int i, uint32_t(&x)[32]) {
+                            if constexpr(!PLAIN)
                             {
-                                uint64_t  unused;
-                                uint32_t *x = &v[i >> 5][i & 31], *y = x + 1;
-                                float     lo, hi;
-                                unpair(score2<CAP, BIAS>(sc, pair(__uint_as_float(*x), __uint_as_float(*y)), from - static_cast<float>(i), -1.0f, unused),
-                                       lo, hi);
-                                *x = __float_as_uint(lo), *y = __float_as_uint(hi);
+#pragma unroll
+                                for(int k = 0; k < 32; k += 2)
+                                {
+                                    uint64_t unused;
+                                    float    lo, hi;
+                                    unpair(score2<CAP, BIAS>(sc, pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])),
+                                                             from - static_cast<float>(32 * i + k), -1.0f, unused),
+                                           lo, hi);
+                                    x[k] = __float_as_uint(lo), x[k + 1] = __float_as_uint(hi);
+                                }
                             }
-                        }
+                        };
+                        float top;
                         if(f & TILE_MASK)
                         {
                             uint32_t see[4];
@@ -287,12 +286,16 @@ namespace b200wmma
                                 for(int i = 0; i < 4; ++i)
                                     see[i] &= same[i];
                             }
+                            top = row_max<true>(s_row, [&](int i, uint32_t(&x)[32]) {
+                                transform(i, x);
 #pragma unroll
-                            for(int i = 0; i < 128; ++i)
-                                if(!(see[i >> 5] >> (i & 31) & 1u))
-                                    v[i >> 5][i & 31] = 0xFF800000u; // -infinity
+                                for(int k = 0; k < 32; ++k)
+                                    if(!(see[i] >> k & 1u))
+                                        x[k] = 0xFF800000u; // -infinity
+                            });
                         }
-                        float top = max_of(v);
+                        else
+                            top = row_max<!PLAIN>(s_row, transform);
                         if constexpr(PLAIN)
                             top *= sc.c; // scale > 0
                         // move the maximum where some row of this warp has outgrown it
@@ -323,7 +326,7 @@ namespace b200wmma
                             }
                         }
                         const float sub = m == -INFINITY ? 0.0f : -m;
-                        l += weights<T>(v, s_tmem[t] + lane_tmem, PLAIN ? sc.c : 1.0f, sub);
+                        l += weights<T>(s_row, PLAIN ? sc.c : 1.0f, sub);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();

@@ -119,19 +119,18 @@ namespace b200wmma
             asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
             return r;
         }
-        // Largest of 128 numbers in four independent chains of three-input steps.
-        __device__ __forceinline__ float max_of(const uint32_t (&v)[4][32])
+        // Largest of 32 numbers and `t`, in two independent chains of three-input steps.
+        __device__ __forceinline__ float max_of(const uint32_t (&v)[32], float t)
         {
-            float t[4];
+            float u = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
-            for(int i = 0; i < 4; ++i)
-                t[i] = fmaxf(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]));
-#pragma unroll
-            for(int k = 2; k < 32; k += 2)
-#pragma unroll
-                for(int i = 0; i < 4; ++i)
-                    t[i] = fmaxf(fmaxf(t[i], __uint_as_float(v[i][k])), __uint_as_float(v[i][k + 1]));
-            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            for(int k = 2; k < 32; k += 4)
+            {
+                t = fmaxf(fmaxf(t, __uint_as_float(v[k])), __uint_as_float(v[k + 1]));
+                if(k + 2 < 32)
+                    u = fmaxf(fmaxf(u, __uint_as_float(v[k + 2])), __uint_as_float(v[k + 3]));
+            }
+            return fmaxf(t, u);
         }
         template <typename T>
         __device__ __forceinline__ uint32_t pack2(float lo, float hi)
@@ -212,21 +211,51 @@ namespace b200wmma
             __syncwarp();
         }
 
-        // P of 128 scores: P = 2^(x c - m) in 16 bits over the scores' own columns; returns the sum of the unrounded P.
-        template <typename T>
-        __device__ __forceinline__ float weights(const uint32_t (&v)[4][32], uint32_t taddr, float c, float sub)
+        // The two passes of a softmax over a row of 128 scores in tensor memory, 32 columns at a time with the next 32 on their
+        // way, so that a thread holds 64 of them and not 128 (which spills, and costs more than reading tensor memory twice).
+        // First pass: the largest.  change(i, x) may alter columns 32 i .. 32 i + 31; WRITE puts them back for the second pass.
+        template <bool WRITE, typename F>
+        __device__ __forceinline__ float row_max(uint32_t taddr, F change)
         {
-            const uint64_t cc = pair(c, c), ss = pair(sub, sub);
-            uint64_t       sum[2] = {0, 0};
+            uint32_t v[2][32];
+            float    top = -INFINITY;
+            ptx::tmem_ld_32x32b_x32(taddr, v[0]);
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
+                ptx::tmem_ld_wait();
+                if(i < 3)
+                    ptx::tmem_ld_32x32b_x32(taddr + 32 * (i + 1), v[(i + 1) & 1]);
+                change(i, v[i & 1]);
+                top = max_of(v[i & 1], top);
+                if(WRITE)
+                    tmem_st_32x32b_x32(taddr + 32 * i, v[i & 1]);
+            }
+            if(WRITE)
+                tmem_st_wait();
+            return top;
+        }
+        // Second pass: P = 2^(x c + sub) in 16 bits over the scores' own first 64 columns, always behind the scores still to be
+        // read; returns the sum of the unrounded P.
+        template <typename T>
+        __device__ __forceinline__ float weights(uint32_t taddr, float c, float sub)
+        {
+            const uint64_t cc = pair(c, c), ss = pair(sub, sub);
+            uint64_t       sum[2] = {0, 0};
+            uint32_t       v[2][32];
+            ptx::tmem_ld_32x32b_x32(taddr, v[0]);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                ptx::tmem_ld_wait();
+                if(i < 3)
+                    ptx::tmem_ld_32x32b_x32(taddr + 32 * (i + 1), v[(i + 1) & 1]);
                 uint32_t w[16];
 #pragma unroll
                 for(int j = 0; j < 16; ++j)
                 {
                     float x, y;
-                    unpair(fma2(pair(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1])), cc, ss), x, y);
+                    unpair(fma2(pair(__uint_as_float(v[i & 1][2 * j]), __uint_as_float(v[i & 1][2 * j + 1])), cc, ss), x, y);
                     x = ex2(x), y = ex2(y);
                     sum[j & 1] = add2(sum[j & 1], pair(x, y));
                     w[j]       = pack2<T>(x, y);

@@ -290,17 +290,11 @@ namespace b200wmma
                     const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + L::VALID) + (n & 7u) * 4;
                     const int32_t   rel0  = int32_t(int64_t(j0) - len); // place of the tile's first token behind the cached ones
                     const bool      masked = (valid[0] & valid[1] & valid[2] & valid[3]) != 0xFFFFFFFFu || rel0 + int32_t(TILE) > 0;
-                    uint32_t        v[4][32];
-#pragma unroll
-                    for(int i = 0; i < 4; ++i)
-                        ptx::tmem_ld_32x32b_x32(s_tmem + u * TILE + lane_tmem + 32 * i, v[i]);
-                    ptx::tmem_ld_wait();
-                    const auto scores = [&](auto mask) {
-                        constexpr bool MASK = decltype(mask)::value;
-#pragma unroll
-                        for(int i = 0; i < 4; ++i)
-                        {
-                            const uint32_t see = MASK ? valid[i] & seen_of(bits, rel0 + 32 * i) : 0u;
+                    const uint32_t  s_row  = s_tmem + u * TILE + lane_tmem;
+                    const auto      scores = [&](auto mask) {
+                        return attn::row_max<true>(s_row, [&](int i, uint32_t(&v)[32]) {
+                            constexpr bool MASK = decltype(mask)::value;
+                            const uint32_t see  = MASK ? valid[i] & seen_of(bits, rel0 + 32 * i) : 0u;
 #pragma unroll
                             for(int k = 0; k < 32; k += 2)
                             {
@@ -321,8 +315,7 @@ namespace b200wmma
                                             step = d(rel + 1) - dist;
                                         }
                                 }
-                                attn::unpair(attn::score2<CAP, BIAS>(sc, attn::pair(__uint_as_float(v[i][k]), __uint_as_float(v[i][k + 1])), dist, step,
-                                                                     unused),
+                                attn::unpair(attn::score2<CAP, BIAS>(sc, attn::pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), dist, step, unused),
                                              y[0], y[1]);
 #pragma unroll
                                 for(int e = 0; e < 2; ++e)
@@ -330,16 +323,12 @@ namespace b200wmma
                                     if constexpr(MASK)
                                         if(!(see >> (k + e) & 1u))
                                             y[e] = -INFINITY;
-                                    v[i][k + e] = __float_as_uint(y[e]);
+                                    v[k + e] = __float_as_uint(y[e]);
                                 }
                             }
-                        }
+                        });
                     };
-                    if(masked)
-                        scores(std::true_type{});
-                    else
-                        scores(std::false_type{});
-                    const float top = attn::max_of(v);
+                    const float top = masked ? scores(std::true_type{}) : scores(std::false_type{});
                     // the maximum moves only where a score passes it by more than 2^8: until then weights grow up to 256
                     if(__any_sync(0xFFFFFFFFu, top > m + 8.0f))
                     {
@@ -367,7 +356,7 @@ namespace b200wmma
                         }
                     }
                     const float sub = m == -INFINITY ? 0.0f : m;
-                    l += attn::weights<T>(v, s_tmem + u * TILE + lane_tmem, 1.0f, -sub);
+                    l += attn::weights<T>(s_row, 1.0f, -sub);
                     attn::tmem_st_wait();
                     ptx::tc_fence_before_sync();
                     __syncwarp();
