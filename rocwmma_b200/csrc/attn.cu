@@ -24,10 +24,11 @@ namespace b200wmma
             DocTile*       dq = static_cast<DocTile*>(workspace);
             const uint32_t nq = uint32_t(tiles_of(p.len_q)), nk = uint32_t(tiles_of(p.len_kv));
             DocTile*       dk = dq + size_t(p.batch) * nq;
-            doc_tiles_kernel<<<ceil_div(p.batch * nq, 4), 128, 0, stream>>>(p.doc_q, p.len_q, nq, p.batch * nq, dq);
-            doc_tiles_kernel<<<ceil_div(p.batch * nk, 4), 128, 0, stream>>>(p.doc_kv, p.len_kv, nk, p.batch * nk, dk);
+            const bool     one = p.doc_q == p.doc_kv && p.len_q == p.len_kv; // queries and keys are the same tokens
+            const uint32_t total_q = one ? 0 : p.batch * nq, total = total_q + p.batch * nk;
+            doc_tiles_kernel<<<ceil_div(total, 4), 128, 0, stream>>>(p.doc_q, p.len_q, nq, total_q, dq, p.doc_kv, p.len_kv, nk, total, dk);
             B200_CHECK_CUDA(cudaGetLastError());
-            *q = dq, *kv = dk;
+            *q = one ? dk : dq, *kv = dk;
             return B200WMMA_OK;
         }
 
@@ -116,12 +117,18 @@ namespace b200wmma
             const uint32_t padded = uint32_t(tiles_of(p.len_q)) * TILE, rows = p.batch * p.heads_q * padded;
             bwd_rows_kernel<T><<<rows / 16, 256, 0, c.stream>>>(p, static_cast<const T*>(c.o), static_cast<const T*>(c.dout), c.lse, c.lse2, c.delta,
                                                                 padded, rows);
-            dkv<<<uint32_t(tiles_of(p.len_kv)) * p.batch * p.heads_kv, BWD_THREADS, BwdSmem<HD>::BYTES, c.stream>>>(
-                c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[5], c.maps[6], p, c.lse2, c.delta, c.docs_q, c.docs_kv,
-                c.status);
-            dq<<<uint32_t(tiles_of(p.len_q)) * p.batch * p.heads_q, BWD_THREADS, BwdSmem<HD>::BYTES, c.stream>>>(
-                c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[4], p, c.lse2, c.delta, c.docs_q, c.docs_kv, c.status);
             B200_CHECK_CUDA(cudaGetLastError());
+            cudaLaunchAttribute early{};
+            early.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+            early.val.programmaticStreamSerializationAllowed = 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.blockDim = dim3(BWD_THREADS), cfg.dynamicSmemBytes = BwdSmem<HD>::BYTES, cfg.stream = c.stream, cfg.attrs = &early, cfg.numAttrs = 1;
+            cfg.gridDim = dim3(uint32_t(tiles_of(p.len_kv)) * p.batch * p.heads_kv);
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dkv, c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[5], c.maps[6], p,
+                                               static_cast<const float*>(c.lse2), static_cast<const float*>(c.delta), c.docs_q, c.docs_kv, c.status));
+            cfg.gridDim = dim3(uint32_t(tiles_of(p.len_q)) * p.batch * p.heads_q);
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dq, c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[4], p, static_cast<const float*>(c.lse2),
+                                               static_cast<const float*>(c.delta), c.docs_q, c.docs_kv, c.status));
             return B200WMMA_OK;
         }
         template <typename T, uint32_t HD>

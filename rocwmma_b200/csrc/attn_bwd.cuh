@@ -4,6 +4,7 @@
 //   dkv: a block owns 128 keys of one key head and walks the queries of all its heads, with keys as tensor memory lanes:
 //        S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   dq:  a block owns 128 queries and walks the keys:  S = Q K^T, dP = dO V^T, dQ += dS K
+// The dq kernel does not need the other one's results and starts when its last blocks leave SMs idle.
 // with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
 // 256 threads compute, two to a lane (64 columns each); one warp issues the products, one the copies.
 #pragma once
@@ -48,6 +49,7 @@ namespace b200wmma
             bwd_rows_kernel(const __grid_constant__ Params p, const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse,
                             float* __restrict__ lse2, float* __restrict__ delta, uint32_t padded, uint32_t total)
         {
+            ptx::grid_dep_launch_dependents();
             const uint32_t at = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15u;
             const uint32_t i = at % padded, bh = at / padded, h = bh % p.heads_q, b = bh / p.heads_q;
             float          sum = 0.0f, s = -INFINITY;
@@ -142,6 +144,8 @@ namespace b200wmma
             ptx::tc_fence_before_sync();
             __syncthreads();
             ptx::tc_fence_after_sync();
+            ptx::grid_dep_wait(); // the row statistics are there; from here on the dq kernel may take SMs that this one leaves idle
+            ptx::grid_dep_launch_dependents();
             const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dv_tmem = tmem + 2 * TILE, dk_tmem = dv_tmem + HD;
 
             const uint32_t   n_stat = q_tiles * TILE; // padded rows of a head
@@ -516,7 +520,7 @@ namespace b200wmma
             if(warp < 8)
             {
                 const size_t stat = (size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row;
-                ls = lse2[stat], de = delta[stat];
+                ls = __ldcg(lse2 + stat), de = __ldcg(delta + stat);
             }
 
             for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
@@ -745,6 +749,9 @@ namespace b200wmma
                 ptx::tc_fence_after_sync();
                 ptx::tmem_dealloc(tmem, 512);
             }
+            // started beside the dkv kernel: the grid ends after it, so that whatever follows finds dk and dv written
+            if(blockIdx.x == gridDim.x - 1)
+                ptx::grid_dep_wait();
         }
     } // namespace attn
 } // namespace b200wmma

@@ -399,13 +399,21 @@ namespace b200wmma
             __syncthreads();
             return *length;
         }
-        // One warp to a tile of a batch entry.
-        static __global__ void __launch_bounds__(128) doc_tiles_kernel(const int32_t* docs, uint32_t len, uint32_t tiles, uint32_t total, DocTile* out)
+        // One warp to a tile of a batch entry: total_q tiles of queries, then tiles of keys up to `total`.
+        static __global__ void __launch_bounds__(128)
+            doc_tiles_kernel(const int32_t* docs_q, uint32_t len_q, uint32_t tiles_q, uint32_t total_q, DocTile* out_q, const int32_t* docs_kv,
+                             uint32_t len_kv, uint32_t tiles_kv, uint32_t total, DocTile* out_kv)
         {
-            const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+            uint32_t       at = blockIdx.x * 4 + (threadIdx.x >> 5);
+            const uint32_t lane = threadIdx.x & 31u;
             if(at >= total)
                 return;
-            const int32_t* d = docs + size_t(at / tiles) * len;
+            const bool     kv = at >= total_q;
+            const uint32_t tiles = kv ? tiles_kv : tiles_q, len = kv ? len_kv : len_q;
+            DocTile*       out = kv ? out_kv : out_q;
+            if(kv)
+                at -= total_q;
+            const int32_t* d  = (kv ? docs_kv : docs_q) + size_t(at / tiles) * len;
             const uint32_t i0 = at % tiles * TILE;
             int32_t        lo = INT32_MAX, hi = -1, neg = 0;
             for(uint32_t i = i0 + lane; i < min(i0 + TILE, len); i += 32)

@@ -5,11 +5,14 @@
 //  - values become 16-bit numbers two at a time, by putting the nibble into the mantissa of 1024 (fp16) or 128 (bf16) and
 //    subtracting that with the zero point: exact, since |q - z| <= 15;
 //  - the products are warp-level matrix instructions (16 outputs x 8 vectors x 16 columns, fp32 sums) even for one vector:
-//    a fused multiply-add per weight and vector would take the issue slots that the conversion needs.  tcgen05 would want
-//    tiles of 128 outputs in shared memory and has nothing to gain at 8 vectors;
+//    a fused multiply-add per weight and vector would take the issue slots that the conversion needs.  Beyond 8 vectors
+//    tcgen05 takes over (gemv_w4_tc05.cuh);
 //  - sums of a group are scaled in fp32, so nothing is rounded before y.
 // The columns' order inside a group of 32 is free as long as weights and x agree: lane t of four takes word t of each 16-byte
 // piece (8 weights), whose nibbles i and i + 4 come out as one pair, and x is permuted to that by four byte selections.
+// Measured (weights from memory): 1 x 16384 x 8192 fp16, groups of 128: 21.1 us (3.2 TB/s); 1 x 2048 x 2048: 2.8 us;
+// 7 x 5003 x 4128 bf16, groups of 32: 12 us; on tcgen05 32 x 14336 x 4096 bf16, groups of 64: 27 us (warp-level: 36 us),
+// 64 x 14336 x 4096: 29 us (50 us).  Neither memory nor one pipe is full then: instructions per weight and their latency bound it.
 #include "attn_common.cuh"
 #include "gemm_tc05_common.cuh"
 
@@ -17,8 +20,7 @@ namespace b200wmma
 {
     namespace gemv_w4
     {
-        constexpr uint32_t WARPS   = 8;
-        constexpr uint32_t THREADS = 32 * WARPS;
+        constexpr uint32_t FEW_VECTORS = 8; // the warp-level kernel's; more take the tcgen05 form
 
         struct Args
         {
@@ -50,21 +52,19 @@ namespace b200wmma
         {
             asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
         }
+        // Plain loads from shared memory at a byte address of the shared window: unlike volatile assembly they may be scheduled
+        // ahead of the products before them.
         __device__ __forceinline__ uint32_t lds32(uint32_t at)
         {
-            uint32_t v;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-            return v;
-        }
-        __device__ __forceinline__ void sts128(uint32_t at, const uint4& v)
-        {
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            return *static_cast<const uint32_t*>(__cvta_shared_to_generic(at));
         }
         __device__ __forceinline__ uint4 lds128(uint32_t at)
         {
-            uint4 v;
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-            return v;
+            return *static_cast<const uint4*>(__cvta_shared_to_generic(at));
+        }
+        __device__ __forceinline__ void sts128(uint32_t at, const uint4& v)
+        {
+            *static_cast<uint4*>(__cvta_shared_to_generic(at)) = v;
         }
         // c = a b + d: `d` is c, or 0 for the first product of a sum
         template <typename T>
@@ -72,11 +72,11 @@ namespace b200wmma
         {
             const float d0 = fresh ? 0.0f : c[0], d1 = fresh ? 0.0f : c[1], d2 = fresh ? 0.0f : c[2], d3 = fresh ? 0.0f : c[3];
             if constexpr(std::is_same<T, __half>::value)
-                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                              : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                              : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
             else
-                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                              : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                              : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
         }
@@ -216,6 +216,20 @@ namespace b200wmma
             }
         }
 
+        // Sum of the same place in the shared memory of a cluster's first `parts` (at most 8) blocks, in order; the loads are all
+        // on their way before the first is added.
+        __device__ __forceinline__ float cluster_sum(const float* at, uint32_t parts)
+        {
+            uint32_t v[8];
+#pragma unroll
+            for(uint32_t c = 0; c < 8; ++c)
+                v[c] = c < parts ? ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(at), c)) : 0u;
+            float s = __uint_as_float(v[0]);
+#pragma unroll
+            for(uint32_t c = 1; c < 8; ++c)
+                s += __uint_as_float(v[c]);
+            return s;
+        }
         template <typename T>
         __device__ __forceinline__ void put(const Args& p, uint32_t r, uint32_t i, float s)
         {
@@ -233,6 +247,15 @@ namespace b200wmma
             }
         }
 
+    } // namespace gemv_w4
+} // namespace b200wmma
+
+#include "gemv_w4_tc05.cuh"
+
+namespace b200wmma
+{
+    namespace gemv_w4
+    {
         // Up to 8 vectors.  A block owns 16 outputs; its W warps share the columns in stretches of 256, each through a ring of its
         // own in shared memory (128 bytes of each row, and the x that belongs to them), so warps never wait for one another
         // before the sums meet.  Few outputs: a cluster of blocks shares the columns too and the sums meet in the first
@@ -245,12 +268,26 @@ namespace b200wmma
         {
             static constexpr uint32_t W_STAGE = FEW_ROWS * FEW_K / 2, ZERO = 512; // zeros: the x of vectors that do not exist
             uint32_t x_warp, bytes; // bytes of a warp's x
-            __host__ __device__ Few(uint32_t w, uint32_t rows, uint32_t n, uint32_t parts)
+            // one vector, kept whole
+            __host__ __device__ Few(uint32_t w, uint32_t n, uint32_t parts)
             {
                 const uint32_t stretches = (n + FEW_K - 1) / FEW_K;
-                x_warp = rows == 1 ? (stretches + w * parts - 1) / (w * parts) * FEW_K * 2 : FEW_STAGES * rows * FEW_K * 2;
-                const uint32_t ring = w * (FEW_STAGES * W_STAGE + x_warp), red = w * 128 * 4; // the sums reuse the ring
-                bytes = ZERO + (ring > red ? ring : red);
+                x_warp = (stretches + w * parts - 1) / (w * parts) * FEW_K * 2;
+                bytes  = total(w, x_warp);
+            }
+            // x in rings
+            static __host__ __device__ uint32_t ring_x(uint32_t rows)
+            {
+                return FEW_STAGES * rows * FEW_K * 2;
+            }
+            static __host__ __device__ uint32_t ring_bytes(uint32_t w, uint32_t rows)
+            {
+                return total(w, ring_x(rows));
+            }
+            static __host__ __device__ uint32_t total(uint32_t w, uint32_t x)
+            {
+                const uint32_t ring = w * (FEW_STAGES * W_STAGE + x), red = w * 128 * 4; // the sums reuse the ring
+                return ZERO + (ring > red ? ring : red);
             }
         };
         template <typename T, bool SIGNED, int W, int STEPS, bool ONE>
@@ -258,11 +295,11 @@ namespace b200wmma
         {
             constexpr int GROUPS = STEPS == 0 ? 8 : 8 / STEPS, INFO = GROUPS > 4 ? 2 : 1;
             extern __shared__ __align__(1024) uint8_t smem[];
-            const Few      f(W, ONE ? 1 : p.rows, p.n, parts);
+            const uint32_t x_warp = ONE ? Few(W, p.n, parts).x_warp : Few::ring_x(p.rows);
             const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
             const uint32_t part_id = parts > 1 ? blockIdx.x % parts : 0, row0 = (parts > 1 ? blockIdx.x / parts : blockIdx.x) * FEW_ROWS;
-            const uint32_t zero = ptx::smem_u32(smem), ring = zero + Few::ZERO + warp * (FEW_STAGES * Few::W_STAGE + f.x_warp);
-            const uint32_t ring_x = ring + FEW_STAGES * Few::W_STAGE, x_stage = f.x_warp / FEW_STAGES;
+            const uint32_t zero = ptx::smem_u32(smem), ring = zero + Few::ZERO + warp * (FEW_STAGES * Few::W_STAGE + x_warp);
+            const uint32_t ring_x = ring + FEW_STAGES * Few::W_STAGE, x_stage = x_warp / FEW_STAGES;
             const uint32_t stretches = (p.n + FEW_K - 1) / FEW_K, stride = W * parts, first = part_id * W + warp;
             const uint32_t mine = first < stretches ? (stretches - first - 1) / stride + 1 : 0;
             const bool     rows_full = row0 + FEW_ROWS <= p.m;
@@ -418,9 +455,7 @@ namespace b200wmma
                 if(part_id == 0)
                     for(uint32_t e = threadIdx.x; e < outs; e += 32 * W)
                     {
-                        float s = red[e];
-                        for(uint32_t c = 1; c < parts; ++c)
-                            s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + e), c)));
+                        const float s = cluster_sum(red + e, parts);
                         if(row0 + e % FEW_ROWS < p.m)
                             put<T>(p, e / FEW_ROWS, row0 + e % FEW_ROWS, s);
                     }
@@ -428,136 +463,9 @@ namespace b200wmma
             }
         }
 
-        // More vectors, 8 NT to a block: its warps own 16 outputs each and share x in shared memory.  A cluster of blocks
-        // shares the columns where there are few blocks.
-        constexpr uint32_t MANY_K = 128, MANY_ROWS = 16 * WARPS;
-        template <int NT>
-        struct Many
-        {
-            static constexpr uint32_t W_BYTES = MANY_ROWS * MANY_K / 2, X_BYTES = 8 * NT * MANY_K * 2, STAGE = W_BYTES + X_BYTES;
-            static constexpr uint32_t STAGES = NT == 8 ? 4 : 6;
-            static constexpr uint32_t BYTES  = STAGES * STAGE;
-            static_assert(BYTES >= MANY_ROWS * 8 * NT * 4, "the sums of a cluster reuse the ring");
-        };
-        template <typename T, bool SIGNED, int NT>
-        __global__ void __launch_bounds__(THREADS) many_kernel(const __grid_constant__ Args p, uint32_t parts)
-        {
-            using S = Many<NT>;
-            extern __shared__ __align__(128) uint8_t smem[];
-            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-            const uint32_t part_id = blockIdx.x % parts, row0 = blockIdx.x / parts * MANY_ROWS, vec0 = blockIdx.y * 8 * NT;
-            const uint32_t ring = ptx::smem_u32(smem), stretches = (p.n + MANY_K - 1) / MANY_K;
-            const uint32_t from = uint32_t(uint64_t(stretches) * part_id / parts), mine = uint32_t(uint64_t(stretches) * (part_id + 1) / parts) - from;
-            const uint32_t ra = min(row0 + warp * 16 + g, p.m - 1), rb = min(row0 + warp * 16 + g + 8, p.m - 1);
-
-            const auto fetch = [&](uint32_t i) {
-                const uint32_t k0 = (from + i) * MANY_K, at = ring + (i % S::STAGES) * S::STAGE;
-#pragma unroll
-                for(uint32_t j = threadIdx.x; j < MANY_ROWS * 4; j += THREADS)
-                {
-                    const uint32_t r = j >> 2, c = j & 3u, k = k0 + c * 32;
-                    const bool     there = k < p.n;
-                    copy16(at + r * 64 + ((c ^ ((r >> 1) & 3u)) << 4), p.a + size_t(min(row0 + r, p.m - 1)) * p.lda + (there ? k / 2 : 0), there);
-                }
-                const T* x = static_cast<const T*>(p.x);
-#pragma unroll
-                for(uint32_t j = threadIdx.x; j < 8 * NT * 16; j += THREADS)
-                {
-                    const uint32_t r = j >> 4, c = j & 15u, k = k0 + c * 8;
-                    const bool     there = k < p.n && vec0 + r < p.rows;
-                    copy16(at + S::W_BYTES + r * 256 + ((c ^ ((r & 1u) << 2)) << 4), x + (there ? size_t(vec0 + r) * p.ldx + k : 0), there);
-                }
-            };
-            float sum[NT][4] = {}, part[NT][4] = {};
-            GroupInfo<T, SIGNED, 1> info, next;
-            const auto groups_of = [&](uint32_t i, GroupInfo<T, SIGNED, 1>& to) {
-                const uint32_t k0 = (from + i) * MANY_K;
-                to.load(p, ra, rb, k0 / p.group + t, min(p.groups - 1, (k0 + MANY_K - 1) / p.group));
-            };
-#pragma unroll
-            for(uint32_t i = 0; i < S::STAGES - 1; ++i)
-            {
-                if(i < mine)
-                    fetch(i);
-                copy_commit();
-            }
-            if(mine)
-                groups_of(0, next);
-            for(uint32_t i = 0; i < mine; ++i)
-            {
-                info = next;
-                if(i + 1 < mine)
-                    groups_of(i + 1, next);
-                copy_wait<S::STAGES - 2>();
-                __syncthreads(); // the stage is there for everyone, and everyone has read the one that is fetched into next
-                if(i + S::STAGES - 1 < mine)
-                    fetch(i + S::STAGES - 1);
-                copy_commit();
-                const uint32_t k0 = (from + i) * MANY_K, at = ring + (i % S::STAGES) * S::STAGE;
-                const uint32_t wa = at + (warp * 16 + g) * 64, flip = (g >> 1) & 3u;
-                uint32_t       grp = 0, left = p.group - k0 % p.group;
-                Offset<T>      z[2];
-                info.offsets(0, lane, z);
-#pragma unroll
-                for(uint32_t c = 0; c < 4; ++c)
-                {
-                    const uint32_t w0 = lds32(wa + ((c ^ flip) << 4) + t * 4), w1 = lds32(wa + 512 + ((c ^ flip) << 4) + t * 4);
-                    uint4          x[NT];
-#pragma unroll
-                    for(int v = 0; v < NT; ++v)
-                        x[v] = pair_up(lds128(at + S::W_BYTES + (v * 8 + g) * 256 + (((c * 4 + t) ^ ((g & 1u) << 2)) << 4)));
-                    step<T, SIGNED, NT>(w0, w1, x, z, part, false);
-                    left -= 32;
-                    if(left == 0 || c == 3)
-                    {
-                        info.template flush<NT>(grp, lane, sum, part);
-#pragma unroll
-                        for(int v = 0; v < NT; ++v)
-                            part[v][0] = part[v][1] = part[v][2] = part[v][3] = 0.0f;
-                        if(left == 0)
-                        {
-                            left = p.group;
-                            ++grp;
-                            if(!SIGNED && c != 3)
-                                info.offsets(grp, lane, z);
-                        }
-                    }
-                }
-            }
-            copy_wait<0>();
-            __syncthreads();
-            // [vector][output] in shared memory, so that outputs are written next to one another
-            float* red = reinterpret_cast<float*>(smem);
-#pragma unroll
-            for(int v = 0; v < NT; ++v)
-#pragma unroll
-                for(int j = 0; j < 4; ++j)
-                    red[(v * 8 + t * 2 + (j & 1)) * MANY_ROWS + warp * 16 + g + 8 * (j >> 1)] = sum[v][j];
-            if(parts > 1)
-                ptx::cluster_sync();
-            else
-                __syncthreads();
-            // the blocks of a cluster share the outputs among them
-            for(uint32_t e = part_id * THREADS + threadIdx.x; e < MANY_ROWS * 8 * NT; e += parts * THREADS)
-            {
-                const uint32_t r = vec0 + e / MANY_ROWS, i = row0 + e % MANY_ROWS;
-                if(r >= p.rows || i >= p.m)
-                    continue;
-                float s = 0.0f;
-                if(parts > 1)
-                    for(uint32_t c = 0; c < parts; ++c)
-                        s += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(ptx::smem_u32(red + e), c)));
-                else
-                    s = red[e];
-                put<T>(p, r, i, s);
-            }
-            if(parts > 1)
-                ptx::cluster_sync(); // no block leaves while another reads its sums
-        }
-
-        template <typename K>
+        template <typename K, typename... More>
         static int launch_clusters(K kern, const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem,
-                                   uint32_t threads, cudaStream_t stream)
+                                   uint32_t threads, cudaStream_t stream, More... more)
         {
             B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
@@ -566,46 +474,68 @@ namespace b200wmma
             attr.id               = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
             cfg.attrs = &attr, cfg.numAttrs = parts > 1 ? 1 : 0;
-            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p, parts));
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p, parts, more...));
             return B200WMMA_OK;
         }
-        // Blocks of a cluster: as many as keep every part busy for a stretch, up to 8 and to two blocks per SM.
-        static uint32_t parts_of(uint64_t blocks, uint32_t most)
+        // Blocks of a cluster: a power of two, up to 8, to `most` (parts with work enough) and to per_sm blocks on an SM.
+        static uint32_t parts_of(uint64_t blocks, uint32_t most, uint32_t per_sm)
         {
             uint32_t parts = 1;
-            while(parts < 8 && 2 * parts <= most && blocks * parts * 2 <= 2 * 148)
+            while(parts < 8 && 2 * parts <= most && blocks * parts * 2 <= per_sm * 148)
                 parts *= 2;
             return parts;
         }
-        template <typename T, bool SIGNED, int NT>
-        static int launch_many(const Args& p, cudaStream_t stream)
-        {
-            const uint32_t blocks = ceil_div(p.m, MANY_ROWS), blocks_y = ceil_div(p.rows, 8 * NT);
-            return launch_clusters(many_kernel<T, SIGNED, NT>, p, blocks, blocks_y, parts_of(uint64_t(blocks) * blocks_y, ceil_div(p.n, 4 * MANY_K)),
-                                   Many<NT>::BYTES, THREADS, stream);
-        }
-#ifndef W4_W
-#define W4_W 8
-#endif
-        template <typename T, bool SIGNED, int W, int STEPS>
-        static int launch_warps(const Args& p, uint32_t blocks, cudaStream_t stream)
-        {
-            const uint32_t parts = parts_of(blocks, ceil_div(p.n, W * FEW_K));
-            const Few      f(W, p.rows, p.n, parts);
-            return p.rows == 1 ? launch_clusters(few_kernel<T, SIGNED, W, STEPS, true>, p, blocks, 1, parts, f.bytes, 32 * W, stream)
-                               : launch_clusters(few_kernel<T, SIGNED, W, STEPS, false>, p, blocks, 1, parts, f.bytes, 32 * W, stream);
-        }
+        // Warps of a block: 8 for one vector (16384 x 8192 fp16: 21 us, 24 with 4), 4 for more, whose rings would leave room for
+        // one or two blocks on an SM (7 x 5003 x 4128 bf16, groups of 32: 12 us, 14 with 8).  One vector that is too long to lie in
+        // shared memory next to the rings goes through them like several.
+        constexpr uint32_t ONE_BYTES = 100 * 1024;
         template <typename T, bool SIGNED, int STEPS>
         static int launch_few(const Args& p, cudaStream_t stream)
         {
-            return launch_warps<T, SIGNED, W4_W, STEPS>(p, ceil_div(p.m, FEW_ROWS), stream);
+            const uint32_t blocks = ceil_div(p.m, FEW_ROWS);
+            if(p.rows == 1)
+            {
+                const uint32_t parts = parts_of(blocks, ceil_div(p.n, 8 * FEW_K), 2);
+                const Few      f(8, p.n, parts);
+                if(f.bytes <= ONE_BYTES)
+                    return launch_clusters(few_kernel<T, SIGNED, 8, STEPS, true>, p, blocks, 1, parts, f.bytes, 256, stream);
+            }
+            const uint32_t parts = parts_of(blocks, ceil_div(p.n, 4 * FEW_K), 2);
+            return launch_clusters(few_kernel<T, SIGNED, 4, STEPS, false>, p, blocks, 1, parts, Few::ring_bytes(4, p.rows), 128, stream);
+        }
+        template <typename T, bool SIGNED, int N, int SETS>
+        static int launch_tc(const Args& p, cudaStream_t stream)
+        {
+            unsigned* status = nullptr;
+            if(int e = status_word_ptr(&status))
+                return e;
+            using L = TcSmem<N, SETS>;
+            const uint32_t blocks = ceil_div(p.m, TC_M), blocks_y = ceil_div(p.rows, uint32_t(N));
+            const uint32_t parts = parts_of(uint64_t(blocks) * blocks_y, ceil_div(p.n, 2 * TC_K), 1);
+            CUtensorMap    map;
+            if(int e = tc05::make_kmajor_tmap(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                              p.x, p.rows, p.n, p.ldx, N))
+                return e;
+            return launch_clusters(tc_kernel<T, SIGNED, N, SETS>, p, blocks, blocks_y, parts, L::BYTES, TC_THREADS, stream, status, map);
+        }
+        template <typename T, bool SIGNED, int SETS>
+        static int launch_tc_rows(const Args& p, cudaStream_t stream)
+        {
+            if constexpr(SETS == 1)
+                if(p.rows > 32)
+                    return launch_tc<T, SIGNED, 64, SETS>(p, stream);
+            if constexpr(SETS <= 2)
+                if(p.rows > 16)
+                    return launch_tc<T, SIGNED, 32, SETS>(p, stream);
+            return launch_tc<T, SIGNED, 16, SETS>(p, stream);
         }
         template <typename T, bool SIGNED>
         static int launch(const Args& p, cudaStream_t stream)
         {
-            if(p.rows > 8)
-                return p.rows <= 16 ? launch_many<T, SIGNED, 2>(p, stream)
-                       : p.rows <= 32 ? launch_many<T, SIGNED, 4>(p, stream) : launch_many<T, SIGNED, 8>(p, stream);
+            if(p.rows > FEW_VECTORS)
+                return p.group % TC_K == 0 ? launch_tc_rows<T, SIGNED, 1>(p, stream)
+                       : p.group == 64     ? launch_tc_rows<T, SIGNED, 2>(p, stream) : launch_tc_rows<T, SIGNED, 4>(p, stream);
+
             if(p.group % FEW_K == 0)
                 return launch_few<T, SIGNED, 8>(p, stream);
             return p.group == 128 ? launch_few<T, SIGNED, 4>(p, stream)

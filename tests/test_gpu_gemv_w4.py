@@ -65,7 +65,7 @@ def check(m, n, rows, group, dtype, zeros=False, out=None, alpha=1.0, beta=0.0, 
 @pytest.mark.parametrize("m,n,rows,group", [
     (1, 32, 1, 32), (16, 256, 1, 128), (17, 96, 2, 64), (100, 4128, 1, 128), (33, 2048, 8, 32), (250, 1056, 3, 96), (64, 8192, 9, 128),
     (129, 544, 16, 64), (70, 320, 17, 1024), (40, 1280, 33, 256), (19, 2080, 64, 32), (24, 64, 65, 32), (13, 288, 130, 160),
-    (2051, 224, 5, 64), (16, 40000, 4, 4000)])
+    (2051, 224, 5, 64), (16, 40000, 4, 4000), (5, 200000, 1, 128), (5, 200000, 2, 96), (130, 96, 12, 32), (260, 1600, 40, 320)])
 def test_matches_the_definition(m, n, rows, group, dtype, zeros):
     check(m, n, rows, group, dtype, zeros, seed=m + n)
 
