@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "librocwmma_b200.so")
@@ -25,6 +26,10 @@ class AttnArgs(C.Structure):
                 + [(n, vp) for n in ("slopes", "prefix", "doc_q", "doc_kv")]
                 + [(n, AttnStrides) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")])
 
+
+# The same bytes from one call of pack(): a Structure of nested ones costs as much as the launch.
+ATTN_ARGS = struct.Struct("=6I2i2f4Q24q")
+assert ATTN_ARGS.size == C.sizeof(AttnArgs)
 
 # name -> (restype, argtypes); mirrors include/rocwmma_b200.h one to one
 SIGNATURES = {
@@ -81,10 +86,10 @@ SIGNATURES = {
     "b200wmma_gemv_w4": (C.c_int, [u32, u32, u32, vp, u32, vp, u32, vp, u32, u32, vp, u32, vp, u32, f32, f32,
                                    C.c_int, C.c_int, vp]),
     "b200wmma_attn_workspace_bytes": (sz, [u32, u32, u32, u32, C.c_int]),
-    "b200wmma_attn_fwd": (C.c_int, [C.POINTER(AttnArgs), vp, vp, vp, vp, vp, vp, sz, vp]),
-    "b200wmma_attn_bwd": (C.c_int, [C.POINTER(AttnArgs), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "b200wmma_attn_fwd": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "b200wmma_attn_bwd": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "b200wmma_attn_tree_workspace_bytes": (sz, [u32, u32, u32, u32, u32, u32]),
-    "b200wmma_attn_tree": (C.c_int, [C.POINTER(AttnArgs), u32, vp, vp, vp, u32, u32, vp, u32, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "b200wmma_attn_tree": (C.c_int, [vp, u32, vp, vp, vp, u32, u32, vp, u32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "b200wmma_mg_unique_id": (C.c_int, [vp]),
     "b200wmma_mg_create": (C.c_int, [C.POINTER(vp), vp, C.c_int, C.c_int]),
     "b200wmma_mg_broadcast": (C.c_int, [vp, vp, C.c_size_t, C.c_int, vp]),

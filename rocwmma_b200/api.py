@@ -12,7 +12,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import AttnArgs, B200WmmaError, check, lib
+from ._lib import ATTN_ARGS, B200WmmaError, check, lib
 
 ROW_MAJOR, COL_MAJOR = 0, 1
 OUT_F16, OUT_F32 = 0, 1
@@ -274,11 +274,17 @@ def gemv(m, n, a, lda, x, y, alpha, beta, layout_a=ROW_MAJOR):
 _DATA_TYPES = {torch.float16: OUT_F16, torch.bfloat16: OUT_BF16}
 
 
-def _need_here(t, dtype, name):
-    """A CUDA tensor of this type on the current device (the library launches there)."""
-    _need(t, dtype, name)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _need_here(t, dtype, name, device):
+    """A CUDA tensor of this type on the current device (the library launches there); returns its address."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
+        _need(t, dtype, name)
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{device}")
+    return t.data_ptr()
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def gemv_w4(m, n, rows, a_packed, lda_bytes, scales, ld_scales, group, x, ldx, y, ldy, alpha, beta, zeros=None, ld_zeros=0):
@@ -286,80 +292,83 @@ def gemv_w4(m, n, rows, a_packed, lda_bytes, scales, ld_scales, group, x, ldx, y
     zero point) to `group` columns of a row.  x and scales fp16 or bf16, y of that type or fp32.  zeros (uint8) makes the
     values unsigned; without it they are signed."""
     dt = x.dtype if isinstance(x, torch.Tensor) else None
+    out = y.dtype if isinstance(y, torch.Tensor) else None
     if dt not in _DATA_TYPES:
         raise TypeError("x must be a float16 or bfloat16 tensor")
-    _need_here(a_packed, torch.uint8, "a_packed"); _need_here(scales, dt, "scales"); _need_here(x, dt, "x")
-    out = y.dtype if isinstance(y, torch.Tensor) else None
-    if out not in (dt, torch.float32):
+    if out is not dt and out is not torch.float32:
         raise TypeError("y must have the type of x, or float32")
-    _need_here(y, out, "y")
-    if zeros is not None:
-        _need_here(zeros, torch.uint8, "zeros")
-    check(lib().b200wmma_gemv_w4(m, n, rows, _ptr(a_packed), lda_bytes, _ptr(scales), ld_scales, _ptr(zeros), ld_zeros, group,
-                                 _ptr(x), ldx, _ptr(y), ldy, alpha, beta, _DATA_TYPES[dt],
-                                 OUT_F32 if out == torch.float32 else _DATA_TYPES[dt], _stream()))
+    here = torch.cuda.current_device() if x.is_cuda else None
+    kind = _DATA_TYPES[dt]
+    check(lib().b200wmma_gemv_w4(m, n, rows, _need_here(a_packed, torch.uint8, "a_packed", here), lda_bytes,
+                                 _need_here(scales, dt, "scales", here), ld_scales,
+                                 None if zeros is None else _need_here(zeros, torch.uint8, "zeros", here), ld_zeros, group,
+                                 _need_here(x, dt, "x", here), ldx, _need_here(y, out, "y", here), ldy, alpha, beta, kind,
+                                 kind if out is dt else OUT_F32, _raw_stream(here)))
 
 
-def _attn_args(q, k, v, o, scale, cap, slopes):
-    """AttnArgs of q, o [batch, tokens, heads_q, dim] and k, v [batch or pages, tokens, heads_kv, dim]."""
+def _attn_tensor(t, dtype, name, device, shape=None):
+    """Address of a four-dimensional tensor with contiguous rows."""
+    at = _need_here(t, dtype, name, device)
+    if t.dim() != 4 or t.stride(3) != 1 or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must have four dimensions, the last one contiguous" + (f", of shape {tuple(shape)}" if shape else ""))
+    return at
+
+
+def _attn_vector(t, dtype, shape, name, device):
+    """Address of a contiguous tensor of this shape, 0 for None."""
+    if t is None:
+        return 0
+    at = _need_here(t, dtype, name, device)
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, of shape {shape}")
+    return at
+
+
+def _attn_type(q):
+    """(type, data_type, current device) of a call whose first tensor is q."""
     dt = q.dtype if isinstance(q, torch.Tensor) else None
-    if dt not in _DATA_TYPES:
-        raise TypeError("q must be a float16 or bfloat16 tensor")
-    a = AttnArgs()
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", o)):
-        _attn_tensor(a, name, t, dt)
-    if k.shape != v.shape or o.shape != q.shape or q.shape[3] != k.shape[3]:
-        raise ValueError("o must have the shape of q, v the shape of k, and both the same head size")
-    a.batch, _, a.heads_q, a.head_dim = q.shape
-    a.heads_kv = k.shape[2]
-    a.data_type, a.scale, a.cap = _DATA_TYPES[dt], scale, cap
-    if slopes is not None:
-        _attn_vector(slopes, torch.float32, (a.heads_q,), "slopes")
-        a.slopes = slopes.data_ptr()
-    return a
+    if dt not in _DATA_TYPES or not q.is_cuda:
+        raise TypeError("q must be a float16 or bfloat16 CUDA tensor")
+    return dt, _DATA_TYPES[dt], torch.cuda.current_device()
 
 
-def _attn_tensor(a, name, t, dt):
-    _need_here(t, dt, name)
-    if t.dim() != 4 or t.stride(3) != 1:
-        raise ValueError(f"{name} must have four dimensions, the last one contiguous")
-    s = getattr(a, name)
-    s.batch, s.token, s.head = t.stride()[:3]
+_NO_STRIDES = (0, 0, 0)
 
 
-def _attn_vector(t, dtype, shape, name):
-    _need_here(t, dtype, name)
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous, of shape {tuple(shape)}")
+def _attn_call(q, k, v, o, lse, scale, causal, cap, slopes, prefix, doc_q, doc_kv, workspace, grads=()):
+    """Checked tensors of attn_fwd and attn_bwd: (packed arguments, addresses, workspace address and size, stream)."""
+    dt, kind, here = _attn_type(q)
+    at = [_attn_tensor(q, dt, "q", here), _attn_tensor(k, dt, "k", here)]
+    batch, len_q, heads_q, dim = q.shape
+    len_kv, heads_kv = k.shape[1], k.shape[2]
+    if k.shape[0] != batch or k.shape[3] != dim:
+        raise ValueError("q and k must have the same batch and head size")
+    at += [_attn_tensor(v, dt, "v", here, k.shape), _attn_tensor(o, dt, "o", here, q.shape)]
+    strides = q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + o.stride()[:3]
+    for name, t, like in grads:
+        at.append(_attn_tensor(t, dt, name, here, like.shape))
+        strides += t.stride()[:3]
+    at.append(_attn_vector(lse, torch.float32, (batch, heads_q, len_q), "lse", here))
+    args = ATTN_ARGS.pack(batch, heads_q, heads_kv, len_q, len_kv, dim, kind, bool(causal), scale, cap,
+                          _attn_vector(slopes, torch.float32, (heads_q,), "slopes", here),
+                          _attn_vector(prefix, torch.int32, (batch,), "prefix", here),
+                          _attn_vector(doc_q, torch.int32, (batch, len_q), "doc_q", here),
+                          _attn_vector(doc_kv, torch.int32, (batch, len_kv), "doc_kv", here),
+                          *strides, *(_NO_STRIDES * (4 - len(grads))))
+    return args, at, *_attn_workspace(workspace, here), _raw_stream(here)
 
 
-def _attn_workspace(workspace):
+def _attn_workspace(workspace, device):
     if workspace is None:
-        return None, 0
-    _need_here(workspace, torch.uint8, "workspace")
+        return 0, 0
+    at = _need_here(workspace, torch.uint8, "workspace", device)
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    return _ptr(workspace), workspace.numel()
-
-
-def _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv):
-    if k.shape[0] != q.shape[0]:
-        raise ValueError("q and k must have the same batch")
-    a.len_q, a.len_kv, a.causal = q.shape[1], k.shape[1], int(causal)
-    if prefix is not None:
-        _attn_vector(prefix, torch.int32, (a.batch,), "prefix")
-        a.prefix = prefix.data_ptr()
-    if doc_q is not None:
-        _attn_vector(doc_q, torch.int32, (a.batch, a.len_q), "doc_q")
-        a.doc_q = doc_q.data_ptr()
-    if doc_kv is not None:
-        _attn_vector(doc_kv, torch.int32, (a.batch, a.len_kv), "doc_kv")
-        a.doc_kv = doc_kv.data_ptr()
-    if lse is not None:
-        _attn_vector(lse, torch.float32, (a.batch, a.heads_q, a.len_q), "lse")
+    return at, workspace.numel()
 
 
 def attn_workspace_bytes(batch, heads_q, len_q, len_kv, backward):
+    """Bytes of scratch for attn_fwd with documents, or for attn_bwd."""
     return lib().b200wmma_attn_workspace_bytes(batch, heads_q, len_q, len_kv, int(backward))
 
 
@@ -367,29 +376,23 @@ def attn_fwd(q, k, v, o, lse, scale, causal=False, cap=0.0, slopes=None, prefix=
     """o = softmax(scores) v with scores = cap * tanh(scale * q k^T / cap) - slope * distance under causal, prefix and
     document masks (b200wmma_attn_fwd has the definition).  q, o: [batch, len_q, heads_q, dim], k, v: [batch, len_kv,
     heads_kv, dim], any strides of whole rows; lse: [batch, heads_q, len_q] fp32 or None."""
-    a = _attn_args(q, k, v, o, scale, cap, slopes)
-    _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv)
-    ws, size = _attn_workspace(workspace)
-    check(lib().b200wmma_attn_fwd(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), ws, size, _stream()))
+    args, (q_, k_, v_, o_, lse_), ws, size, stream = _attn_call(q, k, v, o, lse, scale, causal, cap, slopes, prefix, doc_q, doc_kv, workspace)
+    check(lib().b200wmma_attn_fwd(args, q_, k_, v_, o_, lse_ or None, ws or None, size, stream))
 
 
 def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, scale, causal=False, cap=0.0, slopes=None, prefix=None, doc_q=None, doc_kv=None,
              workspace=None):
     """Gradients dq, dk, dv of attn_fwd for the gradient dout of its o; o and lse are what attn_fwd wrote."""
-    a = _attn_args(q, k, v, o, scale, cap, slopes)
-    for name, t, like in (("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _attn_tensor(a, name, t, q.dtype)
-        if t.shape != like.shape:
-            raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
     if lse is None:
         raise TypeError("attn_bwd needs the lse of attn_fwd")
-    _attn_masks(a, q, k, lse, causal, prefix, doc_q, doc_kv)
-    ws, size = _attn_workspace(workspace)
-    check(lib().b200wmma_attn_bwd(C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk),
-                                  _ptr(dv), ws, size, _stream()))
+    args, (q_, k_, v_, o_, dout_, dq_, dk_, dv_, lse_), ws, size, stream = _attn_call(
+        q, k, v, o, lse, scale, causal, cap, slopes, prefix, doc_q, doc_kv, workspace,
+        (("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, k)))
+    check(lib().b200wmma_attn_bwd(args, q_, k_, v_, o_, dout_, lse_, dq_, dk_, dv_, ws or None, size, stream))
 
 
 def attn_tree_workspace_bytes(batch, drafts, heads_q, heads_kv, head_dim, max_tokens):
+    """Bytes of scratch for attn_tree; max_tokens = pages of a sequence's table x page size."""
     return lib().b200wmma_attn_tree_workspace_bytes(batch, drafts, heads_q, heads_kv, head_dim, max_tokens)
 
 
@@ -399,20 +402,27 @@ def attn_tree(q, k_cache, v_cache, block_table, lens, o, scale, tree=None, depth
     [pages, page_size, heads_kv, dim]; block_table: [batch, pages of a sequence] int32; lens, n_drafts: [batch] int32;
     tree: [batch, drafts] int64, bit j of word i set where drafted token i sees drafted token j (None: j <= i); depths:
     [batch, drafts] int32, for the distances (None: 0, 1, 2, ...)."""
-    a = _attn_args(q, k_cache, v_cache, o, scale, cap, slopes)
-    drafts = q.shape[1]
+    dt, kind, here = _attn_type(q)
+    q_, k_ = _attn_tensor(q, dt, "q", here), _attn_tensor(k_cache, dt, "k_cache", here)
+    batch, drafts, heads_q, dim = q.shape
+    pages, page_size, heads_kv, _ = k_cache.shape
+    if k_cache.shape[3] != dim:
+        raise ValueError("q and the caches must have the same head size")
+    v_, o_ = _attn_tensor(v_cache, dt, "v_cache", here, k_cache.shape), _attn_tensor(o, dt, "o", here, q.shape)
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
         raise ValueError("block_table must have two dimensions")
-    _attn_vector(block_table, torch.int32, (a.batch, block_table.shape[1]), "block_table")
-    _attn_vector(lens, torch.int32, (a.batch,), "lens")
-    for t, dtype, shape, name in ((n_drafts, torch.int32, (a.batch,), "n_drafts"), (tree, torch.int64, (a.batch, drafts), "tree"),
-                                  (depths, torch.int32, (a.batch, drafts), "depths")):
-        if t is not None:
-            _attn_vector(t, dtype, shape, name)
-    ws, size = _attn_workspace(workspace)
-    check(lib().b200wmma_attn_tree(C.byref(a), drafts, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], k_cache.shape[1],
-                                   _ptr(block_table), block_table.shape[1], _ptr(lens), _ptr(n_drafts), _ptr(tree), _ptr(depths),
-                                   _ptr(o), ws, size, _stream()))
+    width = block_table.shape[1]
+    args = ATTN_ARGS.pack(batch, heads_q, heads_kv, 0, 0, dim, kind, 0, scale, cap,
+                          _attn_vector(slopes, torch.float32, (heads_q,), "slopes", here), 0, 0, 0, *q.stride()[:3], *k_cache.stride()[:3],
+                          *v_cache.stride()[:3], *o.stride()[:3], *(_NO_STRIDES * 4))
+    ws, size = _attn_workspace(workspace, here)
+    check(lib().b200wmma_attn_tree(args, drafts, q_, k_, v_, pages, page_size,
+                                   _attn_vector(block_table, torch.int32, (batch, width), "block_table", here), width,
+                                   _attn_vector(lens, torch.int32, (batch,), "lens", here),
+                                   _attn_vector(n_drafts, torch.int32, (batch,), "n_drafts", here) or None,
+                                   _attn_vector(tree, torch.int64, (batch, drafts), "tree", here) or None,
+                                   _attn_vector(depths, torch.int32, (batch, drafts), "depths", here) or None, o_, ws or None, size,
+                                   _raw_stream(here)))
 
 
 class HostContext:
