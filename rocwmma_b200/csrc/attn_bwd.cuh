@@ -1,10 +1,10 @@
 // Backward attention on tcgen05: delta = rowsum(dout * o) in one pass over the rows, then two kernels that both recompute
-// P = 2^(x - lse), so that no sum is shared between blocks and no atomics are needed (seven products where one kernel
+// P = 2^(x - lse), so that no sum is shared between blocks and no atomics are needed (eight products where one kernel
 // with shared sums would do five).
 //   dkv: a block owns 128 keys of one key head and walks the queries of all its heads, with keys as tensor memory lanes:
 //        S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   dq:  a block owns 128 queries and walks the keys:  S = Q K^T, dP = dO V^T, dQ += dS K
-// The dq kernel does not need the other one's results and starts when its last blocks leave SMs idle.
+// The dq kernel runs first and sets delta right (see there).
 // with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
 // 256 threads compute, two to a lane (64 columns each); one warp issues the products, one the copies.
 #pragma once
@@ -144,8 +144,7 @@ namespace b200wmma
             ptx::tc_fence_before_sync();
             __syncthreads();
             ptx::tc_fence_after_sync();
-            ptx::grid_dep_wait(); // the row statistics are there; from here on the dq kernel may take SMs that this one leaves idle
-            ptx::grid_dep_launch_dependents();
+            ptx::grid_dep_wait(); // the row statistics are there
             const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dv_tmem = tmem + 2 * TILE, dk_tmem = dv_tmem + HD;
 
             const uint32_t   n_stat = q_tiles * TILE; // padded rows of a head
@@ -450,13 +449,14 @@ namespace b200wmma
         }
 
         // ---------------------------------------------------------------------------------------------------------------
-        // S has one place in tensor memory, dP (later dS) two, so that the products of the next step run under the arithmetic
-        // of this one.
+        // delta from an o in 16 bits is off by e_i, which moves dQ_i by e_i (P K)_i: as much as the rounding of dS does where a
+        // query sees few keys.  sum_j P (dP - delta) is that error, so this kernel adds it up, adds up P K next to dQ, takes the
+        // product off at the end and leaves the right delta for the dkv kernel.  The steps are interleaved as there.
         template <typename T, uint32_t HD, bool CAP, bool BIAS>
         __global__ void __launch_bounds__(BWD_THREADS, 1)
             bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dq,
-                          const __grid_constant__ Params p, const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                          const __grid_constant__ Params p, const float* __restrict__ lse2, float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
         {
             using L = BwdSmem<HD>;
             extern __shared__ uint8_t smem_raw[];
@@ -487,12 +487,9 @@ namespace b200wmma
                     ptx::mbar_init(base + L::EMPTY + 8 * s, 1);
                 }
                 ptx::mbar_init(base + L::S_FULL, 1);
-                ptx::mbar_init(base + L::P_FULL, 8); // S has been read by a warp
-                for(uint32_t s = 0; s < 2; ++s)
-                {
-                    ptx::mbar_init(base + L::DP_FULL + 8 * s, 1);
-                    ptx::mbar_init(base + L::DS_FULL + 8 * s, 8);
-                }
+                ptx::mbar_init(base + L::DP_FULL, 1);
+                ptx::mbar_init(base + L::P_FULL, 8); // warps
+                ptx::mbar_init(base + L::DS_FULL, 8);
                 ptx::mbar_init(base + L::DONE, 1);
                 *cta_abort = 0u;
                 ptx::fence_barrier_init();
@@ -506,7 +503,9 @@ namespace b200wmma
             ptx::tc_fence_before_sync();
             __syncthreads();
             ptx::tc_fence_after_sync();
-            const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dq_tmem = tmem + 3 * TILE;
+            ptx::grid_dep_wait(); // the row statistics are there
+            ptx::grid_dep_launch_dependents();
+            const uint32_t tmem = misc[0], s_tmem = tmem, dp_tmem = tmem + TILE, dq_tmem = tmem + 2 * TILE, pk_tmem = dq_tmem + HD;
 
             uint32_t         it = 0;
             bool             ok = true;
@@ -516,7 +515,8 @@ namespace b200wmma
             const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
             const int32_t    lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
             const ScoreConst sc  = score_const(p, h);
-            float            ls = 0.0f, de = 0.0f;
+            const float      back = CAP ? 1.0f / sc.cap2 : 0.0f;
+            float            ls = 0.0f, de = 0.0f, rest = 0.0f; // rest: sum of P (dP - delta)
             if(warp < 8)
             {
                 const size_t stat = (size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row;
@@ -564,8 +564,7 @@ namespace b200wmma
                         ptx::tc_fence_after_sync();
                         return ok;
                     };
-                    // S and dP of step n (number `a` over all segments)
-                    const auto products = [&](uint32_t a, uint32_t n) {
+                    const auto scores = [&](uint32_t a, uint32_t n) { // S of step n (number `a` over all segments)
                         const uint32_t st = a & 1u;
                         if(!wait(base + L::FULL + 8 * st, (a >> 1) & 1u, 0))
                             return;
@@ -574,19 +573,20 @@ namespace b200wmma
                             const uint32_t c0 = (list[n] & 0xFFFFFFu) * TILE;
                             clear_padding<HD>(smem + L::RING + st * L::TILE_BYTES, p.doc_kv + size_t(b) * p.len_kv + c0, min(TILE, p.len_kv - c0), lane);
                         }
-                        if(a != 0 && !wait(base + L::P_FULL, (a - 1) & 1u, 1)) // the last S has been read
-                            return;
                         if(elect_one())
                         {
                             mma_over_head<T, HD>(s_tmem, base + L::OWN, base + L::RING + st * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL);
                         }
+                    };
+                    const auto grads = [&](uint32_t a) { // dP
+                        const uint32_t st = a & 1u;
                         if(!wait(base + L::FULL + 16 + 8 * st, (a >> 1) & 1u, 2))
                             return;
                         if(elect_one())
                         {
-                            mma_over_head<T, HD>(dp_tmem + st * TILE, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + st) * L::TILE_BYTES);
-                            ptx::tc_commit(base + L::DP_FULL + 8 * st);
+                            mma_over_head<T, HD>(dp_tmem, base + L::OWN + L::TILE_BYTES, base + L::RING + (2 + st) * L::TILE_BYTES);
+                            ptx::tc_commit(base + L::DP_FULL);
                             ptx::tc_commit(base + L::EMPTY + 16 + 8 * st);
                         }
                     };
@@ -595,19 +595,27 @@ namespace b200wmma
                         if(it == 0)
                             wait(base + L::OWN_FULL, 0, 3);
                         if(ok)
-                            products(it, 0);
+                            scores(it, 0);
+                        if(ok)
+                            grads(it);
                         for(uint32_t n = 0; ok && n < entries; ++n, ++it)
                         {
+                            const uint32_t k_smem = base + L::RING + (it & 1u) * L::TILE_BYTES;
+                            if(!wait(base + L::P_FULL, it & 1u, 1))
+                                break;
+                            if(elect_one())
+                                mma_over_tokens_halves<T, HD>(pk_tmem, s_tmem, k_smem, it != 0);
                             if(n + 1 < entries)
-                                products(it + 1, n + 1);
-                            const uint32_t st = it & 1u;
-                            if(!ok || !wait(base + L::DS_FULL + 8 * st, (it >> 1) & 1u, 4))
+                                scores(it + 1, n + 1);
+                            if(!ok || !wait(base + L::DS_FULL, it & 1u, 4))
                                 break;
                             if(elect_one())
                             {
-                                mma_over_tokens_halves<T, HD>(dq_tmem, dp_tmem + st * TILE, base + L::RING + st * L::TILE_BYTES, it != 0);
-                                ptx::tc_commit(base + L::EMPTY + 8 * st);
+                                mma_over_tokens_halves<T, HD>(dq_tmem, dp_tmem, k_smem, it != 0);
+                                ptx::tc_commit(base + L::EMPTY + 8 * (it & 1u));
                             }
+                            if(n + 1 < entries)
+                                grads(it + 1);
                         }
                     }
                     __syncwarp();
@@ -616,7 +624,7 @@ namespace b200wmma
                 {
                     for(uint32_t n = 0; ok && n < entries; ++n, ++it)
                     {
-                        const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
+                        const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE;
                         int32_t        key_docs[2]; // on their way while the product is
                         if(docs && (e >> 24 & TILE_MASK))
 #pragma unroll
@@ -633,10 +641,6 @@ namespace b200wmma
                         ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem, v[0]);
                         ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
                         ptx::tmem_ld_wait();
-                        ptx::tc_fence_before_sync();
-                        __syncwarp();
-                        if(lane == 0)
-                            ptx::mbar_arrive(base + L::P_FULL);
                         uint64_t seen = ~uint64_t(0); // bit j: key j of the 64 is visible to this query
                         if(e >> 24 & TILE_MASK)
                         {
@@ -650,36 +654,49 @@ namespace b200wmma
                             }
                         }
                         const float from    = static_cast<float>(at - int32_t(c0 + half * 64));
-                        const auto  weights = [&](auto masked) {
+                        const auto  weights = [&](auto masked) { // v becomes P; P (1 - tanh^2) goes over the scores
 #pragma unroll
-                            for(int j = 0; j < 64; j += 2)
+                            for(int i = 0; i < 2; ++i)
                             {
-                                const uint64_t dot = pair(__uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1]));
-                                const uint64_t sub = pair(-ls, -ls);
-                                uint64_t       slip2 = pair(1.0f, 1.0f);
-                                float          x[2], slip[2];
-                                if constexpr(CAP || BIAS)
-                                    unpair(add2(score2<CAP, BIAS>(sc, dot, from - static_cast<float>(j), -1.0f, slip2), sub), x[0], x[1]);
-                                else
-                                    unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
-                                unpair(slip2, slip[0], slip[1]);
+                                uint32_t w[16];
 #pragma unroll
-                                for(int u = 0; u < 2; ++u)
+                                for(int j = 0; j < 32; j += 2)
                                 {
-                                    if constexpr(decltype(masked)::value)
-                                        if(!(seen >> (j + u) & 1u))
-                                            x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
-                                    x[u]                    = ex2(x[u]);
-                                    v[j >> 5][(j & 31) + u] = __float_as_uint(CAP ? x[u] * slip[u] : x[u]);
+                                    const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1])), sub = pair(-ls, -ls);
+                                    uint64_t       slip2 = pair(1.0f, 1.0f);
+                                    float          x[2], slip[2];
+                                    if constexpr(CAP || BIAS)
+                                        unpair(add2(score2<CAP, BIAS>(sc, dot, from - static_cast<float>(32 * i + j), -1.0f, slip2), sub), x[0], x[1]);
+                                    else
+                                        unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
+                                    unpair(slip2, slip[0], slip[1]);
+#pragma unroll
+                                    for(int u = 0; u < 2; ++u)
+                                    {
+                                        if constexpr(decltype(masked)::value)
+                                            if(!(seen >> (32 * i + j + u) & 1u))
+                                                x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
+                                        x[u]        = ex2(x[u]);
+                                        v[i][j + u] = __float_as_uint(x[u]);
+                                        if(CAP)
+                                            x[u] *= slip[u];
+                                    }
+                                    w[j / 2] = pack2<T>(x[0], x[1]);
                                 }
+                                tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
                             }
                         };
                         if(e >> 24 & TILE_MASK)
                             weights(std::true_type{});
                         else
                             weights(std::false_type{});
-                        ok = wait_bounded_warp(base + L::DP_FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
-                                                         DQ_COMPUTE << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
+                        tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        __syncwarp();
+                        if(lane == 0)
+                            ptx::mbar_arrive(base + L::P_FULL);
+
+                        ok = wait_bounded_warp(base + L::DP_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
@@ -688,7 +705,7 @@ namespace b200wmma
                         for(int i = 0; i < 2; ++i)
                         {
                             uint32_t u[32];
-                            ptx::tmem_ld_32x32b_x32(dp_tmem + st * TILE + lane_tmem + 32 * i, u);
+                            ptx::tmem_ld_32x32b_x32(dp_tmem + lane_tmem + 32 * i, u);
                             ptx::tmem_ld_wait();
 #pragma unroll
                             for(int j = 0; j < 16; ++j)
@@ -701,16 +718,26 @@ namespace b200wmma
                                     x[k]           = pr * (__uint_as_float(u[2 * j + k]) - de);
                                     if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
                                         x[k] = pr == 0.0f ? 0.0f : x[k];
+                                    rest += x[k];
+                                    if constexpr(CAP)
+                                    {
+                                        // the capped score again, from its weight: registers for both would not do
+                                        float y = lg2(pr) + ls;
+                                        if constexpr(BIAS)
+                                            y = fmaf(sc.slope, fabsf(from - static_cast<float>(32 * i + 2 * j + k)), y);
+                                        y *= back;
+                                        x[k] = pr == 0.0f ? 0.0f : x[k] * fmaf(-y, y, 1.0f);
+                                    }
                                 }
                                 ds[i * 16 + j] = pack2<T>(x[0], x[1]);
                             }
                         }
-                        tmem_st_32x32b_x32(dp_tmem + st * TILE + lane_tmem, ds);
+                        tmem_st_32x32b_x32(dp_tmem + lane_tmem, ds);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
                         if(lane == 0)
-                            ptx::mbar_arrive(base + L::DS_FULL + 8 * st);
+                            ptx::mbar_arrive(base + L::DS_FULL);
                     }
                 }
                 if(seg + SEG < kv_tiles)
@@ -726,8 +753,15 @@ namespace b200wmma
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
+                    float* rests = reinterpret_cast<float*>(smem + L::STAT);
+                    rests[threadIdx.x] = rest;
+                    ptx::named_bar_sync(1, 256);
+                    rest = rests[threadIdx.x & 127u] + rests[128 + (threadIdx.x & 127u)];
+                    if(half == 0 && row < p.len_q)
+                        delta[(size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row] = de + rest;
                     // every product is done: the tile of Q makes room; both halves of the threads take half of the columns
-                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2), p.scale, it != 0);
+                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2), p.scale, it != 0,
+                                 pk_tmem + ((quad * 32u) << 16), rest);
                     ptx::fence_proxy_async_smem();
                     ptx::named_bar_sync(1, 256);
                     if(threadIdx.x == 0)
@@ -749,9 +783,6 @@ namespace b200wmma
                 ptx::tc_fence_after_sync();
                 ptx::tmem_dealloc(tmem, 512);
             }
-            // started beside the dkv kernel: the grid ends after it, so that whatever follows finds dk and dv written
-            if(blockIdx.x == gridDim.x - 1)
-                ptx::grid_dep_wait();
         }
     } // namespace attn
 } // namespace b200wmma

@@ -84,6 +84,12 @@ namespace b200wmma
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
             return y;
         }
+        __device__ __forceinline__ float lg2(float x)
+        {
+            float y;
+            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+            return y;
+        }
         __device__ __forceinline__ float rcp(float x)
         {
             float y;
@@ -277,9 +283,11 @@ namespace b200wmma
         }
         // Columns [from, to) of this thread's row of an fp32 accumulator, times `by`, as 16-bit values into row `row` of a tile in
         // shared memory with the 128-byte swizzle, from where TMA writes whole rows (a thread's own 16-byte stores to its row
-        // would each touch a line of their own: 2.5 us for a tile).  `live`: the accumulator counts, otherwise zeros.
+        // would each touch a line of their own: 2.5 us for a tile).  `live`: the accumulator counts, otherwise zeros.  `minus`: a
+        // second accumulator (its tensor memory address, 0: none) of which `less` times is taken off first.
         template <typename T>
-        __device__ __forceinline__ void stage_row(uint8_t* tile, uint32_t row, uint32_t taddr, uint32_t from, uint32_t to, float by, bool live)
+        __device__ __forceinline__ void stage_row(uint8_t* tile, uint32_t row, uint32_t taddr, uint32_t from, uint32_t to, float by, bool live,
+                                                  uint32_t minus = 0, float less = 0.0f)
         {
 #pragma unroll 1
             for(uint32_t c = from; c < to; c += 32)
@@ -287,6 +295,15 @@ namespace b200wmma
                 uint32_t w[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32b_x32(taddr + c, w);
+                if(minus != 0)
+                {
+                    uint32_t x[32];
+                    ptx::tmem_ld_32x32b_x32(minus + c, x);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for(int i = 0; i < 32; ++i)
+                        w[i] = __float_as_uint(fmaf(-less, __uint_as_float(x[i]), __uint_as_float(w[i])));
+                }
                 ptx::tmem_ld_wait();
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
