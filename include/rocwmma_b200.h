@@ -355,8 +355,8 @@ int b200wmma_gemv_f64(uint32_t m, uint32_t n, const double* a, uint32_t lda, int
 /* ------------------------------------------------------------------------------------------
  * Matrix-vector products with 4-bit weights and group scales (no counterpart in the reference):
  *   y[r][i] = alpha * sum_k x[r][k] * s[i][k / group] * (q[i][k] - z[i][k / group]) + beta * y[r][i]
- * for `rows` vectors x (one for a single token, a few for several sequences or drafted tokens; any number is right, the
- * kernel is made for up to 64).
+ * for `rows` vectors x (one for a single token, a few for several sequences or drafted tokens; at most 65535, made for up
+ * to 64 - beyond that the weights are read once for every 64, 32 or 16 of them).
  * A is m x n, row major, two 4-bit values per byte along n with the even column in the low nibble (the packing of
  * b200wmma_gemm_i4), lda_bytes bytes per row.  zeros == NULL: q is signed, [-8, 7], and z = 0.  zeros != NULL: q is
  * unsigned, [0, 15], and z = the low four bits of zeros[i * ld_zeros + k / group].
@@ -381,13 +381,16 @@ int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows,
  * data_type is B200WMMA_OUT_F16 or B200WMMA_OUT_BF16 and holds for every matrix; p and the backward pass's ds are rounded
  * to it between the two products, everything else (scores, sums, statistics, accumulators) is fp32.
  * head_dim is a multiple of 8, at most 128.  Rows (one token of one head) are contiguous; the strides of batch entries,
- * tokens and heads are free multiples of 8 elements (any value for an extent of 1), bases 16-byte aligned.
+ * tokens and heads are free positive multiples of 8 elements (any value for an extent of 1), bases 16-byte aligned.  scale,
+ * cap, 1 / cap and scale / cap are at most 1e30.
  * slopes [heads_q] fp32, prefix [batch], doc_q [batch][len_q], doc_kv [batch][len_kv] int32 and may be NULL (doc_q and
  * doc_kv only together).  A negative document marks padding: whatever the rows of padding hold, NaN included, has no
- * influence; their outputs and gradients are zero.  All other elements of q, k, v and dout must be finite, visible or not.
+ * influence; their outputs and gradients are zero.  All other elements of q, k, v and dout must be finite, visible or not
+ * (a mask takes a pair out of the sums by a weight of 0, which does not stop NaN).
  * slopes are constants: there is no gradient for them.
  * lse: [batch][heads_q][len_q] fp32; attn_fwd accepts NULL.  attn_bwd takes o and lse as attn_fwd wrote them and writes
- * dq, dk and dv (sums over the query heads of a key head); results do not depend on the order of execution.
+ * dq, dk and dv (sums over the query heads of a key head); results do not depend on the order of execution.  What 16 bits
+ * took from o is made up for by a sum of the weights, so gradients are as good as with an o in fp32.
  * Outputs must not overlap inputs.  workspace: device scratch of b200wmma_attn_workspace_bytes() bytes, 16-byte aligned;
  * calls that may overlap on the GPU must not share one.  attn_fwd without documents needs none (NULL / 0).
  * ------------------------------------------------------------------------------------------ */
@@ -433,7 +436,7 @@ int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, const void*
  * scale, cap, slopes and the strides q, k, v, o; every other field must be zero.
  * Lengths and pages live on the device and are not checked on the host: a negative length counts as 0, tokens beyond
  * ld_table * page_size and tokens in pages outside [0, num_pages) are not read and not visible.  Rows of the cache that
- * no token of the batch occupies may hold anything, NaN included.
+ * no token of the batch occupies may hold anything, NaN included; those of its tokens must be finite, seen or not.
  * workspace: b200wmma_attn_tree_workspace_bytes() bytes, max_tokens = ld_table * page_size; same rules as above.
  * ------------------------------------------------------------------------------------------ */
 size_t b200wmma_attn_tree_workspace_bytes(uint32_t batch, uint32_t drafts, uint32_t heads_q, uint32_t heads_kv,

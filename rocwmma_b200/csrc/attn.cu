@@ -40,9 +40,10 @@ namespace b200wmma
                 return e;
             B200_REQUIRE(a->len_q && a->len_kv, B200WMMA_ERR_INVALID_ARG, "%s: len_q and len_kv must be non-zero", who);
             B200_REQUIRE(a->len_q < (1u << 30) && a->len_kv < (1u << 30), B200WMMA_ERR_UNSUPPORTED, "%s: len_q and len_kv must be below 2^30", who);
-            B200_REQUIRE(uint64_t(a->batch) * a->heads_q * a->len_q < (uint64_t(1) << 31)
-                             && uint64_t(a->batch) * a->heads_kv * a->len_kv < (uint64_t(1) << 31),
-                         B200WMMA_ERR_UNSUPPORTED, "%s: batch x heads x tokens must be below 2^31", who);
+            const uint64_t most = uint64_t(1) << 31;
+            B200_REQUIRE(uint64_t(a->batch) * a->heads_q < most && uint64_t(a->batch) * a->heads_q * tiles_of(a->len_q) * TILE < most
+                             && uint64_t(a->batch) * a->heads_kv * tiles_of(a->len_kv) * TILE < most,
+                         B200WMMA_ERR_UNSUPPORTED, "%s: batch x heads x tokens, in tiles of 128 tokens, must be below 2^31", who);
             B200_REQUIRE(!a->doc_q == !a->doc_kv, B200WMMA_ERR_INVALID_ARG, "%s: doc_q and doc_kv come together", who);
             if(int e = check_strides(who, "q", q, a->q, a->batch, a->len_q, a->heads_q, &p->q))
                 return e;

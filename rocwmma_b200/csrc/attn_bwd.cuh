@@ -7,6 +7,9 @@
 // The dq kernel runs first and sets delta right (see there).
 // with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
 // 256 threads compute, two to a lane (64 columns each); one warp issues the products, one the copies.
+// Bound: the products.  Each kernel has four to a pair of tiles (2048 cycles at a head of 128); S of the next step runs while dS
+// of this one is computed, dP of the next one while its P is.  Measured, bf16, gradients of 2 x 16 heads of 4096 x 128: 0.91 ms
+// (752 TFLOP/s counting five products), causal 0.53 ms; both kernels take about the same.
 #pragma once
 #include "attn_tc05.cuh"
 
@@ -98,7 +101,8 @@ namespace b200wmma
             bwd_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                            const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ Params p,
-                           const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                           const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q,
+                           const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
         {
             using L = BwdSmem<HD>;
             extern __shared__ uint8_t smem_raw[];
@@ -426,10 +430,10 @@ namespace b200wmma
                     stage_row<T>(smem + L::OWN + half * L::TILE_BYTES, threadIdx.x & 127u, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), 0, HD,
                                  half ? p.scale : 1.0f, it != 0);
                     ptx::fence_proxy_async_smem();
-                    ptx::named_bar_sync(1 + half, TILE);
-                    if((threadIdx.x & 127u) == 0)
-                        store_tile<HD>(half ? &map_dk : &map_dv, base + L::OWN + half * L::TILE_BYTES, c0, g, b);
                 }
+                ptx::named_bar_sync(1 + half, TILE); // warps that gave up come here too
+                if((threadIdx.x & 127u) == 0 && !*cta_abort)
+                    store_tile<HD>(half ? &map_dk : &map_dv, base + L::OWN + half * L::TILE_BYTES, c0, g, b);
             }
             ptx::tc_fence_before_sync();
             __syncthreads();
@@ -455,8 +459,10 @@ namespace b200wmma
         template <typename T, uint32_t HD, bool CAP, bool BIAS>
         __global__ void __launch_bounds__(BWD_THREADS, 1)
             bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dq,
-                          const __grid_constant__ Params p, const float* __restrict__ lse2, float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                          const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ Params p, const float* __restrict__ lse2,
+                          float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q, const DocTile* __restrict__ doc_tiles_kv,
+                          unsigned* status)
         {
             using L = BwdSmem<HD>;
             extern __shared__ uint8_t smem_raw[];
@@ -750,12 +756,12 @@ namespace b200wmma
             {
                 if(ok)
                     ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
+                float* rests       = reinterpret_cast<float*>(smem + L::STAT);
+                rests[threadIdx.x] = rest;
+                ptx::named_bar_sync(1, 256); // warps that gave up come here too
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
-                    float* rests = reinterpret_cast<float*>(smem + L::STAT);
-                    rests[threadIdx.x] = rest;
-                    ptx::named_bar_sync(1, 256);
                     rest = rests[threadIdx.x & 127u] + rests[128 + (threadIdx.x & 127u)];
                     if(half == 0 && row < p.len_q)
                         delta[(size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row] = de + rest;
@@ -763,10 +769,10 @@ namespace b200wmma
                     stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2), p.scale, it != 0,
                                  pk_tmem + ((quad * 32u) << 16), rest);
                     ptx::fence_proxy_async_smem();
-                    ptx::named_bar_sync(1, 256);
-                    if(threadIdx.x == 0)
-                        store_tile<HD>(&map_dq, base + L::OWN, row0, h, b);
                 }
+                ptx::named_bar_sync(1, 256);
+                if(threadIdx.x == 0 && !*cta_abort)
+                    store_tile<HD>(&map_dq, base + L::OWN, row0, h, b);
             }
             ptx::tc_fence_before_sync();
             __syncthreads();

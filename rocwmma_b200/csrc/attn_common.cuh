@@ -31,14 +31,6 @@ namespace b200wmma
             Strides        q, k, v, o, dout, dq, dk, dv;
         };
 
-        // tanh from one exponential: 1 - 2 / (1 + e^2x) is off by a few ulp of 1, absolutely, which is what a score needs
-        // (the hardware's tanh approximation is off by 2^-11 of its value: a capped score of 20 would move by 0.01).
-        // e^2x = infinity and 0 give 1 and -1, NaN stays NaN.
-        __device__ __forceinline__ float tanh_of(float x)
-        {
-            return 1.0f - __fdividef(2.0f, 1.0f + exp2f(x * (2.0f * LOG2E)));
-        }
-
         template <typename T>
         __device__ __forceinline__ float to_f32(T x)
         {
@@ -115,9 +107,13 @@ namespace b200wmma
                          "%s: head_dim must be a multiple of 8, at most %u", who, MAX_DIM);
             B200_REQUIRE(a->data_type == B200WMMA_OUT_F16 || a->data_type == B200WMMA_OUT_BF16, B200WMMA_ERR_INVALID_ARG,
                          "%s: data_type must be B200WMMA_OUT_F16 or B200WMMA_OUT_BF16", who);
-            B200_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, B200WMMA_ERR_INVALID_ARG, "%s: scale must be finite", who);
+            B200_REQUIRE(a->scale - a->scale == 0.0f, B200WMMA_ERR_INVALID_ARG, "%s: scale must be finite", who);
             B200_REQUIRE(a->cap >= 0.0f && a->cap - a->cap == 0.0f, B200WMMA_ERR_INVALID_ARG,
                          "%s: cap must be finite and not negative (0 = none)", who);
+            // constants made of them, 2 log2(e) scale / cap among them, have to be normal numbers
+            const float limit = 1e30f, magnitude = a->scale < 0.0f ? -a->scale : a->scale;
+            B200_REQUIRE(magnitude <= limit && (a->cap == 0.0f || (a->cap >= 1.0f / limit && a->cap <= limit && magnitude / a->cap <= limit)),
+                         B200WMMA_ERR_UNSUPPORTED, "%s: scale, cap, 1 / cap and scale / cap must be at most 1e30", who);
             return B200WMMA_OK;
         }
     } // namespace attn

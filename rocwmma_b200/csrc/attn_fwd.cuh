@@ -6,6 +6,11 @@
 // The two tiles take turns: while the tensor cores work on one, 128 threads (one to a query) do the softmax of the other.
 // The running maximum of a row is only moved when a score passes it by more than 2^8 (RESCALE_STEP): until then P grows up to
 // 256, which both 16-bit types hold, and sums stay fp32, so O is rescaled in a few steps instead of at every one.
+// Bound: a pair of tiles takes 1.9 us at a head of 128, 1.55 us of which remain without any softmax: M = 128, N = 128 products
+// read shared memory at its full 128 bytes a cycle next to the copies' writes, and 2 x 2 of them are 1.1 us by the tensor cores'
+// rate.  Measured, bf16: 1 x 16 heads of 16384 x 128 1.1-1.2 PFLOP/s, 2 x 16 heads of 4096 x 128 0.28 ms (980 TFLOP/s), causal
+// 0.16 ms (870), causal with cap 0.28 ms, 5 packed documents of 8192 tokens 0.11 ms.  What was tried and not kept: announcing P
+// in halves (931 instead of 1064 TFLOP/s then), part of the exponentials as polynomials (892-938).
 #pragma once
 #include "attn_tc05.cuh"
 
@@ -357,12 +362,12 @@ namespace b200wmma
                     // every product of this tile is done: its Q makes room
                     stage_row<T>(smem + L::Q + t * L::TILE_BYTES, threadIdx.x & 127u, o_tmem[t] + ((quad * 32u) << 16), 0, HD, inv, have && l != 0.0f);
                     ptx::fence_proxy_async_smem();
-                    ptx::named_bar_sync(1 + t, TILE);
-                    if((threadIdx.x & 127u) == 0 && row < p.len_q)
-                        store_tile<HD>(&map_o, base + L::Q + t * L::TILE_BYTES, row, h, b);
                     if(lse && row < p.len_q)
                         lse[(size_t(b) * p.heads_q + h) * p.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 }
+                ptx::named_bar_sync(1 + t, TILE); // warps that gave up come here too
+                if((threadIdx.x & 127u) == 0 && row < p.len_q && !*cta_abort)
+                    store_tile<HD>(&map_o, base + L::Q + t * L::TILE_BYTES, row, h, b);
             }
             ptx::tc_fence_before_sync();
             __syncthreads();

@@ -3,11 +3,15 @@
 // Bound: keys and values are read once.  Rows that share a key head (its query heads times the drafted tokens) are the rows of
 // one product, so a block reads 64 tokens of the cache at a time into shared memory and every row uses them.  One warp walks the
 // page table and issues the copies (TMA boxes of as many tokens as surely lie in one page; a page number outside the cache
-// reads as zeros), the others wait for a stage and never for one another.  With up to 64 rows a token's 2 x head_dim values meet
-// 4 x 64 x head_dim flops, which warp-level matrix instructions keep up with; tcgen05 tiles would be 128 rows high and mostly
-// empty.  One pass: running maximum and sum per row, the weights go from accumulators to operands in registers.
+// reads as zeros), the others wait for a stage and never for one another.  With up to 32 rows a token's 2 x head_dim values meet
+// 4 x 32 x head_dim flops, which warp-level matrix instructions keep up with; tcgen05 tiles are 128 rows high and would be mostly
+// empty (more rows take them: attn_tree_tc05.cuh).  One pass: running maximum and sum per row, the weights go from accumulators
+// to operands in registers.
 // The tokens are split over blocks where rows, heads and sequences alone do not fill the machine; a second kernel joins the
 // parts in a fixed order.
+// Measured, bf16, 32/8 heads x 128, one token each: 32 sequences of 4500 tokens 88 us (6.7 TB/s), of 3094 to 6000 tokens 93 us
+// (6.4 TB/s); 8 drafted tokens each, 16 sequences of 8000: 92 us (5.7 TB/s); 5 drafted tokens, 8/2 heads x 64, one sequence of
+// 120000, fp16 with slopes: 22 us (2.8 TB/s; 13 stages to a block, latency).
 #include "attn_tc05.cuh"
 
 namespace b200wmma
@@ -399,6 +403,8 @@ namespace b200wmma
             {
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+                if(m[h] == -INFINITY && l[h] != 0.0f)
+                    m[h] = 0.0f; // nothing but NaN was seen, which is not the same as nothing
             }
             // join the warps that share the rows: [warp][16 rows][HD] sums, [warp][16 rows] maximum and sum of weights
             __syncthreads();
@@ -471,12 +477,11 @@ namespace b200wmma
             constexpr uint32_t E = HD / 32;
             const uint32_t     rows = p.share * p.drafts, row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
             const uint32_t     all_rows = p.batch * p.heads_kv * rows;
-            if(row >= all_rows)
+            const uint32_t     r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
+            const bool         live = row < all_rows && draft < drafts_of(p, b);
+            ptx::grid_dep_wait(); // before anything leaves: the kernel may not end before the one it follows
+            if(!live)
                 return;
-            const uint32_t r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
-            if(draft >= drafts_of(p, b))
-                return;
-            ptx::grid_dep_wait();
             const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (size_t(lane) * all_rows + row) * 2)
                                               : make_float2(-INFINITY, 0.0f);
             float        mx = ml.x;
@@ -600,6 +605,12 @@ namespace b200wmma
             const uint64_t n = want < most ? want : most;
             return n < 1 ? 1u : n > MAX_SPLITS ? MAX_SPLITS : uint32_t(n);
         }
+        // batch x heads_q x drafts (at most 64) counts in 31 bits
+        static bool few_rows(uint32_t batch, uint32_t drafts, uint32_t heads_q)
+        {
+            const uint64_t most = uint64_t(1) << 31, rows = uint64_t(batch) * heads_q;
+            return rows < most && rows * drafts < most;
+        }
         static uint32_t padded_dim(uint32_t dim)
         {
             return dim <= 64 ? 64 : 128;
@@ -665,7 +676,9 @@ using namespace b200wmma;
 extern "C" size_t b200wmma_attn_tree_workspace_bytes(uint32_t batch, uint32_t drafts, uint32_t heads_q, uint32_t heads_kv,
                                                      uint32_t head_dim, uint32_t max_tokens)
 {
-    if(!batch || !drafts || !heads_q || !heads_kv)
+    // shapes that the call refuses need nothing
+    if(!batch || !drafts || drafts > attn_tree::MAX_DRAFTS || !heads_q || !heads_kv || heads_q % heads_kv != 0
+       || !attn_tree::few_rows(batch, drafts, heads_q))
         return 0;
     const uint32_t rows = heads_q / heads_kv * drafts, splits = attn_tree::splits_of(batch, heads_kv, rows, max_tokens);
     return splits == 1 ? 0 : size_t(splits) * batch * heads_kv * rows * (attn_tree::padded_dim(head_dim) + 2) * sizeof(float);
@@ -688,7 +701,7 @@ extern "C" int b200wmma_attn_tree(const b200wmma_attn_args* a, uint32_t drafts, 
     B200_REQUIRE(num_pages < (1u << 31) && uint64_t(ld_table) * page_size < (uint64_t(1) << 31), B200WMMA_ERR_UNSUPPORTED,
                  "%s: num_pages and ld_table x page_size must be below 2^31", who);
     B200_REQUIRE(block_table && lens, B200WMMA_ERR_INVALID_ARG, "%s: block_table and lens must be non-null", who);
-    B200_REQUIRE(uint64_t(a->batch) * a->heads_q * drafts < (uint64_t(1) << 31), B200WMMA_ERR_UNSUPPORTED,
+    B200_REQUIRE(attn_tree::few_rows(a->batch, drafts, a->heads_q), B200WMMA_ERR_UNSUPPORTED,
                  "%s: batch x heads_q x drafts must be below 2^31", who);
     attn_tree::Params p{};
     if(int e = attn::check_strides(who, "q", q, a->q, a->batch, drafts, a->heads_q, &p.q))

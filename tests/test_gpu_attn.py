@@ -2,6 +2,7 @@
 import ctypes as C
 import math
 import os
+import subprocess
 import sys
 
 import pytest
@@ -220,6 +221,87 @@ def test_a_longer_sequence(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("lq,lk", [(3, 66000), (66000, 3), (260, 66100)])
+@pytest.mark.parametrize("docs", [False, True])
+def test_more_tiles_than_one_list_holds(lq, lk, docs):
+    """Key (and query) tiles are listed 512 at a time: 66000 tokens are more."""
+    q, k, v, dout = inputs(1, lq, lk, 1, 1, 64, BF16, seed=37)
+    kw = {}
+    if docs:
+        kw = {"doc_q": (torch.arange(lq) * 3 // lq).to(torch.int32)[None], "doc_kv": (torch.arange(lk) * 3 // lk).to(torch.int32)[None]}
+    check(q, k, v, dout, 0.125, **kw)
+
+
+@gpu
+def test_rows_far_apart():
+    """Offsets that pass 2^31 elements."""
+    n, h, d, stride = 300, 2, 64, 8 << 20
+    big = torch.zeros(n * stride, dtype=BF16, device="cuda")
+    g = torch.Generator().manual_seed(41)
+    q, k, v, dout = inputs(1, n, n, h, h, d, BF16, seed=41)
+    at = iter(range(0, 8 * h * d, h * d))
+    def far(t):
+        x = big.as_strided((1, n, h, d), (n * stride, stride, d, 1), next(at))
+        x.copy_(t)
+        return x
+    assert n * stride > 1 << 31
+    check(q, k, v, dout, 0.125, causal=True, layout=far)
+
+
+@gpu
+def test_two_streams_at_once():
+    """Two calls in flight, each with a workspace of its own."""
+    q, k, v, dout = inputs(1, 900, 900, 4, 4, 128, BF16, seed=43)
+    docs = documents("sorted", 900, 1)[None]
+    alone = run(q, k, v, dout, 0.1, causal=True, doc_q=docs, doc_kv=docs)
+    other = run(q, k, v, dout, 0.2, cap=3.0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                both.append(run(q, k, v, dout, 0.2, cap=3.0) if i else run(q, k, v, dout, 0.1, causal=True, doc_q=docs, doc_kv=docs))
+    torch.cuda.synchronize()
+    for i, got in enumerate(both):
+        for name in got:
+            assert torch.equal(got[name], (other if i % 2 else alone)[name]), name
+
+
+@gpu
+def test_first_call_of_a_process_may_be_captured():
+    code = """
+import torch
+from rocwmma_b200 import api
+q = torch.randn(1, 200, 2, 64, device="cuda").half()
+o, o2, lse = torch.empty_like(q), torch.empty_like(q), torch.empty(1, 2, 200, device="cuda")
+dq, dk, dv = (torch.empty_like(q) for _ in range(3))
+ws = torch.empty(api.attn_workspace_bytes(1, 2, 200, 200, True), dtype=torch.uint8, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    api.attn_fwd(q, q, q, o, lse, 0.125, causal=True)
+    api.attn_bwd(q, q, q, o, q, lse, dq, dk, dv, 0.125, causal=True, workspace=ws)
+g.replay()
+api.attn_fwd(q, q, q, o2, lse, 0.125, causal=True)
+torch.cuda.synchronize()
+assert torch.equal(o, o2) and bool(torch.isfinite(dq).all()) and api.device_status()[0] == 0
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+@gpu
+def test_tensors_of_another_device_are_refused():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    t = torch.zeros(1, 4, 2, 64, dtype=F16, device="cuda:1")
+    with pytest.raises(ValueError):
+        api.attn_fwd(t, t, t, t.clone(), None, 1.0)
+
+
+@gpu
 def test_repeat_stream_and_graph():
     """The same bits again, on another stream, and from a captured graph with new inputs."""
     q, k, v, dout = inputs(2, 300, 300, 4, 2, 64, BF16, seed=29)
@@ -297,7 +379,7 @@ def args(**kw):
     (dict(batch=0), 1), (dict(heads_q=0), 1), (dict(heads_kv=0), 1), (dict(len_q=0), 1), (dict(len_kv=0), 1), (dict(head_dim=0), 1),
     (dict(heads_q=3), 1), (dict(head_dim=60), 2), (dict(head_dim=136), 2), (dict(data_type=1), 1), (dict(cap=-1.0), 1),
     (dict(cap=math.inf), 1), (dict(cap=math.nan), 1), (dict(scale=math.nan), 1), (dict(scale=math.inf), 1), (dict(doc_q=16), 1),
-    (dict(doc_kv=16), 1), (dict(len_q=1 << 30), 2), (dict(q_token=4 * 64 + 4), 3), (dict(k_batch=0), 1), (dict(v_head=-64), 1),
+    (dict(doc_kv=16), 1), (dict(len_q=1 << 30), 2), (dict(batch=1 << 24), 2), (dict(q_token=4 * 64 + 4), 3), (dict(k_batch=0), 1), (dict(v_head=-64), 1),
     (dict(o_head=32), 1), (dict(o_token=64), 1), (dict(q_batch=1 << 38), 2)])
 @pytest.mark.parametrize("backward", [False, True])
 def test_refusals(how, code, backward):

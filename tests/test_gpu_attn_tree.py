@@ -231,6 +231,66 @@ def test_repeat_stream_and_graphs():
 
 
 @gpu
+@pytest.mark.parametrize("t,hq", [(1, 2), (12, 4), (20, 8)])
+@pytest.mark.parametrize("n", [30, 3000])
+def test_a_query_that_is_nan_shows(t, hq, n):
+    """Its row is NaN, also where nothing else is to be seen; the others are what they were."""
+    c = Case([n, n // 2], t, hq, 2, 64, 16, F16, seed=61, kind="chain")
+    a = c.check(0.1)
+    c.q[1, t - 1, 1] = math.nan
+    b = c.run(0.1).cpu()
+    assert bool(torch.isnan(b[1, t - 1, 1]).all())
+    b[1, t - 1, 1] = a[1, t - 1, 1]
+    assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("t,hq", [(4, 2), (40, 4)])
+def test_no_drafted_token_at_all_then_some(t, hq):
+    """A replayed graph of a batch without work writes nothing, and sees the counts that the next replay finds."""
+    c = Case([5000, 70], t, hq, 2, 128, 16, BF16, seed=63, n_drafts=[0, 0])
+    o = c.run(0.1)
+    assert bool((o == 77.0).all())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        c.call()
+    full = Case([5000, 70], t, hq, 2, 128, 16, BF16, seed=63, n_drafts=[t, t - 1])
+    want = full.check(0.1)
+    for name in ("q", "k", "v", "table", "lens", "tree", "depths"):
+        assert c.state[name].shape == full.state[name].shape
+        c.state[name].copy_(full.state[name])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((c.state["o"] == 77.0).all())
+    c.state["n_drafts"].copy_(torch.tensor([t, t - 1], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(c.state["o"].cpu(), want)
+
+
+@gpu
+def test_many_rows_repeat_stream_and_two_graphs():
+    """More than 32 rows to a key head: the same bits again, on another stream, and from two graphs in flight at once."""
+    cases = [Case([2100, 900], 16, 8, 2, 128, 16, BF16, seed=s) for s in (71, 72)]
+    want = [c.check(0.1) for c in cases]
+    graphs, streams = [torch.cuda.CUDAGraph() for _ in cases], [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for c, graph in zip(cases, graphs):
+        with torch.cuda.graph(graph):
+            c.call()
+        c.state["o"].zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for c, w in zip(cases, want):
+        assert torch.equal(c.state["o"].cpu(), w)
+
+
+@gpu
 def test_agrees_with_attention_over_the_same_tokens():
     """A chain of drafted tokens behind a cache is causal attention of the last queries: both kernels, one definition."""
     n, t, hq, hk, d = 301, 11, 4, 2, 128
@@ -283,6 +343,27 @@ def test_refused_calls(how, code):
 
 def test_refused_null_args():
     assert call(None) == 1
+
+
+def test_refused_workspaces():
+    need = _lib.lib().b200wmma_attn_tree_workspace_bytes(2, 5, 4, 2, 64, 64 * 16)
+    assert need > 0
+    assert call(targs(), ld=64, ws=None, size=need) == 1 and call(targs(), ld=64, size=need - 1) == 1 and call(targs(), ld=64, ws=24, size=need) == 3
+    assert _lib.lib().b200wmma_attn_tree_workspace_bytes(2, 5, 4, 2, 64, 16) == 0  # too short to be split
+
+
+@pytest.mark.parametrize("shape", [
+    (0, 5, 4, 2), (2, 0, 4, 2), (2, 65, 4, 2), (2, 5, 0, 2), (2, 5, 4, 0), (2, 5, 4, 3), (2, 5, 1, 2), (1, 64, 1 << 31, 1 << 5),
+    (1 << 31, 4, 1 << 31, 1), (1, 2, 1 << 31, 1)])
+def test_shapes_that_are_refused_need_no_workspace(shape):
+    batch, drafts, hq, hk = shape
+    assert _lib.lib().b200wmma_attn_tree_workspace_bytes(batch, drafts, hq, hk, 64, 1 << 16) == 0
+    assert call(targs(batch=batch, heads_q=hq, heads_kv=hk), drafts=drafts) in (1, 2)
+
+
+@pytest.mark.parametrize("how", [dict(scale=1e31), dict(cap=1e-40), dict(cap=1e-10, scale=1e25), dict(cap=1e31)])
+def test_refused_scales(how):
+    assert call(targs(**how)) == 2
 
 
 def test_wrapper_refuses_wrong_tensors():

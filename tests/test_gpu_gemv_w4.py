@@ -124,6 +124,46 @@ def test_other_stream_and_graph_replay():
         assert torch.equal(y, want)
 
 
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows", [12, 20, 50])
+def test_many_vectors_repeat_and_graph(rows, group):
+    """More than 8 vectors: the same bits again, and from two graphs in flight at once."""
+    m, n = 520, 2400
+    a, s, z, x = make(m, n, rows, group, F16, True)
+    a, s, z, x = torch.from_numpy(a).cuda(), s.cuda(), torch.from_numpy(z).cuda(), x.cuda()
+    groups = -(-n // group)
+    y = [torch.zeros(rows, m, dtype=F16, device="cuda") for _ in range(3)]
+    call = lambda out: api.gemv_w4(m, n, rows, a, n // 2, s, groups, group, x, n, out, m, 1.0, 0.0, zeros=z, ld_zeros=groups)
+    call(y[0])
+    graphs, streams = [torch.cuda.CUDAGraph() for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for graph, out in zip(graphs, y[1:]):
+        with torch.cuda.graph(graph):
+            call(out)
+    for _ in range(3):
+        for graph, side in zip(graphs, streams):
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y[0], y[1]) and torch.equal(y[0], y[2])
+    assert_status_ok()
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_vectors_nan_stays_in_its_row(group):
+    m, n, rows = 150, 544, 18
+    a, s, _, x = make(m, n, rows, group, F16, False)
+    x[2, 7], x[17, 543] = float("nan"), float("inf")
+    groups = -(-n // group)
+    y = torch.zeros(rows, m, dtype=F16, device="cuda")
+    api.gemv_w4(m, n, rows, torch.from_numpy(a).cuda(), n // 2, s.cuda(), groups, group, x.cuda(), n, y, m, 1.0, 0.0)
+    got = torch.isfinite(y.cpu())
+    keep = [r for r in range(rows) if r not in (2, 17)]
+    assert got[keep].all() and not got[2].any() and not got[17].any()
+
+
 def w4(L, m=64, n=128, rows=1, a=16, lda=64, s=16, lds=1, z=None, ldz=0, group=128, x=16, ldx=128, y=16, ldy=64, dt=0, out=0):
     return L.b200wmma_gemv_w4(m, n, rows, a, lda, s, lds, z, ldz, group, x, ldx, y, ldy, 1.0, 0.0, dt, out, None)
 
