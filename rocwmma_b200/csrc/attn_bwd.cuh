@@ -328,7 +328,7 @@ namespace b200wmma
                                 seen = doc < 0 ? 0 : seen & (uint64_t(same[1]) << 32 | same[0]);
                             }
                         }
-                        const auto weights = [&](auto masked) {
+                        const auto weights = [&](auto masked, auto how) {
 #pragma unroll
                             for(int i = 0; i < 2; ++i)
                             {
@@ -348,7 +348,9 @@ namespace b200wmma
                                         uint64_t       slip2 = pair(1.0f, 1.0f);
                                         float          x[2], slip[2];
                                         if constexpr(CAP || BIAS)
-                                            unpair(add2(score2<CAP, BIAS>(sc, dot, from + static_cast<float>(j), 1.0f, slip2), sub), x[0], x[1]);
+                                            unpair(add2(score2<CAP, BIAS, decltype(how)::value>(sc, dot, from + static_cast<float>(j), 1.0f, slip2),
+                                                        sub),
+                                                   x[0], x[1]);
                                         else
                                             unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
                                         unpair(slip2, slip[0], slip[1]);
@@ -367,10 +369,12 @@ namespace b200wmma
                                 tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
                             }
                         };
-                        if(e >> 24 & TILE_MASK)
-                            weights(std::true_type{});
+                        if(!tame<CAP>(sc, v[0]) || !tame<CAP>(sc, v[1]))
+                            weights(std::true_type{}, std::false_type{});
+                        else if(e >> 24 & TILE_MASK)
+                            weights(std::true_type{}, std::true_type{});
                         else
-                            weights(std::false_type{});
+                            weights(std::false_type{}, std::true_type{});
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -660,7 +664,7 @@ namespace b200wmma
                             }
                         }
                         const float from    = static_cast<float>(at - int32_t(c0 + half * 64));
-                        const auto  weights = [&](auto masked) { // v becomes P; P (1 - tanh^2) goes over the scores
+                        const auto  weights = [&](auto masked, auto how) { // v becomes P; P (1 - tanh^2) goes over the scores
 #pragma unroll
                             for(int i = 0; i < 2; ++i)
                             {
@@ -672,7 +676,10 @@ namespace b200wmma
                                     uint64_t       slip2 = pair(1.0f, 1.0f);
                                     float          x[2], slip[2];
                                     if constexpr(CAP || BIAS)
-                                        unpair(add2(score2<CAP, BIAS>(sc, dot, from - static_cast<float>(32 * i + j), -1.0f, slip2), sub), x[0], x[1]);
+                                        unpair(add2(score2<CAP, BIAS, decltype(how)::value>(sc, dot, from - static_cast<float>(32 * i + j), -1.0f,
+                                                                                            slip2),
+                                                    sub),
+                                               x[0], x[1]);
                                     else
                                         unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
                                     unpair(slip2, slip[0], slip[1]);
@@ -692,10 +699,12 @@ namespace b200wmma
                                 tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
                             }
                         };
-                        if(e >> 24 & TILE_MASK)
-                            weights(std::true_type{});
+                        if(!tame<CAP>(sc, v[0]) || !tame<CAP>(sc, v[1]))
+                            weights(std::true_type{}, std::false_type{});
+                        else if(e >> 24 & TILE_MASK)
+                            weights(std::true_type{}, std::true_type{});
                         else
-                            weights(std::false_type{});
+                            weights(std::false_type{}, std::true_type{});
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();

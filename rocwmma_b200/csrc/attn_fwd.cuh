@@ -110,13 +110,13 @@ namespace b200wmma
             const int32_t  at  = int32_t(row) + p.off;
             uint32_t       n_s = 0; // softmax: S tiles so far
             float          m = -INFINITY, l = 0.0f;
-            bool           ok = true, q_here = false;
+            bool           ok = true, q_here = false, steep = false, wild = false;
             const ScoreConst sc = score_const(p, h);
             const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
             // keys [0, lim) of this row are visible as far as causality and lengths go
             const int32_t lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
 
-            for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
+            for(uint32_t seg = (kv_tiles - 1) / SEG * SEG;; seg -= SEG)
             {
                 // the key tiles of this segment that a query of the CTA sees, with the flags of both query tiles
                 const uint32_t entries = list_tiles<FWD_THREADS>(seg, min(SEG, kv_tiles - seg), list, raw, misc + 2, [&](uint32_t tile) {
@@ -156,7 +156,7 @@ namespace b200wmma
                                 if(!ok)
                                     break;
                                 ptx::mbar_arrive_expect_tx(base + L::KV_FULL + 8 * st, L::TILE_BYTES);
-                                load_tile<HD>(base + L::KV + st * L::TILE_BYTES, half ? &map_v : &map_k, (list[e] & 0xFFFFFFu) * TILE, g, b,
+                                load_tile<HD>(base + L::KV + st * L::TILE_BYTES, half ? &map_v : &map_k, (list[entries - 1 - e] & 0xFFFFFFu) * TILE, g, b,
                                               base + L::KV_FULL + 8 * st);
                             }
                     }
@@ -177,16 +177,16 @@ namespace b200wmma
                         const uint32_t st = n % L::STAGES;
                         if(!wait(base + L::KV_FULL + 8 * st, (n / L::STAGES) & 1u, 1))
                             return false;
-                        if(list[e] >> 24 & TILE_DIRTY)
+                        if(list[entries - 1 - e] >> 24 & TILE_DIRTY)
                         {
-                            const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
+                            const uint32_t c0 = (list[entries - 1 - e] & 0xFFFFFFu) * TILE;
                             clear_padding<HD>(smem + L::KV + st * L::TILE_BYTES, p.doc_kv + size_t(b) * p.len_kv + c0, min(TILE, p.len_kv - c0),
                                               lane);
                         }
                         return true;
                     };
                     const auto scores = [&](uint32_t u, uint32_t e, uint32_t n) { // S of query tile u
-                        if((list[e] >> (24 + 2 * u) & TILE_NEED) && elect_one())
+                        if((list[entries - 1 - e] >> (24 + 2 * u) & TILE_NEED) && elect_one())
                         {
                             mma_over_head<T, HD>(s_tmem[u], base + L::Q + u * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL + 8 * u);
@@ -216,7 +216,7 @@ namespace b200wmma
                                 break;
                             for(uint32_t u = 0; ok && u < 2; ++u)
                             {
-                                if(list[e] >> (24 + 2 * u) & TILE_NEED)
+                                if(list[entries - 1 - e] >> (24 + 2 * u) & TILE_NEED)
                                 {
                                     if(!wait(base + L::P_FULL + 8 * u, done[u] & 1u, 2 + u))
                                         break;
@@ -246,10 +246,10 @@ namespace b200wmma
                     const uint32_t lane_tmem = (quad * 32u) << 16;
                     for(uint32_t e = 0; ok && e < entries; ++e)
                     {
-                        const uint32_t f = list[e] >> (24 + 2 * t);
+                        const uint32_t f = list[entries - 1 - e] >> (24 + 2 * t);
                         if(!(f & TILE_NEED))
                             continue;
-                        const uint32_t c0 = (list[e] & 0xFFFFFFu) * TILE;
+                        const uint32_t c0 = (list[entries - 1 - e] & 0xFFFFFFu) * TILE;
                         int32_t        key_docs[4]; // on their way while the product is
                         if(docs && (f & TILE_MASK))
 #pragma unroll
@@ -261,25 +261,33 @@ namespace b200wmma
                         ptx::tc_fence_after_sync();
                         const uint32_t s_row = s_tmem[t] + lane_tmem;
                         const float    from  = static_cast<float>(at - int32_t(c0));
-                        const auto     transform = [&](int i, uint32_t(&x)[32]) {
+                        const auto     transform_as = [&](auto how, int at_col, auto& x) {
+#pragma unroll
+                            for(int k = 0; k < int(sizeof(x) / 4); k += 2)
+                            {
+                                uint64_t unused;
+                                float    lo, hi;
+                                unpair(score2<CAP, BIAS, decltype(how)::value>(sc, pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])),
+                                                                               from - static_cast<float>(at_col + k), -1.0f, unused),
+                                       lo, hi);
+                                x[k] = __float_as_uint(lo), x[k + 1] = __float_as_uint(hi);
+                            }
+                        };
+                        const auto transform = [&](int at_col, auto& x) {
                             if constexpr(!PLAIN)
                             {
-#pragma unroll
-                                for(int k = 0; k < 32; k += 2)
+                                if(tame<CAP>(sc, x))
+                                    transform_as(std::true_type{}, at_col, x);
+                                else
                                 {
-                                    uint64_t unused;
-                                    float    lo, hi;
-                                    unpair(score2<CAP, BIAS>(sc, pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])),
-                                                             from - static_cast<float>(32 * i + k), -1.0f, unused),
-                                           lo, hi);
-                                    x[k] = __float_as_uint(lo), x[k + 1] = __float_as_uint(hi);
+                                    transform_as(std::false_type{}, at_col, x);
+                                    wild = true;
                                 }
                             }
                         };
-                        float top;
+                        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
                         if(f & TILE_MASK)
                         {
-                            uint32_t see[4];
 #pragma unroll
                             for(int i = 0; i < 4; ++i)
                                 see[i] = below(lim - int32_t(c0), i);
@@ -291,20 +299,53 @@ namespace b200wmma
                                 for(int i = 0; i < 4; ++i)
                                     see[i] &= same[i];
                             }
-                            top = row_max<true>(s_row, [&](int i, uint32_t(&x)[32]) {
-                                transform(i, x);
-#pragma unroll
-                                for(int k = 0; k < 32; ++k)
-                                    if(!(see[i] >> k & 1u))
-                                        x[k] = 0xFF800000u; // -infinity
-                            });
                         }
-                        else
-                            top = row_max<!PLAIN>(s_row, transform);
+                        const auto masked = [&](int at_col, auto& x) {
+#pragma unroll
+                            for(int k = 0; k < int(sizeof(x) / 4); ++k)
+                                if(!(see[at_col / 32] >> (at_col % 32 + k) & 1u))
+                                    x[k] = 0xFF800000u; // -infinity
+                        };
+                        float top;
+                        bool  moved = n_s == 0 || steep || wild;
+                        if(!moved)
+                        {
+                            uint32_t    w[4][16];
+                            const float sub = m == -INFINITY ? 0.0f : -m, c = PLAIN ? sc.c : 1.0f;
+                            float       most = 0.0f;
+                            const auto  guess = [&](int at_col, auto& x) {
+                                if constexpr(CAP)
+                                    most = magnitude(x, most);
+                                if constexpr(!PLAIN)
+                                    transform_as(std::true_type{}, at_col, x);
+                            };
+                            const float more = f & TILE_MASK ? weights_at<T>(s_row, c, sub, w, top,
+                                                                             [&](int at_col, auto& x) {
+                                                                                 guess(at_col, x);
+                                                                                 masked(at_col, x);
+                                                                             })
+                                                             : weights_at<T>(s_row, c, sub, w, top, guess);
+                            moved = __any_sync(0xFFFFFFFFu, top * c > m + RESCALE_STEP || (CAP && !(most * fabsf(sc.k2) <= TAME_LIMIT)));
+                            if(!moved)
+                            {
+                                l += more;
+#pragma unroll
+                                for(int i = 0; i < 4; ++i)
+                                    tmem_st_32x32b_x16(s_row + 16 * i, w[i]);
+                            }
+                        }
+                        if(moved)
+                        {
+                        wild = false;
+                        top = row_max<true>(s_row, [&](int at_col, auto& x) {
+                            transform(at_col, x);
+                            masked(at_col, x);
+                        });
                         if constexpr(PLAIN)
                             top *= sc.c; // scale > 0
                         // move the maximum where some row of this warp has outgrown it
-                        if(__any_sync(0xFFFFFFFFu, top > m + RESCALE_STEP))
+                        steep = __any_sync(0xFFFFFFFFu, top > m + RESCALE_STEP);
+                        if(steep)
                         {
                             const float m2 = fmaxf(m, top);
                             const float by = m2 == -INFINITY ? 1.0f : ex2(m - m2);
@@ -332,6 +373,7 @@ namespace b200wmma
                         }
                         const float sub = m == -INFINITY ? 0.0f : -m;
                         l += weights<T>(s_row, PLAIN ? sc.c : 1.0f, sub);
+                        }
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -340,8 +382,9 @@ namespace b200wmma
                         ++n_s;
                     }
                 }
-                if(seg + SEG < kv_tiles)
-                    __syncthreads(); // the list is written anew
+                if(seg == 0)
+                    break;
+                __syncthreads(); // the list is written anew
             }
 
             // ---- results ----

@@ -125,15 +125,16 @@ namespace b200wmma
             asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
             return r;
         }
-        // Largest of 32 numbers and `t`, in two independent chains of three-input steps.
-        __device__ __forceinline__ float max_of(const uint32_t (&v)[32], float t)
+        // Largest of N numbers and `t`, in two independent chains of three-input steps.
+        template <int N>
+        __device__ __forceinline__ float max_of(const uint32_t (&v)[N], float t)
         {
             float u = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
-            for(int k = 2; k < 32; k += 4)
+            for(int k = 2; k < N; k += 4)
             {
                 t = fmaxf(fmaxf(t, __uint_as_float(v[k])), __uint_as_float(v[k + 1]));
-                if(k + 2 < 32)
+                if(k + 2 < N)
                     u = fmaxf(fmaxf(u, __uint_as_float(v[k + 2])), __uint_as_float(v[k + 3]));
             }
             return fmaxf(t, u);
@@ -219,7 +220,7 @@ namespace b200wmma
 
         // The two passes of a softmax over a row of 128 scores in tensor memory, 32 columns at a time with the next 32 on their
         // way, so that a thread holds 64 of them and not 128 (which spills, and costs more than reading tensor memory twice).
-        // First pass: the largest.  change(i, x) may alter columns 32 i .. 32 i + 31; WRITE puts them back for the second pass.
+        // First pass: the largest.  change(at, x) may alter columns at, at + 1, ...; WRITE puts them back for the second pass.
         template <bool WRITE, typename F>
         __device__ __forceinline__ float row_max(uint32_t taddr, F change)
         {
@@ -232,7 +233,7 @@ namespace b200wmma
                 ptx::tmem_ld_wait();
                 if(i < 3)
                     ptx::tmem_ld_32x32b_x32(taddr + 32 * (i + 1), v[(i + 1) & 1]);
-                change(i, v[i & 1]);
+                change(32 * i, v[i & 1]);
                 top = max_of(v[i & 1], top);
                 if(WRITE)
                     tmem_st_32x32b_x32(taddr + 32 * i, v[i & 1]);
@@ -267,6 +268,39 @@ namespace b200wmma
                     w[j]       = pack2<T>(x, y);
                 }
                 tmem_st_32x32b_x16(taddr + 16 * i, w);
+            }
+            float a, b;
+            unpair(add2(sum[0], sum[1]), a, b);
+            return a + b;
+        }
+
+        // Both passes in one, for a maximum that is known already: P stays in registers (16 bits, two to one) until it is clear that
+        // no score of the warp has outgrown `sub` too far.  `top`: the largest of the changed scores (not times c).
+        template <typename T, typename F>
+        __device__ __forceinline__ float weights_at(uint32_t taddr, float c, float sub, uint32_t (&w)[4][16], float& top, F change)
+        {
+            const uint64_t cc = pair(c, c), ss = pair(sub, sub);
+            uint64_t       sum[2] = {0, 0};
+            uint32_t       v[2][16];
+            top = -INFINITY;
+            ptx::tmem_ld_32x32b_x16(taddr, v[0]);
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+            {
+                ptx::tmem_ld_wait();
+                if(i < 7)
+                    ptx::tmem_ld_32x32b_x16(taddr + 16 * (i + 1), v[(i + 1) & 1]);
+                change(16 * i, v[i & 1]);
+                top = max_of(v[i & 1], top);
+#pragma unroll
+                for(int j = 0; j < 8; ++j)
+                {
+                    float x, y;
+                    unpair(fma2(pair(__uint_as_float(v[i & 1][2 * j]), __uint_as_float(v[i & 1][2 * j + 1])), cc, ss), x, y);
+                    x = ex2(x), y = ex2(y);
+                    sum[j & 1]               = add2(sum[j & 1], pair(x, y));
+                    w[i / 2][8 * (i & 1) + j] = pack2<T>(x, y);
+                }
             }
             float a, b;
             unpair(add2(sum[0], sum[1]), a, b);
@@ -451,6 +485,7 @@ namespace b200wmma
         {
             float c;     // log2(e) * scale (no cap)
             float k1;    // 2 log2(e) scale / cap: e^(2 scale dot / cap) = 2^(k1 dot)
+            float k2;    // scale / cap: the argument of tanh is k2 dot
             float cap2;  // log2(e) * cap
             float slope; // log2(e) * slope of this head
         };
@@ -458,7 +493,8 @@ namespace b200wmma
         {
             ScoreConst s;
             s.c     = p.scale * LOG2E;
-            s.k1    = p.cap > 0.0f ? 2.0f * LOG2E * (p.scale / p.cap) : 0.0f;
+            s.k2    = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+            s.k1    = 2.0f * LOG2E * s.k2;
             s.cap2  = p.cap * LOG2E;
             s.slope = p.slopes ? p.slopes[head] * LOG2E : 0.0f;
             return s;
@@ -483,14 +519,49 @@ namespace b200wmma
             return x;
         }
 
-        // The same for two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.  (Powers by a
-        // polynomial on the fused multiply-add pipe and one reciprocal for both measured slower: 332 us against 307 for 2 x 16
-        // heads of 4096 x 128, causal.  Instructions count here, not the unit behind ex2 and rcp.)
-        template <bool CAP, bool BIAS>
+        // Largest magnitude of N numbers and `t`.
+        template <int N>
+        __device__ __forceinline__ float magnitude(const uint32_t (&v)[N], float t)
+        {
+            float u = 0.0f;
+#pragma unroll
+            for(int k = 0; k < N; k += 4)
+            {
+                t = fmaxf(fmaxf(t, fabsf(__uint_as_float(v[k]))), fabsf(__uint_as_float(v[k + 1])));
+                u = fmaxf(fmaxf(u, fabsf(__uint_as_float(v[k + 2]))), fabsf(__uint_as_float(v[k + 3])));
+            }
+            return fmaxf(t, u);
+        }
+        // True where the cap bends the scores of a warp only a little: |k2 dot| <= 1/2, as mostly (NaN counts as small).
+        constexpr float TAME_LIMIT = 0.5f;
+        template <bool CAP, int N>
+        __device__ __forceinline__ bool tame(const ScoreConst& s, const uint32_t (&dot)[N])
+        {
+            if constexpr(CAP)
+                return __all_sync(0xFFFFFFFFu, magnitude(dot, 0.0f) * fabsf(s.k2) <= TAME_LIMIT);
+            else
+                return true;
+        }
+        // The same for two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.
+        // TAME: tanh x / x as a polynomial in x^2, fitted to the smallest largest error over |x| <= 1/2: 1.5e-8 of its value, 4e-8 as
+        // evaluated in fp32, which is closer than the exponential's form.  Three of them and of the softmax's exponentials share a
+        // unit that takes 16 numbers a cycle: 2 x 16 heads of 4096 x 128, causal, TAME_US us with the polynomial, 254 us without.
+        template <bool CAP, bool BIAS, bool TAME>
         __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
         {
             uint64_t x;
-            if constexpr(CAP)
+            if constexpr(CAP && TAME)
+            {
+                const uint64_t u = mul2(dot, pair(s.k2, s.k2)), y = mul2(u, u);
+                uint64_t       q = fma2(y, pair(0.0172414854f, 0.0172414854f), pair(-0.0530454926f, -0.0530454926f));
+                q = fma2(q, y, pair(0.13325879f, 0.13325879f));
+                q = fma2(q, y, pair(-0.333331436f, -0.333331436f));
+                q = fma2(q, y, pair(1.0f, 1.0f));
+                const uint64_t tanh = mul2(u, q);
+                slip = fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
+                x    = mul2(tanh, pair(s.cap2, s.cap2));
+            }
+            else if constexpr(CAP)
             {
                 float a, b;
                 unpair(mul2(dot, pair(s.k1, s.k1)), a, b);

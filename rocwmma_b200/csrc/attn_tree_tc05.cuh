@@ -277,7 +277,7 @@ namespace b200wmma
                 const uint32_t draft = live ? r / p.share : 0;
                 const uint64_t bits  = !live ? 0 : p.tree ? __ldg(p.tree + size_t(b) * p.drafts + draft) : (uint64_t(2) << draft) - 1;
                 attn::ScoreConst sc;
-                sc.c = p.scale * LOG2E, sc.k1 = CAP ? 2.0f * LOG2E * (p.scale / p.cap) : 0.0f, sc.cap2 = p.cap * LOG2E;
+                sc.c = p.scale * LOG2E, sc.k2 = CAP ? p.scale / p.cap : 0.0f, sc.k1 = 2.0f * LOG2E * sc.k2, sc.cap2 = p.cap * LOG2E;
                 sc.slope = BIAS && live ? __ldg(p.slopes + head * p.share + r % p.share) * LOG2E : 0.0f;
                 // distances are taken from token `len`, so that they stay small and exact
                 const int32_t at = BIAS && live ? (p.depths ? __ldg(p.depths + size_t(b) * p.drafts + draft) : int32_t(draft)) : 0;
@@ -294,40 +294,47 @@ namespace b200wmma
                     const bool      masked = (valid[0] & valid[1] & valid[2] & valid[3]) != 0xFFFFFFFFu || rel0 + int32_t(TILE) > 0;
                     const uint32_t  s_row  = s_tmem + u * TILE + lane_tmem;
                     const auto      scores = [&](auto mask) {
-                        return attn::row_max<true>(s_row, [&](int i, uint32_t(&v)[32]) {
-                            constexpr bool MASK = decltype(mask)::value;
-                            const uint32_t see  = MASK ? valid[i] & seen_of(bits, rel0 + 32 * i) : 0u;
+                        return attn::row_max<true>(s_row, [&](int at_col, uint32_t(&v)[32]) {
+                            const int  i      = at_col / 32;
+                            const auto change = [&](auto how) {
+                                constexpr bool MASK = decltype(mask)::value;
+                                const uint32_t see  = MASK ? valid[i] & seen_of(bits, rel0 + 32 * i) : 0u;
 #pragma unroll
-                            for(int k = 0; k < 32; k += 2)
-                            {
-                                uint64_t unused;
-                                float    dist = 0.0f, step = -1.0f, y[2];
-                                if constexpr(BIAS)
+                                for(int k = 0; k < 32; k += 2)
                                 {
-                                    dist = static_cast<float>(at - rel0) - static_cast<float>(i * 32 + k);
-                                    if constexpr(MASK)
-                                        if(p.depths && rel0 + i * 32 + k + 1 >= 0) // drafted tokens stand at their depths
-                                        {
-                                            const int32_t rel = rel0 + i * 32 + k;
-                                            const auto    d   = [&](int32_t to) {
-                                                return static_cast<float>(
-                                                    at - (to >= 0 && to < int32_t(n_drafts) ? __ldg(p.depths + size_t(b) * p.drafts + to) : to));
-                                            };
-                                            dist = d(rel);
-                                            step = d(rel + 1) - dist;
-                                        }
-                                }
-                                attn::unpair(attn::score2<CAP, BIAS>(sc, attn::pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), dist, step, unused),
-                                             y[0], y[1]);
+                                    uint64_t unused;
+                                    float    dist = 0.0f, step = -1.0f, y[2];
+                                    if constexpr(BIAS)
+                                    {
+                                        dist = static_cast<float>(at - rel0) - static_cast<float>(i * 32 + k);
+                                        if constexpr(MASK)
+                                            if(p.depths && rel0 + i * 32 + k + 1 >= 0) // drafted tokens stand at their depths
+                                            {
+                                                const int32_t rel = rel0 + i * 32 + k;
+                                                const auto    d   = [&](int32_t to) {
+                                                    return static_cast<float>(
+                                                        at - (to >= 0 && to < int32_t(n_drafts) ? __ldg(p.depths + size_t(b) * p.drafts + to) : to));
+                                                };
+                                                dist = d(rel);
+                                                step = d(rel + 1) - dist;
+                                            }
+                                    }
+                                    attn::unpair(attn::score2<CAP, BIAS, decltype(how)::value>(sc, attn::pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), dist, step, unused),
+                                                 y[0], y[1]);
 #pragma unroll
-                                for(int e = 0; e < 2; ++e)
-                                {
-                                    if constexpr(MASK)
-                                        if(!(see >> (k + e) & 1u))
-                                            y[e] = -INFINITY;
-                                    v[k + e] = __float_as_uint(y[e]);
+                                    for(int e = 0; e < 2; ++e)
+                                    {
+                                        if constexpr(MASK)
+                                            if(!(see >> (k + e) & 1u))
+                                                y[e] = -INFINITY;
+                                        v[k + e] = __float_as_uint(y[e]);
+                                    }
                                 }
-                            }
+                            };
+                            if(attn::tame<CAP>(sc, v))
+                                change(std::true_type{});
+                            else
+                                change(std::false_type{});
                         });
                     };
                     const float top = masked ? scores(std::true_type{}) : scores(std::false_type{});
