@@ -4,8 +4,10 @@
 //   S = Q K^T (tensor cores, fp32 in tensor memory) -> softmax warps: running maximum and sum, P = 2^(x - m) in 16 bits over S
 //   -> O += P V (tensor cores, P from tensor memory).
 // The two tiles take turns: while the tensor cores work on one, 128 threads (one to a query) do the softmax of the other.
-// The running maximum of a row is only moved when a score passes it by more than 2^8 (RESCALE_STEP): until then P grows up to
-// 256, which both 16-bit types hold, and sums stay fp32, so O is rescaled in a few steps instead of at every one.
+// The running maximum of a row is only moved when a score passes it by more than 2^14 (RESCALE_STEP), so O is rescaled rarely and
+// a tile's weights mostly take one pass over its scores.  Key tiles come from the last to the first: under a causal mask the
+// nearest ones, which a distance bias makes the largest, are first (2 x 16 heads of 4096 x 128 with slopes: 173 us; 270 the other
+// way round, where the maximum moves in every tile).
 // Bound: a pair of tiles takes 1.9 us at a head of 128, 1.55 us of which remain without any softmax: M = 128, N = 128 products
 // read shared memory at its full 128 bytes a cycle next to the copies' writes, and 2 x 2 of them are 1.1 us by the tensor cores'
 // rate.  Measured, bf16: 1 x 16 heads of 16384 x 128 1.1-1.2 PFLOP/s, 2 x 16 heads of 4096 x 128 0.28 ms (980 TFLOP/s), causal
@@ -19,7 +21,6 @@ namespace b200wmma
     namespace attn
     {
         constexpr uint32_t FWD_THREADS  = 320; // warps 0-3: softmax of tile 0, 4-7: of tile 1, 8: TMA, 9: MMA
-        constexpr float    RESCALE_STEP = 8.0f;
 
         template <uint32_t HD>
         struct FwdSmem
@@ -306,6 +307,8 @@ namespace b200wmma
                                 if(!(see[at_col / 32] >> (at_col % 32 + k) & 1u))
                                     x[k] = 0xFF800000u; // -infinity
                         };
+                        // One pass with the maximum as it stands and, under a cap, small scores taken for granted.  Where that turns
+                        // out wrong, two passes; and two at once in the tile after that.
                         float top;
                         bool  moved = n_s == 0 || steep || wild;
                         if(!moved)
@@ -336,43 +339,44 @@ namespace b200wmma
                         }
                         if(moved)
                         {
-                        wild = false;
-                        top = row_max<true>(s_row, [&](int at_col, auto& x) {
-                            transform(at_col, x);
-                            masked(at_col, x);
-                        });
-                        if constexpr(PLAIN)
-                            top *= sc.c; // scale > 0
-                        // move the maximum where some row of this warp has outgrown it
-                        steep = __any_sync(0xFFFFFFFFu, top > m + RESCALE_STEP);
-                        if(steep)
-                        {
-                            const float m2 = fmaxf(m, top);
-                            const float by = m2 == -INFINITY ? 1.0f : ex2(m - m2);
-                            l *= by;
-                            m = m2;
-                            if(n_s != 0)
+                            wild = false;
+                            top = row_max<true>(s_row, [&](int at_col, auto& x) {
+                                transform(at_col, x);
+                                masked(at_col, x);
+                            });
+                            if constexpr(PLAIN)
+                                top *= sc.c; // scale > 0
+                            // move the maximum where some row of this warp has outgrown it
+                            const bool outgrown = __any_sync(0xFFFFFFFFu, top > m + RESCALE_STEP);
+                            steep = outgrown && n_s != 0;
+                            if(outgrown)
                             {
-                                ok = wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
-                                                                 FWD_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
-                                if(!ok)
-                                    break;
-                                ptx::tc_fence_after_sync();
-#pragma unroll 1
-                                for(uint32_t c = 0; c < HD; c += 32)
+                                const float m2 = fmaxf(m, top);
+                                const float by = m2 == -INFINITY ? 1.0f : ex2(m - m2);
+                                l *= by;
+                                m = m2;
+                                if(n_s != 0)
                                 {
-                                    uint32_t w[32];
-                                    ptx::tmem_ld_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
-                                    ptx::tmem_ld_wait();
+                                    ok = wait_bounded_warp(base + L::O_DONE + 8 * t, (n_s - 1) & 1u, cta_abort, status,
+                                                                     FWD_SOFTMAX << 24 | 1u << 20 | (blockIdx.x & 0xFFFFFu));
+                                    if(!ok)
+                                        break;
+                                    ptx::tc_fence_after_sync();
+#pragma unroll 1
+                                    for(uint32_t c = 0; c < HD; c += 32)
+                                    {
+                                        uint32_t w[32];
+                                        ptx::tmem_ld_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
+                                        ptx::tmem_ld_wait();
 #pragma unroll
-                                    for(int i = 0; i < 32; ++i)
-                                        w[i] = __float_as_uint(__uint_as_float(w[i]) * by);
-                                    tmem_st_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
+                                        for(int i = 0; i < 32; ++i)
+                                            w[i] = __float_as_uint(__uint_as_float(w[i]) * by);
+                                        tmem_st_32x32b_x32(o_tmem[t] + lane_tmem + c, w);
+                                    }
                                 }
                             }
-                        }
-                        const float sub = m == -INFINITY ? 0.0f : -m;
-                        l += weights<T>(s_row, PLAIN ? sc.c : 1.0f, sub);
+                            const float sub = m == -INFINITY ? 0.0f : -m;
+                            l += weights<T>(s_row, PLAIN ? sc.c : 1.0f, sub);
                         }
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();

@@ -11,7 +11,7 @@
 // parts in a fixed order.
 // Measured, bf16, 32/8 heads x 128, one token each: 32 sequences of 4500 tokens 88 us (6.7 TB/s), of 3094 to 6000 tokens 93 us
 // (6.4 TB/s); 8 drafted tokens each, 16 sequences of 8000: 92 us (5.7 TB/s); 5 drafted tokens, 8/2 heads x 64, one sequence of
-// 120000, fp16 with slopes: 22 us (2.8 TB/s; 13 stages to a block, latency).
+// 120000, fp16 with slopes: 20.6 us (3.0 TB/s; 13 stages to a block, latency).
 #include "attn_tc05.cuh"
 
 namespace b200wmma
@@ -23,7 +23,7 @@ namespace b200wmma
         constexpr uint32_t MAX_DRAFTS = 64;
         constexpr uint32_t KEYS       = 64; // tokens of a stage
         constexpr uint32_t THREADS    = 160; // warps 0-3 compute, warp 4 copies
-        constexpr uint32_t MAX_SPLITS = 256;
+        constexpr uint32_t MAX_SPLITS = 256; // what 16 warps join
 
         struct Params
         {
@@ -341,8 +341,7 @@ namespace b200wmma
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 2));
                 }
-                // the maximum moves only where a score passes it by more than 2^8: until then weights grow up to 256
-                if(__any_sync(0xFFFFFFFFu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f))
+                if(__any_sync(0xFFFFFFFFu, top[0] > m[0] + attn::RESCALE_STEP || top[1] > m[1] + attn::RESCALE_STEP))
                 {
                     float by[2];
 #pragma unroll
@@ -469,22 +468,35 @@ namespace b200wmma
             }
         }
 
-        // Joins few splits: a warp to a row, a split's maximum and sum to a lane, four (HD = 128) or two elements to a lane; splits
-        // in order.
-        template <typename T, uint32_t HD>
-        __global__ void __launch_bounds__(256) join_few_kernel(const __grid_constant__ Params p, T* __restrict__ o)
+        // Joins the splits of a row: W warps with up to PER splits each, whose parts are all on their way before the first maximum is
+        // known (148 splits of 8 rows: 2.6 us behind the first kernel, 6.8 with a few loads at a time); HD / 32
+        // elements to a lane; everything in a fixed order.
+        template <uint32_t W>
+        struct Join
         {
-            constexpr uint32_t E = HD / 32;
-            const uint32_t     rows = p.share * p.drafts, row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
-            const uint32_t     all_rows = p.batch * p.heads_kv * rows;
-            const uint32_t     r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
-            const bool         live = row < all_rows && draft < drafts_of(p, b);
+            static constexpr uint32_t PER = W == 16 ? 16 : 8, ROWS = W == 16 ? 1 : 8 / W, THREADS = 32 * W * ROWS; // rows of a block
+        };
+        template <typename T, uint32_t HD, uint32_t W>
+        __global__ void __launch_bounds__(Join<W>::THREADS) join_kernel(const __grid_constant__ Params p, T* __restrict__ o)
+        {
+            constexpr uint32_t E = HD / 32, PER = Join<W>::PER, ROWS = Join<W>::ROWS;
+            using Piece          = std::conditional_t<E == 4, float4, float2>;
+            __shared__ float   red[ROWS][W][HD], stats[ROWS][W][2];
+            const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, slot = warp / W, w = warp % W;
+            const uint32_t rows = p.share * p.drafts, row = blockIdx.x * ROWS + slot, all_rows = p.batch * p.heads_kv * rows;
+            const uint32_t r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
+            const bool     live = row < all_rows && draft < drafts_of(p, b);
+            const uint32_t first = w * PER, mine = live && first < p.splits ? min(PER, p.splits - first) : 0;
             ptx::grid_dep_wait(); // before anything leaves: the kernel may not end before the one it follows
-            if(!live)
-                return;
-            const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (size_t(lane) * all_rows + row) * 2)
-                                              : make_float2(-INFINITY, 0.0f);
-            float        mx = ml.x;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if(lane < mine)
+                ml = *reinterpret_cast<const float2*>(p.part_ml + (size_t(first + lane) * all_rows + row) * 2);
+            Piece part[PER];
+#pragma unroll
+            for(uint32_t k = 0; k < PER; ++k)
+                if(k < mine)
+                    part[k] = *reinterpret_cast<const Piece*>(p.part_o + (size_t(first + k) * all_rows + row) * HD + lane * E);
+            float mx = ml.x;
 #pragma unroll
             for(int d = 16; d > 0; d >>= 1)
                 mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
@@ -493,20 +505,47 @@ namespace b200wmma
 #pragma unroll
             for(int d = 16; d > 0; d >>= 1)
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-#pragma unroll 4
-            for(uint32_t s = 0; s < p.splits; ++s)
+#pragma unroll
+            for(uint32_t k = 0; k < PER; ++k)
             {
-                const float w = __shfl_sync(0xFFFFFFFFu, by, s);
-                if(w != 0.0f) // NaN counts
+                const float f = __shfl_sync(0xFFFFFFFFu, by, k);
+                if(k < mine && f != 0.0f) // NaN counts
                 {
-                    const float* from = p.part_o + (size_t(s) * all_rows + row) * HD + lane * E;
+                    const float* from = reinterpret_cast<const float*>(&part[k]);
 #pragma unroll
                     for(uint32_t e = 0; e < E; ++e)
-                        y[e] = fmaf(w, from[e], y[e]);
+                        y[e] = fmaf(f, from[e], y[e]);
+                }
+            }
+            if constexpr(W > 1)
+            {
+#pragma unroll
+                for(uint32_t e = 0; e < E; ++e)
+                    red[slot][w][lane * E + e] = y[e], y[e] = 0.0f;
+                if(lane == 0)
+                    stats[slot][w][0] = mx, stats[slot][w][1] = sum;
+                __syncthreads();
+                if(w != 0)
+                    return;
+                mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for(uint32_t i = 0; i < W; ++i)
+                    mx = fmaxf(mx, stats[slot][i][0]);
+#pragma unroll
+                for(uint32_t i = 0; i < W; ++i)
+                {
+                    const float f = stats[slot][i][0] == -INFINITY ? 0.0f : ex2(stats[slot][i][0] - mx);
+                    if(f != 0.0f)
+                    {
+                        sum = fmaf(f, stats[slot][i][1], sum);
+#pragma unroll
+                        for(uint32_t e = 0; e < E; ++e)
+                            y[e] = fmaf(f, red[slot][i][lane * E + e], y[e]);
+                    }
                 }
             }
             const float inv = sum > 0.0f ? 1.0f / sum : sum;
-            if(lane * E < p.dim)
+            if(live && lane * E < p.dim)
             {
                 uint32_t* out = reinterpret_cast<uint32_t*>(o + row_of(p.o, b, draft, head * p.share + r % p.share) + lane * E);
 #pragma unroll
@@ -514,73 +553,19 @@ namespace b200wmma
                     out[e / 2] = attn::pack2<T>(y[e] * inv, y[e + 1] * inv);
             }
         }
-
-        // Joins many splits: a block to a row.  The splits' maxima and sums become weights in shared memory, then four warps add
-        // up a quarter of the splits each, four (HD = 128) or two elements to a lane; all in a fixed order.
-        template <typename T, uint32_t HD>
-        __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, T* __restrict__ o)
+        template <typename T, uint32_t HD, uint32_t W>
+        static int launch_join(const Params& p, void* o, cudaStream_t stream)
         {
-            constexpr uint32_t E = HD / 32;
-            __shared__ float   by[MAX_SPLITS], red[4][HD], top[4], total[4];
-            ptx::grid_dep_wait();
-            const uint32_t rows = p.share * p.drafts, row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-            const uint32_t all_rows = p.batch * p.heads_kv * rows;
-            const uint32_t r = row % rows, head = row / rows % p.heads_kv, b = row / rows / p.heads_kv, draft = r / p.share;
-            if(draft >= drafts_of(p, b))
-                return;
-            static_assert(MAX_SPLITS == 256, "two splits to a thread");
-            float2 ml[2];
-            float  mx = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for(int i = 0; i < 2; ++i)
-            {
-                const uint32_t s = threadIdx.x + 128 * i;
-                ml[i] = s < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (size_t(s) * all_rows + row) * 2) : make_float2(-INFINITY, 0.0f);
-                mx    = fmaxf(mx, ml[i].x);
-            }
-#pragma unroll
-            for(int d = 16; d > 0; d >>= 1)
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-            if(lane == 0)
-                top[warp] = mx;
-            __syncthreads();
-            mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-#pragma unroll
-            for(int i = 0; i < 2; ++i)
-            {
-                const float w = ml[i].x == -INFINITY ? 0.0f : ex2(ml[i].x - mx);
-                by[threadIdx.x + 128 * i] = w;
-                sum = ml[i].x == -INFINITY ? sum : fmaf(w, ml[i].y, sum);
-            }
-#pragma unroll
-            for(int d = 16; d > 0; d >>= 1)
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-            if(lane == 0)
-                total[warp] = sum;
-            __syncthreads();
-            float y[E] = {};
-#pragma unroll 8
-            for(uint32_t s = warp; s < p.splits; s += 4)
-                if(by[s] != 0.0f) // NaN counts; splits without a visible token have written no sums
-                {
-                    const float* from = p.part_o + (size_t(s) * all_rows + row) * HD + lane * E;
-#pragma unroll
-                    for(uint32_t e = 0; e < E; ++e)
-                        y[e] = fmaf(by[s], from[e], y[e]);
-                }
-#pragma unroll
-            for(uint32_t e = 0; e < E; ++e)
-                red[warp][lane * E + e] = y[e];
-            __syncthreads();
-            sum             = (total[0] + total[1]) + (total[2] + total[3]);
-            const float inv = sum > 0.0f ? 1.0f / sum : sum;
-            const uint32_t d = threadIdx.x * 2;
-            if(d < p.dim)
-            {
-                const float u = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
-                const float v = (red[0][d + 1] + red[1][d + 1]) + (red[2][d + 1] + red[3][d + 1]);
-                *reinterpret_cast<uint32_t*>(o + row_of(p.o, b, draft, head * p.share + r % p.share) + d) = attn::pack2<T>(u * inv, v * inv);
-            }
+            const uint32_t     rows = p.batch * p.heads_kv * p.share * p.drafts;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(ceil_div(rows, Join<W>::ROWS)), cfg.blockDim = dim3(Join<W>::THREADS), cfg.stream = stream;
+            // launched while the last blocks of the kernel before it still run; it waits for them before it reads
+            cudaLaunchAttribute attr{};
+            attr.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr.val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = &attr, cfg.numAttrs = 1;
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T, HD, W>, p, static_cast<T*>(o)));
+            return B200WMMA_OK;
         }
 
         // More rows than 32 take the tcgen05 form: 8 drafted tokens x 4 heads (32 rows) over 16 x 8000 tokens take 92 us with
@@ -634,20 +619,10 @@ namespace b200wmma
                 kern<<<grid, THREADS, Smem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q), static_cast<T*>(o));
             }
             B200_CHECK_CUDA(cudaGetLastError());
-            if(p.splits > 1)
-            {
-                const uint32_t     rows = p.batch * p.heads_kv * p.share * p.drafts;
-                const bool         few  = p.splits <= 32;
-                cudaLaunchConfig_t cfg{};
-                cfg.gridDim = dim3(few ? ceil_div(rows, 8) : rows), cfg.blockDim = dim3(few ? 256 : 128), cfg.stream = stream;
-                // launched while the last blocks of the kernel above still run; it waits for them before it reads
-                cudaLaunchAttribute attr{};
-                attr.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-                attr.val.programmaticStreamSerializationAllowed = 1;
-                cfg.attrs = &attr, cfg.numAttrs = 1;
-                B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, few ? join_few_kernel<T, HD> : join_kernel<T, HD>, p, static_cast<T*>(o)));
-            }
-            return B200WMMA_OK;
+            if(p.splits == 1)
+                return B200WMMA_OK;
+            return p.splits <= Join<1>::PER       ? launch_join<T, HD, 1>(p, o, stream)
+                   : p.splits <= 4 * Join<4>::PER ? launch_join<T, HD, 4>(p, o, stream) : launch_join<T, HD, 16>(p, o, stream);
         }
         template <typename T, uint32_t HD, uint32_t WM>
         static int launch_scores(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)

@@ -338,8 +338,7 @@ namespace b200wmma
                         });
                     };
                     const float top = masked ? scores(std::true_type{}) : scores(std::false_type{});
-                    // the maximum moves only where a score passes it by more than 2^8: until then weights grow up to 256
-                    if(__any_sync(0xFFFFFFFFu, top > m + 8.0f))
+                    if(__any_sync(0xFFFFFFFFu, top > m + attn::RESCALE_STEP))
                     {
                         const float m2 = fmaxf(m, top), by = m2 == -INFINITY ? 1.0f : ex2(m - m2);
                         l *= by;

@@ -231,6 +231,16 @@ def test_repeat_stream_and_graphs():
 
 
 @gpu
+@pytest.mark.parametrize("batch,hk,d", [(1, 1, 64), (1, 2, 128), (6, 2, 128), (30, 2, 64), (40, 1, 128)])
+def test_many_splits_and_few(batch, hk, d):
+    """A long table makes many splits, of which short sequences fill a few: 148 blocks' worth to 4."""
+    g = torch.Generator().manual_seed(batch)
+    lens = [int(x) for x in torch.randint(0, 400, (batch,), generator=g)]
+    lens[0] = 24000 // batch
+    Case(lens, 2, 2 * hk, hk, d, 32, F16, seed=batch).check(0.1)
+
+
+@gpu
 @pytest.mark.parametrize("t,hq", [(1, 2), (12, 4), (20, 8)])
 @pytest.mark.parametrize("n", [30, 3000])
 def test_a_query_that_is_nan_shows(t, hq, n):
