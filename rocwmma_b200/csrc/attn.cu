@@ -72,17 +72,26 @@ namespace b200wmma
             return B200WMMA_OK;
         }
 
-        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
-        static int launch_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
+        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN, uint32_t PER>
+        static int launch_fwd_as(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
                               unsigned* status, cudaStream_t stream)
         {
-            auto kern = fwd_tc05_kernel<T, HD, CAP, BIAS, PLAIN>;
+            auto kern = fwd_tc05_kernel<T, HD, CAP, BIAS, PLAIN, PER>;
             B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<HD>::BYTES));
-            const uint32_t q_blocks = ceil_div(p.len_q, 2 * TILE);
+            const uint32_t q_blocks = ceil_div(p.len_q, PER * TILE);
             kern<<<q_blocks * p.batch * p.heads_q, FWD_THREADS, FwdSmem<HD>::BYTES, stream>>>(maps[0], maps[1], maps[2], maps[3], p, lse,
                                                                                               dq, dk, q_blocks, status);
             B200_CHECK_CUDA(cudaGetLastError());
             return B200WMMA_OK;
+        }
+        // One tile of queries to a block where those blocks still run all at once: 2 x 8 heads of 1024 x 128, causal, 16.6 us (21.5 with
+        // two tiles), with cap and slopes 28 us (38); more of them lose (2 x 16 heads of 4096 x 128, causal: 213 us, 140 with two).
+        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
+        static int launch_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
+                              unsigned* status, cudaStream_t stream)
+        {
+            return tiles_of(p.len_q) * p.batch * p.heads_q <= 148 ? launch_fwd_as<T, HD, CAP, BIAS, PLAIN, 1>(p, maps, lse, dq, dk, status, stream)
+                                                                  : launch_fwd_as<T, HD, CAP, BIAS, PLAIN, 2>(p, maps, lse, dq, dk, status, stream);
         }
         template <typename T, uint32_t HD>
         static int run_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,

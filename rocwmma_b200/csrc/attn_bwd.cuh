@@ -432,7 +432,7 @@ namespace b200wmma
                     ptx::tc_fence_after_sync();
                     // every product is done: the tiles of K and V make room
                     stage_row<T>(smem + L::OWN + half * L::TILE_BYTES, threadIdx.x & 127u, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), 0, HD,
-                                 half ? p.scale : 1.0f, it != 0);
+                                 it == 0 ? 0.0f : half ? p.scale : 1.0f);
                     ptx::fence_proxy_async_smem();
                 }
                 ptx::named_bar_sync(1 + half, TILE); // warps that gave up come here too
@@ -775,8 +775,8 @@ namespace b200wmma
                     if(half == 0 && row < p.len_q)
                         delta[(size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row] = de + rest;
                     // every product is done: the tile of Q makes room; both halves of the threads take half of the columns
-                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2), p.scale, it != 0,
-                                 pk_tmem + ((quad * 32u) << 16), rest);
+                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2),
+                                 it != 0 ? p.scale : 0.0f, pk_tmem + ((quad * 32u) << 16), it != 0 ? -rest * p.scale : 0.0f);
                     ptx::fence_proxy_async_smem();
                 }
                 ptx::named_bar_sync(1, 256);

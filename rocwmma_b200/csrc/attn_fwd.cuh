@@ -1,6 +1,7 @@
 // Forward attention on tcgen05.
 //
-// A CTA owns 256 queries of one head as two tiles of 128 and walks the key tiles that either of them sees.  Per tile
+// A CTA owns 256 queries of one head as two tiles of 128 and walks the key tiles that either of them sees.  (Where the grid is
+// small it owns one tile of queries, whose even and odd key tiles take the places of the two: PER = 1.)  Per tile
 //   S = Q K^T (tensor cores, fp32 in tensor memory) -> softmax warps: running maximum and sum, P = 2^(x - m) in 16 bits over S
 //   -> O += P V (tensor cores, P from tensor memory).
 // The two tiles take turns: while the tensor cores work on one, 128 threads (one to a query) do the softmax of the other.
@@ -31,7 +32,8 @@ namespace b200wmma
             static constexpr uint32_t KV         = Q + 2 * TILE_BYTES;
             static constexpr uint32_t LIST       = KV + STAGES * TILE_BYTES; // SEG words
             static constexpr uint32_t RAW        = LIST + SEG * 4; // SEG bytes of flags before they are listed
-            static constexpr uint32_t BARS       = RAW + SEG;
+            static constexpr uint32_t STATS      = RAW + SEG; // 2 x 128 maxima, 2 x 128 sums
+            static constexpr uint32_t BARS       = STATS + 4 * TILE * 4;
             static constexpr uint32_t Q_FULL = BARS, KV_FULL = Q_FULL + 8, KV_EMPTY = KV_FULL + 8 * STAGES, S_FULL = KV_EMPTY + 8 * STAGES,
                                       P_FULL = S_FULL + 16, O_DONE = P_FULL + 16;
             static constexpr uint32_t MISC  = O_DONE + 16; // tensor memory address, abort flag, list length
@@ -46,7 +48,7 @@ namespace b200wmma
             FWD_SOFTMAX  = 0x33
         };
 
-        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN>
+        template <typename T, uint32_t HD, bool CAP, bool BIAS, bool PLAIN, uint32_t PER>
         __global__ void __launch_bounds__(FWD_THREADS, 1)
             fwd_tc05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
@@ -67,9 +69,10 @@ namespace b200wmma
             // the last queries first: under a causal mask they take longest
             const uint32_t bh = blockIdx.x % (p.batch * p.heads_q), q_block = q_blocks - 1 - blockIdx.x / (p.batch * p.heads_q);
             const uint32_t h = bh % p.heads_q, b = bh / p.heads_q, g = h / (p.heads_q / p.heads_kv);
-            const uint32_t row0 = q_block * 2 * TILE, q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
+            const uint32_t row0 = q_block * PER * TILE, q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
             const int32_t  prefix = p.prefix ? p.prefix[b] : 0;
             const bool     docs   = p.doc_q != nullptr;
+            constexpr uint32_t ahead = PER == 2 ? 1 : 2; // key tiles whose scores are asked for before the weights of one are there
 
             if(threadIdx.x == 0)
             {
@@ -104,10 +107,10 @@ namespace b200wmma
             const uint32_t s_tmem[2] = {tmem, tmem + TILE}, o_tmem[2] = {tmem + 2 * TILE, tmem + 2 * TILE + HD};
 
             // roles keep their place in the rings from one segment of the key tiles to the next
-            uint32_t   it = 0; // producer, MMA: key tiles so far (a key and a value stage each)
+            uint32_t   c = 0; // producer, MMA: place in the ring
             uint32_t   done[2] = {0, 0}; // MMA: S tiles so far of each query tile
             const uint32_t t   = warp >> 2; // softmax: this thread's query tile
-            const uint32_t row = row0 + t * TILE + (threadIdx.x & 127u), quad = warp & 3u;
+            const uint32_t row = row0 + (PER == 2 ? t * TILE : 0) + (threadIdx.x & 127u), quad = warp & 3u;
             const int32_t  at  = int32_t(row) + p.off;
             uint32_t       n_s = 0; // softmax: S tiles so far
             float          m = -INFINITY, l = 0.0f;
@@ -117,13 +120,18 @@ namespace b200wmma
             // keys [0, lim) of this row are visible as far as causality and lengths go
             const int32_t lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
 
+            // TILE_NEED, TILE_MASK of the e-th key tile (of `entries`, from the last) for place u
+            const auto flags = [&](uint32_t entries, uint32_t e, uint32_t u) {
+                const uint32_t f = list[entries - 1 - e] >> 24;
+                return PER == 2 ? f >> (2 * u) : ((e ^ u) & 1u) ? 0u : f;
+            };
             for(uint32_t seg = (kv_tiles - 1) / SEG * SEG;; seg -= SEG)
             {
                 // the key tiles of this segment that a query of the CTA sees, with the flags of both query tiles
                 const uint32_t entries = list_tiles<FWD_THREADS>(seg, min(SEG, kv_tiles - seg), list, raw, misc + 2, [&](uint32_t tile) {
                     uint32_t       f  = 0;
                     const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + tile : nullptr;
-                    for(uint32_t u = 0; u < 2; ++u)
+                    for(uint32_t u = 0; u < PER; ++u)
                     {
                         const uint32_t r0 = row0 + u * TILE;
                         if(r0 < p.len_q)
@@ -142,24 +150,33 @@ namespace b200wmma
                     {
                         if(!q_here)
                         {
-                            const uint32_t n = row0 + TILE < p.len_q ? 2u : 1u;
+                            const uint32_t n = PER == 2 && row0 + TILE < p.len_q ? 2u : 1u;
                             ptx::mbar_arrive_expect_tx(base + L::Q_FULL, n * L::TILE_BYTES);
                             for(uint32_t u = 0; u < n; ++u)
                                 load_tile<HD>(base + L::Q + u * L::TILE_BYTES, &map_q, row0 + u * TILE, h, b, base + L::Q_FULL);
                             q_here = true;
                         }
-                        for(uint32_t e = 0; ok && e < entries; ++e, ++it)
-                            for(uint32_t half = 0; ok && half < 2; ++half)
-                            {
-                                const uint32_t n = 2 * it + half, st = n % L::STAGES, ph = (n / L::STAGES) & 1u;
-                                ok = ptx::mbar_wait_bounded(base + L::KV_EMPTY + 8 * st, ph ^ 1u, cta_abort, status,
-                                                            FWD_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS);
-                                if(!ok)
-                                    break;
-                                ptx::mbar_arrive_expect_tx(base + L::KV_FULL + 8 * st, L::TILE_BYTES);
-                                load_tile<HD>(base + L::KV + st * L::TILE_BYTES, half ? &map_v : &map_k, (list[entries - 1 - e] & 0xFFFFFFu) * TILE, g, b,
-                                              base + L::KV_FULL + 8 * st);
-                            }
+                        const auto load = [&](const CUtensorMap* map, uint32_t e) {
+                            const uint32_t st = c % L::STAGES, ph = (c / L::STAGES) & 1u;
+                            ok = ok
+                                 && ptx::mbar_wait_bounded(base + L::KV_EMPTY + 8 * st, ph ^ 1u, cta_abort, status,
+                                                           FWD_PRODUCER << 24 | (blockIdx.x & 0xFFFFFFu), tc05::WAIT_TIMEOUT_NS);
+                            if(!ok)
+                                return;
+                            ++c;
+                            ptx::mbar_arrive_expect_tx(base + L::KV_FULL + 8 * st, L::TILE_BYTES);
+                            load_tile<HD>(base + L::KV + st * L::TILE_BYTES, map, (list[entries - 1 - e] & 0xFFFFFFu) * TILE, g, b,
+                                          base + L::KV_FULL + 8 * st);
+                        };
+                        // in the order of their use: the keys of the first tiles, then values and the keys `ahead` tiles on
+                        for(uint32_t e = 0; e < min(ahead, entries); ++e)
+                            load(&map_k, e);
+                        for(uint32_t e = 0; ok && e < entries; ++e)
+                        {
+                            load(&map_v, e);
+                            if(e + ahead < entries)
+                                load(&map_k, e + ahead);
+                        }
                     }
                     __syncwarp();
                 }
@@ -187,9 +204,9 @@ namespace b200wmma
                         return true;
                     };
                     const auto scores = [&](uint32_t u, uint32_t e, uint32_t n) { // S of query tile u
-                        if((list[entries - 1 - e] >> (24 + 2 * u) & TILE_NEED) && elect_one())
+                        if((flags(entries, e, u) & TILE_NEED) && elect_one())
                         {
-                            mma_over_head<T, HD>(s_tmem[u], base + L::Q + u * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
+                            mma_over_head<T, HD>(s_tmem[u], base + L::Q + (PER == 2 ? u : 0) * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL + 8 * u);
                         }
                     };
@@ -202,41 +219,42 @@ namespace b200wmma
                         if(!q_here)
                             wait(base + L::Q_FULL, 0, 0);
                         q_here = true;
-                        if(ok && arrive_kv(2 * it, 0))
+                        for(uint32_t e = 0; ok && e < min(ahead, entries); ++e)
+                            if(arrive_kv(c, e))
+                            {
+                                scores(0, e, c);
+                                scores(1, e, c);
+                                free_stage(c++);
+                            }
+                        for(uint32_t e = 0; ok && e < entries; ++e)
                         {
-                            scores(0, 0, 2 * it);
-                            scores(1, 0, 2 * it);
-                            free_stage(2 * it);
-                        }
-                        for(uint32_t e = 0; ok && e < entries; ++e, ++it)
-                        {
-                            if(!arrive_kv(2 * it + 1, e))
+                            if(!arrive_kv(c, e))
                                 break;
-                            const bool more = e + 1 < entries;
-                            if(more && !arrive_kv(2 * it + 2, e + 1))
+                            const bool more = e + ahead < entries;
+                            if(more && !arrive_kv(c + 1, e + ahead))
                                 break;
                             for(uint32_t u = 0; ok && u < 2; ++u)
                             {
-                                if(list[entries - 1 - e] >> (24 + 2 * u) & TILE_NEED)
+                                if(flags(entries, e, u) & TILE_NEED)
                                 {
                                     if(!wait(base + L::P_FULL + 8 * u, done[u] & 1u, 2 + u))
                                         break;
                                     if(elect_one())
                                     {
-                                        mma_over_tokens<T, HD>(o_tmem[u], s_tmem[u], base + L::KV + ((2 * it + 1) % L::STAGES) * L::TILE_BYTES,
+                                        mma_over_tokens<T, HD>(o_tmem[u], s_tmem[u], base + L::KV + (c % L::STAGES) * L::TILE_BYTES,
                                                                done[u] != 0);
                                         ptx::tc_commit(base + L::O_DONE + 8 * u);
                                     }
                                     ++done[u];
                                 }
                                 if(more)
-                                    scores(u, e + 1, 2 * it + 2);
+                                    scores(u, e + ahead, c + 1);
                             }
                             if(!ok)
                                 break;
-                            free_stage(2 * it + 1);
+                            free_stage(c++);
                             if(more)
-                                free_stage(2 * it + 2);
+                                free_stage(c++);
                         }
                     }
                     __syncwarp();
@@ -247,7 +265,7 @@ namespace b200wmma
                     const uint32_t lane_tmem = (quad * 32u) << 16;
                     for(uint32_t e = 0; ok && e < entries; ++e)
                     {
-                        const uint32_t f = list[entries - 1 - e] >> (24 + 2 * t);
+                        const uint32_t f = flags(entries, e, t);
                         if(!(f & TILE_NEED))
                             continue;
                         const uint32_t c0 = (list[entries - 1 - e] & 0xFFFFFFu) * TILE;
@@ -403,18 +421,40 @@ namespace b200wmma
                                                      FWD_SOFTMAX << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                     ptx::tc_fence_after_sync();
                 }
-                if(ok)
+                // every product of this tile is done: its Q makes room for the results
+                const uint32_t tile_smem = L::Q + (PER == 2 ? t * L::TILE_BYTES : 0), tile_row = threadIdx.x & 127u, lane_tmem = (quad * 32u) << 16;
+                if(PER == 2)
                 {
-                    const float inv = l > 0.0f ? 1.0f / l : l; // NaN stays NaN
-                    // every product of this tile is done: its Q makes room
-                    stage_row<T>(smem + L::Q + t * L::TILE_BYTES, threadIdx.x & 127u, o_tmem[t] + ((quad * 32u) << 16), 0, HD, inv, have && l != 0.0f);
-                    ptx::fence_proxy_async_smem();
-                    if(lse && row < p.len_q)
-                        lse[(size_t(b) * p.heads_q + h) * p.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                    if(ok)
+                        stage_row<T>(smem + tile_smem, tile_row, o_tmem[t] + lane_tmem, 0, HD, have && l != 0.0f ? inverse(l) : 0.0f);
                 }
-                ptx::named_bar_sync(1 + t, TILE); // warps that gave up come here too
-                if((threadIdx.x & 127u) == 0 && row < p.len_q && !*cta_abort)
-                    store_tile<HD>(&map_o, base + L::Q + t * L::TILE_BYTES, row, h, b);
+                else
+                {
+                    // the even and the odd key tiles meet; each group of threads takes half of the columns
+                    float* stats = reinterpret_cast<float*>(smem + L::STATS);
+                    stats[threadIdx.x] = m, stats[2 * TILE + threadIdx.x] = l;
+                    ptx::tc_fence_before_sync();
+                    ptx::named_bar_sync(1, 2 * TILE); // warps that gave up come here too
+                    ptx::tc_fence_after_sync();
+                    const float m0 = stats[tile_row], m1 = stats[TILE + tile_row];
+                    float       l0 = stats[2 * TILE + tile_row], l1 = stats[3 * TILE + tile_row];
+                    m = fmaxf(m0, m1);
+                    const float by0 = l0 == 0.0f ? 0.0f : m0 == -INFINITY ? l0 : ex2(m0 - m), by1 = l1 == 0.0f ? 0.0f : m1 == -INFINITY ? l1 : ex2(m1 - m);
+                    l = by0 * l0 + by1 * l1; // l0 of NaN alone, without a maximum, stays NaN
+                    if(ok)
+                        stage_row<T>(smem + tile_smem, tile_row, o_tmem[0] + lane_tmem, t * (HD / 2), (t + 1) * (HD / 2),
+                                     by0 != 0.0f ? by0 * inverse(l) : 0.0f, o_tmem[1] + lane_tmem, by1 != 0.0f ? by1 * inverse(l) : 0.0f);
+                }
+                if(ok)
+                    ptx::fence_proxy_async_smem();
+                if(ok && lse && row < p.len_q && (PER == 2 || t == 0))
+                    lse[(size_t(b) * p.heads_q + h) * p.len_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                if(PER == 2)
+                    ptx::named_bar_sync(1 + t, TILE);
+                else
+                    ptx::named_bar_sync(1, 2 * TILE);
+                if(tile_row == 0 && (PER == 2 || t == 0) && row < p.len_q && !*cta_abort)
+                    store_tile<HD>(&map_o, base + tile_smem, row, h, b);
             }
             ptx::tc_fence_before_sync();
             __syncthreads();

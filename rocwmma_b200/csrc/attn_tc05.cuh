@@ -318,13 +318,18 @@ namespace b200wmma
                          "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src_smem)
                          : "memory");
         }
+        // 1 / l; NaN stays NaN
+        __device__ __forceinline__ float inverse(float l)
+        {
+            return l > 0.0f ? 1.0f / l : l;
+        }
         // Columns [from, to) of this thread's row of an fp32 accumulator, times `by`, as 16-bit values into row `row` of a tile in
         // shared memory with the 128-byte swizzle, from where TMA writes whole rows (a thread's own 16-byte stores to its row
-        // would each touch a line of their own: 2.5 us for a tile).  `live`: the accumulator counts, otherwise zeros.  `minus`: a
-        // second accumulator (its tensor memory address, 0: none) of which `less` times is taken off first.
+        // would each touch a line of their own: 2.5 us for a tile).  `other`: a second accumulator (0: none), which counts `by2`
+        // times.  A factor of 0 takes an accumulator out, whatever it holds.
         template <typename T>
-        __device__ __forceinline__ void stage_row(uint8_t* tile, uint32_t row, uint32_t taddr, uint32_t from, uint32_t to, float by, bool live,
-                                                  uint32_t minus = 0, float less = 0.0f)
+        __device__ __forceinline__ void stage_row(uint8_t* tile, uint32_t row, uint32_t taddr, uint32_t from, uint32_t to, float by,
+                                                  uint32_t other = 0, float by2 = 0.0f)
         {
 #pragma unroll 1
             for(uint32_t c = from; c < to; c += 32)
@@ -332,23 +337,26 @@ namespace b200wmma
                 uint32_t w[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32b_x32(taddr + c, w);
-                if(minus != 0)
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for(int i = 0; i < 32; ++i)
+                    w[i] = by != 0.0f ? __float_as_uint(__uint_as_float(w[i]) * by) : 0u;
+                if(other != 0)
                 {
                     uint32_t x[32];
-                    ptx::tmem_ld_32x32b_x32(minus + c, x);
+                    ptx::tmem_ld_32x32b_x32(other + c, x);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for(int i = 0; i < 32; ++i)
-                        w[i] = __float_as_uint(fmaf(-less, __uint_as_float(x[i]), __uint_as_float(w[i])));
+                        w[i] = by2 != 0.0f ? __float_as_uint(fmaf(by2, __uint_as_float(x[i]), __uint_as_float(w[i]))) : w[i];
                 }
-                ptx::tmem_ld_wait();
 #pragma unroll
                 for(int i = 0; i < 4; ++i)
                 {
                     uint32_t u[4];
 #pragma unroll
                     for(int j = 0; j < 4; ++j)
-                        u[j] = live ? pack2<T>(__uint_as_float(w[8 * i + 2 * j]) * by, __uint_as_float(w[8 * i + 2 * j + 1]) * by) : 0u;
+                        u[j] = pack2<T>(__uint_as_float(w[8 * i + 2 * j]), __uint_as_float(w[8 * i + 2 * j + 1]));
                     const uint32_t at = c / 8 + i; // 16-byte piece of the row
                     *reinterpret_cast<uint4*>(tile + (at / 8) * BOX_BYTES + row * 128 + (((at % 8) ^ (row & 7u)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
                 }

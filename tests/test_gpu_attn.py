@@ -221,6 +221,34 @@ def test_a_longer_sequence(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lq,lk,d", [(300, 300, 128), (257, 390, 64), (384, 150, 80)])
+def test_more_blocks_than_run_at_once(lq, lk, d, dtype):
+    """Grids large enough that a block takes two tiles of queries, with each kind of mask and score."""
+    q, k, v, dout = inputs(4, lq, lk, 20, 5, d, dtype, seed=29, loud=3.0)
+    docs = lambda n: torch.stack([documents(kind, n, 1) for kind in ("sorted", "mixed", "padded", "none")])
+    check(q, k, v, dout, 1 / math.sqrt(d), causal=True)
+    check(q, k, v, dout, 1 / math.sqrt(d), causal=True, cap=20.0, prefix=torch.tensor([0, 30, 140, 600], dtype=torch.int32))
+    check(q, k, v, dout, 1 / math.sqrt(d), slopes=slopes_of(20))
+    check(q, k, v, dout, 1 / math.sqrt(d), causal=lq == lk, doc_q=docs(lq), doc_kv=docs(lk) if lq != lk else docs(lq))
+
+
+@gpu
+@pytest.mark.parametrize("batch", [1, 40])
+@pytest.mark.parametrize("how", ["rising", "falling", "some"])
+@pytest.mark.parametrize("cap", [0.0, 15.0])
+def test_scores_of_very_different_sizes(cap, how, batch):
+    """Key tiles that outgrow one another by more than the maximum may lag behind, in either order and now and then; under a cap
+    some of them bent hard and others hardly."""
+    lq, lk = 200, 1100
+    q, k, v, dout = inputs(batch, lq, lk, 2, 2, 64, BF16, seed=31)
+    at = torch.arange(lk) // 128
+    size = {"rising": 0.02 * 3.0 ** at, "falling": 0.02 * 3.0 ** (8 - at), "some": torch.where(at % 3 == 1, 30.0, 0.1)}[how]
+    k = (k.float() * size[None, :, None, None]).to(BF16)
+    check(q, k, v, dout, 0.125, cap=cap)
+
+
+@gpu
 @pytest.mark.parametrize("lq,lk", [(3, 66000), (66000, 3), (260, 66100)])
 @pytest.mark.parametrize("docs", [False, True])
 def test_more_tiles_than_one_list_holds(lq, lk, docs):
