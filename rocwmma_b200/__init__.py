@@ -1,4 +1,4 @@
-"""rocwmma_b200: the rocWMMA GEMM / DLRM / GEMV hot path as hand-written sm_100a kernels.
+"""rocwmma_b200: the rocWMMA GEMM / DLRM / GEMV hot path, 4-bit products and attention as hand-written sm_100a kernels.
 
 Layout of the package:
   csrc/        CUDA kernels and the C ABI (built into librocwmma_b200.so by build.py)

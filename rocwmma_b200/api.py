@@ -306,12 +306,15 @@ def gemv_w4(m, n, rows, a_packed, lda_bytes, scales, ld_scales, group, x, ldx, y
                                  kind if out is dt else OUT_F32, _raw_stream(here)))
 
 
-def _attn_tensor(t, dtype, name, device, shape=None):
-    """Address of a four-dimensional tensor with contiguous rows."""
-    at = _need_here(t, dtype, name, device)
-    if t.dim() != 4 or t.stride(3) != 1 or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must have four dimensions, the last one contiguous" + (f", of shape {tuple(shape)}" if shape else ""))
-    return at
+def _attn_tensor(t, dtype, name, device, like):
+    """Address and strides of a four-dimensional tensor with contiguous rows, of the shape of `like`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != device:
+        _need_here(t, dtype, name, device)
+    st = t.stride()
+    if len(st) != 4 or st[3] != 1 or (t is not like and t.shape != like.shape):
+        raise ValueError(f"{name} must have four dimensions, the last one contiguous"
+                         + (f", of shape {tuple(like.shape)}" if t is not like else ""))
+    return t.data_ptr(), st[:3]
 
 
 def _attn_vector(t, dtype, shape, name, device):
@@ -338,16 +341,15 @@ _NO_STRIDES = (0, 0, 0)
 def _attn_call(q, k, v, o, lse, scale, causal, cap, slopes, prefix, doc_q, doc_kv, workspace, grads=()):
     """Checked tensors of attn_fwd and attn_bwd: (packed arguments, addresses, workspace address and size, stream)."""
     dt, kind, here = _attn_type(q)
-    at = [_attn_tensor(q, dt, "q", here), _attn_tensor(k, dt, "k", here)]
+    at, strides = [], ()
+    for name, t, like in (("q", q, q), ("k", k, k), ("v", v, k), ("o", o, q), *grads):
+        address, st = _attn_tensor(t, dt, name, here, like)
+        at.append(address)
+        strides += st
     batch, len_q, heads_q, dim = q.shape
-    len_kv, heads_kv = k.shape[1], k.shape[2]
-    if k.shape[0] != batch or k.shape[3] != dim:
+    batch_kv, len_kv, heads_kv, dim_kv = k.shape
+    if batch_kv != batch or dim_kv != dim:
         raise ValueError("q and k must have the same batch and head size")
-    at += [_attn_tensor(v, dt, "v", here, k.shape), _attn_tensor(o, dt, "o", here, q.shape)]
-    strides = q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + o.stride()[:3]
-    for name, t, like in grads:
-        at.append(_attn_tensor(t, dt, name, here, like.shape))
-        strides += t.stride()[:3]
     at.append(_attn_vector(lse, torch.float32, (batch, heads_q, len_q), "lse", here))
     args = ATTN_ARGS.pack(batch, heads_q, heads_kv, len_q, len_kv, dim, kind, bool(causal), scale, cap,
                           _attn_vector(slopes, torch.float32, (heads_q,), "slopes", here),
@@ -403,18 +405,18 @@ def attn_tree(q, k_cache, v_cache, block_table, lens, o, scale, tree=None, depth
     tree: [batch, drafts] int64, bit j of word i set where drafted token i sees drafted token j (None: j <= i); depths:
     [batch, drafts] int32, for the distances (None: 0, 1, 2, ...)."""
     dt, kind, here = _attn_type(q)
-    q_, k_ = _attn_tensor(q, dt, "q", here), _attn_tensor(k_cache, dt, "k_cache", here)
+    (q_, sq), (k_, sk) = _attn_tensor(q, dt, "q", here, q), _attn_tensor(k_cache, dt, "k_cache", here, k_cache)
     batch, drafts, heads_q, dim = q.shape
     pages, page_size, heads_kv, _ = k_cache.shape
     if k_cache.shape[3] != dim:
         raise ValueError("q and the caches must have the same head size")
-    v_, o_ = _attn_tensor(v_cache, dt, "v_cache", here, k_cache.shape), _attn_tensor(o, dt, "o", here, q.shape)
+    (v_, sv), (o_, so) = _attn_tensor(v_cache, dt, "v_cache", here, k_cache), _attn_tensor(o, dt, "o", here, q)
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
         raise ValueError("block_table must have two dimensions")
     width = block_table.shape[1]
     args = ATTN_ARGS.pack(batch, heads_q, heads_kv, 0, 0, dim, kind, 0, scale, cap,
-                          _attn_vector(slopes, torch.float32, (heads_q,), "slopes", here), 0, 0, 0, *q.stride()[:3], *k_cache.stride()[:3],
-                          *v_cache.stride()[:3], *o.stride()[:3], *(_NO_STRIDES * 4))
+                          _attn_vector(slopes, torch.float32, (heads_q,), "slopes", here), 0, 0, 0, *sq, *sk, *sv, *so,
+                          *(_NO_STRIDES * 4))
     ws, size = _attn_workspace(workspace, here)
     check(lib().b200wmma_attn_tree(args, drafts, q_, k_, v_, pages, page_size,
                                    _attn_vector(block_table, torch.int32, (batch, width), "block_table", here), width,

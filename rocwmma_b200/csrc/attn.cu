@@ -77,7 +77,9 @@ namespace b200wmma
                               unsigned* status, cudaStream_t stream)
         {
             auto kern = fwd_tc05_kernel<T, HD, CAP, BIAS, PLAIN, PER>;
-            B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<HD>::BYTES));
+            static Allowed allowed;
+            if(int e = allow_smem(reinterpret_cast<const void*>(kern), FwdSmem<HD>::BYTES, allowed))
+                return e;
             const uint32_t q_blocks = ceil_div(p.len_q, PER * TILE);
             kern<<<q_blocks * p.batch * p.heads_q, FWD_THREADS, FwdSmem<HD>::BYTES, stream>>>(maps[0], maps[1], maps[2], maps[3], p, lse,
                                                                                               dq, dk, q_blocks, status);
@@ -122,8 +124,11 @@ namespace b200wmma
         {
             auto dkv = bwd_dkv_kernel<T, HD, CAP, BIAS>;
             auto dq  = bwd_dq_kernel<T, HD, CAP, BIAS>;
-            B200_CHECK_CUDA(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::BYTES));
-            B200_CHECK_CUDA(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::BYTES));
+            static Allowed allowed[2];
+            if(int e = allow_smem(reinterpret_cast<const void*>(dkv), BwdSmem<HD>::BYTES, allowed[0]))
+                return e;
+            if(int e = allow_smem(reinterpret_cast<const void*>(dq), BwdSmem<HD>::BYTES, allowed[1]))
+                return e;
             const uint32_t padded = uint32_t(tiles_of(p.len_q)) * TILE, rows = p.batch * p.heads_q * padded;
             bwd_rows_kernel<T><<<rows / 16, 256, 0, c.stream>>>(p, static_cast<const T*>(c.o), static_cast<const T*>(c.dout), c.lse, c.lse2, c.delta,
                                                                 padded, rows);

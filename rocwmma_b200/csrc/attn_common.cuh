@@ -3,6 +3,7 @@
 #pragma once
 #include "common.cuh"
 
+#include <atomic>
 #include <cuda_bf16.h>
 #include <type_traits>
 
@@ -46,6 +47,20 @@ namespace b200wmma
                 return __float2half_rn(x);
             else
                 return __float2bfloat16_rn(x);
+        }
+
+        // Lets a kernel use this much dynamic shared memory; asked of the driver once per device and kernel (`allowed` is the
+        // kernel's own), which saves a launch-bound caller half a microsecond a call.
+        using Allowed = std::atomic<uint32_t>[MAX_DEVICES];
+        static int allow_smem(const void* kern, uint32_t bytes, Allowed& allowed)
+        {
+            std::atomic<uint32_t>& most = allowed[current_device_slot()];
+            if(most.load(std::memory_order_relaxed) < bytes)
+            {
+                B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+                most.store(bytes, std::memory_order_relaxed);
+            }
+            return B200WMMA_OK;
         }
 
         // ---- host side: argument checks -------------------------------------------------------

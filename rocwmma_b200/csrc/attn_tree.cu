@@ -606,16 +606,19 @@ namespace b200wmma
         static int launch(const Params& p, const CUtensorMap (&maps)[2], const void* q, void* o, cudaStream_t stream)
         {
             const uint32_t grid = p.batch * p.heads_kv * p.tiles * p.splits;
+            static attn::Allowed allowed;
             if constexpr(WM == 0)
             {
                 auto kern = tree_tc05_kernel<T, HD, CAP, BIAS>;
-                B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<HD>::BYTES));
+                if(int e = attn::allow_smem(reinterpret_cast<const void*>(kern), TcSmem<HD>::BYTES, allowed))
+                    return e;
                 kern<<<grid, TC_THREADS, TcSmem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q), static_cast<T*>(o));
             }
             else
             {
                 auto kern = tree_kernel<T, HD, WM, CAP, BIAS>;
-                B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::BYTES));
+                if(int e = attn::allow_smem(reinterpret_cast<const void*>(kern), Smem<HD>::BYTES, allowed))
+                    return e;
                 kern<<<grid, THREADS, Smem<HD>::BYTES, stream>>>(maps[0], maps[1], p, static_cast<const T*>(q), static_cast<T*>(o));
             }
             B200_CHECK_CUDA(cudaGetLastError());

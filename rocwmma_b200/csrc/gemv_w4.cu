@@ -463,18 +463,20 @@ namespace b200wmma
             }
         }
 
-        template <typename K, typename... More>
-        static int launch_clusters(K kern, const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem,
+        template <auto KERN, typename... More>
+        static int launch_clusters(const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem,
                                    uint32_t threads, cudaStream_t stream, More... more)
         {
-            B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            static attn::Allowed allowed;
+            if(int e = attn::allow_smem(reinterpret_cast<const void*>(KERN), smem, allowed))
+                return e;
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(blocks * parts, blocks_y), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
             cudaLaunchAttribute attr{};
             attr.id               = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
             cfg.attrs = &attr, cfg.numAttrs = parts > 1 ? 1 : 0;
-            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p, parts, more...));
+            B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, KERN, p, parts, more...));
             return B200WMMA_OK;
         }
         // Blocks of a cluster: a power of two, up to 8, to `most` (parts with work enough) and to per_sm blocks on an SM.
@@ -498,10 +500,10 @@ namespace b200wmma
                 const uint32_t parts = parts_of(blocks, ceil_div(p.n, 8 * FEW_K), 2);
                 const Few      f(8, p.n, parts);
                 if(f.bytes <= ONE_BYTES)
-                    return launch_clusters(few_kernel<T, SIGNED, 8, STEPS, true>, p, blocks, 1, parts, f.bytes, 256, stream);
+                    return launch_clusters<few_kernel<T, SIGNED, 8, STEPS, true>>(p, blocks, 1, parts, f.bytes, 256, stream);
             }
             const uint32_t parts = parts_of(blocks, ceil_div(p.n, 4 * FEW_K), 2);
-            return launch_clusters(few_kernel<T, SIGNED, 4, STEPS, false>, p, blocks, 1, parts, Few::ring_bytes(4, p.rows), 128, stream);
+            return launch_clusters<few_kernel<T, SIGNED, 4, STEPS, false>>(p, blocks, 1, parts, Few::ring_bytes(4, p.rows), 128, stream);
         }
         template <typename T, bool SIGNED, int N, int SETS>
         static int launch_tc(const Args& p, cudaStream_t stream)
@@ -516,7 +518,7 @@ namespace b200wmma
             if(int e = tc05::make_kmajor_tmap(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                                               p.x, p.rows, p.n, p.ldx, N))
                 return e;
-            return launch_clusters(tc_kernel<T, SIGNED, N, SETS>, p, blocks, blocks_y, parts, L::BYTES, TC_THREADS, stream, status, map);
+            return launch_clusters<tc_kernel<T, SIGNED, N, SETS>>(p, blocks, blocks_y, parts, L::BYTES, TC_THREADS, stream, status, map);
         }
         template <typename T, bool SIGNED, int SETS>
         static int launch_tc_rows(const Args& p, cudaStream_t stream)
