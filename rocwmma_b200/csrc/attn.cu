@@ -137,7 +137,7 @@ namespace b200wmma
             early.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
             early.val.programmaticStreamSerializationAllowed = 1;
             cudaLaunchConfig_t cfg{};
-            cfg.blockDim = dim3(BWD_THREADS), cfg.dynamicSmemBytes = BwdSmem<HD>::BYTES, cfg.stream = c.stream, cfg.attrs = &early, cfg.numAttrs = 1;
+            cfg.blockDim = dim3(BwdWarps<CAP>::THREADS), cfg.dynamicSmemBytes = BwdSmem<HD>::BYTES, cfg.stream = c.stream, cfg.attrs = &early, cfg.numAttrs = 1;
             cfg.gridDim = dim3(uint32_t(tiles_of(p.len_q)) * p.batch * p.heads_q);
             B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dq, c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[4], p, static_cast<const float*>(c.lse2),
                                                c.delta, c.docs_q, c.docs_kv, c.status));

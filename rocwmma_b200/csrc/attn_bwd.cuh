@@ -6,10 +6,10 @@
 //   dq:  a block owns 128 queries and walks the keys:  S = Q K^T, dP = dO V^T, dQ += dS K
 // The dq kernel runs first and sets delta right (see there).
 // with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
-// 256 threads compute, two to a lane (64 columns each); one warp issues the products, one the copies.
+// 256 or 512 threads compute; one warp issues the products, one the copies.
 // Bound: the products.  Each kernel has four to a pair of tiles (2048 cycles at a head of 128); S of the next step runs while dS
 // of this one is computed, dP of the next one while its P is.  Measured, bf16, gradients of 2 x 16 heads of 4096 x 128: 0.91 ms
-// (752 TFLOP/s counting five products), causal 0.53 ms; both kernels take about the same.
+// (750 TFLOP/s counting five products), causal 0.52 ms, causal with cap and 4 key heads 0.78 ms; both kernels take about the same.
 #pragma once
 #include "attn_tc05.cuh"
 
@@ -17,7 +17,15 @@ namespace b200wmma
 {
     namespace attn
     {
-        constexpr uint32_t BWD_THREADS = 320; // warps 0-7: columns 0-63 (0-3) and 64-127 (4-7); 8: TMA, 9: MMA
+        // Four warps compute a part of a tile's columns, COLS to a lane; then come the warps for TMA and MMA.  Two parts, or four under
+        // a cap, whose longer chain of instructions more warps hide: forward and backward of 2 x 8 heads of 1027 x 80 with cap and
+        // slopes 99 us (109 with two parts); without a cap four parts lose (2 x 16 heads of 4096 x 128, causal: 0.57 ms, 0.52).
+        template <bool CAP>
+        struct BwdWarps
+        {
+            static constexpr uint32_t PARTS = CAP ? 4 : 2, COLS = TILE / PARTS, CHUNKS = COLS / 32;
+            static constexpr uint32_t COMPUTE = 4 * PARTS, TMA = COMPUTE, MMA = COMPUTE + 1, THREADS = 32 * (COMPUTE + 2);
+        };
 
         template <uint32_t HD>
         struct BwdSmem
@@ -84,20 +92,28 @@ namespace b200wmma
             }
         }
 
-        // D (+)= A B over 128 tokens; the left operand's halves of 64 tokens start 64 columns apart
-        template <typename T, uint32_t HD>
-        __device__ __forceinline__ void mma_over_tokens_halves(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem, bool accumulate)
+        __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[16])
+        {
+            tmem_st_32x32b_x16(taddr, r);
+        }
+        __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[32])
+        {
+            tmem_st_32x32b_x32(taddr, r);
+        }
+        // D (+)= A B over 128 tokens; the left operand's parts of COLS tokens start COLS columns apart
+        template <typename T, uint32_t HD, uint32_t COLS>
+        __device__ __forceinline__ void mma_over_tokens_parts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_smem, bool accumulate)
         {
             constexpr uint32_t idesc = tc05::make_idesc<kind_of<T>, TILE, HD, false, true>();
             const uint64_t     b     = ptx::make_mnmajor_sw128_desc(b_smem, BOX_BYTES);
 #pragma unroll
             for(uint32_t k = 0; k < TILE / 16; ++k)
-                mma_f16_ts(d_tmem, a_tmem + (k / 4) * 64 + (k % 4) * 8, b + k * (2048u >> 4), idesc, (accumulate || k != 0) ? 1u : 0u);
+                mma_f16_ts(d_tmem, a_tmem + k * 16 / COLS * COLS + k * 16 % COLS / 2, b + k * (2048u >> 4), idesc, (accumulate || k != 0) ? 1u : 0u);
         }
 
         // ---------------------------------------------------------------------------------------------------------------
         template <typename T, uint32_t HD, bool CAP, bool BIAS>
-        __global__ void __launch_bounds__(BWD_THREADS, 1)
+        __global__ void __launch_bounds__(BwdWarps<CAP>::THREADS, 1)
             bwd_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                            const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ Params p,
@@ -105,6 +121,7 @@ namespace b200wmma
                            const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
         {
             using L = BwdSmem<HD>;
+            using W = BwdWarps<CAP>;
             extern __shared__ uint8_t smem_raw[];
             const uint32_t            base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
             uint8_t*                  smem = smem_raw + (base - ptx::smem_u32(smem_raw));
@@ -133,14 +150,14 @@ namespace b200wmma
                 }
                 ptx::mbar_init(base + L::S_FULL, 1);
                 ptx::mbar_init(base + L::DP_FULL, 1);
-                ptx::mbar_init(base + L::P_FULL, 8); // warps
-                ptx::mbar_init(base + L::DS_FULL, 8);
+                ptx::mbar_init(base + L::P_FULL, W::COMPUTE); // warps
+                ptx::mbar_init(base + L::DS_FULL, W::COMPUTE);
                 ptx::mbar_init(base + L::DONE, 1);
                 *cta_abort = 0u;
                 ptx::fence_barrier_init();
                 ptx::fence_proxy_async_smem();
             }
-            if(warp == 9)
+            if(warp == W::MMA)
             {
                 ptx::tmem_alloc(base + L::MISC, 512);
                 ptx::tmem_relinquish();
@@ -154,21 +171,21 @@ namespace b200wmma
             const uint32_t   n_stat = q_tiles * TILE; // padded rows of a head
             uint32_t         it = 0; // pairs (head, query tile) so far, in every role
             bool             ok = true;
-            const uint32_t   half = warp >> 2, quad = warp & 3u; // compute: columns [64 half, 64 half + 64) of lane 32 quad + lane
+            const uint32_t   part = warp >> 2, quad = warp & 3u; // compute: columns [COLS part, COLS part + COLS) of lane 32 quad + lane
             const uint32_t   col = c0 + quad * 32u + lane; // its key
-            const uint32_t   lane_tmem = ((quad * 32u) << 16) + half * 64u;
+            const uint32_t   lane_tmem = ((quad * 32u) << 16) + part * W::COLS;
             const int32_t    doc = (docs && col < p.len_kv) ? p.doc_kv[size_t(b) * p.len_kv + col] : 0;
 
             for(uint32_t seg = 0; seg < q_tiles; seg += SEG)
             {
                 const uint32_t entries
-                    = list_tiles<BWD_THREADS>(seg, min(SEG, q_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
+                    = list_tiles<W::THREADS>(seg, min(SEG, q_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
                           const DocTile* dq = docs ? doc_tiles_q + size_t(b) * q_tiles + tile : nullptr;
                           const uint32_t f  = tile_flags(p, tile * TILE, c0, prefix, dq, docs ? doc_tiles_kv + size_t(b) * kv_tiles + kv_tile : nullptr);
                           return f && docs && dq->neg ? f | TILE_DIRTY : f;
                       });
                 const uint32_t steps = entries * share; // all tiles of one head, then those of the next
-                if(warp == 8)
+                if(warp == W::TMA)
                 {
                     // ------------------------------ TMA producer ------------------------------
                     if(lane == 0 && ok && steps)
@@ -203,7 +220,7 @@ namespace b200wmma
                     }
                     __syncwarp();
                 }
-                else if(warp == 9)
+                else if(warp == W::MMA)
                 {
                     // ------------------------------- MMA issuer -------------------------------
                     const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
@@ -255,7 +272,7 @@ namespace b200wmma
                                 break;
                             if(elect_one())
                             {
-                                mma_over_tokens_halves<T, HD>(dv_tmem, s_tmem, base + L::RING + (2 + (it & 1u)) * L::TILE_BYTES, it != 0);
+                                mma_over_tokens_parts<T, HD, W::COLS>(dv_tmem, s_tmem, base + L::RING + (2 + (it & 1u)) * L::TILE_BYTES, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 16 + 8 * (it & 1u));
                             }
                             if(more)
@@ -268,7 +285,7 @@ namespace b200wmma
                                 break;
                             if(elect_one())
                             {
-                                mma_over_tokens_halves<T, HD>(dk_tmem, dp_tmem, base + L::RING + (it & 1u) * L::TILE_BYTES, it != 0);
+                                mma_over_tokens_parts<T, HD, W::COLS>(dk_tmem, dp_tmem, base + L::RING + (it & 1u) * L::TILE_BYTES, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 8 * (it & 1u));
                             }
                             if(more)
@@ -294,43 +311,48 @@ namespace b200wmma
                             return ok;
                         };
                         const ScoreConst sc = score_const(p, g * share + n / entries);
-                        int32_t          query_docs[2]; // on their way while the product is
+                        const uint32_t   row0 = r0 + part * W::COLS;
+                        int32_t          query_docs[W::CHUNKS]; // on their way while the product is
                         if(docs && (e >> 24 & TILE_MASK))
 #pragma unroll
-                            for(uint32_t i = 0; i < 2; ++i)
-                            {
-                                const uint32_t r = r0 + half * 64 + 32 * i + lane;
-                                query_docs[i]    = r < p.len_q ? __ldg(p.doc_q + size_t(b) * p.len_q + r) : -1;
-                            }
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                                query_docs[i] = row0 + 32 * i + lane < p.len_q ? __ldg(p.doc_q + size_t(b) * p.len_q + row0 + 32 * i + lane) : -1;
                         // the statistics came with the tiles: an acquire of the same barriers
                         ok = wait_bounded_warp(base + L::FULL + 8 * st, (it >> 1) & 1u, cta_abort, status,
                                                          DKV_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                         if(!ok || !wait(base + L::S_FULL, 0))
                             break;
-                        uint32_t v[2][32];
-                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem, v[0]);
-                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
+                        uint32_t v[W::CHUNKS][32];
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32 * i, v[i]);
                         ptx::tmem_ld_wait();
                         // v becomes P, and then P (1 - tanh^2)
-                        const float4* ls   = reinterpret_cast<const float4*>(smem + L::STAT + st * TILE * 4) + half * 16;
-                        const float   from = static_cast<float>(int32_t(r0 + half * 64) + p.off - int32_t(col));
-                        uint64_t seen = ~uint64_t(0); // bit j: this key is visible to query j of the 64
+                        const float4* ls   = reinterpret_cast<const float4*>(smem + L::STAT + st * TILE * 4) + part * (W::COLS / 4);
+                        const float   from = static_cast<float>(int32_t(row0) + p.off - int32_t(col));
+                        uint32_t seen[W::CHUNKS]; // bit j of word i: this key is visible to query 32 i + j of the part
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            seen[i] = ~0u;
                         if(e >> 24 & TILE_MASK)
                         {
-                            const int32_t first = col >= p.len_kv                           ? 64
-                                                  : (p.causal && int32_t(col) >= prefix) ? int32_t(col) - p.off - int32_t(r0 + half * 64)
+                            const int32_t first = col >= p.len_kv                           ? int32_t(W::COLS)
+                                                  : (p.causal && int32_t(col) >= prefix) ? int32_t(col) - p.off - int32_t(row0)
                                                                                          : 0;
-                            seen = first >= 64 ? 0 : first > 0 ? seen << first : seen;
+                            uint32_t same[W::CHUNKS] = {};
                             if(docs)
-                            {
-                                uint32_t same[2] = {0, 0};
                                 same_docs(query_docs, doc, same);
-                                seen = doc < 0 ? 0 : seen & (uint64_t(same[1]) << 32 | same[0]);
+#pragma unroll
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            {
+                                seen[i] = ~below(first, i);
+                                if(docs)
+                                    seen[i] = doc < 0 ? 0u : seen[i] & same[i];
                             }
                         }
                         const auto weights = [&](auto masked, auto how) {
 #pragma unroll
-                            for(int i = 0; i < 2; ++i)
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             {
                                 uint32_t w[16];
 #pragma unroll
@@ -342,14 +364,13 @@ namespace b200wmma
 #pragma unroll
                                     for(int k = 0; k < 4; k += 2)
                                     {
-                                        const int      j   = i * 32 + j4 * 4 + k;
-                                        const uint64_t dot = pair(__uint_as_float(v[i][j4 * 4 + k]), __uint_as_float(v[i][j4 * 4 + k + 1]));
+                                        const int      j   = j4 * 4 + k;
+                                        const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1]));
                                         const uint64_t sub = pair(-sv[k], -sv[k + 1]);
                                         uint64_t       slip2 = pair(1.0f, 1.0f);
                                         float          x[2], slip[2];
                                         if constexpr(CAP || BIAS)
-                                            unpair(add2(score2<CAP, BIAS, decltype(how)::value>(sc, dot, from + static_cast<float>(j), 1.0f, slip2),
-                                                        sub),
+                                            unpair(add2(score2<CAP, BIAS, decltype(how)::value>(sc, dot, from + static_cast<float>(32 * i + j), 1.0f, slip2), sub),
                                                    x[0], x[1]);
                                         else
                                             unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
@@ -358,10 +379,10 @@ namespace b200wmma
                                         for(int u = 0; u < 2; ++u)
                                         {
                                             if constexpr(decltype(masked)::value)
-                                                if(!(seen >> (j + u) & 1u))
+                                                if(!(seen[i] >> (j + u) & 1u))
                                                     x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
-                                            pr[k + u]            = ex2(x[u]);
-                                            v[i][j4 * 4 + k + u] = __float_as_uint(CAP ? pr[k + u] * slip[u] : pr[k + u]);
+                                            pr[k + u] = ex2(x[u]);
+                                            v[i][j + u]  = __float_as_uint(CAP ? pr[k + u] * slip[u] : pr[k + u]);
                                         }
                                     }
                                     w[2 * j4] = pack2<T>(pr[0], pr[1]), w[2 * j4 + 1] = pack2<T>(pr[2], pr[3]);
@@ -369,7 +390,11 @@ namespace b200wmma
                                 tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
                             }
                         };
-                        if(!tame<CAP>(sc, v[0]) || !tame<CAP>(sc, v[1]))
+                        bool small = true;
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            small = small && tame<CAP>(sc, v[i]);
+                        if(!small)
                             weights(std::true_type{}, std::false_type{});
                         else if(e >> 24 & TILE_MASK)
                             weights(std::true_type{}, std::true_type{});
@@ -383,32 +408,32 @@ namespace b200wmma
 
                         if(!wait(base + L::DP_FULL, 1))
                             break;
-                        const float4* de = reinterpret_cast<const float4*>(smem + L::STAT + (2 + st) * TILE * 4) + half * 16;
-                        uint32_t ds[32];
+                        const float4* de = reinterpret_cast<const float4*>(smem + L::STAT + (2 + st) * TILE * 4) + part * (W::COLS / 4);
+                        uint32_t ds[W::COLS / 2];
 #pragma unroll
-                        for(int i = 0; i < 2; ++i)
+                        for(uint32_t i = 0; i < W::COLS / 16; ++i)
                         {
-                            uint32_t u[32];
-                            ptx::tmem_ld_32x32b_x32(dp_tmem + lane_tmem + 32 * i, u);
+                            uint32_t u[16];
+                            ptx::tmem_ld_32x32b_x16(dp_tmem + lane_tmem + 16 * i, u);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for(int j4 = 0; j4 < 8; ++j4)
+                            for(int j4 = 0; j4 < 4; ++j4)
                             {
-                                const float4 d4    = de[i * 8 + j4];
+                                const float4 d4    = de[i * 4 + j4];
                                 const float  dl[4] = {d4.x, d4.y, d4.z, d4.w};
                                 float        x[4];
 #pragma unroll
                                 for(int k = 0; k < 4; ++k)
                                 {
-                                    const float pr = __uint_as_float(v[i][j4 * 4 + k]);
+                                    const float pr = __uint_as_float(v[i / 2][i % 2 * 16 + j4 * 4 + k]);
                                     x[k]           = pr * (__uint_as_float(u[j4 * 4 + k]) - dl[k]);
                                     if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
                                         x[k] = pr == 0.0f ? 0.0f : x[k];
                                 }
-                                ds[i * 16 + 2 * j4] = pack2<T>(x[0], x[1]), ds[i * 16 + 2 * j4 + 1] = pack2<T>(x[2], x[3]);
+                                ds[i * 8 + 2 * j4] = pack2<T>(x[0], x[1]), ds[i * 8 + 2 * j4 + 1] = pack2<T>(x[2], x[3]);
                             }
                         }
-                        tmem_st_32x32b_x32(dp_tmem + lane_tmem, ds);
+                        store_columns(dp_tmem + lane_tmem, ds);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -420,24 +445,26 @@ namespace b200wmma
                     __syncthreads();
             }
 
-            // ---- results: dv by the first four warps, dk by the next four ----
-            if(warp == 9 && ok && elect_one())
+            // ---- results: dv by the first half of the threads, dk by the other ----
+            if(warp == W::MMA && ok && elect_one())
                 ptx::tc_commit(base + L::DONE);
-            if(warp < 8)
+            if(warp < W::COMPUTE)
             {
+                constexpr uint32_t HALF = W::PARTS / 2; // parts to each
+                const uint32_t     is_dk = part / HALF;
                 if(ok)
                     ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DKV_COMPUTE << 24 | 4u << 20 | (blockIdx.x & 0xFFFFFu));
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
                     // every product is done: the tiles of K and V make room
-                    stage_row<T>(smem + L::OWN + half * L::TILE_BYTES, threadIdx.x & 127u, (half ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), 0, HD,
-                                 it == 0 ? 0.0f : half ? p.scale : 1.0f);
+                    stage_row<T>(smem + L::OWN + is_dk * L::TILE_BYTES, threadIdx.x & 127u, (is_dk ? dk_tmem : dv_tmem) + ((quad * 32u) << 16),
+                                 part % HALF * (HD / HALF), (part % HALF + 1) * (HD / HALF), it == 0 ? 0.0f : is_dk ? p.scale : 1.0f);
                     ptx::fence_proxy_async_smem();
                 }
-                ptx::named_bar_sync(1 + half, TILE); // warps that gave up come here too
-                if((threadIdx.x & 127u) == 0 && !*cta_abort)
-                    store_tile<HD>(half ? &map_dk : &map_dv, base + L::OWN + half * L::TILE_BYTES, c0, g, b);
+                ptx::named_bar_sync(1 + is_dk, HALF * TILE); // warps that gave up come here too
+                if(threadIdx.x % (HALF * TILE) == 0 && !*cta_abort)
+                    store_tile<HD>(is_dk ? &map_dk : &map_dv, base + L::OWN + is_dk * L::TILE_BYTES, c0, g, b);
             }
             ptx::tc_fence_before_sync();
             __syncthreads();
@@ -449,7 +476,7 @@ namespace b200wmma
                     __nanosleep(1000);
                 __syncthreads();
             }
-            if(warp == 9)
+            if(warp == W::MMA)
             {
                 ptx::tc_fence_after_sync();
                 ptx::tmem_dealloc(tmem, 512);
@@ -461,7 +488,7 @@ namespace b200wmma
         // query sees few keys.  sum_j P (dP - delta) is that error, so this kernel adds it up, adds up P K next to dQ, takes the
         // product off at the end and leaves the right delta for the dkv kernel.  The steps are interleaved as there.
         template <typename T, uint32_t HD, bool CAP, bool BIAS>
-        __global__ void __launch_bounds__(BWD_THREADS, 1)
+        __global__ void __launch_bounds__(BwdWarps<CAP>::THREADS, 1)
             bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                           const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ Params p, const float* __restrict__ lse2,
@@ -469,6 +496,7 @@ namespace b200wmma
                           unsigned* status)
         {
             using L = BwdSmem<HD>;
+            using W = BwdWarps<CAP>;
             extern __shared__ uint8_t smem_raw[];
             const uint32_t            base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
             uint8_t*                  smem = smem_raw + (base - ptx::smem_u32(smem_raw));
@@ -498,14 +526,14 @@ namespace b200wmma
                 }
                 ptx::mbar_init(base + L::S_FULL, 1);
                 ptx::mbar_init(base + L::DP_FULL, 1);
-                ptx::mbar_init(base + L::P_FULL, 8); // warps
-                ptx::mbar_init(base + L::DS_FULL, 8);
+                ptx::mbar_init(base + L::P_FULL, W::COMPUTE); // warps
+                ptx::mbar_init(base + L::DS_FULL, W::COMPUTE);
                 ptx::mbar_init(base + L::DONE, 1);
                 *cta_abort = 0u;
                 ptx::fence_barrier_init();
                 ptx::fence_proxy_async_smem();
             }
-            if(warp == 9)
+            if(warp == W::MMA)
             {
                 ptx::tmem_alloc(base + L::MISC, 512);
                 ptx::tmem_relinquish();
@@ -519,15 +547,15 @@ namespace b200wmma
 
             uint32_t         it = 0;
             bool             ok = true;
-            const uint32_t   half = warp >> 2, quad = warp & 3u;
-            const uint32_t   row = row0 + quad * 32u + lane, lane_tmem = ((quad * 32u) << 16) + half * 64u;
+            const uint32_t   part = warp >> 2, quad = warp & 3u;
+            const uint32_t   row = row0 + quad * 32u + lane, lane_tmem = ((quad * 32u) << 16) + part * W::COLS;
             const int32_t    at  = int32_t(row) + p.off;
             const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
             const int32_t    lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
             const ScoreConst sc  = score_const(p, h);
             const float      back = CAP ? 1.0f / sc.cap2 : 0.0f;
             float            ls = 0.0f, de = 0.0f, rest = 0.0f; // rest: sum of P (dP - delta)
-            if(warp < 8)
+            if(warp < W::COMPUTE)
             {
                 const size_t stat = (size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row;
                 ls = __ldcg(lse2 + stat), de = __ldcg(delta + stat);
@@ -536,12 +564,12 @@ namespace b200wmma
             for(uint32_t seg = 0; seg < kv_tiles; seg += SEG)
             {
                 const uint32_t entries
-                    = list_tiles<BWD_THREADS>(seg, min(SEG, kv_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
+                    = list_tiles<W::THREADS>(seg, min(SEG, kv_tiles - seg), list, smem + L::RAW, misc + 2, [&](uint32_t tile) {
                           const DocTile* dk = docs ? doc_tiles_kv + size_t(b) * kv_tiles + tile : nullptr;
                           const uint32_t f  = tile_flags(p, row0, tile * TILE, prefix, docs ? doc_tiles_q + size_t(b) * q_tiles + q_tile : nullptr, dk);
                           return f && docs && dk->neg ? f | TILE_DIRTY : f;
                       });
-                if(warp == 8)
+                if(warp == W::TMA)
                 {
                     if(lane == 0 && ok && entries)
                     {
@@ -566,7 +594,7 @@ namespace b200wmma
                     }
                     __syncwarp();
                 }
-                else if(warp == 9)
+                else if(warp == W::MMA)
                 {
                     const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t what) {
                         ok = ok
@@ -614,14 +642,14 @@ namespace b200wmma
                             if(!wait(base + L::P_FULL, it & 1u, 1))
                                 break;
                             if(elect_one())
-                                mma_over_tokens_halves<T, HD>(pk_tmem, s_tmem, k_smem, it != 0);
+                                mma_over_tokens_parts<T, HD, W::COLS>(pk_tmem, s_tmem, k_smem, it != 0);
                             if(n + 1 < entries)
                                 scores(it + 1, n + 1);
                             if(!ok || !wait(base + L::DS_FULL, it & 1u, 4))
                                 break;
                             if(elect_one())
                             {
-                                mma_over_tokens_halves<T, HD>(dq_tmem, dp_tmem, k_smem, it != 0);
+                                mma_over_tokens_parts<T, HD, W::COLS>(dq_tmem, dp_tmem, k_smem, it != 0);
                                 ptx::tc_commit(base + L::EMPTY + 8 * (it & 1u));
                             }
                             if(n + 1 < entries)
@@ -634,39 +662,42 @@ namespace b200wmma
                 {
                     for(uint32_t n = 0; ok && n < entries; ++n, ++it)
                     {
-                        const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE;
-                        int32_t        key_docs[2]; // on their way while the product is
+                        const uint32_t e = list[n], c0 = (e & 0xFFFFFFu) * TILE + part * W::COLS;
+                        int32_t        key_docs[W::CHUNKS]; // on their way while the product is
                         if(docs && (e >> 24 & TILE_MASK))
 #pragma unroll
-                            for(uint32_t i = 0; i < 2; ++i)
-                            {
-                                const uint32_t c = c0 + half * 64 + 32 * i + lane;
-                                key_docs[i]      = c < p.len_kv ? __ldg(p.doc_kv + size_t(b) * p.len_kv + c) : -1;
-                            }
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                                key_docs[i] = c0 + 32 * i + lane < p.len_kv ? __ldg(p.doc_kv + size_t(b) * p.len_kv + c0 + 32 * i + lane) : -1;
                         ok = wait_bounded_warp(base + L::S_FULL, it & 1u, cta_abort, status, DQ_COMPUTE << 24 | (blockIdx.x & 0xFFFFFFu));
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
-                        uint32_t v[2][32];
-                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem, v[0]);
-                        ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32, v[1]);
+                        uint32_t v[W::CHUNKS][32];
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            ptx::tmem_ld_32x32b_x32(s_tmem + lane_tmem + 32 * i, v[i]);
                         ptx::tmem_ld_wait();
-                        uint64_t seen = ~uint64_t(0); // bit j: key j of the 64 is visible to this query
+                        uint32_t seen[W::CHUNKS]; // bit j of word i: key 32 i + j of the part is visible to this query
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            seen[i] = ~0u;
                         if(e >> 24 & TILE_MASK)
                         {
-                            const int32_t rel = lim - int32_t(c0 + half * 64);
-                            seen              = rel <= 0 ? 0 : rel < 64 ? seen >> (64 - rel) : seen;
+                            uint32_t same[W::CHUNKS] = {};
                             if(docs)
-                            {
-                                uint32_t same[2] = {0, 0};
                                 same_docs(key_docs, doc, same);
-                                seen &= uint64_t(same[1]) << 32 | same[0];
+#pragma unroll
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            {
+                                seen[i] = below(lim - int32_t(c0), i);
+                                if(docs)
+                                    seen[i] &= same[i];
                             }
                         }
-                        const float from    = static_cast<float>(at - int32_t(c0 + half * 64));
+                        const float from    = static_cast<float>(at - int32_t(c0));
                         const auto  weights = [&](auto masked, auto how) { // v becomes P; P (1 - tanh^2) goes over the scores
 #pragma unroll
-                            for(int i = 0; i < 2; ++i)
+                            for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             {
                                 uint32_t w[16];
 #pragma unroll
@@ -687,7 +718,7 @@ namespace b200wmma
                                     for(int u = 0; u < 2; ++u)
                                     {
                                         if constexpr(decltype(masked)::value)
-                                            if(!(seen >> (32 * i + j + u) & 1u))
+                                            if(!(seen[i] >> (j + u) & 1u))
                                                 x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
                                         x[u]        = ex2(x[u]);
                                         v[i][j + u] = __float_as_uint(x[u]);
@@ -699,7 +730,11 @@ namespace b200wmma
                                 tmem_st_32x32b_x16(s_tmem + lane_tmem + 16 * i, w);
                             }
                         };
-                        if(!tame<CAP>(sc, v[0]) || !tame<CAP>(sc, v[1]))
+                        bool small = true;
+#pragma unroll
+                        for(uint32_t i = 0; i < W::CHUNKS; ++i)
+                            small = small && tame<CAP>(sc, v[i]);
+                        if(!small)
                             weights(std::true_type{}, std::false_type{});
                         else if(e >> 24 & TILE_MASK)
                             weights(std::true_type{}, std::true_type{});
@@ -715,21 +750,22 @@ namespace b200wmma
                         if(!ok)
                             break;
                         ptx::tc_fence_after_sync();
-                        uint32_t ds[32];
+                        uint32_t ds[W::COLS / 2];
 #pragma unroll
-                        for(int i = 0; i < 2; ++i)
+                        for(uint32_t i = 0; i < W::COLS / 16; ++i)
                         {
-                            uint32_t u[32];
-                            ptx::tmem_ld_32x32b_x32(dp_tmem + lane_tmem + 32 * i, u);
+                            uint32_t u[16];
+                            ptx::tmem_ld_32x32b_x16(dp_tmem + lane_tmem + 16 * i, u);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for(int j = 0; j < 16; ++j)
+                            for(int j = 0; j < 8; ++j)
                             {
                                 float x[2];
 #pragma unroll
                                 for(int k = 0; k < 2; ++k)
                                 {
-                                    const float pr = __uint_as_float(v[i][2 * j + k]);
+                                    const uint32_t c  = 16 * i + 2 * j + k;
+                                    const float    pr = __uint_as_float(v[c / 32][c % 32]);
                                     x[k]           = pr * (__uint_as_float(u[2 * j + k]) - de);
                                     if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
                                         x[k] = pr == 0.0f ? 0.0f : x[k];
@@ -739,15 +775,15 @@ namespace b200wmma
                                         // the capped score again, from its weight: registers for both would not do
                                         float y = lg2(pr) + ls;
                                         if constexpr(BIAS)
-                                            y = fmaf(sc.slope, fabsf(from - static_cast<float>(32 * i + 2 * j + k)), y);
+                                            y = fmaf(sc.slope, fabsf(from - static_cast<float>(c)), y);
                                         y *= back;
                                         x[k] = pr == 0.0f ? 0.0f : x[k] * fmaf(-y, y, 1.0f);
                                     }
                                 }
-                                ds[i * 16 + j] = pack2<T>(x[0], x[1]);
+                                ds[i * 8 + j] = pack2<T>(x[0], x[1]);
                             }
                         }
-                        tmem_st_32x32b_x32(dp_tmem + lane_tmem, ds);
+                        store_columns(dp_tmem + lane_tmem, ds);
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -759,27 +795,33 @@ namespace b200wmma
                     __syncthreads();
             }
 
-            if(warp == 9 && ok && elect_one())
+            if(warp == W::MMA && ok && elect_one())
                 ptx::tc_commit(base + L::DONE);
-            if(warp < 8)
+            if(warp < W::COMPUTE)
             {
                 if(ok)
                     ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DQ_COMPUTE << 24 | 2u << 20 | (blockIdx.x & 0xFFFFFu));
                 float* rests       = reinterpret_cast<float*>(smem + L::STAT);
                 rests[threadIdx.x] = rest;
-                ptx::named_bar_sync(1, 256); // warps that gave up come here too
+                ptx::named_bar_sync(1, W::PARTS * TILE); // warps that gave up come here too
                 if(ok)
                 {
                     ptx::tc_fence_after_sync();
-                    rest = rests[threadIdx.x & 127u] + rests[128 + (threadIdx.x & 127u)];
-                    if(half == 0 && row < p.len_q)
+                    const uint32_t i = threadIdx.x & 127u;
+                    rest = rests[i];
+#pragma unroll
+                    for(uint32_t k = 1; k < W::PARTS; ++k)
+                        rest += rests[k * TILE + i];
+                    if(part == 0 && row < p.len_q)
                         delta[(size_t(b) * p.heads_q + h) * (q_tiles * TILE) + row] = de + rest;
-                    // every product is done: the tile of Q makes room; both halves of the threads take half of the columns
-                    stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), half * (HD / 2), (half + 1) * (HD / 2),
-                                 it != 0 ? p.scale : 0.0f, pk_tmem + ((quad * 32u) << 16), it != 0 ? -rest * p.scale : 0.0f);
+                    // every product is done: the tile of Q makes room; the parts share its columns, at least 32 to each
+                    constexpr uint32_t SHARE = HD / W::PARTS < 32 ? 32 : HD / W::PARTS;
+                    if(part * SHARE < HD)
+                        stage_row<T>(smem + L::OWN, threadIdx.x & 127u, dq_tmem + ((quad * 32u) << 16), part * SHARE, (part + 1) * SHARE,
+                                     it != 0 ? p.scale : 0.0f, pk_tmem + ((quad * 32u) << 16), it != 0 ? -rest * p.scale : 0.0f);
                     ptx::fence_proxy_async_smem();
                 }
-                ptx::named_bar_sync(1, 256);
+                ptx::named_bar_sync(1, W::PARTS * TILE);
                 if(threadIdx.x == 0 && !*cta_abort)
                     store_tile<HD>(&map_dq, base + L::OWN, row0, h, b);
             }
@@ -793,7 +835,7 @@ namespace b200wmma
                     __nanosleep(1000);
                 __syncthreads();
             }
-            if(warp == 9)
+            if(warp == W::MMA)
             {
                 ptx::tc_fence_after_sync();
                 ptx::tmem_dealloc(tmem, 512);

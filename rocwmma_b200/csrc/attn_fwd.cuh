@@ -12,8 +12,8 @@
 // Bound: a pair of tiles takes 1.9 us at a head of 128, 1.55 us of which remain without any softmax: M = 128, N = 128 products
 // read shared memory at its full 128 bytes a cycle next to the copies' writes, and 2 x 2 of them are 1.1 us by the tensor cores'
 // rate.  Measured, bf16: 1 x 16 heads of 16384 x 128 1.1-1.2 PFLOP/s, 2 x 16 heads of 4096 x 128 0.28 ms (980 TFLOP/s), causal
-// 0.16 ms (870), causal with cap 0.28 ms, 5 packed documents of 8192 tokens 0.11 ms.  What was tried and not kept: announcing P
-// in halves (931 instead of 1064 TFLOP/s then), part of the exponentials as polynomials (892-938).
+// 0.15 ms (930), causal with cap 0.19-0.21 ms, 5 packed documents of 8192 tokens 0.10 ms.  What was tried and not kept: announcing
+// P in halves (931 instead of 1064 TFLOP/s then), part of the exponentials as polynomials (892-938).
 #pragma once
 #include "attn_tc05.cuh"
 
@@ -206,7 +206,8 @@ namespace b200wmma
                     const auto scores = [&](uint32_t u, uint32_t e, uint32_t n) { // S of query tile u
                         if((flags(entries, e, u) & TILE_NEED) && elect_one())
                         {
-                            mma_over_head<T, HD>(s_tmem[u], base + L::Q + (PER == 2 ? u : 0) * L::TILE_BYTES, base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
+                            mma_over_head<T, HD>(s_tmem[u], base + L::Q + (PER == 2 ? u : 0) * L::TILE_BYTES,
+                                                 base + L::KV + (n % L::STAGES) * L::TILE_BYTES);
                             ptx::tc_commit(base + L::S_FULL + 8 * u);
                         }
                     };
@@ -437,10 +438,12 @@ namespace b200wmma
                     ptx::named_bar_sync(1, 2 * TILE); // warps that gave up come here too
                     ptx::tc_fence_after_sync();
                     const float m0 = stats[tile_row], m1 = stats[TILE + tile_row];
-                    float       l0 = stats[2 * TILE + tile_row], l1 = stats[3 * TILE + tile_row];
+                    const float l0 = stats[2 * TILE + tile_row], l1 = stats[3 * TILE + tile_row];
                     m = fmaxf(m0, m1);
-                    const float by0 = l0 == 0.0f ? 0.0f : m0 == -INFINITY ? l0 : ex2(m0 - m), by1 = l1 == 0.0f ? 0.0f : m1 == -INFINITY ? l1 : ex2(m1 - m);
-                    l = by0 * l0 + by1 * l1; // l0 of NaN alone, without a maximum, stays NaN
+                    // a sum without a maximum is NaN and stays it
+                    const float by0 = l0 == 0.0f ? 0.0f : m0 == -INFINITY ? l0 : ex2(m0 - m);
+                    const float by1 = l1 == 0.0f ? 0.0f : m1 == -INFINITY ? l1 : ex2(m1 - m);
+                    l = by0 * l0 + by1 * l1;
                     if(ok)
                         stage_row<T>(smem + tile_smem, tile_row, o_tmem[0] + lane_tmem, t * (HD / 2), (t + 1) * (HD / 2),
                                      by0 != 0.0f ? by0 * inverse(l) : 0.0f, o_tmem[1] + lane_tmem, by1 != 0.0f ? by1 * inverse(l) : 0.0f);

@@ -469,8 +469,8 @@ namespace b200wmma
         }
 
         // Joins the splits of a row: W warps with up to PER splits each, whose parts are all on their way before the first maximum is
-        // known (148 splits of 8 rows: 2.6 us behind the first kernel, 6.8 with a few loads at a time); HD / 32
-        // elements to a lane; everything in a fixed order.
+        // known (148 splits of 8 rows: 2.6 us behind the first kernel, 6.8 with a few loads at a time); HD / 32 elements to a lane;
+        // everything in a fixed order.
         template <uint32_t W>
         struct Join
         {
