@@ -261,6 +261,19 @@ def test_more_tiles_than_one_list_holds(lq, lk, docs):
 
 
 @gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_keys_and_many_blocks(causal):
+    """More key tiles than one list holds, for blocks of two tiles of queries; three of the heads are compared."""
+    lq, lk, hq, d = 129, 66000, 75, 64
+    q, k, v, dout = inputs(1, lq, lk, hq, 1, d, BF16, seed=47)
+    got = run(q, k, v, dout, 0.125, causal=causal, backward=False)
+    few = [0, 37, 74]
+    ref = A.attention(q[:, :, few], k, v, 0.125, causal=causal)
+    A.assert_close(got["o"][:, :, few], ref["o"], ref["o_tol"], "o")
+    A.assert_close(got["lse"][:, few], ref["lse"], ref["lse_tol"], "lse")
+
+
+@gpu
 def test_rows_far_apart():
     """Offsets that pass 2^31 elements."""
     n, h, d, stride = 300, 2, 64, 8 << 20
