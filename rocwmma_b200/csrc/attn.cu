@@ -6,7 +6,9 @@ namespace b200wmma
 {
     namespace attn
     {
-        // Workspace: documents of the query and key tiles, then (backward) lse and delta of each row, padded to whole tiles.
+        constexpr uint32_t SLOTS = 148; // blocks that run at once, one to an SM
+        // Workspace: documents of the query and key tiles, then (backward) lse and delta of each row, padded to whole tiles, then the
+        // parts of dk and dv where the dkv kernel may be split (see dkv_splits; at most a tile of each for every block of SLOTS).
         static size_t tiles_of(uint32_t len)
         {
             return (len + TILE - 1) / TILE;
@@ -14,7 +16,20 @@ namespace b200wmma
         static size_t workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv, int backward)
         {
             const size_t docs = batch * (tiles_of(len_q) + tiles_of(len_kv)) * sizeof(DocTile);
-            return docs + (backward ? 2 * size_t(batch) * heads_q * tiles_of(len_q) * TILE * sizeof(float) : 0);
+            if(!backward)
+                return docs;
+            const size_t rows = 2 * size_t(batch) * heads_q * tiles_of(len_q) * TILE * sizeof(float);
+            const bool   split = 2 * tiles_of(len_kv) * batch <= SLOTS && tiles_of(len_q) * heads_q > 4;
+            return docs + rows + (split ? size_t(SLOTS) * 2 * TILE * MAX_DIM * sizeof(float) : 0);
+        }
+        // Blocks of the dkv kernel to a key tile: where those tiles do not fill the machine the steps (query heads x query tiles) are
+        // split, at least four to a block, and the parts are summed up by a kernel of their own: 8 query heads to one key head, 1700
+        // tokens x 128, causal, gradients 66 us (242 unsplit).
+        static uint32_t dkv_splits(uint32_t batch, uint32_t heads_q, uint32_t heads_kv, uint32_t len_q, uint32_t len_kv)
+        {
+            const uint64_t blocks = tiles_of(len_kv) * batch * heads_kv, most = (tiles_of(len_q) * (heads_q / heads_kv) + 3) / 4;
+            const uint64_t n = SLOTS / blocks < most ? SLOTS / blocks : most;
+            return n > 1 ? uint32_t(n) : 1u;
         }
         static int list_documents(const Params& p, void* workspace, const DocTile** q, const DocTile** kv, cudaStream_t stream)
         {
@@ -92,7 +107,7 @@ namespace b200wmma
         static int launch_fwd(const Params& p, const CUtensorMap (&maps)[4], float* lse, const DocTile* dq, const DocTile* dk,
                               unsigned* status, cudaStream_t stream)
         {
-            return tiles_of(p.len_q) * p.batch * p.heads_q <= 148 ? launch_fwd_as<T, HD, CAP, BIAS, PLAIN, 1>(p, maps, lse, dq, dk, status, stream)
+            return tiles_of(p.len_q) * p.batch * p.heads_q <= SLOTS ? launch_fwd_as<T, HD, CAP, BIAS, PLAIN, 1>(p, maps, lse, dq, dk, status, stream)
                                                                   : launch_fwd_as<T, HD, CAP, BIAS, PLAIN, 2>(p, maps, lse, dq, dk, status, stream);
         }
         template <typename T, uint32_t HD>
@@ -114,7 +129,8 @@ namespace b200wmma
             CUtensorMap    maps[7]; // q, k, v, dout, dq, dk, dv
             const void *   o, *dout;
             const float*   lse;
-            float *        lse2, *delta;
+            float *        lse2, *delta, *partial;
+            void *         dk, *dv;
             const DocTile *docs_q, *docs_kv;
             unsigned*      status;
             cudaStream_t   stream;
@@ -141,9 +157,17 @@ namespace b200wmma
             cfg.gridDim = dim3(uint32_t(tiles_of(p.len_q)) * p.batch * p.heads_q);
             B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dq, c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[4], p, static_cast<const float*>(c.lse2),
                                                c.delta, c.docs_q, c.docs_kv, c.status));
-            cfg.gridDim = dim3(uint32_t(tiles_of(p.len_kv)) * p.batch * p.heads_kv);
+            const uint32_t blocks = uint32_t(tiles_of(p.len_kv)) * p.batch * p.heads_kv;
+            const uint32_t splits = dkv_splits(p.batch, p.heads_q, p.heads_kv, p.len_q, p.len_kv);
+            cfg.gridDim = dim3(blocks * splits);
             B200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dkv, c.maps[0], c.maps[1], c.maps[2], c.maps[3], c.maps[5], c.maps[6], p,
-                                               static_cast<const float*>(c.lse2), static_cast<const float*>(c.delta), c.docs_q, c.docs_kv, c.status));
+                                               static_cast<const float*>(c.lse2), static_cast<const float*>(c.delta), c.docs_q, c.docs_kv, splits, c.partial, c.status));
+            if(splits > 1)
+            {
+                bwd_join_kernel<T, HD><<<blocks * 2 * (TILE * HD / 1024), 256, 0, c.stream>>>(p, c.partial, splits, blocks, static_cast<T*>(c.dk),
+                                                                                           static_cast<T*>(c.dv));
+                B200_CHECK_CUDA(cudaGetLastError());
+            }
             return B200WMMA_OK;
         }
         template <typename T, uint32_t HD>
@@ -250,7 +274,8 @@ extern "C" int b200wmma_attn_bwd(const b200wmma_attn_args* args, const void* q, 
     const size_t doc_tiles = p.batch * (attn::tiles_of(p.len_q) + attn::tiles_of(p.len_kv));
     c.lse2  = reinterpret_cast<float*>(static_cast<attn::DocTile*>(workspace) + doc_tiles);
     c.delta = c.lse2 + size_t(p.batch) * p.heads_q * attn::tiles_of(p.len_q) * attn::TILE;
-    c.o = o, c.dout = dout, c.lse = lse, c.stream = as_stream(stream);
+    c.partial = c.delta + size_t(p.batch) * p.heads_q * attn::tiles_of(p.len_q) * attn::TILE;
+    c.o = o, c.dout = dout, c.lse = lse, c.dk = dk, c.dv = dv, c.stream = as_stream(stream);
     if(int e = attn::list_documents(p, workspace, &c.docs_q, &c.docs_kv, c.stream))
         return e;
     if(args->data_type == B200WMMA_OUT_F16)

@@ -118,7 +118,7 @@ namespace b200wmma
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                            const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ Params p,
                            const float* __restrict__ lse2, const float* __restrict__ delta, const DocTile* __restrict__ doc_tiles_q,
-                           const DocTile* __restrict__ doc_tiles_kv, unsigned* status)
+                           const DocTile* __restrict__ doc_tiles_kv, uint32_t splits, float* __restrict__ partial, unsigned* status)
         {
             using L = BwdSmem<HD>;
             using W = BwdWarps<CAP>;
@@ -130,7 +130,8 @@ namespace b200wmma
             volatile uint32_t*        cta_abort = misc + 1;
 
             const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-            const uint32_t bg = blockIdx.x % (p.batch * p.heads_kv), kv_tile = blockIdx.x / (p.batch * p.heads_kv);
+            const uint32_t split = blockIdx.x % splits, block = blockIdx.x / splits;
+            const uint32_t bg = block % (p.batch * p.heads_kv), kv_tile = block / (p.batch * p.heads_kv);
             const uint32_t g = bg % p.heads_kv, b = bg / p.heads_kv, share = p.heads_q / p.heads_kv;
             const uint32_t c0 = kv_tile * TILE, q_tiles = (p.len_q + TILE - 1) / TILE, kv_tiles = (p.len_kv + TILE - 1) / TILE;
             const int32_t  prefix = p.prefix ? p.prefix[b] : 0;
@@ -184,11 +185,13 @@ namespace b200wmma
                           const uint32_t f  = tile_flags(p, tile * TILE, c0, prefix, dq, docs ? doc_tiles_kv + size_t(b) * kv_tiles + kv_tile : nullptr);
                           return f && docs && dq->neg ? f | TILE_DIRTY : f;
                       });
-                const uint32_t steps = entries * share; // all tiles of one head, then those of the next
+                // all tiles of one head, then those of the next; this block takes steps n0 .. n1 - 1 of them
+                const uint64_t steps = uint64_t(entries) * share;
+                const uint32_t n0 = uint32_t(steps * split / splits), n1 = uint32_t(steps * (split + 1) / splits);
                 if(warp == W::TMA)
                 {
                     // ------------------------------ TMA producer ------------------------------
-                    if(lane == 0 && ok && steps)
+                    if(lane == 0 && ok && n0 < n1)
                     {
                         if(it == 0)
                         {
@@ -196,7 +199,7 @@ namespace b200wmma
                             load_tile<HD>(base + L::OWN, &map_k, c0, g, b, base + L::OWN_FULL);
                             load_tile<HD>(base + L::OWN + L::TILE_BYTES, &map_v, c0, g, b, base + L::OWN_FULL);
                         }
-                        for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                        for(uint32_t n = n0; ok && n < n1; ++n, ++it)
                         {
                             const uint32_t h = g * share + n / entries, r0 = (list[n % entries] & 0xFFFFFFu) * TILE;
                             const uint32_t st = it & 1u, ph = (it >> 1) & 1u;
@@ -257,17 +260,17 @@ namespace b200wmma
                             ptx::tc_commit(base + L::DP_FULL);
                         }
                     };
-                    if(steps && ok)
+                    if(n0 < n1 && ok)
                     {
                         if(it == 0)
                             wait(base + L::OWN_FULL, 0, 2);
-                        if(ok && arrive(0, it, 0))
+                        if(ok && arrive(0, it, n0))
                             scores(it);
-                        if(ok && arrive(1, it, 0))
+                        if(ok && arrive(1, it, n0))
                             grads(it);
-                        for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                        for(uint32_t n = n0; ok && n < n1; ++n, ++it)
                         {
-                            const bool more = n + 1 < steps;
+                            const bool more = n + 1 < n1;
                             if(!wait(base + L::P_FULL, it & 1u, 3))
                                 break;
                             if(elect_one())
@@ -301,7 +304,7 @@ namespace b200wmma
                 else
                 {
                     // --------------------------------- compute --------------------------------
-                    for(uint32_t n = 0; ok && n < steps; ++n, ++it)
+                    for(uint32_t n = n0; ok && n < n1; ++n, ++it)
                     {
                         const uint32_t e = list[n % entries], r0 = (e & 0xFFFFFFu) * TILE, st = it & 1u;
                         const auto     wait = [&](uint32_t bar, uint32_t what) {
@@ -454,16 +457,31 @@ namespace b200wmma
                 const uint32_t     is_dk = part / HALF;
                 if(ok)
                     ok = wait_bounded_warp(base + L::DONE, 0, cta_abort, status, DKV_COMPUTE << 24 | 4u << 20 | (blockIdx.x & 0xFFFFFu));
-                if(ok)
+                const uint32_t acc = (is_dk ? dk_tmem : dv_tmem) + ((quad * 32u) << 16), from = part % HALF * (HD / HALF), to = from + HD / HALF;
+                ptx::tc_fence_after_sync();
+                if(ok && splits > 1)
                 {
-                    ptx::tc_fence_after_sync();
+                    float* out = partial + ((size_t(split * 2 + is_dk) * (gridDim.x / splits) + block) * TILE + (threadIdx.x & 127u)) * HD;
+#pragma unroll 1
+                    for(uint32_t c = from; c < to; c += 32)
+                    {
+                        uint32_t w[32];
+                        ptx::tmem_ld_32x32b_x32(acc + c, w);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for(int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(out + c + 4 * i)
+                                = it != 0 ? make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]) : make_uint4(0, 0, 0, 0);
+                    }
+                }
+                else if(ok)
+                {
                     // every product is done: the tiles of K and V make room
-                    stage_row<T>(smem + L::OWN + is_dk * L::TILE_BYTES, threadIdx.x & 127u, (is_dk ? dk_tmem : dv_tmem) + ((quad * 32u) << 16),
-                                 part % HALF * (HD / HALF), (part % HALF + 1) * (HD / HALF), it == 0 ? 0.0f : is_dk ? p.scale : 1.0f);
+                    stage_row<T>(smem + L::OWN + is_dk * L::TILE_BYTES, threadIdx.x & 127u, acc, from, to, it == 0 ? 0.0f : is_dk ? p.scale : 1.0f);
                     ptx::fence_proxy_async_smem();
                 }
                 ptx::named_bar_sync(1 + is_dk, HALF * TILE); // warps that gave up come here too
-                if(threadIdx.x % (HALF * TILE) == 0 && !*cta_abort)
+                if(threadIdx.x % (HALF * TILE) == 0 && splits == 1 && !*cta_abort)
                     store_tile<HD>(is_dk ? &map_dk : &map_dv, base + L::OWN + is_dk * L::TILE_BYTES, c0, g, b);
             }
             ptx::tc_fence_before_sync();
@@ -481,6 +499,30 @@ namespace b200wmma
                 ptx::tc_fence_after_sync();
                 ptx::tmem_dealloc(tmem, 512);
             }
+        }
+
+        // Sums the partial dk and dv of a tile's splits, in order: four elements to a thread.
+        template <typename T, uint32_t HD>
+        __global__ void __launch_bounds__(256)
+            bwd_join_kernel(const __grid_constant__ Params p, const float* __restrict__ partial, uint32_t splits, uint32_t blocks, T* __restrict__ dk,
+                            T* __restrict__ dv)
+        {
+            const size_t   at = (size_t(blockIdx.x) * 256 + threadIdx.x) * 4, tile = size_t(TILE) * HD;
+            const uint32_t d = at % HD, row = at / HD % TILE, block = uint32_t(at / tile % blocks), is_dk = uint32_t(at / tile / blocks);
+            const uint32_t bg = block % (p.batch * p.heads_kv), token = block / (p.batch * p.heads_kv) * TILE + row;
+            if(is_dk > 1 || token >= p.len_kv || d >= p.dim)
+                return;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for(uint32_t s = 0; s < splits; ++s)
+            {
+                const float4 x = *reinterpret_cast<const float4*>(partial + at + size_t(s) * 2 * blocks * tile);
+                y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+            }
+            const float    by = is_dk ? p.scale : 1.0f;
+            const Strides& st = is_dk ? p.dk : p.dv;
+            T* out = (is_dk ? dk : dv) + int64_t(bg / p.heads_kv) * st.batch + int64_t(token) * st.token + int64_t(bg % p.heads_kv) * st.head + d;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(y.x * by, y.y * by), pack2<T>(y.z * by, y.w * by));
         }
 
         // ---------------------------------------------------------------------------------------------------------------

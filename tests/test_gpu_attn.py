@@ -261,6 +261,20 @@ def test_more_tiles_than_one_list_holds(lq, lk, docs):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d", [(1, 1500, 900, 8, 1, 128), (2, 700, 700, 12, 2, 72), (1, 40, 130, 16, 1, 64), (1, 5000, 100, 1, 1, 128)])
+def test_few_key_heads(b, lq, lk, hq, hk, d, dtype):
+    """Few blocks for dk and dv, whose steps are split; bits do not depend on the call."""
+    q, k, v, dout = inputs(b, lq, lk, hq, hk, d, dtype, seed=53)
+    got = check(q, k, v, dout, 1 / math.sqrt(d), causal=True)
+    again = run(q, k, v, dout, 1 / math.sqrt(d), causal=True)
+    for name in got:
+        assert torch.equal(got[name], again[name]), name
+    docs = lambda n: torch.stack([documents(("sorted", "mixed")[i], n, 3) for i in range(b)])
+    check(q, k, v, dout, 1 / math.sqrt(d), cap=9.0, slopes=slopes_of(hq), doc_q=docs(lq), doc_kv=docs(lk))
+
+
+@gpu
 @pytest.mark.parametrize("causal", [False, True])
 def test_long_keys_and_many_blocks(causal):
     """More key tiles than one list holds, for blocks of two tiles of queries; three of the heads are compared."""
