@@ -397,12 +397,10 @@ namespace b200wmma
 #pragma unroll
                         for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             small = small && tame<CAP>(sc, v[i]);
-                        if(!small)
-                            weights(std::true_type{}, std::false_type{});
-                        else if(e >> 24 & TILE_MASK)
-                            weights(std::true_type{}, std::true_type{});
+                        if(small && !(e >> 24 & TILE_MASK))
+                            weights(std::false_type{}, Bent<TAME>{});
                         else
-                            weights(std::false_type{}, std::true_type{});
+                            bend<CAP>(sc, small, [&](auto how) { weights(std::true_type{}, how); });
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -776,12 +774,10 @@ namespace b200wmma
 #pragma unroll
                         for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             small = small && tame<CAP>(sc, v[i]);
-                        if(!small)
-                            weights(std::true_type{}, std::false_type{});
-                        else if(e >> 24 & TILE_MASK)
-                            weights(std::true_type{}, std::true_type{});
+                        if(small && !(e >> 24 & TILE_MASK))
+                            weights(std::false_type{}, Bent<TAME>{});
                         else
-                            weights(std::false_type{}, std::true_type{});
+                            bend<CAP>(sc, small, [&](auto how) { weights(std::true_type{}, how); });
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();

@@ -296,13 +296,9 @@ namespace b200wmma
                         const auto transform = [&](int at_col, auto& x) {
                             if constexpr(!PLAIN)
                             {
-                                if(tame<CAP>(sc, x))
-                                    transform_as(std::true_type{}, at_col, x);
-                                else
-                                {
-                                    transform_as(std::false_type{}, at_col, x);
-                                    wild = true;
-                                }
+                                const bool small = tame<CAP>(sc, x);
+                                wild |= !small;
+                                bend<CAP>(sc, small, [&](auto how) { transform_as(how, at_col, x); });
                             }
                         };
                         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
@@ -339,7 +335,7 @@ namespace b200wmma
                                 if constexpr(CAP)
                                     most = magnitude(x, most);
                                 if constexpr(!PLAIN)
-                                    transform_as(std::true_type{}, at_col, x);
+                                    transform_as(Bent<TAME>{}, at_col, x);
                             };
                             const float more = f & TILE_MASK ? weights_at<T>(s_row, c, sub, w, top,
                                                                              [&](int at_col, auto& x) {

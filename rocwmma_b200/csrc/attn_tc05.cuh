@@ -510,26 +510,6 @@ namespace b200wmma
             s.slope = p.slopes ? p.slopes[head] * LOG2E : 0.0f;
             return s;
         }
-        // tanh from one exponential: 1 - 2 / (1 + 2^(k1 dot)) is off by a few ulp of 1, absolutely, which is what a score
-        // needs (the hardware's tanh approximation is off by 2^-11 of its value: a capped score of 20 would move by 0.01).
-        // An infinite or zero power gives 1 and -1, NaN stays NaN.
-        template <bool CAP, bool BIAS>
-        __device__ __forceinline__ float score(const ScoreConst& s, float dot, float dist, float& slip)
-        {
-            float x;
-            if constexpr(CAP)
-            {
-                const float tanh = fmaf(-2.0f, rcp(1.0f + ex2(dot * s.k1)), 1.0f);
-                slip             = fmaf(-tanh, tanh, 1.0f); // the cap's derivative
-                x                = s.cap2 * tanh;
-            }
-            else
-                x = dot * s.c;
-            if constexpr(BIAS)
-                x = fmaf(-s.slope, fabsf(dist), x);
-            return x;
-        }
-
         // Largest magnitude of N numbers and `t`.
         template <int N>
         __device__ __forceinline__ float magnitude(const uint32_t (&v)[N], float t)
@@ -545,39 +525,91 @@ namespace b200wmma
         }
         // True where the cap bends the scores of a warp only a little: |k2 dot| <= 1/2, as mostly (NaN counts as small).
         constexpr float TAME_LIMIT = 0.5f;
-        template <bool CAP, int N>
-        __device__ __forceinline__ bool tame(const ScoreConst& s, const uint32_t (&dot)[N])
+        template <bool CAP>
+        __device__ __forceinline__ bool tame(const ScoreConst& s, float largest)
         {
             if constexpr(CAP)
-                return __all_sync(0xFFFFFFFFu, magnitude(dot, 0.0f) * fabsf(s.k2) <= TAME_LIMIT);
+                return __all_sync(0xFFFFFFFFu, largest * fabsf(s.k2) <= TAME_LIMIT);
             else
                 return true;
         }
-        // The same for two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.
-        // TAME: tanh x / x as a polynomial in x^2, fitted to the smallest largest error over |x| <= 1/2: 1.5e-8 of its value, 4e-8 as
-        // evaluated in fp32, which is closer than the exponential's form.  Three of them and of the softmax's exponentials share a
-        // unit that takes 16 numbers a cycle: 2 x 16 heads of 4096 x 128, causal, 187 us with the polynomial, 254 us without.
-        template <bool CAP, bool BIAS, bool TAME>
-        __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
+        template <bool CAP, int N>
+        __device__ __forceinline__ bool tame(const ScoreConst& s, const uint32_t (&dot)[N])
         {
-            uint64_t x;
-            if constexpr(CAP && TAME)
+            return tame<CAP>(s, CAP ? magnitude(dot, 0.0f) : 0.0f);
+        }
+        // How scores of a warp are bent: all of them a little, or not; the latter under any cap, or under one of at most MODEST_CAP.
+        enum Bend : int
+        {
+            TAME,
+            MODEST,
+            ANY
+        };
+        template <Bend B>
+        using Bent = std::integral_constant<Bend, B>;
+        // tanh x of two x = k2 dot.
+        // TAME (|x| <= 1/2): tanh x / x as a polynomial in x^2, fitted to the smallest largest error: 1.5e-8 of its value, 4e-8 as
+        // evaluated in fp32.
+        // MODEST: 1 - 2 / (1 + 2^(k1 dot)), off by some ulp of 1: a score by up to 1.3e-7 of the cap, 8e-6 at the largest that this is
+        // for, which is nothing next to the rounding of its weight to 16 bits (the hardware's tanh approximation is off by 2^-11 of its
+        // value: a capped score of 20 would move by 0.01).  An infinite or zero power gives 1 and -1.  Its three numbers of a score and
+        // the softmax's exponential share a unit that takes 16 numbers a cycle: 2 x 16 heads of 4096 x 128, causal, 187 us with the
+        // polynomial, 254 us with this.
+        // ANY: each by its own size, off by a few ulp of itself, as the cap may be much larger than a score (scores around a cap of 2,
+        // 2 x 16 heads of 4096 x 128, causal: 346 us, MODEST 301).
+        // NaN stays NaN.
+        constexpr float MODEST_CAP = 64.0f;
+        template <Bend HOW>
+        __device__ __forceinline__ uint64_t tanh2(const ScoreConst& s, uint64_t dot)
+        {
+            uint64_t u = 0, near = 0, far = 0;
+            if constexpr(HOW != MODEST)
             {
-                const uint64_t u = mul2(dot, pair(s.k2, s.k2)), y = mul2(u, u);
+                u = mul2(dot, pair(s.k2, s.k2));
+                const uint64_t y = mul2(u, u);
                 uint64_t       q = fma2(y, pair(0.0172414854f, 0.0172414854f), pair(-0.0530454926f, -0.0530454926f));
-                q = fma2(q, y, pair(0.13325879f, 0.13325879f));
-                q = fma2(q, y, pair(-0.333331436f, -0.333331436f));
-                q = fma2(q, y, pair(1.0f, 1.0f));
-                const uint64_t tanh = mul2(u, q);
-                slip = fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
-                x    = mul2(tanh, pair(s.cap2, s.cap2));
+                q    = fma2(q, y, pair(0.13325879f, 0.13325879f));
+                q    = fma2(q, y, pair(-0.333331436f, -0.333331436f));
+                q    = fma2(q, y, pair(1.0f, 1.0f));
+                near = mul2(u, q);
             }
-            else if constexpr(CAP)
+            if constexpr(HOW != TAME)
             {
                 float a, b;
                 unpair(mul2(dot, pair(s.k1, s.k1)), a, b);
                 unpair(add2(pair(ex2(a), ex2(b)), pair(1.0f, 1.0f)), a, b);
-                const uint64_t tanh = fma2(pair(rcp(a), rcp(b)), pair(-2.0f, -2.0f), pair(1.0f, 1.0f));
+                far = fma2(pair(rcp(a), rcp(b)), pair(-2.0f, -2.0f), pair(1.0f, 1.0f));
+            }
+            if constexpr(HOW == ANY)
+            {
+                float x[2], t[2], f[2];
+                unpair(u, x[0], x[1]);
+                unpair(near, t[0], t[1]);
+                unpair(far, f[0], f[1]);
+                return pair(fabsf(x[0]) > TAME_LIMIT ? f[0] : t[0], fabsf(x[1]) > TAME_LIMIT ? f[1] : t[1]);
+            }
+            else
+                return HOW == TAME ? near : far;
+        }
+        // Calls f with the Bend of a warp's scores.
+        template <bool CAP, typename F>
+        __device__ __forceinline__ void bend(const ScoreConst& s, bool all_tame, F f)
+        {
+            if(!CAP || all_tame)
+                f(Bent<TAME>{});
+            else if(__builtin_expect(s.cap2 > MODEST_CAP * LOG2E, false))
+                f(Bent<ANY>{});
+            else
+                f(Bent<MODEST>{});
+        }
+        // Two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.
+        template <bool CAP, bool BIAS, Bend HOW>
+        __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
+        {
+            uint64_t x;
+            if constexpr(CAP)
+            {
+                const uint64_t tanh = tanh2<HOW>(s, dot);
                 slip = fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
                 x    = mul2(tanh, pair(s.cap2, s.cap2));
             }

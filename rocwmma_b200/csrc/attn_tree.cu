@@ -172,7 +172,7 @@ namespace b200wmma
                 at[i] = BIAS && live[i] ? (p.depths ? __ldg(p.depths + size_t(b) * p.drafts + draft[i]) : int32_t(draft[i])) : 0;
             }
             attn::ScoreConst sc;
-            sc.c = p.scale * LOG2E, sc.k1 = CAP ? 2.0f * LOG2E * (p.scale / p.cap) : 0.0f, sc.cap2 = p.cap * LOG2E, sc.slope = 0.0f;
+            sc.c = p.scale * LOG2E, sc.k2 = CAP ? p.scale / p.cap : 0.0f, sc.k1 = 2.0f * LOG2E * sc.k2, sc.cap2 = p.cap * LOG2E, sc.slope = 0.0f;
 
             uint32_t qf[HD / 16][4];
 #pragma unroll
@@ -291,7 +291,7 @@ namespace b200wmma
                 const bool     masked = (v0 & v1) != 0xFFFFFFFFu || (from + i + 1) * KEYS > len;
                 const int32_t  rel0   = int32_t(int64_t(j0) - len); // place of the warp's first token behind the cached ones
                 float          top[2] = {-INFINITY, -INFINITY};
-                const auto     scores = [&](auto mask) {
+                const auto     scores = [&](auto mask, auto how) {
                     constexpr bool MASK = decltype(mask)::value;
                     uint32_t       see[2][(MINE + 31) / 32]; // of this lane's first token on
                     if constexpr(MASK)
@@ -307,34 +307,57 @@ namespace b200wmma
 #pragma unroll
                     for(uint32_t n = 0; n < MINE / 8; ++n)
 #pragma unroll
-                        for(int e = 0; e < 4; ++e)
+                        for(int h = 0; h < 2; ++h)
                         {
-                            const uint32_t off = n * 8 + (e & 1); // and t * 2
-                            const int      h   = e >> 1;
-                            float          dist = 0.0f, unused;
+                            const uint32_t off  = n * 8; // and t * 2: the first of two tokens
+                            float          dist = 0.0f, step = -1.0f, y[2];
                             if constexpr(BIAS)
                             {
                                 dist = static_cast<float>(at[h] - rel0 - int32_t(t * 2)) - static_cast<float>(off);
                                 if constexpr(MASK)
                                 {
                                     const int32_t rel = rel0 + int32_t(off + t * 2);
-                                    if(rel >= 0 && p.depths && j0 + off + t * 2 < end)
-                                        dist = static_cast<float>(at[h] - __ldg(p.depths + size_t(b) * p.drafts + rel));
+                                    if(rel + 1 >= 0 && p.depths) // drafted tokens stand at their depths
+                                    {
+                                        const auto d = [&](uint32_t e) {
+                                            const int32_t to = rel + int32_t(e);
+                                            return static_cast<float>(
+                                                at[h] - (to >= 0 && j0 + off + t * 2 + e < end ? __ldg(p.depths + size_t(b) * p.drafts + to) : to));
+                                        };
+                                        dist = d(0);
+                                        step = d(1) - dist;
+                                    }
                                 }
                             }
                             sc.slope = slope[h];
-                            float y  = attn::score<CAP, BIAS>(sc, s[n][e], dist, unused);
-                            if constexpr(MASK)
-                                if(!(see[h][off / 32] >> (off & 31u) & 1u))
-                                    y = -INFINITY;
-                            s[n][e] = y;
-                            top[h]  = fmaxf(top[h], y);
+                            uint64_t unused;
+                            attn::unpair(attn::score2<CAP, BIAS, decltype(how)::value>(sc, attn::pair(s[n][2 * h], s[n][2 * h + 1]), dist, step, unused),
+                                         y[0], y[1]);
+#pragma unroll
+                            for(int e = 0; e < 2; ++e)
+                            {
+                                if constexpr(MASK)
+                                    if(!(see[h][off / 32] >> ((off & 31u) + e) & 1u))
+                                        y[e] = -INFINITY;
+                                s[n][2 * h + e] = y[e];
+                                top[h]          = fmaxf(top[h], y[e]);
+                            }
                         }
                 };
+                float largest = 0.0f;
+                if constexpr(CAP)
+#pragma unroll
+                    for(uint32_t n = 0; n < MINE / 8; ++n)
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                            largest = fmaxf(largest, fabsf(s[n][e]));
+                const auto masked_scores = [&](auto mask) {
+                    attn::bend<CAP>(sc, attn::tame<CAP>(sc, largest), [&](auto how) { scores(mask, how); });
+                };
                 if(masked)
-                    scores(std::true_type{});
+                    masked_scores(std::true_type{});
                 else
-                    scores(std::false_type{});
+                    masked_scores(std::false_type{});
 #pragma unroll
                 for(int h = 0; h < 2; ++h)
                 {

@@ -331,10 +331,7 @@ namespace b200wmma
                                     }
                                 }
                             };
-                            if(attn::tame<CAP>(sc, v))
-                                change(std::true_type{});
-                            else
-                                change(std::false_type{});
+                            attn::bend<CAP>(sc, attn::tame<CAP>(sc, v), change);
                         });
                     };
                     const float top = masked ? scores(std::true_type{}) : scores(std::false_type{});
