@@ -593,7 +593,6 @@ namespace b200wmma
             const int32_t    doc = (docs && row < p.len_q) ? p.doc_q[size_t(b) * p.len_q + row] : 0;
             const int32_t    lim = (row >= p.len_q || doc < 0) ? 0 : (p.causal ? min(max(at + 1, prefix), int32_t(p.len_kv)) : int32_t(p.len_kv));
             const ScoreConst sc  = score_const(p, h);
-            const float      back = CAP ? 1.0f / sc.cap2 : 0.0f;
             float            ls = 0.0f, de = 0.0f, rest = 0.0f; // rest: sum of P (dP - delta)
             if(warp < W::COMPUTE)
             {
@@ -735,7 +734,11 @@ namespace b200wmma
                             }
                         }
                         const float from    = static_cast<float>(at - int32_t(c0));
-                        const auto  weights = [&](auto masked, auto how) { // v becomes P; P (1 - tanh^2) goes over the scores
+                        // v becomes P, or under a cap the tanh, from which P and the cap's derivative come again below (registers for both
+                        // would not do, and from a weight a tanh comes back only as well as the cap is large); P (1 - tanh^2) goes over
+                        // the scores.  -infinity stands for pairs that are not visible.
+                        const uint64_t sub = pair(-ls, -ls);
+                        const auto     weights = [&](auto masked, auto how) {
 #pragma unroll
                             for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             {
@@ -743,25 +746,28 @@ namespace b200wmma
 #pragma unroll
                                 for(int j = 0; j < 32; j += 2)
                                 {
-                                    const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1])), sub = pair(-ls, -ls);
-                                    uint64_t       slip2 = pair(1.0f, 1.0f);
-                                    float          x[2], slip[2];
-                                    if constexpr(CAP || BIAS)
-                                        unpair(add2(score2<CAP, BIAS, decltype(how)::value>(sc, dot, from - static_cast<float>(32 * i + j), -1.0f,
-                                                                                            slip2),
-                                                    sub),
-                                               x[0], x[1]);
+                                    const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1]));
+                                    [[maybe_unused]] const float dist = from - static_cast<float>(32 * i + j);
+                                    float                        x[2], tanh[2], slip[2] = {1.0f, 1.0f};
+                                    if constexpr(CAP)
+                                    {
+                                        const uint64_t t = tanh2<decltype(how)::value>(sc, dot);
+                                        unpair(t, tanh[0], tanh[1]);
+                                        unpair(slip_of(t), slip[0], slip[1]);
+                                        unpair(add2(capped<BIAS>(sc, t, dist, -1.0f), sub), x[0], x[1]);
+                                    }
+                                    else if constexpr(BIAS)
+                                        unpair(add2(biased<BIAS>(sc, mul2(dot, pair(sc.c, sc.c)), dist, -1.0f), sub), x[0], x[1]);
                                     else
                                         unpair(fma2(dot, pair(sc.c, sc.c), sub), x[0], x[1]);
-                                    unpair(slip2, slip[0], slip[1]);
 #pragma unroll
                                     for(int u = 0; u < 2; ++u)
                                     {
                                         if constexpr(decltype(masked)::value)
                                             if(!(seen[i] >> (j + u) & 1u))
-                                                x[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
+                                                x[u] = tanh[u] = -INFINITY, slip[u] = 0.0f; // the product may be NaN
                                         x[u]        = ex2(x[u]);
-                                        v[i][j + u] = __float_as_uint(x[u]);
+                                        v[i][j + u] = __float_as_uint(CAP ? tanh[u] : x[u]);
                                         if(CAP)
                                             x[u] *= slip[u];
                                     }
@@ -798,25 +804,24 @@ namespace b200wmma
 #pragma unroll
                             for(int j = 0; j < 8; ++j)
                             {
-                                float x[2];
+                                const uint32_t c = 16 * i + 2 * j;
+                                float          x[2], pr[2] = {__uint_as_float(v[c / 32][c % 32]), __uint_as_float(v[c / 32][c % 32 + 1])}, slip[2];
+                                if constexpr(CAP)
+                                {
+                                    const uint64_t t = pair(pr[0], pr[1]);
+                                    unpair(slip_of(t), slip[0], slip[1]);
+                                    unpair(add2(capped<BIAS>(sc, t, from - static_cast<float>(c), -1.0f), sub), pr[0], pr[1]);
+                                    pr[0] = ex2(pr[0]), pr[1] = ex2(pr[1]);
+                                }
 #pragma unroll
                                 for(int k = 0; k < 2; ++k)
                                 {
-                                    const uint32_t c  = 16 * i + 2 * j + k;
-                                    const float    pr = __uint_as_float(v[c / 32][c % 32]);
-                                    x[k]           = pr * (__uint_as_float(u[2 * j + k]) - de);
+                                    x[k] = pr[k] * (__uint_as_float(u[2 * j + k]) - de);
                                     if(e >> 24 & TILE_MASK) // a row of padding may have made the product NaN
-                                        x[k] = pr == 0.0f ? 0.0f : x[k];
+                                        x[k] = pr[k] == 0.0f ? 0.0f : x[k];
                                     rest += x[k];
                                     if constexpr(CAP)
-                                    {
-                                        // the capped score again, from its weight: registers for both would not do
-                                        float y = lg2(pr) + ls;
-                                        if constexpr(BIAS)
-                                            y = fmaf(sc.slope, fabsf(from - static_cast<float>(c)), y);
-                                        y *= back;
-                                        x[k] = pr == 0.0f ? 0.0f : x[k] * fmaf(-y, y, 1.0f);
-                                    }
+                                        x[k] = pr[k] == 0.0f ? 0.0f : x[k] * slip[k];
                                 }
                                 ds[i * 8 + j] = pack2<T>(x[0], x[1]);
                             }

@@ -87,12 +87,6 @@ namespace b200wmma
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
             return y;
         }
-        __device__ __forceinline__ float lg2(float x)
-        {
-            float y;
-            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-            return y;
-        }
         __device__ __forceinline__ float rcp(float x)
         {
             float y;
@@ -602,19 +596,10 @@ namespace b200wmma
             else
                 f(Bent<MODEST>{});
         }
-        // Two scores whose distances are `dist` and `dist` + `step`; slip: the cap's derivative.
-        template <bool CAP, bool BIAS, Bend HOW>
-        __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
+        // Two scores whose distances are `dist` and `dist` + `step`, without a cap and from their tanh; the cap's derivative there.
+        template <bool BIAS>
+        __device__ __forceinline__ uint64_t biased(const ScoreConst& s, uint64_t x, float dist, float step)
         {
-            uint64_t x;
-            if constexpr(CAP)
-            {
-                const uint64_t tanh = tanh2<HOW>(s, dot);
-                slip = fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
-                x    = mul2(tanh, pair(s.cap2, s.cap2));
-            }
-            else
-                x = mul2(dot, pair(s.c, s.c));
             if constexpr(BIAS)
             {
                 float a, b;
@@ -622,6 +607,28 @@ namespace b200wmma
                 x = pair(fmaf(-s.slope, fabsf(dist), a), fmaf(-s.slope, fabsf(dist + step), b));
             }
             return x;
+        }
+        template <bool BIAS>
+        __device__ __forceinline__ uint64_t capped(const ScoreConst& s, uint64_t tanh, float dist, float step)
+        {
+            return biased<BIAS>(s, mul2(tanh, pair(s.cap2, s.cap2)), dist, step);
+        }
+        __device__ __forceinline__ uint64_t slip_of(uint64_t tanh)
+        {
+            return fma2(mul2(tanh, pair(-1.0f, -1.0f)), tanh, pair(1.0f, 1.0f));
+        }
+        // Either of them; slip: the cap's derivative.
+        template <bool CAP, bool BIAS, Bend HOW>
+        __device__ __forceinline__ uint64_t score2(const ScoreConst& s, uint64_t dot, float dist, float step, uint64_t& slip)
+        {
+            if constexpr(CAP)
+            {
+                const uint64_t tanh = tanh2<HOW>(s, dot);
+                slip = slip_of(tanh);
+                return capped<BIAS>(s, tanh, dist, step);
+            }
+            else
+                return biased<BIAS>(s, mul2(dot, pair(s.c, s.c)), dist, step);
         }
 
         // ---- host side ------------------------------------------------------------------------
