@@ -50,15 +50,16 @@ namespace b200wmma
         }
 
         // Lets a kernel use this much dynamic shared memory; asked of the driver once per device and kernel (`allowed` is the
-        // kernel's own), which saves a launch-bound caller half a microsecond a call.
-        using Allowed = std::atomic<uint32_t>[MAX_DEVICES];
+        // kernel's own), which saves a launch-bound caller half a microsecond a call.  `bytes` has to be the same in every call of
+        // a kernel, the most that any launch of it takes: threads that come here for the first time at once all ask the driver.
+        using Allowed = std::atomic<bool>[MAX_DEVICES];
         static int allow_smem(const void* kern, uint32_t bytes, Allowed& allowed)
         {
-            std::atomic<uint32_t>& most = allowed[current_device_slot()];
-            if(most.load(std::memory_order_relaxed) < bytes)
+            std::atomic<bool>& asked = allowed[current_device_slot()];
+            if(!asked.load(std::memory_order_acquire))
             {
                 B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-                most.store(bytes, std::memory_order_relaxed);
+                asked.store(true, std::memory_order_release);
             }
             return B200WMMA_OK;
         }

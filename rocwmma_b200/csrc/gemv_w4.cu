@@ -276,15 +276,15 @@ namespace b200wmma
                 bytes  = total(w, x_warp);
             }
             // x in rings
-            static __host__ __device__ uint32_t ring_x(uint32_t rows)
+            static constexpr __host__ __device__ uint32_t ring_x(uint32_t rows)
             {
                 return FEW_STAGES * rows * FEW_K * 2;
             }
-            static __host__ __device__ uint32_t ring_bytes(uint32_t w, uint32_t rows)
+            static constexpr __host__ __device__ uint32_t ring_bytes(uint32_t w, uint32_t rows)
             {
                 return total(w, ring_x(rows));
             }
-            static __host__ __device__ uint32_t total(uint32_t w, uint32_t x)
+            static constexpr __host__ __device__ uint32_t total(uint32_t w, uint32_t x)
             {
                 const uint32_t ring = w * (FEW_STAGES * W_STAGE + x), red = w * 128 * 4; // the sums reuse the ring
                 return ZERO + (ring > red ? ring : red);
@@ -463,12 +463,13 @@ namespace b200wmma
             }
         }
 
-        template <auto KERN, typename... More>
+        // MOST: what any call of KERN asks for.
+        template <auto KERN, uint32_t MOST, typename... More>
         static int launch_clusters(const Args& p, uint32_t blocks, uint32_t blocks_y, uint32_t parts, uint32_t smem,
                                    uint32_t threads, cudaStream_t stream, More... more)
         {
             static attn::Allowed allowed;
-            if(int e = attn::allow_smem(reinterpret_cast<const void*>(KERN), smem, allowed))
+            if(int e = attn::allow_smem(reinterpret_cast<const void*>(KERN), MOST, allowed))
                 return e;
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(blocks * parts, blocks_y), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
@@ -490,7 +491,7 @@ namespace b200wmma
         // Warps of a block: 8 for one vector (16384 x 8192 fp16: 21 us, 24 with 4), 4 for more, whose rings would leave room for
         // one or two blocks on an SM (7 x 5003 x 4128 bf16, groups of 32: 12 us, 14 with 8).  One vector that is too long to lie in
         // shared memory next to the rings goes through them like several.
-        constexpr uint32_t ONE_BYTES = 100 * 1024;
+        constexpr uint32_t ONE_BYTES = 100 * 1024, RING_BYTES = Few::ring_bytes(4, FEW_VECTORS);
         template <typename T, bool SIGNED, int STEPS>
         static int launch_few(const Args& p, cudaStream_t stream)
         {
@@ -500,10 +501,10 @@ namespace b200wmma
                 const uint32_t parts = parts_of(blocks, ceil_div(p.n, 8 * FEW_K), 2);
                 const Few      f(8, p.n, parts);
                 if(f.bytes <= ONE_BYTES)
-                    return launch_clusters<few_kernel<T, SIGNED, 8, STEPS, true>>(p, blocks, 1, parts, f.bytes, 256, stream);
+                    return launch_clusters<few_kernel<T, SIGNED, 8, STEPS, true>, ONE_BYTES>(p, blocks, 1, parts, f.bytes, 256, stream);
             }
             const uint32_t parts = parts_of(blocks, ceil_div(p.n, 4 * FEW_K), 2);
-            return launch_clusters<few_kernel<T, SIGNED, 4, STEPS, false>>(p, blocks, 1, parts, Few::ring_bytes(4, p.rows), 128, stream);
+            return launch_clusters<few_kernel<T, SIGNED, 4, STEPS, false>, RING_BYTES>(p, blocks, 1, parts, Few::ring_bytes(4, p.rows), 128, stream);
         }
         template <typename T, bool SIGNED, int N, int SETS>
         static int launch_tc(const Args& p, cudaStream_t stream)
@@ -518,7 +519,7 @@ namespace b200wmma
             if(int e = tc05::make_kmajor_tmap(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                                               p.x, p.rows, p.n, p.ldx, N))
                 return e;
-            return launch_clusters<tc_kernel<T, SIGNED, N, SETS>>(p, blocks, blocks_y, parts, L::BYTES, TC_THREADS, stream, status, map);
+            return launch_clusters<tc_kernel<T, SIGNED, N, SETS>, L::BYTES>(p, blocks, blocks_y, parts, L::BYTES, TC_THREADS, stream, status, map);
         }
         template <typename T, bool SIGNED, int SETS>
         static int launch_tc_rows(const Args& p, cudaStream_t stream)
