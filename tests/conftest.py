@@ -25,6 +25,12 @@ def _has_gpu():
 def pytest_collection_modifyitems(config, items):
     # GPU tests are selected with -m gpu; without a device they are skipped, never silently passed.
     if _has_gpu():
+        # The refusals next to them hand addresses that are none to the entry points; a call that is not refused (attn_bwd takes an
+        # o with overlapping rows, which it only reads) is harmless only where nothing can be launched.
+        skip = pytest.mark.skip(reason="calls with made-up addresses: only without a CUDA device")
+        for item in items:
+            if "gpu" not in item.keywords and item.path.name.startswith("test_gpu_"):
+                item.add_marker(skip)
         return
     skip = pytest.mark.skip(reason="no CUDA device")
     for item in items:
