@@ -7,20 +7,9 @@ namespace b200wmma
     namespace attn
     {
         constexpr uint32_t SLOTS = 148; // blocks that run at once, one to an SM
-        // Workspace: documents of the query and key tiles, then (backward) lse and delta of each row, padded to whole tiles, then the
-        // parts of dk and dv where the dkv kernel may be split (see dkv_splits; at most a tile of each for every block of SLOTS).
         static size_t tiles_of(uint32_t len)
         {
             return (len + TILE - 1) / TILE;
-        }
-        static size_t workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv, int backward)
-        {
-            const size_t docs = batch * (tiles_of(len_q) + tiles_of(len_kv)) * sizeof(DocTile);
-            if(!backward)
-                return docs;
-            const size_t rows = 2 * size_t(batch) * heads_q * tiles_of(len_q) * TILE * sizeof(float);
-            const bool   split = 2 * tiles_of(len_kv) * batch <= SLOTS && tiles_of(len_q) * heads_q > 4;
-            return docs + rows + (split ? size_t(SLOTS) * 2 * TILE * MAX_DIM * sizeof(float) : 0);
         }
         // Blocks of the dkv kernel to a key tile: where those tiles do not fill the machine the steps (query heads x query tiles) are
         // split, at least four to a block, and the parts are summed up by a kernel of their own: 8 query heads to one key head, 1700
@@ -30,6 +19,30 @@ namespace b200wmma
             const uint64_t blocks = tiles_of(len_kv) * batch * heads_kv, most = (tiles_of(len_q) * (heads_q / heads_kv) + 3) / 4;
             const uint64_t n = SLOTS / blocks < most ? SLOTS / blocks : most;
             return n > 1 ? uint32_t(n) : 1u;
+        }
+        // Blocks of a dkv kernel that is split, for whatever number of key heads makes them most.
+        static size_t dkv_parts(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv)
+        {
+            const size_t tiles = tiles_of(len_kv) * batch; // of one key head
+            size_t       most  = 0;
+            for(uint32_t heads_kv = 1; tiles && heads_kv <= heads_q && 2 * tiles * heads_kv <= SLOTS; ++heads_kv)
+                if(heads_q % heads_kv == 0)
+                {
+                    const uint32_t splits = dkv_splits(batch, heads_q, heads_kv, len_q, len_kv);
+                    if(splits > 1 && splits * tiles * heads_kv > most)
+                        most = splits * tiles * heads_kv;
+                }
+            return most;
+        }
+        // Workspace: documents of the query and key tiles, then (backward) lse and delta of each row, padded to whole tiles, then the
+        // parts of dk and dv, a tile of each for every block of a dkv kernel that is split.
+        static size_t workspace_bytes(uint32_t batch, uint32_t heads_q, uint32_t len_q, uint32_t len_kv, int backward)
+        {
+            const size_t docs = batch * (tiles_of(len_q) + tiles_of(len_kv)) * sizeof(DocTile);
+            if(!backward)
+                return docs;
+            const size_t rows = 2 * size_t(batch) * heads_q * tiles_of(len_q) * TILE * sizeof(float);
+            return docs + rows + dkv_parts(batch, heads_q, len_q, len_kv) * 2 * TILE * MAX_DIM * sizeof(float);
         }
         static int list_documents(const Params& p, void* workspace, const DocTile** q, const DocTile** kv, cudaStream_t stream)
         {
