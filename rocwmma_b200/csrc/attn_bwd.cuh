@@ -397,10 +397,10 @@ namespace b200wmma
 #pragma unroll
                         for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             small = small && tame<CAP>(sc, v[i]);
-                        if(small && !(e >> 24 & TILE_MASK))
-                            weights(std::false_type{}, Bent<TAME>{});
-                        else
+                        if(!small || (e >> 24 & TILE_MASK))
                             bend<CAP>(sc, small, [&](auto how) { weights(std::true_type{}, how); });
+                        else
+                            weights(std::false_type{}, Bent<TAME>{});
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -737,8 +737,7 @@ namespace b200wmma
                         // v becomes P, or under a cap the tanh, from which P and the cap's derivative come again below (registers for both
                         // would not do, and from a weight a tanh comes back only as well as the cap is large); P (1 - tanh^2) goes over
                         // the scores.  -infinity stands for pairs that are not visible.
-                        const uint64_t sub = pair(-ls, -ls);
-                        const auto     weights = [&](auto masked, auto how) {
+                        const auto weights = [&](auto masked, auto how) {
 #pragma unroll
                             for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             {
@@ -746,7 +745,7 @@ namespace b200wmma
 #pragma unroll
                                 for(int j = 0; j < 32; j += 2)
                                 {
-                                    const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1]));
+                                    const uint64_t dot = pair(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1])), sub = pair(-ls, -ls);
                                     [[maybe_unused]] const float dist = from - static_cast<float>(32 * i + j);
                                     float                        x[2], tanh[2], slip[2] = {1.0f, 1.0f};
                                     if constexpr(CAP)
@@ -780,10 +779,10 @@ namespace b200wmma
 #pragma unroll
                         for(uint32_t i = 0; i < W::CHUNKS; ++i)
                             small = small && tame<CAP>(sc, v[i]);
-                        if(small && !(e >> 24 & TILE_MASK))
-                            weights(std::false_type{}, Bent<TAME>{});
-                        else
+                        if(!small || (e >> 24 & TILE_MASK))
                             bend<CAP>(sc, small, [&](auto how) { weights(std::true_type{}, how); });
+                        else
+                            weights(std::false_type{}, Bent<TAME>{});
                         tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -810,7 +809,7 @@ namespace b200wmma
                                 {
                                     const uint64_t t = pair(pr[0], pr[1]);
                                     unpair(slip_of(t), slip[0], slip[1]);
-                                    unpair(add2(capped<BIAS>(sc, t, from - static_cast<float>(c), -1.0f), sub), pr[0], pr[1]);
+                                    unpair(add2(capped<BIAS>(sc, t, from - static_cast<float>(c), -1.0f), pair(-ls, -ls)), pr[0], pr[1]);
                                     pr[0] = ex2(pr[0]), pr[1] = ex2(pr[1]);
                                 }
 #pragma unroll
