@@ -382,7 +382,8 @@ int b200wmma_gemv_w4(uint32_t m, uint32_t n, uint32_t rows,
  * to it between the two products, everything else (scores, sums, statistics, accumulators) is fp32.
  * head_dim is a multiple of 8, at most 128.  Rows (one token of one head) are contiguous; the strides of batch entries,
  * tokens and heads are free positive multiples of 8 elements (any value for an extent of 1), bases 16-byte aligned.  scale,
- * cap, 1 / cap and scale / cap are at most 1e30.
+ * cap, 1 / cap and scale / cap are at most 1e30, scale / cap is 0 or at least 1e-37.  tanh is right to some units of its last
+ * place, up to a cap of 64 to some of 2^-24; its derivative is 1 - tanh^2 of that number.
  * slopes [heads_q] fp32, prefix [batch], doc_q [batch][len_q], doc_kv [batch][len_kv] int32 and may be NULL (doc_q and
  * doc_kv only together).  A negative document marks padding: whatever the rows of padding hold, NaN included, has no
  * influence; their outputs and gradients are zero.  All other elements of q, k, v and dout must be finite, visible or not

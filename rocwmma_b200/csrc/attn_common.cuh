@@ -130,6 +130,8 @@ namespace b200wmma
             const float limit = 1e30f, magnitude = a->scale < 0.0f ? -a->scale : a->scale;
             B200_REQUIRE(magnitude <= limit && (a->cap == 0.0f || (a->cap >= 1.0f / limit && a->cap <= limit && magnitude / a->cap <= limit)),
                          B200WMMA_ERR_UNSUPPORTED, "%s: scale, cap, 1 / cap and scale / cap must be at most 1e30", who);
+            B200_REQUIRE(a->cap == 0.0f || magnitude == 0.0f || magnitude / a->cap >= 1e-37f, B200WMMA_ERR_UNSUPPORTED,
+                         "%s: scale / cap must be 0 or at least 1e-37", who);
             return B200WMMA_OK;
         }
     } // namespace attn
