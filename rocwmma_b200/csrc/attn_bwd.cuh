@@ -8,8 +8,9 @@
 // with dS = P (dP - delta) (1 - tanh^2).  P^T and dS overwrite the products that they come from in tensor memory.
 // 256 or 512 threads compute; one warp issues the products, one the copies.
 // Bound: the products.  Each kernel has four to a pair of tiles (2048 cycles at a head of 128); S of the next step runs while dS
-// of this one is computed, dP of the next one while its P is.  Measured, bf16, gradients of 2 x 16 heads of 4096 x 128: 0.91 ms
-// (750 TFLOP/s counting five products), causal 0.52 ms, causal with cap and 4 key heads 0.78 ms; both kernels take about the same.
+// of this one is computed, dP of the next one while its P is.  Measured, bf16, gradients of 2 x 16 heads of 4096 x 128: 0.92 ms
+// (735-750 TFLOP/s counting five products), causal 0.51 ms, causal with cap and 4 key heads 0.65 ms; both kernels take about the
+// same.
 #pragma once
 #include "attn_tc05.cuh"
 
@@ -19,7 +20,8 @@ namespace b200wmma
     {
         // Four warps compute a part of a tile's columns, COLS to a lane; then come the warps for TMA and MMA.  Two parts, or four under
         // a cap, whose longer chain of instructions more warps hide: forward and backward of 2 x 8 heads of 1027 x 80 with cap and
-        // slopes 99 us (109 with two parts); without a cap four parts lose (2 x 16 heads of 4096 x 128, causal: 0.57 ms, 0.52).
+        // slopes 97 us (at that step 99, 109 with two parts); without a cap four parts lose (2 x 16 heads of 4096 x 128, causal: 0.57 ms,
+        // 0.52).
         template <bool CAP>
         struct BwdWarps
         {

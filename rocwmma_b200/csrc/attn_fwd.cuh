@@ -8,11 +8,11 @@
 // The running maximum of a row is only moved when a score passes it by more than 2^14 (RESCALE_STEP), so O is rescaled rarely and
 // a tile's weights mostly take one pass over its scores.  Key tiles come from the last to the first: under a causal mask the
 // nearest ones, which a distance bias makes the largest, are first (2 x 16 heads of 4096 x 128 with slopes: 173 us; 270 the other
-// way round, where the maximum moves in every tile).
+// way round, where the maximum moves in every tile, at that step).
 // Bound: a pair of tiles takes 1.9 us at a head of 128, 1.55 us of which remain without any softmax: M = 128, N = 128 products
 // read shared memory at its full 128 bytes a cycle next to the copies' writes, and 2 x 2 of them are 1.1 us by the tensor cores'
-// rate.  Measured, bf16: 1 x 16 heads of 16384 x 128 1.1-1.2 PFLOP/s, 2 x 16 heads of 4096 x 128 0.28 ms (980 TFLOP/s), causal
-// 0.15 ms (930), causal with cap 0.19-0.21 ms, 5 packed documents of 8192 tokens 0.10 ms.  What was tried and not kept: announcing
+// rate.  Measured, bf16: 1 x 16 heads of 16384 x 128 1.1-1.2 PFLOP/s, 2 x 16 heads of 4096 x 128 0.28 ms (990 TFLOP/s), causal
+// 0.15 ms (930), causal with cap 0.19-0.21 ms, with slopes 0.15 ms, 5 packed documents of 8192 tokens 0.11 ms.  What was tried and not kept: announcing
 // P in halves (931 instead of 1064 TFLOP/s then), part of the exponentials as polynomials (892-938).
 #pragma once
 #include "attn_tc05.cuh"

@@ -9,9 +9,10 @@
 // to operands in registers.
 // The tokens are split over blocks where rows, heads and sequences alone do not fill the machine; a second kernel joins the
 // parts in a fixed order.
-// Measured, bf16, 32/8 heads x 128, one token each: 32 sequences of 4500 tokens 88 us (6.7 TB/s), of 3094 to 6000 tokens 93 us
-// (6.4 TB/s); 8 drafted tokens each, 16 sequences of 8000: 92 us (5.7 TB/s); 5 drafted tokens, 8/2 heads x 64, one sequence of
-// 120000, fp16 with slopes: 20.6 us (3.0 TB/s; 13 stages to a block, latency).
+// Measured, bf16, 32/8 heads x 128, one token each: 32 sequences of 4500 tokens 89 us (6.6 TB/s), of 3094 to 6000 tokens 94 us
+// (6.4 TB/s; a copy, which also writes, reaches 6.5, the dgemv kernel, which only reads, 7.3); 8 drafted tokens each, 16 sequences
+// of 8000: 89 us (5.9 TB/s); 5 drafted tokens, 8/2 heads x 64, one sequence of 120000, fp16 with slopes: 19-21 us (3.0-3.2 TB/s;
+// 13 stages to a block, latency); one token after 8192: 13 us.
 #include "attn_tc05.cuh"
 
 namespace b200wmma
@@ -592,7 +593,8 @@ namespace b200wmma
         }
 
         // More rows than 32 take the tcgen05 form: 8 drafted tokens x 4 heads (32 rows) over 16 x 8000 tokens take 92 us with
-        // warp-level products and 145 us with tiles of 128 rows that are mostly empty; 128 rows take 212 us and 69 us.
+        // warp-level products and 145 us with tiles of 128 rows that are mostly empty; 128 rows took 212 us and 69 us
+        // when this was chosen (32 rows now 89 us).
         constexpr uint32_t WARP_ROWS = 32;
         static bool many_rows(uint32_t rows)
         {

